@@ -348,7 +348,7 @@ def _run_own(s):
         return {"k": k, "v": v}
     if case["kind"] == "prompt":
         return prompt_attention(s["q"], s["k"], s["v"], s["ends"], s["ends_k"], causal=case["causal"], window=case["window"])
-    return paged_attention(s["q"], PagedKVCache(**s["cache"]), s["pages"], s["lens_dev"], s["ends"], window=case["window"])
+    return paged_attention(s["q"], PagedKVCache(**s["cache"]), s["pages"], s["lens_dev"], s["ends"], max_new=max(s["new"]), window=case["window"])
 
 
 def run(state):
