@@ -400,6 +400,90 @@ int sngguf_grouped_linear_ws(const void* x, int64_t M, const uint8_t* indicator,
                              int numerics, void* stream);
 
 /*
+ * ---- Between a layer's projections: rotary positions, a paged cache of keys and values, attention -----------------
+ * What modeling_qwen3.py:431-505 and :583-745 do with tensor operations between the q / k / v projections and the output
+ * projection.  All values are bf16 [tokens][heads][dim], the elements of a head next to each other; tokens and heads may lie
+ * any distance apart (strides in elements, a tensor's views into the projections' stacked output among them).
+ */
+
+/* Rotation of pairs of a head's elements: a pair at position p turns by 2 pi p turns[i], i < pairs, and is scaled by
+ * `magnitude`.  Pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with interleaved != 0; the elements from 2 * pairs on are
+ * left as they are.  Angles are formed in 64 bits, cosine and sine are rounded to fp32, a product sum to bf16 once. */
+typedef struct sngguf_rotary_table {
+    const double* turns;  /* device, [pairs]                 */
+    int64_t pairs;        /* 1 .. dim / 2                     */
+    double magnitude;
+    int32_t interleaved;
+} sngguf_rotary_table;
+
+/* Keys and values of `pages` * `page_size` tokens.  qtype SNGGUF_TYPE_BF16: k, v are bf16 [pages][kv_heads][page_size][dim].
+ * SNGGUF_TYPE_Q8_0: k, v are int8 of that shape and k_scale, v_scale fp16 [pages][kv_heads][dim / 32][page_size]; 32 elements
+ * of a token share a scale d = fp16(max |x| / 127), at most 512, and are held as rint(x / d), at most 127 in magnitude (the
+ * arithmetic of a Q8_0 block; larger values than 65024 saturate, a NaN makes its 32 elements NaN).  All four 16-byte aligned.
+ * page_size: a power of two, 16 .. 4096.  dim: a multiple of 32 up to 256.  Token t of a sequence lies at slot
+ * table[t / page_size] * page_size + t % page_size. */
+typedef struct sngguf_kv_cache {
+    void *k, *v, *k_scale, *v_scale;
+    int64_t pages, page_size, kv_heads, dim;
+    int32_t qtype;
+} sngguf_kv_cache;
+
+/* q_out = q turned, and the same for k (k_heads = 0: q alone).  dim % 8 == 0, up to 1024.  An output may be its input (same address and
+ * strides), else they must not overlap.  Any alignment; fastest with rows of whole 16-byte pieces. */
+int sngguf_rotary(const sngguf_rotary_table* table, const int64_t* positions, int64_t tokens, int64_t dim,
+                  const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                  const void* k, int64_t k_heads, int64_t k_token, int64_t k_head, void* k_out, int64_t k_out_token, int64_t k_out_head,
+                  void* stream);
+
+/* k, v [tokens][cache heads][dim] into the cache's slots, one slot a token.  Negative slots and slots behind the last page are passed over.
+ * Where two tokens have one slot, that slot holds an unspecified mixture of them. */
+int sngguf_cache_write(const sngguf_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                       int64_t v_token, int64_t v_head, const int64_t* slots, int64_t tokens, void* stream);
+
+/* sngguf_rotary of q, and sngguf_cache_write of the turned k (rounded to bf16, as sngguf_rotary does) and of v, in one launch. */
+int sngguf_cache_write_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_table* table, const int64_t* positions,
+                              const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                              const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                              const int64_t* slots, int64_t tokens, void* stream);
+
+/* The cache's slots as bf16 rows: k_out, v_out [tokens][kv_heads][dim], contiguous, 16-byte aligned.  Slots outside the cache
+ * give zeros. */
+int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of packed sequences: sequence i has the queries [ends_q[i], ends_q[i + 1]) and the keys [ends_k[i], ends_k[i + 1])
+ * (device, [sequences + 1], not decreasing).  out = softmax(scale q . k) v, each query over the keys that it sees: all, or
+ * with causal != 0 those up to its own place, the last query standing at the last key; with window > 0 (causal only) the last
+ * `window` of them.  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, those of out not
+ * written.  heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads).  dim: a multiple of 32 up to 256.
+ * q, k, v, out: rows of whole 16-byte pieces.  Scores, maxima and sums are fp32, the weights are rounded to bf16 for the product
+ * with v.  A key or value that is not finite reaches every query of its sequence that sees it, and may reach those that share
+ * a tile of 64 keys with it; other sequences' never do.
+ * workspace (16-byte aligned) of sngguf_attention_workspace_bytes(...): partial results where few rows meet many keys; with
+ * less, or NULL, such a call is slower.  Nothing in it outlives the call.
+ */
+int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim);
+int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head,
+                     const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                     int64_t tokens_k, int64_t kv_heads, int64_t dim, const int32_t* ends_q, const int32_t* ends_k, int64_t sequences,
+                     float scale, int causal, int64_t window, void* out, int64_t out_token, int64_t out_head,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of new tokens over sequences that lie in a paged cache, their own keys and values already written: sequence i has
+ * lens[i] tokens in all, in the pages table[i][0 .. ], of which the last ends_q[i + 1] - ends_q[i] are the queries; ends_q NULL:
+ * one query a sequence, in order.  Causal.  max_new: the most queries of any sequence as far as the caller knows, 0 if it does
+ * not (a wrong value costs time only).  Lengths beyond the table's width count as its width; page numbers outside the cache are
+ * read as the nearest page.  table: rows table_stride apart, table_width numbers each.  An 8-bit cache is multiplied in fp16,
+ * its values rounded to 11 bits.  Everything else as sngguf_attention.
+ */
+int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim);
+int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
+                           const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* lens, const int32_t* ends_q,
+                           int64_t sequences, int64_t max_new, float scale, int64_t window, void* out, int64_t out_token, int64_t out_head,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * ---- GGUF container reader (host only, no GPU call) -----------------------------------
  * What the reference gets from gguf.GGUFReader at
  * src/sensenova_u1/utils/gguf_loader.py:29-44: open the file, walk `reader.tensors`, read each

@@ -1,0 +1,359 @@
+"""What stands between a decoder layer's projections: rotary positions, a paged cache of keys and values, and attention over
+whole prompts or over that cache (``modeling_qwen3.py:431-505,583-745``, where the reference runs tensor operations).
+
+All of it takes and gives bf16 ``[tokens][heads][dim]`` on one HIP device, enqueues on the current stream, never synchronises,
+and reads every length, position, slot and page number on the device: a captured step replays with new ones.  Views into a
+stacked projection's output go in as they are.  Forward only: nothing here records a gradient.
+
+A layer's attention for new tokens of sequences that lie in a cache::
+
+    q, k, v = (y.view(tokens, -1, dim) for y in qkv(hidden, norm_weight, eps))     # FusedProjections
+    q = cache.write_rotary(q, k, v, positions, table, slots)
+    out = paged_attention(q, cache, pages, lens, ends)                              # [tokens][heads][dim]
+    hidden = o_proj.forward_residual(out.view(tokens, -1), hidden)
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import ops
+from .ops import SnGgufError
+
+_BF16 = torch.bfloat16
+
+
+class _TableStruct(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double), ("interleaved", ctypes.c_int32)]
+
+
+class _CacheStruct(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("qtype", ctypes.c_int32)]
+
+
+def _same_device(what: str, index: int, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise SnGgufError(f"{what}: tensors on different devices (or on the host; there is no CPU implementation)")
+
+
+def _heads(x: torch.Tensor, what: str, name: str) -> torch.Tensor:
+    """``x`` as [tokens][heads][dim] rows whose elements are neighbours."""
+    if not x.is_cuda:
+        raise SnGgufError(f"sn_gguf ops run on a HIP device only, got {name} on '{x.device}'; there is no CPU implementation")
+    if x.dtype != _BF16 or x.dim() != 3:
+        raise SnGgufError(f"{what}: {name} must be bf16 [tokens][heads][dim], got {x.dtype} {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise SnGgufError(f"{what}: forward only, but {name} requires a gradient")
+    return x if x.stride(2) == 1 or x.numel() == 0 else x.contiguous()
+
+
+def _pieces(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with every row at a 16-byte boundary (copied where it is not; strides of one row or none do not count)."""
+    t, h, _ = x.stride()
+    if (t % 8 == 0 or x.shape[0] < 2) and (h % 8 == 0 or x.shape[1] < 2) and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(x: torch.Tensor):
+    """(token, head) strides; those of an axis of one entry are never stepped over and count as whole pieces."""
+    t, h, _ = x.stride()
+    return (t if x.shape[0] > 1 else 0), (h if x.shape[1] > 1 else 0)
+
+
+def _numbers(x: torch.Tensor, dtype: torch.dtype, count: Optional[int], what: str, name: str) -> torch.Tensor:
+    if x.dtype != dtype or x.dim() != 1 or (count is not None and x.shape[0] != count):
+        raise SnGgufError(f"{what}: {name} must be {dtype} [{count if count is not None else 'n'}], got {x.dtype} {tuple(x.shape)}")
+    return x if x.stride(0) == 1 or x.shape[0] < 2 else x.contiguous()
+
+
+class RotaryTable:
+    """How the pairs of a head turn: pair i by ``turns[i]`` turns (of 2 pi) a position, and the result scaled by ``magnitude``.
+
+    ``turns``: float64 on the device, one for each pair; pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with
+    ``interleaved``; elements behind the 2 * pairs first are left as they are.  ``for_model`` makes it of a checkpoint's settings."""
+
+    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address")
+
+    def __init__(self, turns: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0) -> None:
+        if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
+            raise SnGgufError(f"RotaryTable: turns must be float64 [pairs] on a HIP device, got {turns.dtype} {tuple(turns.shape)} on '{turns.device}'")
+        if not math.isfinite(magnitude):
+            raise SnGgufError("RotaryTable: the magnitude is not finite")
+        self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
+        self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
+        self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self.magnitude, self.interleaved)
+        self._address = ctypes.addressof(self._struct)
+
+    @classmethod
+    def for_model(cls, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_context: int = 0,
+                  beta_fast: float = 32.0, beta_slow: float = 1.0, magnitude: Optional[float] = None, interleaved: bool = False,
+                  device="cuda") -> "RotaryTable":
+        """The table of ``rotary_dim`` elements with wavelengths from 2 pi to 2 pi ``base`` positions.
+
+        ``scaling`` (a GGUF file's ``rope.scaling.type``): ``"none"``; ``"linear"``: positions count 1 / ``factor``;
+        ``"yarn"``: pairs that turn more than ``beta_fast`` times over ``original_context`` positions are left, those that turn
+        less than ``beta_slow`` times are stretched by ``factor``, with a ramp between, and the magnitude is 0.1 ln(factor) + 1."""
+        if rotary_dim < 2 or rotary_dim % 2:
+            raise SnGgufError(f"RotaryTable: {rotary_dim} elements are no pairs")
+        if scaling not in ("none", "linear", "yarn") or not factor > 0 or not base > 1:
+            raise SnGgufError(f"RotaryTable: scaling '{scaling}' by {factor} on base {base} is not known")
+        half = rotary_dim // 2
+        pair = torch.arange(half, dtype=torch.float64)
+        turns = float(base) ** (-pair / half) / (2 * math.pi)
+        size = 1.0
+        if scaling == "linear":
+            turns = turns / factor
+        elif scaling == "yarn":
+            if original_context < 1:
+                raise SnGgufError("RotaryTable: yarn scaling needs the original context")
+            at = [half * math.log(original_context / (beta * 2 * math.pi)) / math.log(base) for beta in (beta_fast, beta_slow)]
+            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
+            keep = 1 - ((pair - low) / max(high - low, 0.001)).clamp(0, 1)
+            turns = turns * keep + turns / factor * (1 - keep)
+            size = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+        return cls(turns.to(device), interleaved, size if magnitude is None else magnitude)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: RotaryTable, inplace: bool = False):
+    """Queries and keys turned by their positions: ``(q, k)``, new tensors or with ``inplace`` the given ones.
+
+    q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None.  positions: int64 [tokens].  A model whose head
+    has parts with positions of their own calls it on views of the parts."""
+    q0, k0 = q, k
+    q = _heads(q, "rotary", "q")
+    tokens, heads, dim = q.shape
+    index = q.get_device()
+    positions = _numbers(positions, torch.int64, tokens, "rotary", "positions")
+    _same_device("rotary", index, k, positions, table.turns)
+    if k is not None:
+        k = _heads(k, "rotary", "k")
+        if k.shape[0] != tokens or k.shape[2] != dim:
+            raise SnGgufError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
+    if inplace and (q is not q0 or k is not k0):
+        raise SnGgufError("rotary: in place needs the elements of a head next to each other")
+    q_out = q if inplace else torch.empty((tokens, heads, dim), dtype=_BF16, device=q.device)
+    k_out = k if inplace or k is None else torch.empty(k.shape, dtype=_BF16, device=q.device)
+    if tokens and heads:
+        kt, kh, kot, koh = (*_strides(k), *_strides(k_out)) if k is not None else (0, 0, 0, 0)
+        kp, kop, kn = (k.data_ptr(), k_out.data_ptr(), k.shape[1]) if k is not None else (None, None, 0)
+        dev = q.device
+        with ops._on(dev):
+            rc = ops.load_library().sngguf_rotary(table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, *_strides(q), q_out.data_ptr(),
+                                                  *_strides(q_out), kp, kn, kt, kh, kop, kot, koh, ops._stream(dev))
+        ops._check(rc, "sngguf_rotary")
+    return q_out, k_out
+
+
+class PagedKVCache:
+    """Keys and values of ``pages`` * ``page_size`` tokens of one layer.
+
+    bf16: ``k`` and ``v`` are bf16 ``[pages][kv_heads][page_size][dim]``.  8 bits: int8 of that shape, with fp16 ``k_scale`` and
+    ``v_scale`` ``[pages][kv_heads][dim / 32][page_size]``; 32 elements of a token share a scale, as in a Q8_0 block (magnitudes
+    beyond 65024 saturate, a NaN makes its 32 elements NaN).  ``page_size`` is a power of two from 16 to 4096, ``dim`` a multiple
+    of 32 up to 256.  ``PagedKVCache.empty`` allocates one; the constructor takes tensors that are there.
+
+    Token t of a sequence lies at slot ``page_of_the_sequence[t // page_size] * page_size + t % page_size``."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+        if not k.is_cuda:
+            raise SnGgufError(f"sn_gguf ops run on a HIP device only, got a cache on '{k.device}'; there is no CPU implementation")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or k.dtype not in (_BF16, torch.int8) or not k.is_contiguous() or not v.is_contiguous():
+            raise SnGgufError("PagedKVCache: k and v must be contiguous bf16 or int8 [pages][kv_heads][page_size][dim]")
+        pages, kv_heads, page, dim = shape
+        if pages < 1 or kv_heads < 1 or page < 16 or page > 4096 or page & (page - 1) or dim % 32 or not 32 <= dim <= 256:
+            raise SnGgufError(f"PagedKVCache: pages of 16 .. 4096 tokens (a power of two) and heads of 32 .. 256 elements (a multiple of 32) are needed, got {tuple(shape)}")
+        q8 = k.dtype == torch.int8
+        for s in (k_scale, v_scale):
+            if (s is not None) != q8 or (q8 and (s.dtype != torch.float16 or s.shape != (pages, kv_heads, dim // 32, page) or not s.is_contiguous())):
+                raise SnGgufError("PagedKVCache: an int8 cache has contiguous fp16 scales [pages][kv_heads][dim / 32][page_size], a bf16 cache none")
+        index = k.get_device()
+        _same_device("PagedKVCache", index, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.quant_type = ops.Q8_0 if q8 else ops.BF16
+        self.pages, self.kv_heads, self.page_size, self.dim, self._index = pages, kv_heads, page, dim, index
+        self._struct = _CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None, pages, page,
+                                    kv_heads, dim, self.quant_type)
+        self._address = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, dim: int, quant_type: int = ops.Q8_0, device="cuda") -> "PagedKVCache":
+        """A cache of uninitialised pages: ``quant_type`` ``ops.Q8_0`` (8 bits) or ``ops.BF16``."""
+        if quant_type not in (ops.Q8_0, ops.BF16):
+            raise SnGgufError(f"PagedKVCache: quant type {quant_type} is not implemented (have Q8_0=8, BF16=30)")
+        q8 = quant_type == ops.Q8_0
+        k, v = (torch.empty((pages, kv_heads, page_size, dim), dtype=torch.int8 if q8 else _BF16, device=device) for _ in range(2))
+        scales = [torch.empty((pages, kv_heads, dim // 32, page_size), dtype=torch.float16, device=device) for _ in range(2)] if q8 else [None, None]
+        return cls(k, v, *scales)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+
+    def _rows(self, k, v, slots, what):
+        k, v = _heads(k, what, "k"), _heads(v, what, "v")
+        if k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[2] != self.dim:
+            raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with a cache of {self.kv_heads} heads of {self.dim}")
+        slots = _numbers(slots, torch.int64, k.shape[0], what, "slots")
+        _same_device(what, self._index, k, v, slots)
+        return k, v, slots
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Keys and values [tokens][kv_heads][dim] into ``slots`` (int64 [tokens], different ones; negative ones and those behind
+        the last page are passed over)."""
+        k, v, slots = self._rows(k, v, slots, "PagedKVCache.write")
+        if k.shape[0]:
+            dev = k.device
+            with ops._on(dev):
+                rc = ops.load_library().sngguf_cache_write(self._address, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), k.shape[0],
+                                                           ops._stream(dev))
+            ops._check(rc, "sngguf_cache_write")
+
+    def write_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: RotaryTable, slots: torch.Tensor,
+                     inplace: bool = False) -> torch.Tensor:
+        """``rotary`` of q and k, then ``write`` of the turned k and of v, in one launch; returns the turned q (with ``inplace`` in
+        q's own memory; k is left as it is)."""
+        what = "PagedKVCache.write_rotary"
+        q0 = q
+        q = _heads(q, what, "q")
+        k, v, slots = self._rows(k, v, slots, what)
+        tokens = k.shape[0]
+        if q.shape[0] != tokens or q.shape[2] != self.dim:
+            raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
+        if inplace and q is not q0:
+            raise SnGgufError(f"{what}: in place needs the elements of a head next to each other")
+        positions = _numbers(positions, torch.int64, tokens, what, "positions")
+        _same_device(what, self._index, q, positions, table.turns)
+        out = q if inplace else torch.empty(q.shape, dtype=_BF16, device=q.device)
+        if tokens:
+            dev = q.device
+            with ops._on(dev):
+                rc = ops.load_library().sngguf_cache_write_rotary(
+                    self._address, table._address, positions.data_ptr(), q.data_ptr(), q.shape[1], *_strides(q), out.data_ptr(), *_strides(out),
+                    k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), tokens, ops._stream(dev))
+            ops._check(rc, "sngguf_cache_write_rotary")
+        return out
+
+    def read(self, slots: torch.Tensor):
+        """``(k, v)`` of ``slots`` (int64 [tokens]) as bf16 [tokens][kv_heads][dim]; a slot outside the cache gives zeros."""
+        slots = _numbers(slots, torch.int64, None, "PagedKVCache.read", "slots")
+        _same_device("PagedKVCache.read", self._index, slots)
+        dev = self.k.device
+        k, v = (torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=_BF16, device=dev) for _ in range(2))
+        if slots.shape[0]:
+            with ops._on(dev):
+                rc = ops.load_library().sngguf_cache_read(self._address, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(), ops._stream(dev))
+            ops._check(rc, "sngguf_cache_read")
+        return k, v
+
+
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=_BF16, device=q.device)
+    if out.dtype != _BF16 or out.shape != q.shape or out.get_device() != q.get_device() or out.stride(2) != 1 or _pieces(out) is not out:
+        raise SnGgufError(f"{what}: out must be bf16 {tuple(q.shape)} on q's device, its rows of whole 16-byte pieces")
+    return out
+
+
+def _check_options(what: str, heads: int, kv_heads: int, dim: int, scale: Optional[float], window: int) -> float:
+    if kv_heads < 1 or heads % kv_heads or heads < 1:
+        raise SnGgufError(f"{what}: {heads} query heads cannot share {kv_heads} key / value heads")
+    if dim % 32 or not 32 <= dim <= 256:
+        raise SnGgufError(f"{what}: heads of {dim} elements (a multiple of 32 up to 256 is needed)")
+    if window < 0:
+        raise SnGgufError(f"{what}: a window of {window} tokens")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise SnGgufError(f"{what}: a scale of {scale}")
+    return scale
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: torch.Tensor, ends_k: Optional[torch.Tensor] = None,
+                     causal: bool = True, scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of packed sequences: sequence i has the queries ``ends_q[i] : ends_q[i + 1]`` and the keys ``ends_k[i] :
+    ends_k[i + 1]`` (int32 [sequences + 1], not decreasing; ``ends_k`` defaults to ``ends_q``).
+
+    q [tokens][heads][dim], k and v [keys][kv_heads][dim], ``heads`` a multiple of ``kv_heads``, ``dim`` a multiple of 32 up to
+    256.  Causal: the last query of a sequence stands at its last key, and none sees a key behind its own place; ``window`` > 0: only the last
+    ``window`` keys up to it.  A query that sees nothing gives zeros.  ``scale`` defaults to dim ** -0.5.  Rows of ``out`` behind
+    the last sequence are not written."""
+    what = "prompt_attention"
+    q, k, v = _pieces(_heads(q, what, "q")), _pieces(_heads(k, what, "k")), _pieces(_heads(v, what, "v"))
+    tokens, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[2] != dim:
+        raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
+    scale = _check_options(what, heads, k.shape[1], dim, scale, window)
+    if window and not causal:
+        raise SnGgufError(f"{what}: a window needs causal attention")
+    ends_q = _numbers(ends_q, torch.int32, None, what, "ends_q")
+    ends_k = ends_q if ends_k is None else _numbers(ends_k, torch.int32, ends_q.shape[0], what, "ends_k")
+    if ends_q.shape[0] < 1:
+        raise SnGgufError(f"{what}: ends_q has no entry")
+    _same_device(what, q.get_device(), k, v, ends_q, ends_k)
+    out = _output(out, q, what)
+    sequences = ends_q.shape[0] - 1
+    if tokens and sequences:
+        dev = q.device
+        lib = ops.load_library()
+        nbytes = lib.sngguf_attention_workspace_bytes(tokens, sequences, heads, k.shape[1], dim)
+        with ops._on(dev), ops._whole_call(dev):
+            ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
+            rc = lib.sngguf_attention(q.data_ptr(), tokens, heads, *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), k.shape[0],
+                                      k.shape[1], dim, ends_q.data_ptr(), ends_k.data_ptr(), sequences, scale, int(causal), window,
+                                      out.data_ptr(), *_strides(out), ops._ptr(ws), nbytes, ops._stream(dev))
+        ops._check(rc, "sngguf_attention")
+    return out
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, lens: torch.Tensor, ends_q: Optional[torch.Tensor] = None,
+                    max_new: int = 0, scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of new tokens over sequences in a paged cache, their own keys and values already written.
+
+    pages: int32 [sequences][width], the pages of each sequence in order.  lens: int32 [sequences], its tokens in all.  The queries
+    of sequence i are ``ends_q[i] : ends_q[i + 1]`` (int32 [sequences + 1]) and stand at its last places; without ``ends_q`` every
+    sequence has one, in order.  ``max_new``: the most queries of any sequence, where the program knows it (0: unknown); it
+    decides which kernels are launched and never what they compute.  ``scale``, ``window``, ``out``: as ``prompt_attention``."""
+    what = "paged_attention"
+    q = _pieces(_heads(q, what, "q"))
+    tokens, heads, dim = q.shape
+    if dim != cache.dim:
+        raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with a cache of heads of {cache.dim}")
+    scale = _check_options(what, heads, cache.kv_heads, dim, scale, window)
+    if max_new < 0:
+        raise SnGgufError(f"{what}: max_new is {max_new}")
+    lens = _numbers(lens, torch.int32, None, what, "lens")
+    sequences = lens.shape[0]
+    if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != sequences:
+        raise SnGgufError(f"{what}: pages must be int32 [{sequences}][width], got {pages.dtype} {tuple(pages.shape)}")
+    width = pages.shape[1]
+    if width * cache.page_size >= 1 << 31:
+        raise SnGgufError(f"{what}: {width} pages of {cache.page_size} tokens a sequence are too many")
+    if (width > 1 and pages.stride(1) != 1) or (sequences > 1 and pages.stride(0) < width):
+        pages = pages.contiguous()
+    if ends_q is not None:
+        ends_q = _numbers(ends_q, torch.int32, sequences + 1, what, "ends_q")
+    elif tokens != sequences:
+        raise SnGgufError(f"{what}: {tokens} queries of {sequences} sequences need ends_q")
+    _same_device(what, cache._index, q, pages, lens, ends_q)
+    out = _output(out, q, what)
+    if tokens and sequences:
+        dev = q.device
+        lib = ops.load_library()
+        if ends_q is None:
+            max_new = 1
+        nbytes = lib.sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, heads, cache.kv_heads, dim)
+        with ops._on(dev), ops._whole_call(dev):
+            ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
+            rc = lib.sngguf_paged_attention(q.data_ptr(), tokens, heads, *_strides(q), cache._address, pages.data_ptr(), pages.stride(0), width,
+                                            lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), *_strides(out),
+                                            ops._ptr(ws), nbytes, ops._stream(dev))
+        ops._check(rc, "sngguf_paged_attention")
+    return out

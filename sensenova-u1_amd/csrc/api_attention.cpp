@@ -1,0 +1,359 @@
+// extern "C" entry points between a layer's projections: rotary positions, the paged cache, attention.  Argument checks and
+// the choice of kernels; nothing here allocates, synchronises or throws.
+#include <hip/hip_runtime_api.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "attention.hpp"
+#include "rotary_cache.hpp"
+
+namespace sngguf {
+int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream);
+int launch_attention_tiles(const AttentionArgs& a, int dim, int source, hipStream_t stream);
+}  // namespace sngguf
+
+namespace {
+
+using sngguf::AttentionArgs;
+using sngguf::bf16_t;
+using sngguf::RotaryCacheArgs;
+
+constexpr int64_t kMost = (int64_t)1 << 31;           // tokens, heads, pages: numbered with 32 bits
+constexpr int64_t kMostStride = (int64_t)1 << 26;     // elements between tokens: sixteen rows within 32-bit byte offsets
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int check_cache(const sngguf_kv_cache* c) {
+    if (!c) return SNGGUF_E_NULLPTR;
+    if (c->qtype != SNGGUF_TYPE_BF16 && c->qtype != SNGGUF_TYPE_Q8_0) return SNGGUF_E_BADTYPE;
+    if (c->pages < 1 || c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)) != 0 || c->pages >= kMost ||
+        c->kv_heads < 1 || c->kv_heads > 65535 || c->dim < 32 || c->dim > 256 || c->dim % 32 != 0)
+        return SNGGUF_E_BADSHAPE;
+    if (!c->k || !c->v) return SNGGUF_E_NULLPTR;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return SNGGUF_E_ALIGN;
+    if (c->qtype == SNGGUF_TYPE_Q8_0) {
+        if (!c->k_scale || !c->v_scale) return SNGGUF_E_NULLPTR;
+        if (!aligned(c->k_scale, 16) || !aligned(c->v_scale, 16)) return SNGGUF_E_ALIGN;
+    }
+    return SNGGUF_OK;
+}
+
+int log2_of(int64_t v) {
+    int s = 0;
+    while (((int64_t)1 << s) < v) s++;
+    return s;
+}
+
+void set_cache(RotaryCacheArgs& a, const sngguf_kv_cache* c) {
+    a.k_pages = c->k;
+    a.v_pages = c->v;
+    a.k_scales = static_cast<uint16_t*>(c->k_scale);
+    a.v_scales = static_cast<uint16_t*>(c->v_scale);
+    a.page_shift = log2_of(c->page_size);
+    a.slot_count = c->pages * c->page_size;
+    a.kv_heads = (int32_t)c->kv_heads;
+}
+
+// Rows of whole 16-byte pieces
+bool whole_pieces(const void* p, int64_t token, int64_t head) { return aligned(p, 16) && token % 8 == 0 && head % 8 == 0; }
+
+int check_table(const sngguf_rotary_table* t, const int64_t* positions, int64_t tokens, int64_t dim, int64_t heads) {
+    if (!t) return SNGGUF_E_NULLPTR;
+    if (tokens < 0 || tokens >= kMost || dim < 8 || dim > 1024 || dim % 8 != 0 || heads < 1 || heads > 65535 || t->pairs < 1 || 2 * t->pairs > dim ||
+        !isfinite(t->magnitude))
+        return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!t->turns || !positions) return SNGGUF_E_NULLPTR;
+    if (!aligned(t->turns, 8) || !aligned(positions, 8)) return SNGGUF_E_ALIGN;
+    return SNGGUF_OK;
+}
+
+void set_table(RotaryCacheArgs& a, const sngguf_rotary_table* t, const int64_t* positions) {
+    a.turns = t->turns;
+    a.magnitude = t->magnitude;
+    a.positions = positions;
+    a.pairs = (int32_t)t->pairs;
+    a.interleaved = t->interleaved != 0;
+}
+
+// ---- attention: how much is launched ----------------------------------------------------------------------------------
+
+constexpr int kRowsWant = 768, kRowsLeast = 2, kRowsKeys = 128;    // three workgroups a compute unit; at least 256 keys each
+constexpr int kTilesWant = 512, kTilesLeast = 4, kTilesRows = 128, kTilesKeys = 64;
+
+int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// (row tile, head) pairs at most: every sequence's last tile may be cut short
+int64_t tiles_most(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int rows) {
+    return kv_heads * (tokens * (heads / kv_heads) / rows + sequences);
+}
+
+struct Launch {
+    int64_t tiles, grid, partial_bytes;
+};
+
+// Split only where unsplit workgroups do not fill the device.
+Launch plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int dim, int rows, int want) {
+    Launch p;
+    p.tiles = tiles_most(tokens, sequences, heads, kv_heads, rows);
+    const bool split = p.tiles < want;
+    p.grid = p.tiles + (split ? want : 0);
+    p.partial_bytes = split ? p.grid * rows * (dim + 2) * 4 : 0;
+    return p;
+}
+
+struct PagedPlan {
+    int rows;              // of a tile of the kernel for few rows
+    bool few, many;        // which kernels run
+    int64_t few_rows;      // sequences of at most so many rows go to the first where both run
+    Launch a, b;
+};
+
+PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim) {
+    PagedPlan p;
+    const int64_t group = heads / kv_heads;
+    const int64_t most = (max_new > 0 && max_new < tokens ? max_new : tokens) * group;
+    const int d = kernel_dim(dim), widest = d == 256 ? 32 : 64;
+    // one kernel where no sequence has more rows than its tile; else single tokens and chunks each have their own
+    const int64_t r = most <= widest ? most : group;
+    p.rows = r <= 16 ? 16 : r <= 32 ? 32 : widest;
+    p.few = r <= widest;
+    p.many = most > widest;
+    p.few_rows = p.many ? (p.few ? p.rows : 0) : kMost - 1;
+    p.a = plan(tokens, sequences, heads, kv_heads, d, p.rows, kRowsWant);
+    p.b = plan(tokens, sequences, heads, kv_heads, d, kTilesRows, kTilesWant);
+    return p;
+}
+
+bool heads_fit(int64_t heads, int64_t kv_heads, int64_t dim) {
+    return heads >= 1 && heads <= 65535 && kv_heads >= 1 && heads % kv_heads == 0 && dim >= 32 && dim <= 256 && dim % 32 == 0;
+}
+
+int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* partial, hipStream_t stream) {
+    a.partial = partial;
+    a.want = kTilesWant;
+    a.least = kTilesLeast;
+    a.grid = partial ? p.grid : p.tiles;
+    const int rc = sngguf::launch_attention_tiles(a, dim, source, stream);
+    if (rc != SNGGUF_OK || !partial) return rc;
+    return sngguf::launch_attention_combine(a, kTilesRows, kTilesKeys, dim, p.tiles, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sngguf_rotary(const sngguf_rotary_table* table, const int64_t* positions, int64_t tokens, int64_t dim, const void* q,
+                  int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
+                  const void* k, int64_t k_heads, int64_t k_token, int64_t k_head, void* k_out, int64_t k_out_token,
+                  int64_t k_out_head, void* stream) {
+    const int rc = check_table(table, positions, tokens, dim, q_heads);
+    if (rc != SNGGUF_OK) return rc;
+    if (k_heads < 0 || k_heads > 65535) return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!q || !q_out || (k_heads && (!k || !k_out))) return SNGGUF_E_NULLPTR;
+    if (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(k, 2) || !aligned(k_out, 2)) return SNGGUF_E_ALIGN;
+    RotaryCacheArgs a = {};
+    set_table(a, table, positions);
+    a.q = static_cast<const bf16_t*>(q);
+    a.q_out = static_cast<bf16_t*>(q_out);
+    a.k = static_cast<const bf16_t*>(k);
+    a.k_out = static_cast<bf16_t*>(k_out);
+    a.q_token = q_token, a.q_head = q_head, a.q_out_token = q_out_token, a.q_out_head = q_out_head;
+    a.k_token = k_token, a.k_head = k_head, a.k_out_token = k_out_token, a.k_out_head = k_out_head;
+    a.tokens = tokens;
+    a.dim = (int32_t)dim;
+    a.q_heads = (int32_t)q_heads;
+    a.k_heads = (int32_t)k_heads;
+    a.wide = whole_pieces(q, q_token, q_head) && whole_pieces(q_out, q_out_token, q_out_head) &&
+             (!k_heads || (whole_pieces(k, k_token, k_head) && whole_pieces(k_out, k_out_token, k_out_head)));
+    return sngguf::launch_rotary_cache(a, 0, static_cast<hipStream_t>(stream));
+}
+
+int sngguf_cache_write(const sngguf_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                       int64_t v_token, int64_t v_head, const int64_t* slots, int64_t tokens, void* stream) {
+    const int rc = check_cache(cache);
+    if (rc != SNGGUF_OK) return rc;
+    if (tokens < 0 || tokens >= kMost) return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!k || !v || !slots) return SNGGUF_E_NULLPTR;
+    if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return SNGGUF_E_ALIGN;
+    RotaryCacheArgs a = {};
+    set_cache(a, cache);
+    a.k = static_cast<const bf16_t*>(k);
+    a.v = static_cast<const bf16_t*>(v);
+    a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+    a.slots = slots;
+    a.tokens = tokens;
+    a.dim = (int32_t)cache->dim;
+    a.wide = whole_pieces(k, k_token, k_head) && whole_pieces(v, v_token, v_head);
+    return sngguf::launch_rotary_cache(a, cache->qtype == SNGGUF_TYPE_Q8_0 ? 2 : 1, static_cast<hipStream_t>(stream));
+}
+
+int sngguf_cache_write_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_table* table, const int64_t* positions,
+                              const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token,
+                              int64_t q_out_head, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, const int64_t* slots, int64_t tokens, void* stream) {
+    int rc = check_cache(cache);
+    if (rc == SNGGUF_OK) rc = check_table(table, positions, tokens, cache->dim, q_heads);
+    if (rc != SNGGUF_OK || tokens == 0) return rc;
+    if (!q || !q_out || !k || !v || !slots) return SNGGUF_E_NULLPTR;
+    if (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return SNGGUF_E_ALIGN;
+    RotaryCacheArgs a = {};
+    set_cache(a, cache);
+    set_table(a, table, positions);
+    a.q = static_cast<const bf16_t*>(q);
+    a.q_out = static_cast<bf16_t*>(q_out);
+    a.k = static_cast<const bf16_t*>(k);
+    a.v = static_cast<const bf16_t*>(v);
+    a.q_token = q_token, a.q_head = q_head, a.q_out_token = q_out_token, a.q_out_head = q_out_head;
+    a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+    a.slots = slots;
+    a.tokens = tokens;
+    a.dim = (int32_t)cache->dim;
+    a.q_heads = (int32_t)q_heads;
+    a.wide = whole_pieces(q, q_token, q_head) && whole_pieces(q_out, q_out_token, q_out_head) && whole_pieces(k, k_token, k_head) &&
+             whole_pieces(v, v_token, v_head);
+    return sngguf::launch_rotary_cache(a, cache->qtype == SNGGUF_TYPE_Q8_0 ? 2 : 1, static_cast<hipStream_t>(stream));
+}
+
+int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream) {
+    const int rc = check_cache(cache);
+    if (rc != SNGGUF_OK) return rc;
+    // (one thread for eight elements, workgroups of 256 numbered with 31 bits)
+    if (tokens < 0 || tokens >= kMost || tokens * cache->kv_heads * (cache->dim / 8) >= kMost * 256) return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!slots || !k_out || !v_out) return SNGGUF_E_NULLPTR;
+    if (!aligned(slots, 8) || !aligned(k_out, 16) || !aligned(v_out, 16)) return SNGGUF_E_ALIGN;
+    RotaryCacheArgs a = {};
+    set_cache(a, cache);
+    a.slots = slots;
+    a.tokens = tokens;
+    a.dim = (int32_t)cache->dim;
+    a.k_out = static_cast<bf16_t*>(k_out);
+    a.v_out = static_cast<bf16_t*>(v_out);
+    return sngguf::launch_cache_read(a, cache->qtype == SNGGUF_TYPE_Q8_0, static_cast<hipStream_t>(stream));
+}
+
+int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || !heads_fit(heads, kv_heads, dim)) return 0;
+    return plan(tokens_q, sequences, heads, kv_heads, kernel_dim(dim), kTilesRows, kTilesWant).partial_bytes;
+}
+
+int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const void* k,
+                     int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int64_t tokens_k,
+                     int64_t kv_heads, int64_t dim, const int32_t* ends_q, const int32_t* ends_k, int64_t sequences, float scale,
+                     int causal, int64_t window, void* out, int64_t out_token, int64_t out_head, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+    if (tokens_q < 0 || tokens_q >= kMost || tokens_k < 0 || tokens_k >= kMost || sequences < 0 || sequences >= kMost ||
+        !heads_fit(heads, kv_heads, dim) || tokens_q * (heads / kv_heads) >= kMost || window < 0 || (window && !causal) || !(scale >= 1e-30f) || scale > 1e30f ||
+        k_token < 0 || k_token >= kMostStride || v_token < 0 || v_token >= kMostStride)
+        return SNGGUF_E_BADSHAPE;
+    if (tokens_q == 0 || sequences == 0) return SNGGUF_OK;
+    if (!q || !out || !ends_q || !ends_k || (tokens_k && (!k || !v))) return SNGGUF_E_NULLPTR;
+    if (!whole_pieces(q, q_token, q_head) || !whole_pieces(k, k_token, k_head) || !whole_pieces(v, v_token, v_head) ||
+        !whole_pieces(out, out_token, out_head) || !aligned(ends_q, 4) || !aligned(ends_k, 4) || !aligned(workspace, 16))
+        return SNGGUF_E_ALIGN;
+    const int d = kernel_dim(dim);
+    const Launch p = plan(tokens_q, sequences, heads, kv_heads, d, kTilesRows, kTilesWant);
+    if (p.grid >= kMost) return SNGGUF_E_BADSHAPE;
+    AttentionArgs a = {};
+    a.q = static_cast<const bf16_t*>(q);
+    a.k = static_cast<const bf16_t*>(k);
+    a.v = static_cast<const bf16_t*>(v);
+    a.out = static_cast<bf16_t*>(out);
+    a.q_token = q_token, a.q_head = q_head, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+    a.out_token = out_token, a.out_head = out_head;
+    a.ends_q = ends_q;
+    a.ends_k = ends_k;
+    a.sequences = (int32_t)sequences;
+    a.tokens_q = tokens_q;
+    a.tokens_k = tokens_k;
+    a.heads = (int32_t)heads;
+    a.kv_heads = (int32_t)kv_heads;
+    a.group = (int32_t)(heads / kv_heads);
+    a.dim = (int32_t)dim;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.causal = causal != 0;
+    a.window = window;
+    a.min_rows = 1;
+    a.max_rows = (int32_t)(kMost - 1);
+    float* partial = p.partial_bytes && workspace && workspace_bytes >= p.partial_bytes ? static_cast<float*>(workspace) : nullptr;
+    return launch_many(a, p, d, 0, partial, static_cast<hipStream_t>(stream));
+}
+
+int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || max_new < 0 || !heads_fit(heads, kv_heads, dim)) return 0;
+    const PagedPlan p = paged_plan(tokens_q, sequences, max_new, heads, kv_heads, dim);
+    return (p.few ? p.a.partial_bytes : 0) + (p.many ? p.b.partial_bytes : 0);
+}
+
+int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
+                           const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* lens, const int32_t* ends_q,
+                           int64_t sequences, int64_t max_new, float scale, int64_t window, void* out, int64_t out_token,
+                           int64_t out_head, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = check_cache(cache);
+    if (rc != SNGGUF_OK) return rc;
+    if (tokens_q < 0 || tokens_q >= kMost || sequences < 0 || sequences >= kMost || !heads_fit(heads, cache->kv_heads, cache->dim) ||
+        tokens_q * (heads / cache->kv_heads) >= kMost || max_new < 0 || window < 0 || !(scale >= 1e-30f) || scale > 1e30f || table_width < 0 || table_width * cache->page_size >= kMost ||
+        (sequences > 1 && table_stride < table_width) || (!ends_q && tokens_q < sequences))
+        return SNGGUF_E_BADSHAPE;
+    if (tokens_q == 0 || sequences == 0) return SNGGUF_OK;
+    if (!q || !out || !lens || (table_width && !table)) return SNGGUF_E_NULLPTR;
+    if (!whole_pieces(q, q_token, q_head) || !whole_pieces(out, out_token, out_head) || !aligned(table, 4) || !aligned(lens, 4) ||
+        !aligned(ends_q, 4) || !aligned(workspace, 16))
+        return SNGGUF_E_ALIGN;
+    const int64_t kv_heads = cache->kv_heads;
+    const int d = kernel_dim(cache->dim);
+    const bool q8 = cache->qtype == SNGGUF_TYPE_Q8_0;
+    const PagedPlan p = paged_plan(tokens_q, sequences, ends_q ? max_new : 1, heads, kv_heads, cache->dim);
+    if (p.a.grid >= kMost || p.b.grid >= kMost) return SNGGUF_E_BADSHAPE;
+    AttentionArgs a = {};
+    a.q = static_cast<const bf16_t*>(q);
+    a.out = static_cast<bf16_t*>(out);
+    a.q_token = q_token, a.q_head = q_head, a.out_token = out_token, a.out_head = out_head;
+    a.k_pages = cache->k;
+    a.v_pages = cache->v;
+    a.k_scales = static_cast<const uint16_t*>(cache->k_scale);
+    a.v_scales = static_cast<const uint16_t*>(cache->v_scale);
+    a.table = table;
+    a.lens = lens;
+    a.table_stride = table_stride;
+    a.table_width = (int32_t)table_width;
+    a.pages = (int32_t)cache->pages;
+    a.page_shift = log2_of(cache->page_size);
+    a.ends_q = ends_q;
+    a.sequences = (int32_t)sequences;
+    a.tokens_q = tokens_q;
+    a.heads = (int32_t)heads;
+    a.kv_heads = (int32_t)kv_heads;
+    a.group = (int32_t)(heads / kv_heads);
+    a.dim = (int32_t)cache->dim;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.causal = 1;
+    a.window = window;
+    const int64_t need = (p.few ? p.a.partial_bytes : 0) + (p.many ? p.b.partial_bytes : 0);
+    float* partial = workspace && workspace_bytes >= need ? static_cast<float*>(workspace) : nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p.few) {
+        AttentionArgs f = a;
+        f.min_rows = 1;
+        f.max_rows = (int32_t)p.few_rows;
+        f.partial = p.a.partial_bytes ? partial : nullptr;
+        f.want = kRowsWant;
+        f.least = kRowsLeast;
+        f.grid = f.partial ? p.a.grid : p.a.tiles;
+        int r = sngguf::launch_attention_rows(f, p.rows, d, q8, s);
+        if (r == SNGGUF_OK && f.partial) r = sngguf::launch_attention_combine(f, p.rows, kRowsKeys, d, p.a.tiles, s);
+        if (r != SNGGUF_OK) return r;
+    }
+    if (p.many) {
+        a.min_rows = (int32_t)p.few_rows + 1;
+        a.max_rows = (int32_t)(kMost - 1);
+        float* rest = partial && p.b.partial_bytes ? partial + (p.few ? p.a.partial_bytes / 4 : 0) : nullptr;
+        return launch_many(a, p.b, d, q8 ? 2 : 1, rest, s);
+    }
+    return SNGGUF_OK;
+}
+
+}  // extern "C"

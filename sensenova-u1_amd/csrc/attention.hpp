@@ -1,0 +1,191 @@
+// What the attention kernels share: their arguments, and how a launch's workgroups find their share of the work.
+//
+// The lengths of the sequences lie in device memory (a captured launch sees new ones at every replay), so the host knows
+// only how many sequences and tokens there are at most.  Every workgroup scans the lengths itself, 64 sequences at a time,
+// and finds its (sequence, row tile, key / value head, split) from its number; workgroups beyond the last one leave.
+//
+// A row is one (token, query head) pair of the heads that share a key / value head: row r of a sequence is token r / group,
+// head r % group, so a tile of keys and values serves all heads of the group.
+#pragma once
+
+#include "sngguf_common.hpp"
+
+namespace sngguf {
+
+struct AttentionArgs {
+    const bf16_t* q;        // [tokens_q][heads][dim]
+    bf16_t* out;
+    int64_t q_token, q_head, out_token, out_head;     // strides in elements
+    // keys and values: packed rows ...
+    const bf16_t *k, *v;    // [tokens_k][kv_heads][dim]
+    int64_t k_token, k_head, v_token, v_head;
+    const int32_t* ends_k;  // [sequences + 1]
+    // ... or pages [pages][kv_heads][page][dim], scales [pages][kv_heads][dim / 32][page]
+    const void *k_pages, *v_pages;
+    const uint16_t *k_scales, *v_scales;
+    const int32_t* table;   // [sequences][table_width], rows table_stride apart
+    const int32_t* lens;    // [sequences]
+    int64_t table_stride;
+    int32_t pages, page_shift, table_width;
+    const int32_t* ends_q;  // [sequences + 1], or NULL: one token each
+    int32_t sequences;
+    int64_t tokens_q, tokens_k;
+    int32_t heads, kv_heads, group, dim;
+    float scale_log2;       // softmax scale x log2(e)
+    int32_t causal;
+    int64_t window;         // 0: none
+    int32_t min_rows, max_rows;   // rows of the sequences that this launch takes
+    // split of a sequence's keys over workgroups (NULL: none)
+    float* partial;         // [workgroups][tile rows][dim of the kernel], then [workgroups][tile rows][2]: maximum, sum
+    int32_t want;           // workgroups that fill the device
+    int32_t least;          // key tiles of a split at least
+    int64_t grid;           // workgroups of the main launch
+};
+
+struct AttentionSequence {
+    int64_t q0, k0;
+    int32_t lq, lk;
+};
+
+__device__ __forceinline__ AttentionSequence attention_sequence(const AttentionArgs& a, int i) {
+    AttentionSequence s;
+    if (a.ends_q) {
+        // (values that are no cumulative lengths stay within the tensors)
+        int64_t e0 = a.ends_q[i], e1 = a.ends_q[i + 1];
+        e0 = e0 < 0 ? 0 : e0 > a.tokens_q ? a.tokens_q : e0;
+        e1 = e1 < e0 ? e0 : e1 > a.tokens_q ? a.tokens_q : e1;
+        s.q0 = e0;
+        s.lq = (int32_t)(e1 - e0);
+    } else {
+        s.q0 = i;
+        s.lq = 1;
+    }
+    if (a.lens) {
+        const int64_t cap = (int64_t)a.table_width << a.page_shift;
+        int64_t n = a.lens[i];
+        s.k0 = 0;
+        s.lk = (int32_t)(n < 0 ? 0 : n > cap ? cap : n);
+    } else {
+        int64_t e0 = a.ends_k[i], e1 = a.ends_k[i + 1];
+        e0 = e0 < 0 ? 0 : e0 > a.tokens_k ? a.tokens_k : e0;
+        e1 = e1 < e0 ? e0 : e1 > a.tokens_k ? a.tokens_k : e1;
+        s.k0 = e0;
+        s.lk = (int32_t)(e1 - e0);
+    }
+    return s;
+}
+
+// Row tiles of a sequence, and key tiles that its rows see between them.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void attention_tiles(const AttentionArgs& a, const AttentionSequence& s, uint32_t& row_tiles, uint32_t& key_tiles) {
+    const int64_t rows = (int64_t)s.lq * a.group;
+    if (rows < a.min_rows || rows > a.max_rows) {
+        row_tiles = key_tiles = 0;
+        return;
+    }
+    row_tiles = (uint32_t)((rows + ROWS - 1) / ROWS);
+    int64_t lo = a.window ? (int64_t)s.lk - s.lq - a.window + 1 : 0;
+    lo = lo < 0 ? 0 : lo / KEYS;
+    const int64_t hi = ((int64_t)s.lk + KEYS - 1) / KEYS;
+    key_tiles = (uint32_t)(hi > lo ? hi - lo : 1);
+}
+
+struct AttentionBlock {
+    AttentionSequence s;
+    int32_t seq, row_tile, split, splits, kv_head;
+    int64_t slot;           // number of this workgroup's (combining: of split 0's) partial result; splits lie kv_heads apart
+    bool there;
+};
+
+// COMBINE: `id` counts (row tile, head) pairs and not (row tile, split, head) triples.
+template <int ROWS, int KEYS, bool COMBINE>
+__device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a, uint32_t id) {
+    const int lane = threadIdx.x & 63;
+    AttentionBlock b;
+    b.there = false;
+    // heads of one row tile are neighbours: with 8 key / value heads each XCD keeps to one head's keys and values
+    b.kv_head = id % (uint32_t)a.kv_heads;
+    const uint32_t want = id / (uint32_t)a.kv_heads;
+    uint64_t chunk = 0;     // key tiles of a split; 0: not split
+    if (a.partial) {
+        uint64_t total = 0;
+        for (int base = 0; base < a.sequences; base += 64) {
+            uint64_t mine = 0;
+            if (base + lane < a.sequences) {
+                uint32_t rt, kt;
+                attention_tiles<ROWS, KEYS>(a, attention_sequence(a, base + lane), rt, kt);
+                mine = (uint64_t)rt * kt;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
+            total += mine;
+        }
+        chunk = (total * a.kv_heads + a.want - 1) / (uint32_t)a.want;
+        if (chunk < (uint32_t)a.least) chunk = a.least;
+    }
+    uint32_t before = 0, before_slots = 0;
+    for (int base = 0; base < a.sequences; base += 64) {
+        uint32_t rt = 0, kt = 0, splits = 1;
+        if (base + lane < a.sequences) {
+            attention_tiles<ROWS, KEYS>(a, attention_sequence(a, base + lane), rt, kt);
+            if (chunk) splits = (uint32_t)((kt + chunk - 1) / chunk);
+            if (splits < 1) splits = 1;
+        }
+        const uint32_t slots = rt * splits, mine = COMBINE ? rt : slots;
+        uint32_t sum = mine, sum_slots = slots;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(sum, o), y = __shfl_up(sum_slots, o);
+            if (lane >= o) {
+                sum += x;
+                sum_slots += y;
+            }
+        }
+        const uint64_t hit = __ballot(want >= before + sum - mine && want < before + sum);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            const uint32_t first = before + (uint32_t)__builtin_amdgcn_readlane((int)(sum - mine), l);
+            const uint32_t first_slot = before_slots + (uint32_t)__builtin_amdgcn_readlane((int)(sum_slots - slots), l);
+            const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)rt, l);
+            b.seq = base + l;
+            b.splits = __builtin_amdgcn_readlane((int)splits, l);
+            const uint32_t within = want - first;
+            const uint32_t t = COMBINE ? within : within / (uint32_t)b.splits;
+            b.split = COMBINE ? 0 : (int32_t)(within - t * (uint32_t)b.splits);
+            // the last rows of a causal sequence see the most keys: first
+            b.row_tile = (int32_t)(tiles - 1 - t);
+            b.slot = ((int64_t)first_slot + (int64_t)t * b.splits + b.split) * a.kv_heads + b.kv_head;
+            b.s = attention_sequence(a, b.seq);
+            b.there = true;
+            return b;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        before_slots += (uint32_t)__builtin_amdgcn_readlane((int)sum_slots, 63);
+    }
+    return b;
+}
+
+// Keys [lo, hi) that some row of rows [r0, r1) of a sequence sees.
+__device__ __forceinline__ void attention_keys(const AttentionArgs& a, const AttentionSequence& s, int64_t r0, int64_t r1, int32_t& lo, int32_t& hi) {
+    const int64_t back = (int64_t)s.lk - s.lq;
+    lo = 0;
+    hi = s.lk;
+    if (a.causal) {
+        const int64_t last = back + (r1 - 1) / a.group + 1;
+        if (last < hi) hi = (int32_t)(last < 0 ? 0 : last);
+    }
+    if (a.window) {
+        const int64_t first = back + r0 / a.group - a.window + 1;
+        if (first > 0) lo = (int32_t)(first < hi ? first : hi);
+    }
+}
+
+// Page of a sequence's key; numbers that are no pages are read as the nearest one, so that no table reaches beyond the cache.
+__device__ __forceinline__ int64_t attention_page(const AttentionArgs& a, int seq, int32_t key) {
+    const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+    return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
+}
+
+int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, hipStream_t stream);
+
+}  // namespace sngguf
