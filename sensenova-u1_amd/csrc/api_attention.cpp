@@ -9,7 +9,7 @@
 
 namespace sngguf {
 int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream);
-int launch_attention_tiles(const AttentionArgs& a, int dim, int source, hipStream_t stream);
+int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream);
 }  // namespace sngguf
 
 namespace {
@@ -79,7 +79,9 @@ void set_table(RotaryCacheArgs& a, const sngguf_rotary_table* t, const int64_t* 
 // ---- attention: how much is launched ----------------------------------------------------------------------------------
 
 constexpr int kRowsWant = 768, kRowsLeast = 2, kRowsKeys = 128;    // three workgroups a compute unit; at least 256 keys each
-constexpr int kTilesWant = 512, kTilesLeast = 4, kTilesRows = 128, kTilesKeys = 64;
+constexpr int kTilesWant = 512, kTilesLeast = 4, kTilesKeys = 64;
+
+constexpr int64_t kWide = 512;      // 256-row workgroups from which on they are taken
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
@@ -89,17 +91,25 @@ int64_t tiles_most(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_
 }
 
 struct Launch {
+    int rows;
     int64_t tiles, grid, partial_bytes;
 };
 
 // Split only where unsplit workgroups do not fill the device.
 Launch plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int dim, int rows, int want) {
     Launch p;
+    p.rows = rows;
     p.tiles = tiles_most(tokens, sequences, heads, kv_heads, rows);
     const bool split = p.tiles < want;
     p.grid = p.tiles + (split ? want : 0);
     p.partial_bytes = split ? p.grid * rows * (dim + 2) * 4 : 0;
     return p;
+}
+
+// The kernel for many rows
+Launch plan_many(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
+    const int rows = dim <= 128 && tiles_most(tokens, 0, heads, kv_heads, 256) >= kWide ? 256 : 128;
+    return plan(tokens, sequences, heads, kv_heads, dim, rows, kTilesWant);
 }
 
 struct PagedPlan {
@@ -121,7 +131,7 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t
     p.many = most > widest;
     p.few_rows = p.many ? (p.few ? p.rows : 0) : kMost - 1;
     p.a = plan(tokens, sequences, heads, kv_heads, d, p.rows, kRowsWant);
-    p.b = plan(tokens, sequences, heads, kv_heads, d, kTilesRows, kTilesWant);
+    p.b = plan_many(tokens, sequences, heads, kv_heads, d);
     return p;
 }
 
@@ -134,9 +144,9 @@ int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* p
     a.want = kTilesWant;
     a.least = kTilesLeast;
     a.grid = partial ? p.grid : p.tiles;
-    const int rc = sngguf::launch_attention_tiles(a, dim, source, stream);
+    const int rc = sngguf::launch_attention_tiles(a, p.rows, dim, source, stream);
     if (rc != SNGGUF_OK || !partial) return rc;
-    return sngguf::launch_attention_combine(a, kTilesRows, kTilesKeys, dim, p.tiles, stream);
+    return sngguf::launch_attention_combine(a, p.rows, kTilesKeys, dim, p.tiles, stream);
 }
 
 }  // namespace
@@ -237,7 +247,7 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
 
 int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
     if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || !heads_fit(heads, kv_heads, dim)) return 0;
-    return plan(tokens_q, sequences, heads, kv_heads, kernel_dim(dim), kTilesRows, kTilesWant).partial_bytes;
+    return plan_many(tokens_q, sequences, heads, kv_heads, kernel_dim(dim)).partial_bytes;
 }
 
 int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const void* k,
@@ -255,7 +265,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
         !whole_pieces(out, out_token, out_head) || !aligned(ends_q, 4) || !aligned(ends_k, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
     const int d = kernel_dim(dim);
-    const Launch p = plan(tokens_q, sequences, heads, kv_heads, d, kTilesRows, kTilesWant);
+    const Launch p = plan_many(tokens_q, sequences, heads, kv_heads, d);
     if (p.grid >= kMost) return SNGGUF_E_BADSHAPE;
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);

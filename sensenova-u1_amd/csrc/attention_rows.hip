@@ -407,6 +407,8 @@ int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim
     SNGGUF_GO_DIM(32, 128)
     SNGGUF_GO_DIM(64, 128)
     SNGGUF_GO_DIM(128, 64)
+    SNGGUF_GO(256, 64, 64)
+    SNGGUF_GO(256, 64, 128)
 #undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;

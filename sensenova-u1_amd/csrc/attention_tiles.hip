@@ -1,15 +1,24 @@
 // Attention of many rows: whole prompts over their own packed keys and values, and chunks of new tokens over a paged cache.
 //
-// A workgroup takes 128 rows of one sequence and key / value head (row = token x query heads of the group, so the heads that
-// share keys and values share their tiles), four wavefronts of 32 rows, and walks over tiles of 64 keys in two LDS stages.
-// One pass with a running maximum m and sum l, in base 2.  Bound by the matrix instructions (32 x 32 x 16):
-//  * S^T = K Q^T: a lane holds sixteen of a row's 32 scores (row = lane % 32), so maxima and sums are taken in registers, and
-//    the two halves of a row meet in one exchange.  Register i of lane half h is key 8 (i / 4) + 4 h + i % 4;
+// A workgroup takes 128 CT rows of one sequence and key / value head (row = token x query heads of the group, so the heads that
+// share keys and values share their tiles), four wavefronts of 32 CT rows, and walks over tiles of 64 keys in a ring of LDS
+// stages.  One pass with a running maximum m and sum l, in base 2.  Bound by the matrix instructions (32 x 32 x 16):
+//  * S^T = K Q^T: a lane holds sixteen of a row's 32 scores (row = lane % 32).  Register i of lane half h is key 8 (i / 4) +
+//    4 h + i % 4;
 //  * O^T += V^T P^T wants eight keys of a row in each lane, in any order that V^T shares: those registers are taken as they
 //    are, and V, which lies row by row in LDS, is read with the transposing read, four keys of one element at a time.
 // In LDS a row's 16-byte pieces are permuted so that the eight or sixteen rows that one read touches lie in different banks;
 // copies go from global memory to LDS directly, and permute on the global side.
+//
+// A step takes 32 keys, and three of them at once: the product with V of the step before, the weights of its own scores, and the
+// scores of the step after depend on nothing of each other, so the vector instructions of the weights are dealt over the
+// matrix instructions.  What would put the maximum in front of the weights is left out: they are formed with the maximum known
+// so far, whatever the scores, and only if a row's 32 weights sum to more than a limit far within range (or to nothing that
+// is a number) are maximum, sums and weights set right, behind the step.
 // An 8-bit cache is widened on its way to LDS: fp16 there (see attention_rows.hip), and p is scaled by 2^12.
+#include <type_traits>
+#include <utility>
+
 #include "attention.hpp"
 
 namespace sngguf {
@@ -17,7 +26,6 @@ namespace sngguf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 128;
 constexpr int kKeys = 64;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -60,6 +68,12 @@ __device__ __forceinline__ void copy_request(uint32_t lds, uint32_t off, const v
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
+// f(0), f(1), ... f(N - 1), each number a constant (an unrolled loop of this size is given up by the compiler)
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>()), ...);
+}
+
 // What piece c of row r is exchanged with: rows that one read touches together get different pieces.
 template <int DT>
 __device__ __forceinline__ int swizzle(int r) {
@@ -71,36 +85,45 @@ __device__ __forceinline__ int swizzle(int r) {
 
 enum { kPacked = 0, kPaged = 1, kPagedQ8 = 2 };
 
-template <int DT, int SOURCE>
-__global__ __launch_bounds__(kThreads) void attention_tiles_kernel(AttentionArgs a) {
+// CT: 32-row tiles of a wavefront.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
+template <int DT, int SOURCE, int CT, int NS>
+__global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
+    constexpr int ROWS = 128 * CT;
     constexpr int PIECES = DT / 8;                     // of a row
     constexpr int TILE = kKeys * DT * 2;               // bytes
     constexpr int KS = DT / 16, DTILES = DT / 32;
+    constexpr int VF = 2 * DTILES, NF = VF + KS;       // operand fragments of a step: of values, in all
+    constexpr int NP = 8 * CT;                         // pairs of weights of a step that a lane forms
+    constexpr float kLimit = Q8 ? 32768.f : 1e9f;      // (fp16 weights are scaled by 2^12)
+    constexpr float kUp = Q8 ? 12.f : 0.f;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // [stage][keys, values]
 
-    const AttentionBlock b = attention_block<kRows, kKeys, false>(a, blockIdx.x);
+    const AttentionBlock b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
     if (!b.there) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
     const int64_t rows = (int64_t)b.s.lq * a.group;
-    const int64_t r0 = (int64_t)b.row_tile * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
+    const int64_t r0 = (int64_t)b.row_tile * ROWS, r1 = r0 + ROWS < rows ? r0 + ROWS : rows;
     int32_t lo, hi;
     attention_keys(a, b.s, r0, r1, lo, hi);
     const int32_t back = b.s.lk - b.s.lq;
 
-    // ---- this lane's row: its query as operand fragments, and the keys that it sees ------------------------------------
-    const int64_t r = r0 + 32 * wave + col;
-    const bool there = r < r1;
-    const int64_t rr = there ? r : r1 - 1;
-    const int32_t token = (int32_t)(rr / a.group), head = b.kv_head * a.group + (int32_t)(rr - (int64_t)token * a.group);
-    const int32_t place = back + token;
-    const int32_t last = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
-    const int32_t first = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
-    op_t qf[KS];
-    float c = a.scale_log2;
-    {
+    // ---- this lane's rows: their queries as operand fragments, and the keys that they see --------------------------------
+    op_t qf[CT][KS];
+    float c[CT];
+    int32_t first[CT], last[CT];
+    int64_t row_of[CT];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        row_of[n] = r0 + 32 * (CT * wave + n) + col;
+        const int64_t rr = row_of[n] < r1 ? row_of[n] : r1 - 1;
+        const int32_t token = (int32_t)(rr / a.group), head = b.kv_head * a.group + (int32_t)(rr - (int64_t)token * a.group);
+        const int32_t place = back + token;
+        last[n] = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
+        first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
+        c[n] = a.scale_log2;
         const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
         u32x4_t raw[KS];
 #pragma unroll
@@ -125,12 +148,12 @@ __global__ __launch_bounds__(kThreads) void attention_tiles_kernel(AttentionArgs
                 u32x4_t w;
 #pragma unroll
                 for (int j = 0; j < 4; j++) w[j] = pack_f16(__builtin_ldexpf(bf16lo_to_f32(raw[i][j]), -ex), __builtin_ldexpf(bf16hi_to_f32(raw[i][j]), -ex));
-                qf[i] = __builtin_bit_cast(op_t, w);
+                qf[n][i] = __builtin_bit_cast(op_t, w);
             }
-            c = fmaxf(__builtin_ldexpf(c, ex), 1.2e-38f);
+            c[n] = fmaxf(__builtin_ldexpf(c[n], ex), 1.2e-38f);
         } else {
 #pragma unroll
-            for (int i = 0; i < KS; i++) qf[i] = __builtin_bit_cast(op_t, raw[i]);
+            for (int i = 0; i < KS; i++) qf[n][i] = __builtin_bit_cast(op_t, raw[i]);
         }
     }
 
@@ -141,18 +164,24 @@ __global__ __launch_bounds__(kThreads) void attention_tiles_kernel(AttentionArgs
         s0 += per * b.split;
         s1 = s0 + per < s1 ? s0 + per : s1;
     }
+    const int32_t count = s1 - s0;
     // rows whose visible keys are the fewest: tiles inside these bounds need no mask
-    const int64_t tail = r1 - 1;
-    const int32_t place0 = back + (int32_t)(r0 / a.group), place1 = back + (int32_t)(tail / a.group);
+    const int32_t place0 = back + (int32_t)(r0 / a.group), place1 = back + (int32_t)((r1 - 1) / a.group);
     const int32_t all_last = a.causal && place0 < b.s.lk - 1 ? place0 : b.s.lk - 1;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
-    f32x16_t acc[DTILES];
+    f32x16_t acc[CT][DTILES];
+    float m[CT], l[CT], nb[CT];      // nb: what is added to a scaled score, kUp - m
 #pragma unroll
-    for (int t = 0; t < DTILES; t++)
+    for (int n = 0; n < CT; n++) {
+        m[n] = -__builtin_inff();
+        nb[n] = __builtin_inff();    // nothing known yet: whatever is formed with it is set right
+        l[n] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[t][i] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;
+        for (int t = 0; t < DTILES; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[n][t][i] = 0.f;
+    }
 
     // ---- tiles into LDS ------------------------------------------------------------------------------------------------
     // Sixteen rows a wavefront.  Rows behind the last key are the last key's: masked, but finite wherever the keys are.
@@ -162,215 +191,334 @@ __global__ __launch_bounds__(kThreads) void attention_tiles_kernel(AttentionArgs
     const int crow = lane / PIECES, cpiece = lane % PIECES;
     constexpr int QP = DT / 16;                        // 8-bit: 16-byte pieces of a row
     constexpr int QN = 16 * QP / 64;                   // ... a lane has of each tile
-    u32x4_t kq[Q8 ? QN : 1], vq[Q8 ? QN : 1];
-    uint16_t ksc[Q8 ? QN : 1], vsc[Q8 ? QN : 1];
-    auto request = [&](int32_t tile, int stage) {
-        const int32_t base = tile * kKeys + 16 * wave;
-        const int32_t most = b.s.lk - 1;
+    u32x4_t held[2][Q8 ? QN : 1];
+    uint16_t held_scale[2][Q8 ? QN : 1];
+    // keys (half 0) or values (half 1) of a tile into the stage's half
+    auto request_half = [&](int32_t tile, int stage, auto half_) {
+        constexpr int half = decltype(half_)::value;
+        const int32_t base = tile * kKeys + 16 * wave, most = b.s.lk - 1;
+        const int32_t lead = base < most ? base : most;
+        uint8_t* to = lds + (2 * stage + half) * TILE + 16 * wave * DT * 2;
         if constexpr (SOURCE == kPacked) {
-            const int32_t lead = base < most ? base : most;
-            const uint8_t* kb = uniform_ptr(a.k + (b.s.k0 + lead) * a.k_token + (int64_t)b.kv_head * a.k_head);
-            const uint8_t* vb = uniform_ptr(a.v + (b.s.k0 + lead) * a.v_token + (int64_t)b.kv_head * a.v_head);
+            const int64_t stride = half ? a.v_token : a.k_token;
+            const uint8_t* from = uniform_ptr((half ? a.v + (int64_t)b.kv_head * a.v_head : a.k + (int64_t)b.kv_head * a.k_head) + (b.s.k0 + lead) * stride);
 #pragma unroll
             for (int i = 0; i < REQ; i++) {
                 const int row = RQ * i + crow;
                 int piece = cpiece ^ swizzle<DT>(row);
                 piece = 8 * piece < a.dim ? piece : 0;
                 const int32_t at = base + row < most ? base + row - lead : most - lead;
-                copy_request(lds_offset(lds + (2 * stage) * TILE + (16 * wave + RQ * i) * DT * 2), (uint32_t)(2 * (at * a.k_token + 8 * piece)), kb);
-                copy_request(lds_offset(lds + (2 * stage + 1) * TILE + (16 * wave + RQ * i) * DT * 2), (uint32_t)(2 * (at * a.v_token + 8 * piece)), vb);
+                copy_request(lds_offset(to + RQ * i * DT * 2), (uint32_t)(2 * (at * (int32_t)stride + 8 * piece)), from);
             }
         } else {
             // (sixteen rows lie in one page)
-            const int32_t lead = base < most ? base : most;
-            const int64_t page = __builtin_amdgcn_readfirstlane((int)attention_page(a, b.seq, lead));
-            const int64_t at_page = page * a.kv_heads + b.kv_head;
+            const int64_t at_page = (int64_t)__builtin_amdgcn_readfirstlane((int)attention_page(a, b.seq, lead)) * a.kv_heads + b.kv_head;
             if constexpr (SOURCE == kPaged) {
-                const uint8_t* kb = uniform_ptr(static_cast<const bf16_t*>(a.k_pages) + (at_page << a.page_shift) * a.dim);
-                const uint8_t* vb = uniform_ptr(static_cast<const bf16_t*>(a.v_pages) + (at_page << a.page_shift) * a.dim);
+                const uint8_t* from = uniform_ptr(static_cast<const bf16_t*>(half ? a.v_pages : a.k_pages) + (at_page << a.page_shift) * a.dim);
 #pragma unroll
                 for (int i = 0; i < REQ; i++) {
                     const int row = RQ * i + crow;
                     int piece = cpiece ^ swizzle<DT>(row);
                     piece = 8 * piece < a.dim ? piece : 0;
                     const int32_t at = (base + row < most ? base + row : most) & page_mask;
-                    const uint32_t off = (uint32_t)(2 * (at * a.dim + 8 * piece));
-                    copy_request(lds_offset(lds + (2 * stage) * TILE + (16 * wave + RQ * i) * DT * 2), off, kb);
-                    copy_request(lds_offset(lds + (2 * stage + 1) * TILE + (16 * wave + RQ * i) * DT * 2), off, vb);
+                    copy_request(lds_offset(to + RQ * i * DT * 2), (uint32_t)(2 * (at * a.dim + 8 * piece)), from);
                 }
             } else {
-                const uint8_t* kb = static_cast<const uint8_t*>(a.k_pages) + (at_page << a.page_shift) * a.dim;
-                const uint8_t* vb = static_cast<const uint8_t*>(a.v_pages) + (at_page << a.page_shift) * a.dim;
-                const uint16_t* ks = a.k_scales + (at_page * (a.dim >> 5) << a.page_shift);
-                const uint16_t* vs = a.v_scales + (at_page * (a.dim >> 5) << a.page_shift);
+                const uint8_t* from = static_cast<const uint8_t*>(half ? a.v_pages : a.k_pages) + (at_page << a.page_shift) * a.dim;
+                const uint16_t* scales = (half ? a.v_scales : a.k_scales) + (at_page * (a.dim >> 5) << a.page_shift);
 #pragma unroll
                 for (int i = 0; i < QN; i++) {
                     const int p = lane + 64 * i, row = p / QP;
                     int piece = p % QP;
                     piece = 16 * piece < a.dim ? piece : 0;
                     const int32_t at = (base + row < most ? base + row : most) & page_mask;
-                    kq[i] = *reinterpret_cast<const u32x4_t*>(kb + at * a.dim + 16 * piece);
-                    vq[i] = *reinterpret_cast<const u32x4_t*>(vb + at * a.dim + 16 * piece);
-                    ksc[i] = ks[((piece >> 1) << a.page_shift) + at];
-                    vsc[i] = vs[((piece >> 1) << a.page_shift) + at];
+                    held[half][i] = *reinterpret_cast<const u32x4_t*>(from + at * a.dim + 16 * piece);
+                    held_scale[half][i] = scales[((piece >> 1) << a.page_shift) + at];
                 }
             }
         }
     };
-    // 8-bit tiles: widened from the registers that request() filled
-    auto widen = [&](int stage) {
+    // 8-bit tiles: widened from the registers that the request filled
+    auto widen_half = [&](int stage, int half) {
         if constexpr (Q8) {
 #pragma unroll
-            for (int half = 0; half < 2; half++)
+            for (int i = 0; i < QN; i++) {
+                const int p = lane + 64 * i, row = p / QP, piece = p % QP;
+                const u32x4_t w = held[half][i];
+                const _Float16 d1 = __builtin_bit_cast(_Float16, held_scale[half][i]);
+                const f16x2_t d = {d1, d1};
+                uint8_t* to = lds + (2 * stage + half) * TILE + (16 * wave + row) * DT * 2;
 #pragma unroll
-                for (int i = 0; i < QN; i++) {
-                    const int p = lane + 64 * i, row = p / QP, piece = p % QP;
-                    const u32x4_t w = half ? vq[i] : kq[i];
-                    const _Float16 d1 = __builtin_bit_cast(_Float16, half ? vsc[i] : ksc[i]);
-                    const f16x2_t d = {d1, d1};
-                    uint8_t* to = lds + (2 * stage + half) * TILE + (16 * wave + row) * DT * 2;
+                for (int y = 0; y < 2; y++) {
+                    u32x4_t f;
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        u32x4_t f;
-#pragma unroll
-                        for (int z = 0; z < 2; z++) {
-                            const uint32_t flipped = w[2 * y + z] ^ 0x80808080u;
-                            f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * d);
-                            f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * d);
-                        }
-                        *reinterpret_cast<u32x4_t*>(to + 16 * ((2 * piece + y) ^ swizzle<DT>(row))) = f;
+                    for (int z = 0; z < 2; z++) {
+                        const uint32_t flipped = w[2 * y + z] ^ 0x80808080u;
+                        f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * d);
+                        f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * d);
                     }
+                    *reinterpret_cast<u32x4_t*>(to + 16 * ((2 * piece + y) ^ swizzle<DT>(row))) = f;
+                }
+            }
+        }
+    };
+    typedef std::integral_constant<int, 0> Keys;
+    typedef std::integral_constant<int, 1> Values;
+    // stage i: keys of tile i, values of tile i - 1 (behind the last tile: of the last, read by nobody, so that the loop neither asks
+    // whether there are more nor counts what is under way)
+    auto request = [&](int32_t i) {
+        const int stage = i % NS;
+        request_half(s0 + (i < count ? i : count - 1), stage, Keys());
+        request_half(s0 + (i <= count ? i : count) - 1, stage, Values());
+    };
+
+    // ---- fragments ---------------------------------------------------------------------------------------------------
+    // keys: row col, piece 2 ks + h; values: keys 4 h + (lane % 16) / 4, elements 16 ((lane % 32) / 16) + 4 (lane % 4) ...: the rows of one
+    // transposing read are four keys
+    const int vkey = 4 * h + ((lane & 15) >> 2), velem = 16 * ((lane & 31) >> 4) + 4 * (lane & 3);
+    auto key_fragment = [&](const uint8_t* kt, int half, int ks) -> op_t {
+        const int row = 32 * half + col;
+        return *reinterpret_cast<const op_t*>(kt + row * DT * 2 + 16 * ((2 * ks + h) ^ swizzle<DT>(col)));
+    };
+    auto value_fragment = [&](const uint8_t* vt, int half, int t, int x) -> op_t {
+        u32x2_t part[2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            const int row = 16 * x + 8 * y + vkey, e = 32 * t + velem;
+            part[y] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(
+                vt + (32 * half + row) * DT * 2 + 16 * ((e >> 3) ^ swizzle<DT>(row)) + 2 * (e & 7))));
+        }
+        return __builtin_bit_cast(op_t, u32x4_t{part[0][0], part[0][1], part[1][0], part[1][1]});
+    };
+
+    // ---- pieces of a step ----------------------------------------------------------------------------------------------
+    typedef f32x16_t scores_t[CT];
+    typedef uint32_t weights_t[CT][2][4];     // [16 keys][pair]
+    auto clear = [&](scores_t& s) {
+#pragma unroll
+        for (int n = 0; n < CT; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+    };
+    auto mask = [&](scores_t& s, int32_t key0) {
+        if (key0 + 31 > all_last || key0 < all_first) {
+#pragma unroll
+            for (int n = 0; n < CT; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int32_t key = key0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (key < first[n] || key > last[n]) s[n][i] = -__builtin_inff();
                 }
         }
     };
+    auto weights_pair = [&](const scores_t& s, weights_t& w, float (&sum)[CT], const float (&add)[CT], int p) {
+        const int n = p / 8, i = 2 * (p % 8);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c[n], add[n]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], c[n], add[n]));
+        if constexpr (Q8) {
+            w[n][i / 8][(i / 2) % 4] = pack_f16(p0, p1);
+            sum[n] += p0 + p1;
+        } else {
+            // the rounded weights are summed
+            const uint32_t both = pack_bf16(p0, p1);
+            w[n][i / 8][(i / 2) % 4] = both;
+            sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), sum[n], false);
+        }
+    };
+    // maximum, sums and weights from the scores
+    auto set_right = [&](const scores_t& s, weights_t& w, float (&sum)[CT]) {
+        float add[CT];
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            float top = s[n][0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, s[n][i]);
+            top = fmaxf(top, other_half(top));
+            top = fmaxf(top * c[n], m[n]);
+            const bool none = top == -__builtin_inff();
+            const float base = none ? 0.f : top;
+            const float keep = __builtin_amdgcn_exp2f(m[n] - base);
+            m[n] = top;
+            add[n] = kUp - base;
+            nb[n] = none ? __builtin_inff() : add[n];
+            l[n] *= keep;
+#pragma unroll
+            for (int t = 0; t < DTILES; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[n][t][i] *= keep;
+            sum[n] = 0.f;
+        }
+#pragma unroll
+        for (int p = 0; p < NP; p++) weights_pair(s, w, sum, add, p);
+    };
+    auto settle = [&](const scores_t& s, weights_t& w, float (&sum)[CT]) {
+        bool fine = true;
+#pragma unroll
+        for (int n = 0; n < CT; n++) fine = fine && sum[n] <= kLimit;
+        if (__any(!fine)) set_right(s, w, sum);
+#pragma unroll
+        for (int n = 0; n < CT; n++) l[n] += sum[n];
+    };
+    auto weights_operand = [&](const weights_t& w, int n, int x) -> op_t {
+        return __builtin_bit_cast(op_t, u32x4_t{w[n][x][0], w[n][x][1], w[n][x][2], w[n][x][3]});
+    };
 
-    // fragment addresses within a tile: keys: row col, piece 2 ks + h; values: key 4 h + (lane % 16) / 4, elements 16 ((lane %
-    // 32) / 16) + 4 (lane % 4) ..., the rows of one transposing read being four keys
-    const int vkey = 4 * h + ((lane & 15) >> 2), velem = 16 * ((lane & 31) >> 4) + 4 * (lane & 3);
+    op_t ring[4];
+    // One step: values of keys 32 half ... of vt times w0; weights of s into w1; scores of keys 32 half ... of kt into s1.
+    // The first two fragments are in the ring; the next step's are fetched by its end, from half 1 of vt or from `vnext`, behind the
+    // barrier that its stage needs (LAST).
+    auto step = [&](scores_t& s, scores_t& s1, const weights_t& w0, weights_t& w1, const uint8_t* kt, const uint8_t* vt, const uint8_t* vnext, int32_t key0,
+                    auto half_, auto arrive) {
+        constexpr int half = decltype(half_)::value;
+        mask(s, key0);
+        clear(s1);
+        float sum[CT];
+#pragma unroll
+        for (int n = 0; n < CT; n++) sum[n] = 0.f;
+        each_of(
+            [&](auto f_) {
+                constexpr int f = decltype(f_)::value, g = f + 2;
+                if constexpr (half == 1 && f == NF - 2) arrive();
+                if constexpr (g < VF) ring[g & 3] = value_fragment(vt, half, g >> 1, g & 1);
+                else if constexpr (g < NF) ring[g & 3] = key_fragment(kt, half, g - VF);
+                else ring[g & 3] = value_fragment(vnext, half ^ 1, 0, g - NF);
+#pragma unroll
+                for (int n = 0; n < CT; n++) {
+                    if constexpr (f < VF) acc[n][f >> 1] = mfma(ring[f & 3], weights_operand(w0, n, f & 1), acc[n][f >> 1]);
+                    else s1[n] = mfma(ring[f & 3], qf[n][f - VF], s1[n]);
+                }
+#pragma unroll
+                for (int p = f * NP / NF; p < (f + 1) * NP / NF; p++) weights_pair(s, w1, sum, nb, p);
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            std::make_integer_sequence<int, NF>());
+        settle(s, w1, sum);
+    };
+    auto scores = [&](scores_t& s, const uint8_t* kt, int half) {
+        clear(s);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const op_t k = key_fragment(kt, half, ks);
+#pragma unroll
+            for (int n = 0; n < CT; n++) s[n] = mfma(k, qf[n][ks], s[n]);
+        }
+    };
+    auto values = [&](const weights_t& w, const uint8_t* vt, int half) {
+#pragma unroll
+        for (int f = 0; f < VF; f++) {
+            const op_t v = value_fragment(vt, half, f >> 1, f & 1);
+#pragma unroll
+            for (int n = 0; n < CT; n++) acc[n][f >> 1] = mfma(v, weights_operand(w, n, f & 1), acc[n][f >> 1]);
+        }
+    };
 
-    if (s0 < s1) {
-        request(s0, 0);
-        widen(0);
-    }
-    for (int32_t s = s0; s < s1; s++) {
-        const int stage = (s - s0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (count > 0) {
+        scores_t sa, sb;
+        weights_t wa, wb;
+        float sum[CT];
+        auto stage_keys = [&](int32_t i) { return lds + (2 * (i % NS)) * TILE; };
+        auto stage_values = [&](int32_t i) { return lds + (2 * (i % NS) + 1) * TILE; };
+        // the requests of all stages but the NS - 2 last asked for have arrived, from every wavefront
+        auto wait_stage = [&] {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ * (NS - 2)) : "memory");
+            __syncthreads();
+        };
+        request_half(s0, 0, Keys());
+        if constexpr (Q8) widen_half(0, 0);
+        request(1);
+        if constexpr (!Q8) {
+            if constexpr (NS > 2) request(2);
+            // the keys of tile 0
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ * (NS - 1)) : "memory");
+        }
         __syncthreads();
-        if (s + 1 < s1) request(s + 1, stage ^ 1);
-        const uint8_t* kt = lds + (2 * stage) * TILE;
-        const uint8_t* vt = kt + TILE;
-        f32x16_t sc[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) sc[t][i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const int row = 32 * t + col;
-                const op_t kf = *reinterpret_cast<const op_t*>(kt + row * DT * 2 + 16 * ((2 * ks + h) ^ swizzle<DT>(row)));
-                sc[t] = mfma(kf, qf[ks], sc[t]);
-            }
+        scores(sa, stage_keys(0), 0);
+        scores(sb, stage_keys(0), 1);
+        if constexpr (Q8) {
+            widen_half(1 % NS, 0);
+            widen_half(1 % NS, 1);
         }
-        const int32_t key0 = s * kKeys;
-        if (key0 + kKeys - 1 > all_last || key0 < all_first) {
+        mask(sa, s0 * kKeys);
+        set_right(sa, wa, sum);
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int32_t key = key0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (key < first || key > last) sc[t][i] = -__builtin_inff();
+        for (int n = 0; n < CT; n++) l[n] += sum[n];
+        wait_stage();
+        ring[0] = value_fragment(stage_values(1), 0, 0, 0);
+        ring[1] = value_fragment(stage_values(1), 0, 0, 1);
+        for (int32_t i = 1; i < count; i++) {
+            const uint8_t *kt = stage_keys(i), *vt = stage_values(i), *vnext = stage_values(i + 1);
+            request(i + NS - 1);
+            const int32_t key0 = (s0 + i - 1) * kKeys + 32;
+            step(sb, sa, wa, wb, kt, vt, vt, key0, Keys(), [] {});
+            step(sa, sb, wb, wa, kt, vt, vnext, key0 + 32, Values(), [&] {
+                if constexpr (Q8) {
+                    widen_half((i + 1) % NS, 0);
+                    widen_half((i + 1) % NS, 1);
                 }
+                wait_stage();
+            });
         }
-        float top = sc[0][0];
+        const uint8_t* vt = stage_values(count);
+        values(wa, vt, 0);
+        mask(sb, (s1 - 1) * kKeys + 32);
+        set_right(sb, wb, sum);
 #pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, sc[t][i]);
-        top = fmaxf(top, other_half(top));
-        top = fmaxf(top * c, m);
-        const float base = top == -__builtin_inff() ? 0.f : top;
-        const float keep = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        float sum = 0.f;
-        op_t pf[4];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                u32x4_t w;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * half + 2 * j], c, -base));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * half + 2 * j + 1], c, -base));
-                    sum += p0 + p1;
-                    w[j] = Q8 ? pack_f16(p0 * 4096.f, p1 * 4096.f) : pack_bf16(p0, p1);
-                }
-                pf[2 * t + half] = __builtin_bit_cast(op_t, w);
-            }
-        l = l * keep + sum;
-#pragma unroll
-        for (int t = 0; t < DTILES; t++) {
-            acc[t] *= keep;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                u32x2_t half[2];
-#pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    const int row = 16 * x + 8 * y + vkey, e = 32 * t + velem;
-                    half[y] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(
-                        vt + row * DT * 2 + 16 * ((e >> 3) ^ swizzle<DT>(row)) + 2 * (e & 7))));
-                }
-                const u32x4_t w = {half[0][0], half[0][1], half[1][0], half[1][1]};
-                acc[t] = mfma(__builtin_bit_cast(op_t, w), pf[x], acc[t]);
-            }
-        }
-        if (s + 1 < s1) widen(stage ^ 1);
+        for (int n = 0; n < CT; n++) l[n] += sum[n];
+        values(wb, vt, 1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no request outlives the workgroup's LDS
     }
-    l += other_half(l);
-    if (!there) return;
-    // acc[t][i]: row `col`, element 32 t + 8 (i / 4) + 4 h + i % 4
-    const float unit = Q8 ? 1.f / 4096.f : 1.f;
-    if (b.splits > 1) {
-        const int64_t at = b.slot * kRows + 32 * wave + col;
+
+    // ---- out: acc[n][t][i]: row row_of[n], element 32 t + 8 (i / 4) + 4 h + i % 4 --------------------------------------------
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        l[n] += other_half(l[n]);
+        if (row_of[n] >= r1) continue;
+        if (b.splits > 1) {
+            const int64_t at = b.slot * ROWS + (row_of[n] - r0);
+#pragma unroll
+            for (int t = 0; t < DTILES; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4_t*>(a.partial + at * DT + 32 * t + 2 * i + 4 * h) = f32x4_t{acc[n][t][i], acc[n][t][i + 1], acc[n][t][i + 2], acc[n][t][i + 3]};
+            if (h == 0) {
+                float* st = a.partial + a.grid * ROWS * DT + at * 2;
+                st[0] = m[n];
+                st[1] = l[n];
+            }
+            continue;
+        }
+        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+        const int32_t token = (int32_t)(row_of[n] / a.group), head = b.kv_head * a.group + (int32_t)(row_of[n] - (int64_t)token * a.group);
+        bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head;
 #pragma unroll
         for (int t = 0; t < DTILES; t++)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4_t*>(a.partial + at * DT + 32 * t + 2 * i + 4 * h) =
-                    f32x4_t{acc[t][i] * unit, acc[t][i + 1] * unit, acc[t][i + 2] * unit, acc[t][i + 3] * unit};
-        if (h == 0) {
-            float* st = a.partial + a.grid * kRows * DT + at * 2;
-            st[0] = m;
-            st[1] = l;
-        }
-        return;
+            for (int i = 0; i < 16; i += 4) {
+                const int e = 32 * t + 2 * i + 4 * h;
+                if (e < a.dim)
+                    *reinterpret_cast<u32x2_t*>(out + e) =
+                        u32x2_t{pack_bf16(acc[n][t][i] * inv, acc[n][t][i + 1] * inv), pack_bf16(acc[n][t][i + 2] * inv, acc[n][t][i + 3] * inv)};
+            }
     }
-    const float inv = l == 0.f ? 0.f : unit / l;
-    bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head;
-#pragma unroll
-    for (int t = 0; t < DTILES; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int e = 32 * t + 2 * i + 4 * h;
-            if (e < a.dim)
-                *reinterpret_cast<u32x2_t*>(out + e) = u32x2_t{pack_bf16(acc[t][i] * inv, acc[t][i + 1] * inv), pack_bf16(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
-        }
 }
 
-int launch_attention_tiles(const AttentionArgs& a, int dim, int source, hipStream_t stream) {
-#define SNGGUF_GO(D, S)                                                                                                 \
-    if (dim == D && source == S) {                                                                                      \
-        constexpr int kLds = 4 * kKeys * D * 2;                                                                         \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S>), \
+// rows: of a workgroup, 128 or (up to 128 elements) 256
+int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
+#define SNGGUF_GO(D, S, C, N)                                                                                           \
+    if (dim == D && source == S && rows == 128 * C) {                                                                   \
+        constexpr int kLds = N * 2 * kKeys * D * 2;                                                                     \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, C, N>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_tiles_kernel<D, S><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                            \
+        attention_tiles_kernel<D, S, C, N><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                      \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
-#define SNGGUF_GO_DIM(D) SNGGUF_GO(D, kPacked) SNGGUF_GO(D, kPaged) SNGGUF_GO(D, kPagedQ8)
-    SNGGUF_GO_DIM(64)
-    SNGGUF_GO_DIM(128)
-    SNGGUF_GO_DIM(256)
+#define SNGGUF_GO_DIM(D, C, N) SNGGUF_GO(D, kPacked, C, N) SNGGUF_GO(D, kPaged, C, N) SNGGUF_GO(D, kPagedQ8, C, 2)
+    SNGGUF_GO_DIM(64, 1, 3)
+    SNGGUF_GO_DIM(64, 2, 3)
+    SNGGUF_GO_DIM(128, 1, 2)
+    SNGGUF_GO_DIM(128, 2, 3)
+    SNGGUF_GO_DIM(256, 1, 2)
 #undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
