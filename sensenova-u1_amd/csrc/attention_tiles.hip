@@ -7,8 +7,11 @@
 //    4 h + i % 4;
 //  * O^T += V^T P^T wants eight keys of a row in each lane, in any order that V^T shares: those registers are taken as they
 //    are, and V, which lies row by row in LDS, is read with the transposing read, four keys of one element at a time.
-// In LDS a row's 16-byte pieces are permuted so that the eight or sixteen rows that one read touches lie in different banks;
-// copies go from global memory to LDS directly, and permute on the global side.
+// In LDS a tile is blocks of 8 rows x 128 bytes, the order that one copy request (1 KB, global memory to LDS directly) makes of
+// whole cache lines: piece by piece (16 bytes), and within a piece row by row, so that a read of one piece of many rows is
+// contiguous and every address of a tile is a lane's constant and an immediate offset.  Pieces 2, 3, 6, 7 have the halves of
+// their eight rows exchanged: the transposing read takes four pieces of four rows, which then fill all banks; blocks of
+// neighbouring rows lie half a turn of the banks apart for the same reason.
 //
 // A step takes 32 keys, and three of them at once: the product with V of the step before, the weights of its own scores, and the
 // scores of the step after depend on nothing of each other, so the vector instructions of the weights are dealt over the
@@ -74,12 +77,14 @@ __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>()), ...);
 }
 
-// What piece c of row r is exchanged with: rows that one read touches together get different pieces.
-template <int DT>
-__device__ __forceinline__ int swizzle(int r) {
-    // 128-byte rows lie two to a line of the 64 banks, so that rows of one parity have to differ
-    return DT == 64 ? ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : (((r & 3) << 2) | ((r >> 2) & 3));
-}
+// Place of (row % 8, piece % 8) in its block, in pieces.
+__device__ __forceinline__ int block_place(int row, int piece) { return 8 * (piece & 7) + ((row & 7) ^ (4 * ((piece >> 1) & 1))); }
+
+template <int DT> struct Tile {
+    static constexpr int kBlocks = DT / 64;                    // of eight rows
+    static constexpr int kRowBlock = kBlocks * 1024 + 128;     // bytes from eight rows to the next
+    static constexpr int kBytes = kKeys / 8 * kRowBlock;
+};
 
 }  // namespace
 
@@ -91,8 +96,7 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
     constexpr int ROWS = 128 * CT;
-    constexpr int PIECES = DT / 8;                     // of a row
-    constexpr int TILE = kKeys * DT * 2;               // bytes
+    constexpr int TILE = Tile<DT>::kBytes, RB = Tile<DT>::kRowBlock, PB = Tile<DT>::kBlocks;
     constexpr int KS = DT / 16, DTILES = DT / 32;
     constexpr int VF = 2 * DTILES, NF = VF + KS;       // operand fragments of a step: of values, in all
     constexpr int NP = 8 * CT;                         // pairs of weights of a step that a lane forms
@@ -186,108 +190,118 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     // ---- tiles into LDS ------------------------------------------------------------------------------------------------
     // Sixteen rows a wavefront.  Rows behind the last key are the last key's: masked, but finite wherever the keys are.
     const int32_t page_mask = (1 << a.page_shift) - 1;
-    constexpr int RQ = 1024 / (DT * 2);                // rows of one request (1 KB)
-    constexpr int REQ = 16 / RQ;
-    const int crow = lane / PIECES, cpiece = lane % PIECES;
+    constexpr int REQ = 2 * PB;                        // requests of a wavefront for a tile: blocks of its sixteen rows
     constexpr int QP = DT / 16;                        // 8-bit: 16-byte pieces of a row
     constexpr int QN = 16 * QP / 64;                   // ... a lane has of each tile
     u32x4_t held[2][Q8 ? QN : 1];
     uint16_t held_scale[2][Q8 ? QN : 1];
-    // keys (half 0) or values (half 1) of a tile into the stage's half
-    auto request_half = [&](int32_t tile, int stage, auto half_) {
-        constexpr int half = decltype(half_)::value;
-        const int32_t base = tile * kKeys + 16 * wave, most = b.s.lk - 1;
-        const int32_t lead = base < most ? base : most;
-        uint8_t* to = lds + (2 * stage + half) * TILE + 16 * wave * DT * 2;
+    // this lane's part of a request: row and piece of a block
+    const int crow = (lane & 7) ^ (4 * ((lane >> 4) & 1)), cpiece = lane >> 3;
+    const int64_t k_stride = SOURCE == kPacked ? a.k_token : a.dim, v_stride = SOURCE == kPacked ? a.v_token : a.dim;
+    // byte offsets of this lane's pieces behind the first of the wavefront's sixteen rows, and the last row known to be there
+    uint32_t coff[2][REQ];
+    int32_t rows_there[2] = {-1, -1};
+    auto set_offsets = [&](int half, int32_t spare) {
+        spare = spare < 15 ? spare : 15;
+        if (spare == rows_there[half]) return;
+        rows_there[half] = spare;
+#pragma unroll
+        for (int j = 0; j < REQ; j++) {
+            const int i = j / PB, p = j % PB, row = 8 * i + crow < spare ? 8 * i + crow : spare;
+            // (pieces behind dim: the first, whose elements meet queries of zero, or are never stored)
+            coff[half][j] = (uint32_t)(2 * row * (int32_t)(half ? v_stride : k_stride)) + (64 * p + 8 * cpiece < a.dim ? 128 * p + 16 * cpiece : 0);
+        }
+    };
+    const uint8_t* k_base = reinterpret_cast<const uint8_t*>(SOURCE == kPacked ? a.k + b.s.k0 * a.k_token + (int64_t)b.kv_head * a.k_head : nullptr);
+    const uint8_t* v_base = reinterpret_cast<const uint8_t*>(SOURCE == kPacked ? a.v + b.s.k0 * a.v_token + (int64_t)b.kv_head * a.v_head : nullptr);
+    const int32_t most = b.s.lk - 1;
+    const int32_t* table = SOURCE == kPacked ? nullptr : a.table + (int64_t)b.seq * a.table_stride;
+    // page of the wavefront's rows of a tile (sixteen rows lie in one)
+    auto page_of = [&](int32_t tile) -> int32_t {
+        if constexpr (SOURCE == kPacked) return 0;
+        const int32_t base = tile * kKeys + 16 * wave, lead = base < most ? base : most;
+        const int32_t p = *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(table + __builtin_amdgcn_readfirstlane(lead >> a.page_shift));
+        return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
+    };
+    // where the wavefront's rows of a tile start, for the requests of half 0 (keys) or 1 (values)
+    const uint8_t* from[2] = {nullptr, nullptr};
+    auto aim = [&](int half, int32_t tile, int32_t page) {
+        const int32_t base = tile * kKeys + 16 * wave, lead = base < most ? base : most;
+        const int32_t spare = most - lead;             // rows behind the first that there are
         if constexpr (SOURCE == kPacked) {
-            const int64_t stride = half ? a.v_token : a.k_token;
-            const uint8_t* from = uniform_ptr((half ? a.v + (int64_t)b.kv_head * a.v_head : a.k + (int64_t)b.kv_head * a.k_head) + (b.s.k0 + lead) * stride);
-#pragma unroll
-            for (int i = 0; i < REQ; i++) {
-                const int row = RQ * i + crow;
-                int piece = cpiece ^ swizzle<DT>(row);
-                piece = 8 * piece < a.dim ? piece : 0;
-                const int32_t at = base + row < most ? base + row - lead : most - lead;
-                copy_request(lds_offset(to + RQ * i * DT * 2), (uint32_t)(2 * (at * (int32_t)stride + 8 * piece)), from);
-            }
+            from[half] = uniform_ptr((half ? v_base : k_base) + 2 * lead * (half ? v_stride : k_stride));
+            set_offsets(half, spare);
         } else {
-            // (sixteen rows lie in one page)
-            const int64_t at_page = (int64_t)__builtin_amdgcn_readfirstlane((int)attention_page(a, b.seq, lead)) * a.kv_heads + b.kv_head;
-            if constexpr (SOURCE == kPaged) {
-                const uint8_t* from = uniform_ptr(static_cast<const bf16_t*>(half ? a.v_pages : a.k_pages) + (at_page << a.page_shift) * a.dim);
-#pragma unroll
-                for (int i = 0; i < REQ; i++) {
-                    const int row = RQ * i + crow;
-                    int piece = cpiece ^ swizzle<DT>(row);
-                    piece = 8 * piece < a.dim ? piece : 0;
-                    const int32_t at = (base + row < most ? base + row : most) & page_mask;
-                    copy_request(lds_offset(to + RQ * i * DT * 2), (uint32_t)(2 * (at * a.dim + 8 * piece)), from);
-                }
+            const int64_t at_page = (int64_t)page * a.kv_heads + b.kv_head;
+            const int64_t at = (at_page << a.page_shift) + (lead & page_mask);
+            from[half] = uniform_ptr(static_cast<const uint8_t*>(half ? a.v_pages : a.k_pages) + at * a.dim * (Q8 ? 1 : 2));
+            if constexpr (!Q8) {
+                set_offsets(half, spare);
             } else {
-                const uint8_t* from = static_cast<const uint8_t*>(half ? a.v_pages : a.k_pages) + (at_page << a.page_shift) * a.dim;
-                const uint16_t* scales = (half ? a.v_scales : a.k_scales) + (at_page * (a.dim >> 5) << a.page_shift);
+                const uint16_t* scales = (half ? a.v_scales : a.k_scales) + (at_page * (a.dim >> 5) << a.page_shift) + (lead & page_mask);
 #pragma unroll
                 for (int i = 0; i < QN; i++) {
-                    const int p = lane + 64 * i, row = p / QP;
+                    const int p = lane + 64 * i, row = p / QP < spare ? p / QP : spare;
                     int piece = p % QP;
                     piece = 16 * piece < a.dim ? piece : 0;
-                    const int32_t at = (base + row < most ? base + row : most) & page_mask;
-                    held[half][i] = *reinterpret_cast<const u32x4_t*>(from + at * a.dim + 16 * piece);
-                    held_scale[half][i] = scales[((piece >> 1) << a.page_shift) + at];
+                    held[half][i] = *reinterpret_cast<const u32x4_t*>(from[half] + row * a.dim + 16 * piece);
+                    held_scale[half][i] = scales[((piece >> 1) << a.page_shift) + row];
                 }
             }
         }
+    };
+    const uint32_t lds0 = lds_offset(lds);
+    // request j of REQ into the half of the stage at `stage`
+    auto request = [&](int half, uint32_t stage, int j) {
+        if constexpr (!Q8) copy_request(stage + half * TILE + (2 * wave + j / PB) * RB + (j % PB) * 1024, coff[half][j], from[half]);
     };
     // 8-bit tiles: widened from the registers that the request filled
-    auto widen_half = [&](int stage, int half) {
+    auto widen = [&](int half, uint32_t stage, int i) {
         if constexpr (Q8) {
+            const int p = lane + 64 * i, row = 16 * wave + p / QP, piece = p % QP;
+            const u32x4_t w = held[half][i];
+            const _Float16 d1 = __builtin_bit_cast(_Float16, held_scale[half][i]);
+            const f16x2_t d = {d1, d1};
+            const uint32_t to = stage + half * TILE + (row >> 3) * RB + (piece >> 2) * 1024;
 #pragma unroll
-            for (int i = 0; i < QN; i++) {
-                const int p = lane + 64 * i, row = p / QP, piece = p % QP;
-                const u32x4_t w = held[half][i];
-                const _Float16 d1 = __builtin_bit_cast(_Float16, held_scale[half][i]);
-                const f16x2_t d = {d1, d1};
-                uint8_t* to = lds + (2 * stage + half) * TILE + (16 * wave + row) * DT * 2;
+            for (int y = 0; y < 2; y++) {
+                u32x4_t f;
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    u32x4_t f;
-#pragma unroll
-                    for (int z = 0; z < 2; z++) {
-                        const uint32_t flipped = w[2 * y + z] ^ 0x80808080u;
-                        f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * d);
-                        f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * d);
-                    }
-                    *reinterpret_cast<u32x4_t*>(to + 16 * ((2 * piece + y) ^ swizzle<DT>(row))) = f;
+                for (int z = 0; z < 2; z++) {
+                    const uint32_t flipped = w[2 * y + z] ^ 0x80808080u;
+                    f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * d);
+                    f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * d);
                 }
+                *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)(to + 16 * block_place(row, 2 * piece + y)) = f;
             }
         }
     };
-    typedef std::integral_constant<int, 0> Keys;
-    typedef std::integral_constant<int, 1> Values;
-    // stage i: keys of tile i, values of tile i - 1 (behind the last tile: of the last, read by nobody, so that the loop neither asks
-    // whether there are more nor counts what is under way)
-    auto request = [&](int32_t i) {
-        const int stage = i % NS;
-        request_half(s0 + (i < count ? i : count - 1), stage, Keys());
-        request_half(s0 + (i <= count ? i : count) - 1, stage, Values());
-    };
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, 1> Second;
 
     // ---- fragments ---------------------------------------------------------------------------------------------------
-    // keys: row col, piece 2 ks + h; values: keys 4 h + (lane % 16) / 4, elements 16 ((lane % 32) / 16) + 4 (lane % 4) ...: the rows of one
-    // transposing read are four keys
-    const int vkey = 4 * h + ((lane & 15) >> 2), velem = 16 * ((lane & 31) >> 4) + 4 * (lane & 3);
-    auto key_fragment = [&](const uint8_t* kt, int half, int ks) -> op_t {
-        const int row = 32 * half + col;
-        return *reinterpret_cast<const op_t*>(kt + row * DT * 2 + 16 * ((2 * ks + h) ^ swizzle<DT>(col)));
+    // keys: row 32 half + col, piece 2 ks + h; values: keys 32 half + 16 x + 8 y + 4 h + (lane % 16) / 4 (the rows of one transposing
+    // read are four keys), elements 32 t + 16 ((lane % 32) / 16) + 4 (lane % 4) ...
+    const uint32_t k_at[2] = {lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, h)), lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, 2 + h))};
+    const uint32_t v_at = lds0 + (uint32_t)(TILE + 16 * block_place(4 * h + ((lane & 15) >> 2), 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1)) + 8 * (lane & 1));
+    // one lane's addresses in a stage; everything else is an immediate offset
+    struct At {
+        uint32_t k[2], v;
     };
-    auto value_fragment = [&](const uint8_t* vt, int half, int t, int x) -> op_t {
+    auto at_stage = [&](uint32_t stage) -> At {
+        At x = {{k_at[0] + stage, k_at[1] + stage}, v_at + stage};
+        asm volatile("" : "+v"(x.k[0]), "+v"(x.k[1]), "+v"(x.v));     // (or every address would be formed by itself)
+        return x;
+    };
+    auto key_fragment = [&](const At& x, int half, int ks) -> op_t {
+        return *(const __attribute__((address_space(3))) op_t*)(uintptr_t)(x.k[ks & 1] + 4 * half * RB + (ks >> 2) * 1024 + ((ks & 2) ? 512 : 0));
+    };
+    auto value_fragment = [&](const At& x, int half, int t, int y) -> op_t {
         u32x2_t part[2];
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
-            const int row = 16 * x + 8 * y + vkey, e = 32 * t + velem;
-            part[y] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(
-                vt + (32 * half + row) * DT * 2 + 16 * ((e >> 3) ^ swizzle<DT>(row)) + 2 * (e & 7))));
-        }
+        for (int z = 0; z < 2; z++)
+            part[z] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)(
+                x.v + (4 * half + 2 * y + z) * RB + (t >> 1) * 1024 + (t & 1) * 512)));
         return __builtin_bit_cast(op_t, u32x4_t{part[0][0], part[0][1], part[1][0], part[1][1]});
     };
 
@@ -311,10 +325,13 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
                 }
         }
     };
-    auto weights_pair = [&](const scores_t& s, weights_t& w, float (&sum)[CT], const float (&add)[CT], int p) {
+    auto raise_pair = [&](const scores_t& s, const float (&add)[CT], int p, float& p0, float& p1) {
         const int n = p / 8, i = 2 * (p % 8);
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c[n], add[n]));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], c[n], add[n]));
+        p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c[n], add[n]));
+        p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], c[n], add[n]));
+    };
+    auto pack_pair = [&](weights_t& w, float (&sum)[CT], int p, float p0, float p1) {
+        const int n = p / 8, i = 2 * (p % 8);
         if constexpr (Q8) {
             w[n][i / 8][(i / 2) % 4] = pack_f16(p0, p1);
             sum[n] += p0 + p1;
@@ -349,7 +366,11 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
             sum[n] = 0.f;
         }
 #pragma unroll
-        for (int p = 0; p < NP; p++) weights_pair(s, w, sum, add, p);
+        for (int p = 0; p < NP; p++) {
+            float p0, p1;
+            raise_pair(s, add, p, p0, p1);
+            pack_pair(w, sum, p, p0, p1);
+        }
     };
     auto settle = [&](const scores_t& s, weights_t& w, float (&sum)[CT]) {
         bool fine = true;
@@ -364,49 +385,59 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     };
 
     op_t ring[4];
-    // One step: values of keys 32 half ... of vt times w0; weights of s into w1; scores of keys 32 half ... of kt into s1.
-    // The first two fragments are in the ring; the next step's are fetched by its end, from half 1 of vt or from `vnext`, behind the
-    // barrier that its stage needs (LAST).
-    auto step = [&](scores_t& s, scores_t& s1, const weights_t& w0, weights_t& w1, const uint8_t* kt, const uint8_t* vt, const uint8_t* vnext, int32_t key0,
-                    auto half_, auto arrive) {
+    // One step: values of keys 32 half ... of a stage times w0; weights of s into w1; scores of keys 32 half ... into s1.
+    // The first three fragments are in the ring; the next step's are fetched by its end, from the same stage or from `next`, behind
+    // the barrier that this needs.  beside(f): what else is done beside fragment f.
+    auto step = [&](scores_t& s, scores_t& s1, const weights_t& w0, weights_t& w1, const At& at, const At& next, int32_t key0, auto half_, auto beside) {
         constexpr int half = decltype(half_)::value;
         mask(s, key0);
         clear(s1);
         float sum[CT];
 #pragma unroll
         for (int n = 0; n < CT; n++) sum[n] = 0.f;
+        // (a pair is packed one fragment after it was raised: the exponential's result is a while coming)
+        constexpr int PF = (NP + NF - 1) / NF;         // pairs of a fragment at most
+        float up[2][PF][2];
+        auto pack_of = [&](auto f_) {
+            constexpr int f = decltype(f_)::value, p0 = f * NP / NF, p1 = (f + 1) * NP / NF;
+#pragma unroll
+            for (int p = p0; p < p1; p++) pack_pair(w1, sum, p, up[f & 1][p - p0][0], up[f & 1][p - p0][1]);
+        };
         each_of(
             [&](auto f_) {
-                constexpr int f = decltype(f_)::value, g = f + 2;
-                if constexpr (half == 1 && f == NF - 2) arrive();
-                if constexpr (g < VF) ring[g & 3] = value_fragment(vt, half, g >> 1, g & 1);
-                else if constexpr (g < NF) ring[g & 3] = key_fragment(kt, half, g - VF);
-                else ring[g & 3] = value_fragment(vnext, half ^ 1, 0, g - NF);
+                constexpr int f = decltype(f_)::value, g = f + 3;
+                beside(f_);
+                if constexpr (g < VF) ring[g & 3] = value_fragment(at, half, g >> 1, g & 1);
+                else if constexpr (g < NF) ring[g & 3] = key_fragment(at, half, g - VF);
+                else ring[g & 3] = value_fragment(next, half ^ 1, (g - NF) >> 1, (g - NF) & 1);
 #pragma unroll
                 for (int n = 0; n < CT; n++) {
                     if constexpr (f < VF) acc[n][f >> 1] = mfma(ring[f & 3], weights_operand(w0, n, f & 1), acc[n][f >> 1]);
                     else s1[n] = mfma(ring[f & 3], qf[n][f - VF], s1[n]);
                 }
+                constexpr int p0 = f * NP / NF, p1 = (f + 1) * NP / NF;
 #pragma unroll
-                for (int p = f * NP / NF; p < (f + 1) * NP / NF; p++) weights_pair(s, w1, sum, nb, p);
+                for (int p = p0; p < p1; p++) raise_pair(s, nb, p, up[f & 1][p - p0][0], up[f & 1][p - p0][1]);
+                if constexpr (f > 0) pack_of(std::integral_constant<int, f - 1>());
                 __builtin_amdgcn_sched_barrier(0);
             },
             std::make_integer_sequence<int, NF>());
+        pack_of(std::integral_constant<int, NF - 1>());
         settle(s, w1, sum);
     };
-    auto scores = [&](scores_t& s, const uint8_t* kt, int half) {
+    auto scores = [&](scores_t& s, const At& at, int half) {
         clear(s);
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            const op_t k = key_fragment(kt, half, ks);
+            const op_t k = key_fragment(at, half, ks);
 #pragma unroll
             for (int n = 0; n < CT; n++) s[n] = mfma(k, qf[n][ks], s[n]);
         }
     };
-    auto values = [&](const weights_t& w, const uint8_t* vt, int half) {
+    auto values = [&](const weights_t& w, const At& at, int half) {
 #pragma unroll
         for (int f = 0; f < VF; f++) {
-            const op_t v = value_fragment(vt, half, f >> 1, f & 1);
+            const op_t v = value_fragment(at, half, f >> 1, f & 1);
 #pragma unroll
             for (int n = 0; n < CT; n++) acc[n][f >> 1] = mfma(v, weights_operand(w, n, f & 1), acc[n][f >> 1]);
         }
@@ -416,55 +447,90 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
         scores_t sa, sb;
         weights_t wa, wb;
         float sum[CT];
-        auto stage_keys = [&](int32_t i) { return lds + (2 * (i % NS)) * TILE; };
-        auto stage_values = [&](int32_t i) { return lds + (2 * (i % NS) + 1) * TILE; };
+        // A stage: keys of tile i, values of tile i - 1 (behind the last tile: of the last, read by nobody, so that the loop neither
+        // asks whether there are more nor counts what is under way)
+        constexpr uint32_t kStage = 2 * TILE, kRing = NS * kStage;
+        auto after = [&](uint32_t stage) { return stage + kStage < kRing ? stage + kStage : 0u; };
         // the requests of all stages but the NS - 2 last asked for have arrived, from every wavefront
         auto wait_stage = [&] {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ * (NS - 2)) : "memory");
             __syncthreads();
         };
-        request_half(s0, 0, Keys());
-        if constexpr (Q8) widen_half(0, 0);
-        request(1);
-        if constexpr (!Q8) {
-            if constexpr (NS > 2) request(2);
-            // the keys of tile 0
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ * (NS - 1)) : "memory");
-        }
-        __syncthreads();
-        scores(sa, stage_keys(0), 0);
-        scores(sb, stage_keys(0), 1);
+        int32_t page_k = page_of(s0), page_v = page_k;
+        auto aim_stage = [&](int32_t i) {
+            const int32_t tk = s0 + (i < count ? i : count - 1), tv = s0 + (i <= count ? i : count) - 1;
+            page_v = page_k;
+            page_k = page_of(tk);
+            aim(0, tk, page_k);
+            aim(1, tv, page_v);
+        };
+        aim(0, s0, page_k);
+#pragma unroll
+        for (int j = 0; j < REQ; j++) request(0, lds0, j);
         if constexpr (Q8) {
-            widen_half(1 % NS, 0);
-            widen_half(1 % NS, 1);
+#pragma unroll
+            for (int i = 0; i < QN; i++) widen(0, lds0, i);
+        }
+#pragma unroll
+        for (int n = 1; n < NS; n++) {
+            aim_stage(n);
+#pragma unroll
+            for (int j = 0; j < 2 * REQ; j++) request(j / REQ, lds0 + n * kStage, j % REQ);
+        }
+        if constexpr (!Q8) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ * (NS - 1)) : "memory");     // the keys of tile 0
+        __syncthreads();
+        At at = at_stage(0);
+        scores(sa, at, 0);
+        scores(sb, at, 1);
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < 2 * QN; i++) widen(i / QN, lds0 + kStage, i % QN);
         }
         mask(sa, s0 * kKeys);
         set_right(sa, wa, sum);
 #pragma unroll
         for (int n = 0; n < CT; n++) l[n] += sum[n];
         wait_stage();
-        ring[0] = value_fragment(stage_values(1), 0, 0, 0);
-        ring[1] = value_fragment(stage_values(1), 0, 0, 1);
+        uint32_t stage = kStage;                       // of tile i's keys
+        uint32_t ahead = NS == 2 ? 0u : after(kStage); // the last one asked for
+        at = at_stage(stage);
+        ring[0] = value_fragment(at, 0, 0, 0);
+        ring[1] = value_fragment(at, 0, 0, 1);
+        ring[2] = value_fragment(at, 0, 1, 0);
         for (int32_t i = 1; i < count; i++) {
-            const uint8_t *kt = stage_keys(i), *vt = stage_values(i), *vnext = stage_values(i + 1);
-            request(i + NS - 1);
+            if constexpr (NS > 2) ahead = after(ahead);
+            else ahead = after(stage);
+            stage = after(stage);
+            const At next = at_stage(stage);
+            aim_stage(i + NS - 1);
             const int32_t key0 = (s0 + i - 1) * kKeys + 32;
-            step(sb, sa, wa, wb, kt, vt, vt, key0, Keys(), [] {});
-            step(sa, sb, wb, wa, kt, vt, vnext, key0 + 32, Values(), [&] {
-                if constexpr (Q8) {
-                    widen_half((i + 1) % NS, 0);
-                    widen_half((i + 1) % NS, 1);
-                }
-                wait_stage();
+            const uint32_t to = lds0 + ahead;
+            // requests and widened pieces are dealt over the fragments: close together they fill the memory pipeline's queue
+            step(sb, sa, wa, wb, at, at, key0, First(), [&](auto f_) {
+                constexpr int f = decltype(f_)::value;
+#pragma unroll
+                for (int j = f * REQ / NF; j < (f + 1) * REQ / NF; j++) request(0, to, j);
             });
+            step(sa, sb, wb, wa, at, next, key0 + 32, Second(), [&](auto f_) {
+                constexpr int f = decltype(f_)::value, before = NF - 3;
+                if constexpr (f < before) {
+#pragma unroll
+                    for (int j = f * REQ / before; j < (f + 1) * REQ / before; j++) request(1, to, j);
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int j = f * 2 * QN / before; j < (f + 1) * 2 * QN / before; j++) widen(j / QN, to, j % QN);
+                    }
+                }
+                if constexpr (f == before) wait_stage();
+            });
+            at = next;
         }
-        const uint8_t* vt = stage_values(count);
-        values(wa, vt, 0);
+        values(wa, at, 0);
         mask(sb, (s1 - 1) * kKeys + 32);
         set_right(sb, wb, sum);
 #pragma unroll
         for (int n = 0; n < CT; n++) l[n] += sum[n];
-        values(wb, vt, 1);
+        values(wb, at, 1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no request outlives the workgroup's LDS
     }
 
@@ -506,7 +572,7 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
 #define SNGGUF_GO(D, S, C, N)                                                                                           \
     if (dim == D && source == S && rows == 128 * C) {                                                                   \
-        constexpr int kLds = N * 2 * kKeys * D * 2;                                                                     \
+        constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                    \
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, C, N>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
