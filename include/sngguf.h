@@ -462,7 +462,7 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
  * workspace (16-byte aligned) of sngguf_attention_workspace_bytes(...): partial results where few rows meet many keys; with
  * less, or NULL, such a call is slower.  Nothing in it outlives the call.
  */
-int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim);
+int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim);
 int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head,
                      const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                      int64_t tokens_k, int64_t kv_heads, int64_t dim, const int32_t* ends_q, const int32_t* ends_k, int64_t sequences,
@@ -474,10 +474,11 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
  * lens[i] tokens in all, in the pages table[i][0 .. ], of which the last ends_q[i + 1] - ends_q[i] are the queries; ends_q NULL:
  * one query a sequence, in order.  Causal.  max_new: the most queries of any sequence as far as the caller knows, 0 if it does
  * not (a wrong value costs time only).  Lengths beyond the table's width count as its width; page numbers outside the cache are
- * read as the nearest page.  table: rows table_stride apart, table_width numbers each.  An 8-bit cache is multiplied in fp16,
+ * read as the nearest page.  table: rows table_stride apart, table_width numbers each.  max_keys (of the workspace): table_width *
+ * page_size, below 2^31 - 65536.  An 8-bit cache is multiplied in fp16,
  * its values rounded to 11 bits.  Everything else as sngguf_attention.
  */
-int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim);
+int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads, int64_t dim);
 int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
                            const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* lens, const int32_t* ends_q,
                            int64_t sequences, int64_t max_new, float scale, int64_t window, void* out, int64_t out_token, int64_t out_head,

@@ -303,7 +303,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
     if tokens and sequences:
         dev = q.device
         lib = ops.load_library()
-        nbytes = lib.sngguf_attention_workspace_bytes(tokens, sequences, heads, k.shape[1], dim)
+        nbytes = lib.sngguf_attention_workspace_bytes(tokens, k.shape[0], sequences, heads, k.shape[1], dim)
         with ops._on(dev), ops._whole_call(dev):
             ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
             rc = lib.sngguf_attention(q.data_ptr(), tokens, heads, *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), k.shape[0],
@@ -334,7 +334,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != sequences:
         raise SnGgufError(f"{what}: pages must be int32 [{sequences}][width], got {pages.dtype} {tuple(pages.shape)}")
     width = pages.shape[1]
-    if width * cache.page_size >= 1 << 31:
+    if width * cache.page_size > (1 << 31) - 65536:
         raise SnGgufError(f"{what}: {width} pages of {cache.page_size} tokens a sequence are too many")
     if (width > 1 and pages.stride(1) != 1) or (sequences > 1 and pages.stride(0) < width):
         pages = pages.contiguous()
@@ -349,7 +349,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
         lib = ops.load_library()
         if ends_q is None:
             max_new = 1
-        nbytes = lib.sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, heads, cache.kv_heads, dim)
+        nbytes = lib.sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
         with ops._on(dev), ops._whole_call(dev):
             ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
             rc = lib.sngguf_paged_attention(q.data_ptr(), tokens, heads, *_strides(q), cache._address, pages.data_ptr(), pages.stride(0), width,

@@ -41,7 +41,7 @@ def _hipcc() -> str:
 # results the vector ALU consumes at once: they must land in ordinary VGPRs, not in accumulation
 # registers that need one v_accvgpr_read per value.
 SOURCE_FLAGS = {"gemv_kq_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "gemm_mid.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                "attention_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                "attention_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "attention_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 # sources compiled once per variant: gemm_mid.hip holds the kernels of one block format (ggml type ids)
 SOURCE_VARIANTS = {"gemm_mid.hip": [(f"_t{t}", [f"-DSNGGUF_MID_TYPE={t}"]) for t in (8, 14, 13, 12, 11, 10, 7, 6, 3, 2)]}
 

@@ -78,60 +78,63 @@ void set_table(RotaryCacheArgs& a, const sngguf_rotary_table* t, const int64_t* 
 
 // ---- attention: how much is launched ----------------------------------------------------------------------------------
 
-constexpr int kRowsWant = 768, kRowsLeast = 2, kRowsKeys = 128;    // three workgroups a compute unit; at least 256 keys each
-constexpr int kTilesWant = 512, kTilesLeast = 4, kTilesKeys = 64;
+constexpr int64_t kMostKeys = kMost - 65536;          // of a sequence: a few tiles more still have 32-bit numbers
 
-constexpr int64_t kWide = 512;      // 256-row workgroups from which on they are taken
+// Workgroups that fill the device (three a compute unit, two), key tiles that a split has at least, keys of a tile
+constexpr int kRowsLeast = 2, kRowsKeys = 128;
+int rows_want(int rows, int dim) { return rows * dim <= 16 * 128 ? 768 : rows * dim <= 16 * 256 ? 512 : 256; }
+constexpr int kTilesWant = 512, kTilesLeast = 4, kTilesKeys = 64;
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// (row tile, head) pairs at most: every sequence's last tile may be cut short
-int64_t tiles_most(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int rows) {
-    return kv_heads * (tokens * (heads / kv_heads) / rows + sequences);
-}
-
 struct Launch {
-    int rows;
-    int64_t tiles, grid, partial_bytes;
+    int rows;              // of a tile
+    int64_t tiles;         // (row tile, head) pairs at most
+    int64_t grid, partial_bytes;
 };
 
-// Split only where unsplit workgroups do not fill the device.
-Launch plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int dim, int rows, int want) {
+// Split only where unsplit workgroups do not fill the device, and a sequence can have the keys for two.
+Launch plan(int64_t tiles, int64_t keys, int dim, int rows, int want, int64_t least) {
     Launch p;
     p.rows = rows;
-    p.tiles = tiles_most(tokens, sequences, heads, kv_heads, rows);
-    const bool split = p.tiles < want;
-    p.grid = p.tiles + (split ? want : 0);
+    p.tiles = tiles;
+    const bool split = tiles < want && keys > least;
+    p.grid = tiles + (split ? want : 0);
     p.partial_bytes = split ? p.grid * rows * (dim + 2) * 4 : 0;
     return p;
 }
 
-// The kernel for many rows
-Launch plan_many(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
-    const int rows = dim <= 128 && tiles_most(tokens, 0, heads, kv_heads, 256) >= kWide ? 256 : 128;
-    return plan(tokens, sequences, heads, kv_heads, dim, rows, kTilesWant);
+// Row tiles of all sequences at most: every sequence's last one may be cut short
+int64_t row_tiles(int64_t tokens, int64_t sequences, int64_t group, int rows) { return tokens * group / rows + sequences; }
+
+// The kernel for many rows: 256 a workgroup unless that leaves most of a sequence's only tile empty.
+Launch plan_many(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
+    const int64_t group = heads / kv_heads;
+    const int rows = dim <= 128 && tokens * group >= 512 * sequences ? 256 : 128;
+    return plan(kv_heads * row_tiles(tokens, sequences, group, rows), keys / kTilesKeys + 1, dim, rows, kTilesWant, kTilesLeast);
 }
 
 struct PagedPlan {
-    int rows;              // of a tile of the kernel for few rows
     bool few, many;        // which kernels run
-    int64_t few_rows;      // sequences of at most so many rows go to the first where both run
+    int64_t few_rows;      // sequences of at most so many rows go to the first
+    int64_t most_rows;     // of a tile of the first, as far as is known
     Launch a, b;
 };
 
-PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim) {
+PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
     PagedPlan p;
     const int64_t group = heads / kv_heads;
     const int64_t most = (max_new > 0 && max_new < tokens ? max_new : tokens) * group;
     const int d = kernel_dim(dim), widest = d == 256 ? 32 : 64;
     // one kernel where no sequence has more rows than its tile; else single tokens and chunks each have their own
     const int64_t r = most <= widest ? most : group;
-    p.rows = r <= 16 ? 16 : r <= 32 ? 32 : widest;
+    const int rows = r <= 16 ? 16 : r <= 32 ? 32 : widest;
     p.few = r <= widest;
     p.many = most > widest;
-    p.few_rows = p.many ? (p.few ? p.rows : 0) : kMost - 1;
-    p.a = plan(tokens, sequences, heads, kv_heads, d, p.rows, kRowsWant);
-    p.b = plan_many(tokens, sequences, heads, kv_heads, d);
+    p.few_rows = !p.many ? kMost - 1 : p.few ? rows : 0;
+    p.most_rows = most < rows ? most : rows;
+    p.a = plan(kv_heads * (p.many ? sequences : row_tiles(tokens, sequences, group, rows)), keys / kRowsKeys + 1, d, rows, rows_want(rows, d), kRowsLeast);
+    p.b = plan_many(tokens, keys, sequences, heads, kv_heads, d);
     return p;
 }
 
@@ -140,13 +143,14 @@ bool heads_fit(int64_t heads, int64_t kv_heads, int64_t dim) {
 }
 
 int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* partial, hipStream_t stream) {
+    const int64_t most_rows = a.tokens_q * a.group;
     a.partial = partial;
     a.want = kTilesWant;
     a.least = kTilesLeast;
     a.grid = partial ? p.grid : p.tiles;
     const int rc = sngguf::launch_attention_tiles(a, p.rows, dim, source, stream);
     if (rc != SNGGUF_OK || !partial) return rc;
-    return sngguf::launch_attention_combine(a, p.rows, kTilesKeys, dim, p.tiles, stream);
+    return sngguf::launch_attention_combine(a, p.rows, kTilesKeys, dim, p.tiles, most_rows, stream);
 }
 
 }  // namespace
@@ -245,9 +249,10 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
     return sngguf::launch_cache_read(a, cache->qtype == SNGGUF_TYPE_Q8_0, static_cast<hipStream_t>(stream));
 }
 
-int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
-    if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || !heads_fit(heads, kv_heads, dim)) return 0;
-    return plan_many(tokens_q, sequences, heads, kv_heads, kernel_dim(dim)).partial_bytes;
+int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (tokens_q <= 0 || tokens_q >= kMost || tokens_k < 0 || tokens_k > kMostKeys || sequences <= 0 || sequences >= kMost || !heads_fit(heads, kv_heads, dim))
+        return 0;
+    return plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, kernel_dim(dim)).partial_bytes;
 }
 
 int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const void* k,
@@ -255,7 +260,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
                      int64_t kv_heads, int64_t dim, const int32_t* ends_q, const int32_t* ends_k, int64_t sequences, float scale,
                      int causal, int64_t window, void* out, int64_t out_token, int64_t out_head, void* workspace,
                      int64_t workspace_bytes, void* stream) {
-    if (tokens_q < 0 || tokens_q >= kMost || tokens_k < 0 || tokens_k >= kMost || sequences < 0 || sequences >= kMost ||
+    if (tokens_q < 0 || tokens_q >= kMost || tokens_k < 0 || tokens_k > kMostKeys || sequences < 0 || sequences >= kMost ||
         !heads_fit(heads, kv_heads, dim) || tokens_q * (heads / kv_heads) >= kMost || window < 0 || (window && !causal) || !(scale >= 1e-30f) || scale > 1e30f ||
         k_token < 0 || k_token >= kMostStride || v_token < 0 || v_token >= kMostStride)
         return SNGGUF_E_BADSHAPE;
@@ -265,7 +270,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
         !whole_pieces(out, out_token, out_head) || !aligned(ends_q, 4) || !aligned(ends_k, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
     const int d = kernel_dim(dim);
-    const Launch p = plan_many(tokens_q, sequences, heads, kv_heads, d);
+    const Launch p = plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, d);
     if (p.grid >= kMost) return SNGGUF_E_BADSHAPE;
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);
@@ -292,9 +297,10 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
     return launch_many(a, p, d, 0, partial, static_cast<hipStream_t>(stream));
 }
 
-int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t heads, int64_t kv_heads, int64_t dim) {
-    if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || max_new < 0 || !heads_fit(heads, kv_heads, dim)) return 0;
-    const PagedPlan p = paged_plan(tokens_q, sequences, max_new, heads, kv_heads, dim);
+int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    if (tokens_q <= 0 || tokens_q >= kMost || sequences <= 0 || sequences >= kMost || max_new < 0 || max_keys < 0 || max_keys > kMostKeys || !heads_fit(heads, kv_heads, dim))
+        return 0;
+    const PagedPlan p = paged_plan(tokens_q, sequences, max_new, max_keys, heads, kv_heads, dim);
     return (p.few ? p.a.partial_bytes : 0) + (p.many ? p.b.partial_bytes : 0);
 }
 
@@ -305,7 +311,7 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
     const int rc = check_cache(cache);
     if (rc != SNGGUF_OK) return rc;
     if (tokens_q < 0 || tokens_q >= kMost || sequences < 0 || sequences >= kMost || !heads_fit(heads, cache->kv_heads, cache->dim) ||
-        tokens_q * (heads / cache->kv_heads) >= kMost || max_new < 0 || window < 0 || !(scale >= 1e-30f) || scale > 1e30f || table_width < 0 || table_width * cache->page_size >= kMost ||
+        tokens_q * (heads / cache->kv_heads) >= kMost || max_new < 0 || window < 0 || !(scale >= 1e-30f) || scale > 1e30f || table_width < 0 || table_width > kMostKeys / cache->page_size ||
         (sequences > 1 && table_stride < table_width) || (!ends_q && tokens_q < sequences))
         return SNGGUF_E_BADSHAPE;
     if (tokens_q == 0 || sequences == 0) return SNGGUF_OK;
@@ -316,7 +322,7 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
     const int64_t kv_heads = cache->kv_heads;
     const int d = kernel_dim(cache->dim);
     const bool q8 = cache->qtype == SNGGUF_TYPE_Q8_0;
-    const PagedPlan p = paged_plan(tokens_q, sequences, ends_q ? max_new : 1, heads, kv_heads, cache->dim);
+    const PagedPlan p = paged_plan(tokens_q, sequences, ends_q ? max_new : 1, table_width * cache->page_size, heads, kv_heads, cache->dim);
     if (p.a.grid >= kMost || p.b.grid >= kMost) return SNGGUF_E_BADSHAPE;
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);
@@ -350,11 +356,11 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
         f.min_rows = 1;
         f.max_rows = (int32_t)p.few_rows;
         f.partial = p.a.partial_bytes ? partial : nullptr;
-        f.want = kRowsWant;
+        f.want = rows_want(p.a.rows, d);
         f.least = kRowsLeast;
         f.grid = f.partial ? p.a.grid : p.a.tiles;
-        int r = sngguf::launch_attention_rows(f, p.rows, d, q8, s);
-        if (r == SNGGUF_OK && f.partial) r = sngguf::launch_attention_combine(f, p.rows, kRowsKeys, d, p.a.tiles, s);
+        int r = sngguf::launch_attention_rows(f, p.a.rows, d, q8, s);
+        if (r == SNGGUF_OK && f.partial) r = sngguf::launch_attention_combine(f, p.a.rows, kRowsKeys, d, p.a.tiles, p.most_rows, s);
         if (r != SNGGUF_OK) return r;
     }
     if (p.many) {

@@ -108,19 +108,27 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
     const uint32_t want = id / (uint32_t)a.kv_heads;
     uint64_t chunk = 0;     // key tiles of a split; 0: not split
     if (a.partial) {
-        uint64_t total = 0;
+        uint64_t total = 0, tiles = 0;
         for (int base = 0; base < a.sequences; base += 64) {
             uint64_t mine = 0;
+            uint32_t rt = 0, kt = 0;
             if (base + lane < a.sequences) {
-                uint32_t rt, kt;
                 attention_tiles<ROWS, KEYS>(a, attention_sequence(a, base + lane), rt, kt);
                 mine = (uint64_t)rt * kt;
             }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
+            for (int o = 32; o > 0; o >>= 1) {
+                mine += __shfl_xor((unsigned long long)mine, o);
+                rt += __shfl_xor(rt, o);
+            }
             total += mine;
+            tiles += rt;
         }
-        chunk = (total * a.kv_heads + a.want - 1) / (uint32_t)a.want;
+        // the last split of a row tile is half as long as the others on average: so many workgroups less, or the device would have
+        // a few to do in a second round
+        const uint64_t cut = tiles * a.kv_heads / 2, most = a.want;
+        const uint64_t target = cut < most / 2 ? most - cut : most / 2;
+        chunk = (total * a.kv_heads + target - 1) / target;
         if (chunk < (uint32_t)a.least) chunk = a.least;
     }
     uint32_t before = 0, before_slots = 0;
@@ -186,6 +194,6 @@ __device__ __forceinline__ int64_t attention_page(const AttentionArgs& a, int se
     return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
 }
 
-int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, hipStream_t stream);
+int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, int64_t most_rows, hipStream_t stream);
 
 }  // namespace sngguf

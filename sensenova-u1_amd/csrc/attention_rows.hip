@@ -49,26 +49,120 @@ __device__ __forceinline__ f16x2_t whole_pair(uint32_t flipped) {
 
 }  // namespace
 
-// DT: elements of a head, rounded up.  NT: 16-row tiles.
-template <int DT, bool Q8, int NT>
-__global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs a) {
+// Workgroups that a compute unit takes at a time (as many wavefronts a SIMD: four a workgroup)
+constexpr int rows_workgroups(int dt, int nt) { return nt * dt <= 128 ? 3 : nt * dt <= 256 ? 2 : 1; }
+
+// DT: elements of a head, rounded up (FULL: exactly).  NT: 16-row tiles.
+template <int DT, bool FULL, bool Q8, int NT>
+__global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_rows_kernel(AttentionArgs a) {
     typedef typename Operand<Q8>::T op_t;
     constexpr int ROWS = 16 * NT;
     constexpr int KP = DT / 4;              // elements of a key that a lane reads
     constexpr int VP = DT / 16;             // elements of a value that a lane reads
     constexpr int KC = KP / 8;              // instructions of a score
+    constexpr int KW = Q8 ? KC / 2 : KC;    // 16-byte words of a key
+    constexpr int KR = DT / 128 > 0 ? DT / 128 : 1;   // scales of a key
+    constexpr int VW = Q8 ? VP / 4 : VP / 2;          // dwords of a value
+    constexpr int E = Q8 ? 1 : 2;           // bytes of an element
+    constexpr float kUp = Q8 ? 12.f : 0.f;
+    constexpr float kLimit = Q8 ? 32768.f : 1e9f;
     extern __shared__ __attribute__((aligned(16))) float lds[];   // [wave][16][DT] sums, then [wave][ROWS][2]
     float* stats = lds + kWaves * 16 * DT;
 
     const AttentionBlock b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
     if (!b.there) return;
+    const int dim = FULL ? DT : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int64_t rows = (int64_t)b.s.lq * a.group;
     const int64_t r0 = (int64_t)b.row_tile * ROWS, r1 = r0 + ROWS < rows ? r0 + ROWS : rows;
     int32_t lo, hi;
     attention_keys(a, b.s, r0, r1, lo, hi);
-    const int32_t back = b.s.lk - b.s.lq;
+    const int32_t back = b.s.lk - b.s.lq, most = b.s.lk - 1;
+
+    // ---- this split's runs, and the cache's words of a run -----------------------------------------------------------------
+    int32_t s0 = lo / kKeys, s1 = (hi + kKeys - 1) / kKeys;
+    {
+        const int32_t per = (s1 - s0 + b.splits - 1) / b.splits;
+        s0 += per * b.split;
+        s1 = s0 + per < s1 ? s0 + per : s1;
+    }
+    const int32_t end = s1 * kKeys < hi ? s1 * kKeys : hi;
+    const int32_t page_mask = (1 << a.page_shift) - 1;
+    const int32_t* table = a.table + (int64_t)b.seq * a.table_stride;
+    auto page_of = [&](int32_t key) -> int32_t {
+        const int32_t p = table[(key < most ? key : most) >> a.page_shift];
+        return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
+    };
+    // key of matrix row `col` in the two score instructions: 8 (col / 4) + col % 4 (+ 4); values: keys 8 g .. 8 g + 7
+    const int k_key = 8 * (col >> 2) + (col & 3), v_key = 8 * g;
+    int k_e[KW];                            // (pieces behind dim: the first, whose elements meet queries of zero)
+#pragma unroll
+    for (int x = 0; x < KW; x++) {
+        const int e = Q8 ? KP * g + 16 * x : 32 * x + 8 * g;
+        k_e[x] = FULL || e < dim ? e : 0;
+    }
+    const int v_e = FULL || VP * col < dim ? VP * col : 0;      // (behind dim: never stored)
+    u32x4_t k_raw[2][KW];
+    uint16_t k_scale[2][KR];
+    uint32_t v_raw[8][VW];
+    u32x4_t v_scale;
+    auto load_keys = [&](int32_t key0, int32_t page) {
+        const int64_t at = (int64_t)page * a.kv_heads + b.kv_head;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int32_t key = key0 + k_key + 4 * i, row = (key < most ? key : most) & page_mask;
+            const uint8_t* p = static_cast<const uint8_t*>(a.k_pages) + ((at << a.page_shift) + row) * (dim * E);
+#pragma unroll
+            for (int x = 0; x < KW; x++) k_raw[i][x] = *reinterpret_cast<const u32x4_t*>(p + E * k_e[x]);
+            if constexpr (Q8) {
+                const uint16_t* sc = a.k_scales + (at * (dim >> 5) << a.page_shift) + row;
+#pragma unroll
+                for (int x = 0; x < KR; x++) k_scale[i][x] = sc[(int64_t)(k_e[x * (KW / KR)] >> 5) << a.page_shift];
+            }
+        }
+    };
+    auto load_values = [&](int32_t key0, int32_t page) {
+        const int64_t at = (int64_t)page * a.kv_heads + b.kv_head;
+        const int32_t lead = key0 + v_key < most ? key0 + v_key : most, row = lead & page_mask & ~7;
+        const uint8_t* p = static_cast<const uint8_t*>(a.v_pages) + ((at << a.page_shift) + row) * (dim * E) + E * v_e;
+        auto word = [&](int j, int r) {
+            const uint8_t* q = p + r * (dim * E);
+            if constexpr (VW == 1) v_raw[j][0] = *reinterpret_cast<const uint32_t*>(q);
+            else if constexpr (VW == 2) {
+                const u32x2_t w = *reinterpret_cast<const u32x2_t*>(q);
+                v_raw[j][0] = w[0], v_raw[j][1] = w[1];
+            } else {
+#pragma unroll
+                for (int x = 0; x < VW; x += 4) {
+                    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + 4 * x);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) v_raw[j][x + y] = w[y];
+                }
+            }
+        };
+        if (key0 + kRun <= b.s.lk) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) word(j, j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int32_t last = (most & page_mask) - row;     // of these eight, or of the eight that are read in their place
+                word(j, key0 + v_key + j <= most ? j : last);
+            }
+        }
+        if constexpr (Q8) v_scale = *reinterpret_cast<const u32x4_t*>(a.v_scales + ((at * (dim >> 5) + (v_e >> 5)) << a.page_shift) + row);
+    };
+    int32_t key0 = s0 * kKeys + wave * kRun;
+    int32_t page_k = 0, page_v = 0;
+    if (key0 < end) {
+        page_k = page_of(key0 + (k_key & ~7));
+        page_v = page_of(key0 + v_key);
+        load_keys(key0, page_k);
+        load_values(key0, page_v);
+        page_k = page_of(key0 + kKeys + (k_key & ~7));
+        page_v = page_of(key0 + kKeys + v_key);
+    }
 
     // ---- queries: operand fragments, and which keys each column sees ---------------------------------------------------
     op_t qf[NT][KC];
@@ -77,18 +171,17 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int64_t r = r0 + 16 * n + col;
-        const bool there = r < r1;
-        const int64_t rr = there ? r : r0;
+        const int64_t rr = r < r1 ? r : r1 - 1;
         const int32_t token = (int32_t)(rr / a.group), head = b.kv_head * a.group + (int32_t)(rr - (int64_t)token * a.group);
         const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
         const int32_t place = back + token;
-        last[n] = !there ? -1 : a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
+        last[n] = a.causal && place < most ? place : most;
         first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
         u32x4_t raw[KC];
 #pragma unroll
         for (int i = 0; i < KC; i++) {
-            const int e = KP * g + 8 * i;
-            raw[i] = there && e < a.dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
+            const int e = Q8 ? KP * g + 8 * i : 32 * i + 8 * g;
+            raw[i] = FULL || e < dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
         }
         c[n] = a.scale_log2;
         if constexpr (Q8) {
@@ -99,9 +192,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const uint32_t x = raw[i][j] & 0x7F807F80u;
-                    const uint32_t h = x >> 16, l = x & 0xFFFFu;
-                    top = top > h ? top : h;
-                    top = top > l ? top : l;
+                    top = max(top, max(x >> 16, x & 0xFFFFu));
                 }
             top = max(top, (uint32_t)__shfl_xor((int)top, 16));
             top = max(top, (uint32_t)__shfl_xor((int)top, 32));
@@ -119,177 +210,159 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
             for (int i = 0; i < KC; i++) qf[n][i] = __builtin_bit_cast(op_t, raw[i]);
         }
     }
+    // keys that every row of the tile sees
+    const int32_t place0 = back + (int32_t)(r0 / a.group), place1 = back + (int32_t)((r1 - 1) / a.group);
+    const int32_t all_last = a.causal && place0 < most ? place0 : most;
+    const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
     f32x4_t acc[NT][VP];
-    float m[NT], l[NT];
+    float m[NT], l[NT], nb[NT];             // nb: what is added to a scaled score, kUp - m
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         m[n] = -__builtin_inff();
+        nb[n] = __builtin_inff();           // nothing known yet: whatever is formed with it is set right
         l[n] = 0.f;
 #pragma unroll
         for (int t = 0; t < VP; t++) acc[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- this split's steps --------------------------------------------------------------------------------------------
-    int32_t s0 = lo / kKeys, s1 = (hi + kKeys - 1) / kKeys;
-    {
-        const int32_t per = (s1 - s0 + b.splits - 1) / b.splits;
-        s0 += per * b.split;
-        s1 = s0 + per < s1 ? s0 + per : s1;
-    }
-    const int32_t page_mask = (1 << a.page_shift) - 1;
-    // key of matrix row `col` in the two score instructions: 8 (col / 4) + col % 4 (+ 4); values: keys 8 g .. 8 g + 7
-    const int k_key = 8 * (col >> 2) + (col & 3), v_key = 8 * g;
-    const int v_e = VP * col < a.dim ? VP * col : 0;      // (columns behind dim: any finite-or-not values of the same row, never stored)
-    const int64_t run_stride = (int64_t)1 << a.page_shift;
-    for (int32_t s = s0; s < s1; s++) {
-        const int32_t key0 = s * kKeys + wave * kRun;
-        if (key0 >= hi) break;
-        const bool edge = key0 + kRun > b.s.lk;
-        // -- keys
-        int64_t kat[2];
+    for (; key0 < end; key0 += kKeys) {
+        const bool more = key0 + kKeys < end;
+        float sc[NT][8];
         {
-            const int32_t lead = min(key0 + (k_key & ~7), b.s.lk - 1);
-            const int64_t page = (attention_page(a, b.seq, lead) * a.kv_heads + b.kv_head) << a.page_shift;
-            kat[0] = page + (min(key0 + k_key, b.s.lk - 1) & page_mask);
-            kat[1] = page + (min(key0 + k_key + 4, b.s.lk - 1) & page_mask);
-        }
-        op_t kf[2][KC];
+            op_t kf[2][KC];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if constexpr (Q8) {
-                const int64_t pg = kat[i] >> a.page_shift, row = kat[i] & page_mask;
-                const uint16_t* sc = a.k_scales + (pg * (a.dim >> 5) << a.page_shift) + row;
-                const uint8_t* p = static_cast<const uint8_t*>(a.k_pages) + kat[i] * a.dim;
+            for (int i = 0; i < 2; i++) {
+                if constexpr (Q8) {
 #pragma unroll
-                for (int x = 0; x < KC / 2; x++) {
-                    const int e = KP * g + 16 * x < a.dim ? KP * g + 16 * x : 0;
-                    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + e);
-                    const _Float16 d = __builtin_bit_cast(_Float16, sc[(e >> 5) * run_stride]);
-                    const f16x2_t dd = {d, d};
+                    for (int x = 0; x < KW; x++) {
+                        const _Float16 d = __builtin_bit_cast(_Float16, k_scale[i][x / (KW / KR)]);
+                        const f16x2_t dd = {d, d};
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        u32x4_t f;
+                        for (int y = 0; y < 2; y++) {
+                            u32x4_t f;
 #pragma unroll
-                        for (int z = 0; z < 2; z++) {
-                            const uint32_t flipped = w[2 * y + z] ^ 0x80808080u;
-                            f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * dd);
-                            f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * dd);
+                            for (int z = 0; z < 2; z++) {
+                                const uint32_t flipped = k_raw[i][x][2 * y + z] ^ 0x80808080u;
+                                f[2 * z] = __builtin_bit_cast(uint32_t, whole_pair<false>(flipped) * dd);
+                                f[2 * z + 1] = __builtin_bit_cast(uint32_t, whole_pair<true>(flipped) * dd);
+                            }
+                            kf[i][2 * x + y] = __builtin_bit_cast(op_t, f);
                         }
-                        kf[i][2 * x + y] = __builtin_bit_cast(op_t, f);
                     }
-                }
-            } else {
-                const bf16_t* p = static_cast<const bf16_t*>(a.k_pages) + kat[i] * a.dim;
+                } else {
 #pragma unroll
-                for (int x = 0; x < KC; x++) {
-                    const int e = KP * g + 8 * x < a.dim ? KP * g + 8 * x : 0;
-                    kf[i][x] = __builtin_bit_cast(op_t, *reinterpret_cast<const u32x4_t*>(p + e));
+                    for (int x = 0; x < KC; x++) kf[i][x] = __builtin_bit_cast(op_t, k_raw[i][x]);
                 }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int x = 0; x < KC; x++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) s[i] = mfma(kf[i][x], qf[n][x], s[i]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) sc[n][j] = s[j >> 2][j & 3];
+            }
         }
-        // -- values: vf[t] holds element t of keys 8 g .. 8 g + 7
-        op_t vf[VP];
-        {
-            const int32_t lead = min(key0 + v_key, b.s.lk - 1);
-            const int64_t page = attention_page(a, b.seq, lead) * a.kv_heads + b.kv_head;
-            const int32_t row = lead & page_mask & ~7;
-            int32_t at[8];
+        if (more) load_keys(key0 + kKeys, page_k);
+        if (key0 + kRun - 1 > all_last || key0 < all_first) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) at[j] = min(key0 + v_key + j, b.s.lk - 1) & page_mask;
-            if constexpr (Q8) {
-                u32x4_t sw = *reinterpret_cast<const u32x4_t*>(a.v_scales + ((page * (a.dim >> 5) + (v_e >> 5)) << a.page_shift) + row);
-                if (edge) {
-                    // scales behind the last key were never written: not even a zero may meet them
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (key0 + v_key + j >= b.s.lk) sw[j >> 1] &= (j & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-                }
-                const uint8_t* p = static_cast<const uint8_t*>(a.v_pages) + (page << a.page_shift) * a.dim + v_e;
-                uint32_t w[8][VP / 4];
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int x = 0; x < VP / 4; x++) w[j][x] = *reinterpret_cast<const uint32_t*>(p + (int64_t)at[j] * a.dim + 4 * x) ^ 0x80808080u;
-#pragma unroll
-                for (int x = 0; x < VP / 4; x++) {
-                    u32x4_t f[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t dw = sw[j];      // (a bit cast of a vector's element itself takes element 0)
-                        const f16x2_t d = __builtin_bit_cast(f16x2_t, dw);
-                        const uint32_t a0 = w[2 * j][x], a1 = w[2 * j + 1][x];
-                        // pairs of elements of each key -> pairs of keys of each element
-                        const uint32_t l0 = __builtin_bit_cast(uint32_t, whole_pair<false>(a0)), l1 = __builtin_bit_cast(uint32_t, whole_pair<false>(a1));
-                        const uint32_t h0 = __builtin_bit_cast(uint32_t, whole_pair<true>(a0)), h1 = __builtin_bit_cast(uint32_t, whole_pair<true>(a1));
-                        f[0][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(l1, l0, 0x05040100u)) * d);
-                        f[1][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(l1, l0, 0x07060302u)) * d);
-                        f[2][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(h1, h0, 0x05040100u)) * d);
-                        f[3][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(h1, h0, 0x07060302u)) * d);
-                    }
-#pragma unroll
-                    for (int t = 0; t < 4; t++) vf[4 * x + t] = __builtin_bit_cast(op_t, f[t]);
-                }
-            } else {
-                const bf16_t* p = static_cast<const bf16_t*>(a.v_pages) + (page << a.page_shift) * a.dim + v_e;
-                uint32_t w[8][VP / 2];
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const uint32_t* pj = reinterpret_cast<const uint32_t*>(p + (int64_t)at[j] * a.dim);
-#pragma unroll
-                    for (int x = 0; x < VP / 2; x++) w[j][x] = pj[x];
+                    const int32_t key = key0 + v_key + j;
+                    if (key < first[n] || key > last[n]) sc[n][j] = -__builtin_inff();
                 }
+        }
+        // weights with the maximum known so far; only where they run away are maximum, sums and weights set right
+        float p[NT][8], sum[NT];
+        bool fine = true;
 #pragma unroll
-                for (int x = 0; x < VP / 2; x++) {
-                    u32x4_t f0, f1;
+        for (int n = 0; n < NT; n++) {
+            sum[n] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        f0[j] = __builtin_amdgcn_perm(w[2 * j + 1][x], w[2 * j][x], 0x05040100u);
-                        f1[j] = __builtin_amdgcn_perm(w[2 * j + 1][x], w[2 * j][x], 0x07060302u);
-                    }
-                    vf[2 * x] = __builtin_bit_cast(op_t, f0);
-                    vf[2 * x + 1] = __builtin_bit_cast(op_t, f1);
+            for (int j = 0; j < 8; j++) {
+                p[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j], c[n], nb[n]));
+                sum[n] += p[n][j];
+            }
+            fine = fine && sum[n] <= kLimit;
+        }
+        if (__any(!fine)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float top = sc[n][0];
+#pragma unroll
+                for (int j = 1; j < 8; j++) top = fmaxf(top, sc[n][j]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(top * c[n], m[n]);
+                const bool none = top == -__builtin_inff();
+                const float base = none ? 0.f : top, keep = __builtin_amdgcn_exp2f(m[n] - base);
+                m[n] = top;
+                nb[n] = none ? __builtin_inff() : kUp - base;
+                l[n] *= keep;
+#pragma unroll
+                for (int t = 0; t < VP; t++) acc[n][t] *= keep;
+                sum[n] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][j], c[n], kUp - base));
+                    sum[n] += p[n][j];
                 }
             }
         }
+        op_t pf[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            f32x4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            l[n] += sum[n];
+            u32x4_t w;
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int j = 0; j < 4; j++) w[j] = Q8 ? pack_f16(p[n][2 * j], p[n][2 * j + 1]) : pack_bf16(p[n][2 * j], p[n][2 * j + 1]);
+            pf[n] = __builtin_bit_cast(op_t, w);
+        }
+        // vf: element t of keys 8 g .. 8 g + 7
+        u32x4_t vf[VP];
+        if constexpr (Q8) {
+            if (key0 + kRun > b.s.lk) {
+                // scales behind the last key were never written: not even a zero may meet them
 #pragma unroll
-                for (int x = 0; x < KC; x++) sc[i] = mfma(kf[i][x], qf[n][x], sc[i]);
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int32_t key = key0 + 8 * g + j;
-                p[j] = key >= first[n] && key <= last[n] ? sc[j >> 2][j & 3] : -__builtin_inff();
+                for (int j = 0; j < 8; j++)
+                    if (key0 + v_key + j > most) v_scale[j >> 1] &= (j & 1) ? 0x0000FFFFu : 0xFFFF0000u;
             }
-            float top = p[0];
 #pragma unroll
-            for (int j = 1; j < 8; j++) top = fmaxf(top, p[j]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(top * c[n], m[n]);
-            const float base = top == -__builtin_inff() ? 0.f : top;
-            const float keep = __builtin_amdgcn_exp2f(m[n] - base);
-            m[n] = top;
-            float sum = 0.f;
+            for (int x = 0; x < VW; x++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], c[n], -base));
-                sum += p[j];
-            }
-            l[n] = l[n] * keep + sum;
-            u32x4_t pw;
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t dw = v_scale[j];      // (a bit cast of a vector's element itself takes element 0)
+                    const f16x2_t d = __builtin_bit_cast(f16x2_t, dw);
+                    const uint32_t a0 = v_raw[2 * j][x] ^ 0x80808080u, a1 = v_raw[2 * j + 1][x] ^ 0x80808080u;
+                    // pairs of elements of each key -> pairs of keys of each element
+                    const uint32_t l0 = __builtin_bit_cast(uint32_t, whole_pair<false>(a0)), l1 = __builtin_bit_cast(uint32_t, whole_pair<false>(a1));
+                    const uint32_t h0 = __builtin_bit_cast(uint32_t, whole_pair<true>(a0)), h1 = __builtin_bit_cast(uint32_t, whole_pair<true>(a1));
+                    vf[4 * x][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(l1, l0, 0x05040100u)) * d);
+                    vf[4 * x + 1][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(l1, l0, 0x07060302u)) * d);
+                    vf[4 * x + 2][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(h1, h0, 0x05040100u)) * d);
+                    vf[4 * x + 3][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(h1, h0, 0x07060302u)) * d);
+                }
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) pw[j] = Q8 ? pack_f16(p[2 * j] * 4096.f, p[2 * j + 1] * 4096.f) : pack_bf16(p[2 * j], p[2 * j + 1]);
-            const op_t pf = __builtin_bit_cast(op_t, pw);
+            for (int x = 0; x < VW; x++)
 #pragma unroll
-            for (int t = 0; t < VP; t++) {
-                acc[n][t] *= keep;
-                acc[n][t] = mfma(vf[t], pf, acc[n][t]);
-            }
+                for (int j = 0; j < 4; j++) {
+                    vf[2 * x][j] = __builtin_amdgcn_perm(v_raw[2 * j + 1][x], v_raw[2 * j][x], 0x05040100u);
+                    vf[2 * x + 1][j] = __builtin_amdgcn_perm(v_raw[2 * j + 1][x], v_raw[2 * j][x], 0x07060302u);
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int t = 0; t < VP; t++) acc[n][t] = mfma(__builtin_bit_cast(op_t, vf[t]), pf[n], acc[n][t]);
+        if (more) {
+            load_values(key0 + kKeys, page_v);
+            page_k = page_of(key0 + 2 * kKeys + (k_key & ~7));
+            page_v = page_of(key0 + 2 * kKeys + v_key);
         }
     }
 
@@ -310,7 +383,6 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
 #pragma unroll
         for (int w = 0; w < kWaves; w++) top = fmaxf(top, stats[(w * ROWS + 16 * n + col) * 2]);
         mine = m[n] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
-        if constexpr (Q8) mine *= 1.f / 4096.f;
         // acc[n][t][i]: column col, element VP (4 g + i) + t
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -322,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
         // thread: row tid / 16 of the tile, elements VP (tid % 16) ...
         const int row = threadIdx.x >> 4, e = VP * (threadIdx.x & 15);
         const int64_t r = r0 + 16 * n + row;
-        if (r < r1 && e < a.dim) {
+        if (r < r1 && e < dim) {
             float o[VP];
 #pragma unroll
             for (int t = 0; t < VP; t++) {
@@ -360,46 +432,98 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(AttentionArgs 
     }
 }
 
-// Joins the splits of a row: one wavefront a row, lanes along its elements.
-template <int ROWS, int KEYS, int DT>
+// Joins the splits of rows: WIDE: a workgroup a row, its wavefronts taking every fourth pair of splits; else a wavefront a row.
+// Lanes: 32 along the row's elements, two splits at a time.
+template <int ROWS, int KEYS, int DT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionArgs a) {
+    constexpr int PER = DT / 32;            // elements of a lane
+    __shared__ float part[WIDE ? kWaves : 1][DT + 1];
+    __shared__ float tops[kWaves];
     const AttentionBlock b = attention_block<ROWS, KEYS, true>(a, blockIdx.x);
     if (!b.there || b.splits < 2) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = blockIdx.y * kWaves + wave;
-    const int64_t r = (int64_t)b.row_tile * ROWS + row;
-    if (r >= (int64_t)b.s.lq * a.group) return;
+    const int half = lane >> 5, e = PER * (lane & 31);
     const float* stats = a.partial + a.grid * ROWS * DT;
-    float top = -__builtin_inff();
-    for (int s = 0; s < b.splits; s++) top = fmaxf(top, stats[((b.slot + (int64_t)s * a.kv_heads) * ROWS + row) * 2]);
-    float o[DT / 64];
+    const int64_t r0 = (int64_t)b.row_tile * ROWS, left = (int64_t)b.s.lq * a.group - r0;
+    const int rows = left < ROWS ? (int)left : ROWS;
+    // (the launch has as many workgroups as the caller takes for the most rows; more rows are taken in turn)
+    for (int row = WIDE ? blockIdx.y : blockIdx.y * kWaves + wave; row < rows; row += gridDim.y * (WIDE ? 1 : kWaves)) {
+        auto slot = [&](int s) { return (b.slot + (int64_t)s * a.kv_heads) * ROWS + row; };
+        float top = -__builtin_inff();
+        for (int s = WIDE ? threadIdx.x : lane; s < b.splits; s += WIDE ? kThreads : 64) top = fmaxf(top, stats[slot(s) * 2]);
 #pragma unroll
-    for (int t = 0; t < DT / 64; t++) o[t] = 0.f;
-    float l = 0.f;
-    for (int s = 0; s < b.splits; s++) {
-        const int64_t at = (b.slot + (int64_t)s * a.kv_heads) * ROWS + row;
-        const float ms = stats[at * 2];
-        if (ms == -__builtin_inff()) continue;
-        const float w = __builtin_amdgcn_exp2f(ms - top);
-        l += stats[at * 2 + 1] * w;
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if constexpr (WIDE) {
+            if (lane == 0) tops[wave] = top;
+            __syncthreads();
 #pragma unroll
-        for (int t = 0; t < DT / 64; t++) o[t] += a.partial[at * DT + 64 * t + lane] * w;
+            for (int w = 0; w < kWaves; w++) top = fmaxf(top, tops[w]);
+        }
+        float o[PER], l = 0.f;
+#pragma unroll
+        for (int t = 0; t < PER; t++) o[t] = 0.f;
+#pragma unroll 8
+        for (int s = WIDE ? 2 * wave + half : half; s < b.splits; s += WIDE ? 2 * kWaves : 2) {
+            const int64_t at = slot(s);
+            const float ms = stats[at * 2], ls = stats[at * 2 + 1];
+            // (a split in which the row sees nothing holds zeros)
+            const float w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - top);
+            l += ls * w;
+            const float* p = a.partial + at * DT + e;
+            if constexpr (PER == 2) {
+                const float2 x = *reinterpret_cast<const float2*>(p);
+                o[0] += x.x * w, o[1] += x.y * w;
+            } else {
+#pragma unroll
+                for (int t = 0; t < PER; t += 4) {
+                    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + t);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) o[t + y] += x[y] * w;
+                }
+            }
+        }
+        l += __shfl_xor(l, 32);
+#pragma unroll
+        for (int t = 0; t < PER; t++) o[t] += __shfl_xor(o[t], 32);
+        if constexpr (WIDE) {
+            if (half == 0) {
+#pragma unroll
+                for (int t = 0; t < PER; t++) part[wave][e + t] = o[t];
+                if (lane == 0) part[wave][DT] = l;
+            }
+            __syncthreads();
+            if (wave == 0) {
+                l = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) l += part[w][DT];
+#pragma unroll
+                for (int t = 0; t < PER; t++) {
+                    o[t] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWaves; w++) o[t] += part[w][e + t];
+                }
+            }
+        }
+        if ((!WIDE || wave == 0) && half == 0 && e < a.dim) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int64_t r = r0 + row;
+            const int32_t token = (int32_t)(r / a.group), head = b.kv_head * a.group + (int32_t)(r - (int64_t)token * a.group);
+            bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e;
+#pragma unroll
+            for (int t = 0; t < PER; t += 2) *reinterpret_cast<uint32_t*>(out + t) = pack_bf16(o[t] * inv, o[t + 1] * inv);
+        }
+        if constexpr (WIDE) __syncthreads();       // (part and tops are written again)
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int32_t token = (int32_t)(r / a.group), head = b.kv_head * a.group + (int32_t)(r - (int64_t)token * a.group);
-    bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head;
-#pragma unroll
-    for (int t = 0; t < DT / 64; t++)
-        if (64 * t + lane < a.dim) out[64 * t + lane] = f32_to_bf16(o[t] * inv);
 }
 
-int64_t attention_rows_keys() { return kKeys; }
-
-// tiles: (row tile, head) pairs at most
-int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, hipStream_t stream) {
+// tiles: (row tile, head) pairs at most; most_rows: of a tile, as far as is known
+int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, int64_t most_rows, hipStream_t stream) {
+    const unsigned count = (unsigned)(most_rows < rows ? most_rows : rows);
+    // few rows have many splits each
 #define SNGGUF_GO(R, K, D)                                                                                              \
     if (rows == R && keys == K && dim == D) {                                                                           \
-        attention_combine_kernel<R, K, D><<<dim3((unsigned)tiles, R / kWaves), kThreads, 0, stream>>>(a);               \
+        constexpr bool kWide = R <= 64;                                                                                 \
+        attention_combine_kernel<R, K, D, kWide><<<dim3((unsigned)tiles, kWide ? count : (count + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a); \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
 #define SNGGUF_GO_DIM(R, K) SNGGUF_GO(R, K, 64) SNGGUF_GO(R, K, 128) SNGGUF_GO(R, K, 256)
@@ -414,21 +538,27 @@ int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim
     return SNGGUF_E_BADSHAPE;
 }
 
+// dim: of the kernel, 64, 128 or 256; rows: of a tile, 16, 32 or (up to 128 elements) 64
 int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream) {
-#define SNGGUF_GO(D, Q, N)                                                                                              \
-    if (dim == D && q8 == Q && rows == 16 * N) {                                                                        \
+#define SNGGUF_GO(D, F, Q, N)                                                                                           \
+    if (dim == D && (a.dim == D) == F && q8 == Q && rows == 16 * N) {                                                   \
         constexpr int kLds = (kWaves * 16 * D + kWaves * 16 * N * 2) * 4;                                               \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_rows_kernel<D, Q, N>), \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_rows_kernel<D, F, Q, N>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_rows_kernel<D, Q, N><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                          \
+        attention_rows_kernel<D, F, Q, N><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                       \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
-#define SNGGUF_GO_DIM(D) SNGGUF_GO(D, false, 1) SNGGUF_GO(D, false, 2) SNGGUF_GO(D, false, 4) SNGGUF_GO(D, true, 1) SNGGUF_GO(D, true, 2) SNGGUF_GO(D, true, 4)
-    SNGGUF_GO_DIM(64)
-    SNGGUF_GO_DIM(128)
-    SNGGUF_GO_DIM(256)
-#undef SNGGUF_GO_DIM
+#define SNGGUF_GO_TYPES(D, N) SNGGUF_GO(D, true, false, N) SNGGUF_GO(D, false, false, N) SNGGUF_GO(D, true, true, N) SNGGUF_GO(D, false, true, N)
+    SNGGUF_GO_TYPES(64, 1)
+    SNGGUF_GO_TYPES(64, 2)
+    SNGGUF_GO_TYPES(64, 4)
+    SNGGUF_GO_TYPES(128, 1)
+    SNGGUF_GO_TYPES(128, 2)
+    SNGGUF_GO_TYPES(128, 4)
+    SNGGUF_GO_TYPES(256, 1)
+    SNGGUF_GO_TYPES(256, 2)
+#undef SNGGUF_GO_TYPES
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
 }

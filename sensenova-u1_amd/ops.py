@@ -160,12 +160,12 @@ def load_library() -> ctypes.CDLL:
     lib.sngguf_cache_write_rotary.restype = ci
     lib.sngguf_cache_read.argtypes = [vp, vp, i64, vp, vp, vp]
     lib.sngguf_cache_read.restype = ci
-    lib.sngguf_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64]
+    lib.sngguf_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
     lib.sngguf_attention_workspace_bytes.restype = i64
     lib.sngguf_attention.argtypes = [vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, i64, i64, i64, i64, vp, vp, i64, cf, ci, i64, vp, i64, i64,
                                      vp, i64, vp]
     lib.sngguf_attention.restype = ci
-    lib.sngguf_paged_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+    lib.sngguf_paged_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i64]
     lib.sngguf_paged_attention_workspace_bytes.restype = i64
     lib.sngguf_paged_attention.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, cf, i64, vp, i64, i64, vp, i64, vp]
     lib.sngguf_paged_attention.restype = ci

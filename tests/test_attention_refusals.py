@@ -88,7 +88,7 @@ def _attention(q=P, tokens=4, heads=4, kv_heads=2, dim=64, k=P, v=P, keys=4, end
 
 
 def test_attention_refusals():
-    for bad in (dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=1 << 30, heads=4, kv_heads=2), dict(keys=-1), dict(n=-1), dict(heads=3), dict(heads=0), dict(kv_heads=0),
+    for bad in (dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=1 << 30, heads=4, kv_heads=2), dict(keys=-1), dict(keys=(1 << 31) - 1), dict(n=-1), dict(heads=3), dict(heads=0), dict(kv_heads=0),
                 dict(dim=80), dict(dim=16), dict(dim=288), dict(scale=0.0), dict(scale=-1.0), dict(scale=NAN), dict(scale=INF), dict(window=-1),
                 dict(window=5, causal=0), dict(kt=1 << 26), dict(kt=-128)):
         assert _attention(**bad) == E_SHAPE, bad
@@ -98,8 +98,9 @@ def test_attention_refusals():
         assert _attention(**bad) == E_ALIGN, bad
     assert _attention(tokens=0, q=None) == 0 and _attention(n=0, ends_q=None) == 0
     lib = ops.load_library()
-    assert lib.sngguf_attention_workspace_bytes(0, 1, 4, 2, 64) == 0 and lib.sngguf_attention_workspace_bytes(4, 1, 4, 3, 64) == 0
-    assert lib.sngguf_attention_workspace_bytes(1 << 20, 1, 32, 8, 128) == 0 and lib.sngguf_attention_workspace_bytes(64, 1, 32, 8, 128) > 0
+    assert lib.sngguf_attention_workspace_bytes(0, 9, 1, 4, 2, 64) == 0 and lib.sngguf_attention_workspace_bytes(4, 9, 1, 4, 3, 64) == 0
+    assert lib.sngguf_attention_workspace_bytes(1 << 20, 1 << 20, 1, 32, 8, 128) == 0 and lib.sngguf_attention_workspace_bytes(64, 5000, 1, 32, 8, 128) > 0
+    assert lib.sngguf_attention_workspace_bytes(64, 64, 1, 32, 8, 128) == 0
 
 
 def _paged(q=P, tokens=2, heads=4, cache=_cache(), table=P, stride=4, width=4, lens=P, ends=None, n=2, max_new=0, scale=0.1, window=0, out=P, ws=None, nbytes=0):

@@ -66,7 +66,7 @@ def test_prompt_packed_with_empty_sequences_and_rows_that_see_nothing(dev, causa
 
 def test_prompt_few_rows_over_many_keys_are_split(dev):
     for tokens, keys, causal in ((1, 5000, True), (40, 9001, True), (40, 9001, False)):
-        assert ops.load_library().sngguf_attention_workspace_bytes(tokens, 1, 8, 2, 128) > 0
+        assert ops.load_library().sngguf_attention_workspace_bytes(tokens, keys, 1, 8, 2, 128) > 0
         _prompt(dev, [tokens], [keys], 8, 2, 128, causal)
     _prompt(dev, [3, 1, 30], [4000, 1, 700], 8, 2, 128, True, 900)
 
