@@ -78,12 +78,12 @@ __device__ __forceinline__ AttentionSequence attention_sequence(const AttentionA
 // Row tiles of a sequence, and key tiles that its rows see between them.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ void attention_tiles(const AttentionArgs& a, const AttentionSequence& s, uint32_t& row_tiles, uint32_t& key_tiles) {
-    const int64_t rows = (int64_t)s.lq * a.group;
-    if (rows < a.min_rows || rows > a.max_rows) {
+    const uint32_t rows = (uint32_t)s.lq * (uint32_t)a.group;     // (tokens_q x group is below 2^31)
+    if ((int32_t)rows < a.min_rows || (int32_t)rows > a.max_rows) {
         row_tiles = key_tiles = 0;
         return;
     }
-    row_tiles = (uint32_t)((rows + ROWS - 1) / ROWS);
+    row_tiles = (rows + ROWS - 1) / ROWS;
     int64_t lo = a.window ? (int64_t)s.lk - s.lq - a.window + 1 : 0;
     lo = lo < 0 ? 0 : lo / KEYS;
     const int64_t hi = ((int64_t)s.lk + KEYS - 1) / KEYS;
@@ -106,7 +106,7 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
     // heads of one row tile are neighbours: with 8 key / value heads each XCD keeps to one head's keys and values
     b.kv_head = id % (uint32_t)a.kv_heads;
     const uint32_t want = id / (uint32_t)a.kv_heads;
-    uint64_t chunk = 0;     // key tiles of a split; 0: not split
+    uint32_t chunk = 0;     // key tiles of a split; 0: not split
     if (a.partial) {
         uint64_t total = 0, tiles = 0;
         for (int base = 0; base < a.sequences; base += 64) {
@@ -128,15 +128,19 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
         // a few to do in a second round
         const uint64_t cut = tiles * a.kv_heads / 2, most = a.want;
         const uint64_t target = cut < most / 2 ? most - cut : most / 2;
-        chunk = (total * a.kv_heads + target - 1) / target;
+        // (rounded up by one at most where the quotient is whole: the grid has room for `want`)
+        const double exact = (double)(total * a.kv_heads) / (double)target;
+        chunk = exact < 2147483647.0 ? (uint32_t)exact + 1 : 0x7FFFFFFFu;
         if (chunk < (uint32_t)a.least) chunk = a.least;
     }
     uint32_t before = 0, before_slots = 0;
     for (int base = 0; base < a.sequences; base += 64) {
         uint32_t rt = 0, kt = 0, splits = 1;
+        AttentionSequence mine_s = {0, 0, 0, 0};
         if (base + lane < a.sequences) {
-            attention_tiles<ROWS, KEYS>(a, attention_sequence(a, base + lane), rt, kt);
-            if (chunk) splits = (uint32_t)((kt + chunk - 1) / chunk);
+            mine_s = attention_sequence(a, base + lane);
+            attention_tiles<ROWS, KEYS>(a, mine_s, rt, kt);
+            if (chunk) splits = (kt + chunk - 1) / chunk;
             if (splits < 1) splits = 1;
         }
         const uint32_t slots = rt * splits, mine = COMBINE ? rt : slots;
@@ -163,7 +167,10 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
             // the last rows of a causal sequence see the most keys: first
             b.row_tile = (int32_t)(tiles - 1 - t);
             b.slot = ((int64_t)first_slot + (int64_t)t * b.splits + b.split) * a.kv_heads + b.kv_head;
-            b.s = attention_sequence(a, b.seq);
+            b.s.q0 = (uint32_t)__builtin_amdgcn_readlane((int)mine_s.q0, l);     // (both below 2^31)
+            b.s.k0 = (uint32_t)__builtin_amdgcn_readlane((int)mine_s.k0, l);
+            b.s.lq = __builtin_amdgcn_readlane(mine_s.lq, l);
+            b.s.lk = __builtin_amdgcn_readlane(mine_s.lk, l);
             b.there = true;
             return b;
         }
@@ -173,25 +180,26 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
     return b;
 }
 
+// Token of a row, and its head of the group
+__device__ __forceinline__ int32_t attention_token(const AttentionArgs& a, int64_t row, int32_t& head) {
+    const uint32_t token = (uint32_t)row / (uint32_t)a.group;
+    head = (int32_t)((uint32_t)row - token * (uint32_t)a.group);
+    return (int32_t)token;
+}
+
 // Keys [lo, hi) that some row of rows [r0, r1) of a sequence sees.
 __device__ __forceinline__ void attention_keys(const AttentionArgs& a, const AttentionSequence& s, int64_t r0, int64_t r1, int32_t& lo, int32_t& hi) {
     const int64_t back = (int64_t)s.lk - s.lq;
     lo = 0;
     hi = s.lk;
     if (a.causal) {
-        const int64_t last = back + (r1 - 1) / a.group + 1;
+        const int64_t last = back + (uint32_t)(r1 - 1) / (uint32_t)a.group + 1;
         if (last < hi) hi = (int32_t)(last < 0 ? 0 : last);
     }
     if (a.window) {
-        const int64_t first = back + r0 / a.group - a.window + 1;
+        const int64_t first = back + (uint32_t)r0 / (uint32_t)a.group - a.window + 1;
         if (first > 0) lo = (int32_t)(first < hi ? first : hi);
     }
-}
-
-// Page of a sequence's key; numbers that are no pages are read as the nearest one, so that no table reaches beyond the cache.
-__device__ __forceinline__ int64_t attention_page(const AttentionArgs& a, int seq, int32_t key) {
-    const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
-    return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
 }
 
 int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, int64_t most_rows, hipStream_t stream);

@@ -172,7 +172,9 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     for (int n = 0; n < NT; n++) {
         const int64_t r = r0 + 16 * n + col;
         const int64_t rr = r < r1 ? r : r1 - 1;
-        const int32_t token = (int32_t)(rr / a.group), head = b.kv_head * a.group + (int32_t)(rr - (int64_t)token * a.group);
+        int32_t head;
+        const int32_t token = attention_token(a, rr, head);
+        head += b.kv_head * a.group;
         const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
         const int32_t place = back + token;
         last[n] = a.causal && place < most ? place : most;
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         }
     }
     // keys that every row of the tile sees
-    const int32_t place0 = back + (int32_t)(r0 / a.group), place1 = back + (int32_t)((r1 - 1) / a.group);
+    const int32_t place0 = back + (int32_t)((uint32_t)r0 / (uint32_t)a.group), place1 = back + (int32_t)((uint32_t)(r1 - 1) / (uint32_t)a.group);
     const int32_t all_last = a.causal && place0 < most ? place0 : most;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
@@ -421,7 +423,9 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
                 }
             } else {
                 const float inv = rl == 0.f ? 0.f : 1.f / rl;
-                const int32_t token = (int32_t)(r / a.group), head = b.kv_head * a.group + (int32_t)(r - (int64_t)token * a.group);
+                int32_t head;
+            const int32_t token = attention_token(a, r, head);
+            head += b.kv_head * a.group;
                 bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e;
 #pragma unroll
                 for (int t = 0; t < VP; t += 4)
@@ -507,7 +511,9 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
         if ((!WIDE || wave == 0) && half == 0 && e < a.dim) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t r = r0 + row;
-            const int32_t token = (int32_t)(r / a.group), head = b.kv_head * a.group + (int32_t)(r - (int64_t)token * a.group);
+            int32_t head;
+            const int32_t token = attention_token(a, r, head);
+            head += b.kv_head * a.group;
             bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e;
 #pragma unroll
             for (int t = 0; t < PER; t += 2) *reinterpret_cast<uint32_t*>(out + t) = pack_bf16(o[t] * inv, o[t + 1] * inv);

@@ -28,7 +28,6 @@ namespace sngguf {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kKeys = 64;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -90,12 +89,12 @@ template <int DT> struct Tile {
 
 enum { kPacked = 0, kPaged = 1, kPagedQ8 = 2 };
 
-// CT: 32-row tiles of a wavefront.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
-template <int DT, int SOURCE, int CT, int NS>
-__global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
+// W: wavefronts.  CT: 32-row tiles of each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
+template <int DT, int SOURCE, int W, int CT, int NS>
+__global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
-    constexpr int ROWS = 128 * CT;
+    constexpr int ROWS = 32 * W * CT;
     constexpr int TILE = Tile<DT>::kBytes, RB = Tile<DT>::kRowBlock, PB = Tile<DT>::kBlocks;
     constexpr int KS = DT / 16, DTILES = DT / 32;
     constexpr int VF = 2 * DTILES, NF = VF + KS;       // operand fragments of a step: of values, in all
@@ -123,7 +122,9 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     for (int n = 0; n < CT; n++) {
         row_of[n] = r0 + 32 * (CT * wave + n) + col;
         const int64_t rr = row_of[n] < r1 ? row_of[n] : r1 - 1;
-        const int32_t token = (int32_t)(rr / a.group), head = b.kv_head * a.group + (int32_t)(rr - (int64_t)token * a.group);
+        int32_t head;
+        const int32_t token = attention_token(a, rr, head);
+        head += b.kv_head * a.group;
         const int32_t place = back + token;
         last[n] = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
         first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     }
     const int32_t count = s1 - s0;
     // rows whose visible keys are the fewest: tiles inside these bounds need no mask
-    const int32_t place0 = back + (int32_t)(r0 / a.group), place1 = back + (int32_t)((r1 - 1) / a.group);
+    const int32_t place0 = back + (int32_t)((uint32_t)r0 / (uint32_t)a.group), place1 = back + (int32_t)((uint32_t)(r1 - 1) / (uint32_t)a.group);
     const int32_t all_last = a.causal && place0 < b.s.lk - 1 ? place0 : b.s.lk - 1;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
@@ -188,21 +189,23 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     }
 
     // ---- tiles into LDS ------------------------------------------------------------------------------------------------
-    // Sixteen rows a wavefront.  Rows behind the last key are the last key's: masked, but finite wherever the keys are.
+    // Rows behind the last key are the last key's: masked, but finite wherever the keys are.
     const int32_t page_mask = (1 << a.page_shift) - 1;
-    constexpr int REQ = 2 * PB;                        // requests of a wavefront for a tile: blocks of its sixteen rows
+    constexpr int LOAD = kKeys / W;                    // rows of a tile that a wavefront brings, 8 or 16
+    constexpr int REQ = LOAD / 8 * PB;                 // requests for them: blocks
     constexpr int QP = DT / 16;                        // 8-bit: 16-byte pieces of a row
-    constexpr int QN = 16 * QP / 64;                   // ... a lane has of each tile
+    constexpr int QN = LOAD * QP / 64;                 // ... a lane has of each tile
+    static_assert(LOAD % 8 == 0 && (!Q8 || LOAD * QP % 64 == 0), "whole requests");
     u32x4_t held[2][Q8 ? QN : 1];
     uint16_t held_scale[2][Q8 ? QN : 1];
     // this lane's part of a request: row and piece of a block
     const int crow = (lane & 7) ^ (4 * ((lane >> 4) & 1)), cpiece = lane >> 3;
     const int64_t k_stride = SOURCE == kPacked ? a.k_token : a.dim, v_stride = SOURCE == kPacked ? a.v_token : a.dim;
-    // byte offsets of this lane's pieces behind the first of the wavefront's sixteen rows, and the last row known to be there
+    // byte offsets of this lane's pieces behind the first of the wavefront's rows, and the last row known to be there
     uint32_t coff[2][REQ];
     int32_t rows_there[2] = {-1, -1};
     auto set_offsets = [&](int half, int32_t spare) {
-        spare = spare < 15 ? spare : 15;
+        spare = spare < LOAD - 1 ? spare : LOAD - 1;
         if (spare == rows_there[half]) return;
         rows_there[half] = spare;
 #pragma unroll
@@ -216,17 +219,17 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     const uint8_t* v_base = reinterpret_cast<const uint8_t*>(SOURCE == kPacked ? a.v + b.s.k0 * a.v_token + (int64_t)b.kv_head * a.v_head : nullptr);
     const int32_t most = b.s.lk - 1;
     const int32_t* table = SOURCE == kPacked ? nullptr : a.table + (int64_t)b.seq * a.table_stride;
-    // page of the wavefront's rows of a tile (sixteen rows lie in one)
+    // page of the wavefront's rows of a tile (they lie in one)
     auto page_of = [&](int32_t tile) -> int32_t {
         if constexpr (SOURCE == kPacked) return 0;
-        const int32_t base = tile * kKeys + 16 * wave, lead = base < most ? base : most;
+        const int32_t base = tile * kKeys + LOAD * wave, lead = base < most ? base : most;
         const int32_t p = *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(table + __builtin_amdgcn_readfirstlane(lead >> a.page_shift));
         return p < 0 ? 0 : p >= a.pages ? a.pages - 1 : p;
     };
     // where the wavefront's rows of a tile start, for the requests of half 0 (keys) or 1 (values)
     const uint8_t* from[2] = {nullptr, nullptr};
     auto aim = [&](int half, int32_t tile, int32_t page) {
-        const int32_t base = tile * kKeys + 16 * wave, lead = base < most ? base : most;
+        const int32_t base = tile * kKeys + LOAD * wave, lead = base < most ? base : most;
         const int32_t spare = most - lead;             // rows behind the first that there are
         if constexpr (SOURCE == kPacked) {
             from[half] = uniform_ptr((half ? v_base : k_base) + 2 * lead * (half ? v_stride : k_stride));
@@ -253,12 +256,12 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
     const uint32_t lds0 = lds_offset(lds);
     // request j of REQ into the half of the stage at `stage`
     auto request = [&](int half, uint32_t stage, int j) {
-        if constexpr (!Q8) copy_request(stage + half * TILE + (2 * wave + j / PB) * RB + (j % PB) * 1024, coff[half][j], from[half]);
+        if constexpr (!Q8) copy_request(stage + half * TILE + (LOAD / 8 * wave + j / PB) * RB + (j % PB) * 1024, coff[half][j], from[half]);
     };
     // 8-bit tiles: widened from the registers that the request filled
     auto widen = [&](int half, uint32_t stage, int i) {
         if constexpr (Q8) {
-            const int p = lane + 64 * i, row = 16 * wave + p / QP, piece = p % QP;
+            const int p = lane + 64 * i, row = LOAD * wave + p / QP, piece = p % QP;
             const u32x4_t w = held[half][i];
             const _Float16 d1 = __builtin_bit_cast(_Float16, held_scale[half][i]);
             const f16x2_t d = {d1, d1};
@@ -407,19 +410,18 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
             [&](auto f_) {
                 constexpr int f = decltype(f_)::value, g = f + 3;
                 beside(f_);
-                if constexpr (g < VF) ring[g & 3] = value_fragment(at, half, g >> 1, g & 1);
+                if constexpr (g < VF) ring[g & 3] = value_fragment(at, half, g % DTILES, g / DTILES);
                 else if constexpr (g < NF) ring[g & 3] = key_fragment(at, half, g - VF);
-                else ring[g & 3] = value_fragment(next, half ^ 1, (g - NF) >> 1, (g - NF) & 1);
+                else ring[g & 3] = value_fragment(next, half ^ 1, (g - NF) % DTILES, (g - NF) / DTILES);
 #pragma unroll
                 for (int n = 0; n < CT; n++) {
-                    if constexpr (f < VF) acc[n][f >> 1] = mfma(ring[f & 3], weights_operand(w0, n, f & 1), acc[n][f >> 1]);
+                    if constexpr (f < VF) acc[n][f % DTILES] = mfma(ring[f & 3], weights_operand(w0, n, f / DTILES), acc[n][f % DTILES]);
                     else s1[n] = mfma(ring[f & 3], qf[n][f - VF], s1[n]);
                 }
                 constexpr int p0 = f * NP / NF, p1 = (f + 1) * NP / NF;
 #pragma unroll
                 for (int p = p0; p < p1; p++) raise_pair(s, nb, p, up[f & 1][p - p0][0], up[f & 1][p - p0][1]);
                 if constexpr (f > 0) pack_of(std::integral_constant<int, f - 1>());
-                __builtin_amdgcn_sched_barrier(0);
             },
             std::make_integer_sequence<int, NF>());
         pack_of(std::integral_constant<int, NF - 1>());
@@ -495,8 +497,8 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
         uint32_t ahead = NS == 2 ? 0u : after(kStage); // the last one asked for
         at = at_stage(stage);
         ring[0] = value_fragment(at, 0, 0, 0);
-        ring[1] = value_fragment(at, 0, 0, 1);
-        ring[2] = value_fragment(at, 0, 1, 0);
+        ring[1] = value_fragment(at, 0, 1 % DTILES, 1 / DTILES);
+        ring[2] = value_fragment(at, 0, 2 % DTILES, 2 / DTILES);
         for (int32_t i = 1; i < count; i++) {
             if constexpr (NS > 2) ahead = after(ahead);
             else ahead = after(stage);
@@ -554,7 +556,9 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
             continue;
         }
         const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-        const int32_t token = (int32_t)(row_of[n] / a.group), head = b.kv_head * a.group + (int32_t)(row_of[n] - (int64_t)token * a.group);
+        int32_t head;
+        const int32_t token = attention_token(a, row_of[n], head);
+        head += b.kv_head * a.group;
         bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head;
 #pragma unroll
         for (int t = 0; t < DTILES; t++)
@@ -570,22 +574,27 @@ __global__ __launch_bounds__(kThreads, CT == 1 && DT <= 128 ? 2 : 1) void attent
 
 // rows: of a workgroup, 128 or (up to 128 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
-#define SNGGUF_GO(D, S, C, N)                                                                                           \
-    if (dim == D && source == S && rows == 128 * C) {                                                                   \
-        constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                    \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, C, N>), \
+#define SNGGUF_GO(D, S, W, C, N)                                                                                        \
+    if (dim == D && source == S && rows == 32 * W * C) {                                                                \
+        constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                   \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, C, N>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_tiles_kernel<D, S, C, N><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                      \
+        attention_tiles_kernel<D, S, W, C, N><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                     \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
-#define SNGGUF_GO_DIM(D, C, N) SNGGUF_GO(D, kPacked, C, N) SNGGUF_GO(D, kPaged, C, N) SNGGUF_GO(D, kPagedQ8, C, 2)
-    SNGGUF_GO_DIM(64, 1, 3)
-    SNGGUF_GO_DIM(64, 2, 3)
-    SNGGUF_GO_DIM(128, 1, 2)
-    SNGGUF_GO_DIM(128, 2, 3)
-    SNGGUF_GO_DIM(256, 1, 2)
-#undef SNGGUF_GO_DIM
+#define SNGGUF_GO_PLAIN(D, W, C, N) SNGGUF_GO(D, kPacked, W, C, N) SNGGUF_GO(D, kPaged, W, C, N)
+    SNGGUF_GO_PLAIN(64, 4, 1, 3)
+    SNGGUF_GO_PLAIN(64, 4, 2, 3)
+    SNGGUF_GO_PLAIN(128, 4, 1, 2)
+    SNGGUF_GO_PLAIN(128, 8, 1, 3)
+    SNGGUF_GO_PLAIN(256, 4, 1, 2)
+    SNGGUF_GO(64, kPagedQ8, 4, 1, 2)
+    SNGGUF_GO(64, kPagedQ8, 4, 2, 2)
+    SNGGUF_GO(128, kPagedQ8, 4, 1, 2)
+    SNGGUF_GO(128, kPagedQ8, 8, 1, 2)
+    SNGGUF_GO(256, kPagedQ8, 4, 1, 2)
+#undef SNGGUF_GO_PLAIN
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
 }
