@@ -36,6 +36,29 @@ class _CacheStruct(ctypes.Structure):
                 ("qtype", ctypes.c_int32)]
 
 
+def _new(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """``lib.<name>(*args, current stream)`` with device ``index`` current."""
+    fn = getattr(ops.load_library(), name)
+    if index == ops._current_device():
+        rc = fn(*args, ops._stream(torch.device("cuda", index)) if ops._raw_stream is None else ops._raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        ops._check(rc, name)
+
+
+def _launch_with_workspace(dev: torch.device, nbytes: int, name: str, *args) -> None:
+    if not nbytes:
+        return _launch(dev.index, name, *args, None, 0)
+    with ops._on(dev), ops._whole_call(dev):
+        _launch(dev.index, name, *args, ops.pooled_workspace(dev, nbytes).data_ptr(), nbytes)
+
+
 def _same_device(what: str, index: int, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:
@@ -138,16 +161,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             raise SnGgufError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
     if inplace and (q is not q0 or k is not k0):
         raise SnGgufError("rotary: in place needs the elements of a head next to each other")
-    q_out = q if inplace else torch.empty((tokens, heads, dim), dtype=_BF16, device=q.device)
-    k_out = k if inplace or k is None else torch.empty(k.shape, dtype=_BF16, device=q.device)
+    q_out = q if inplace else _new(q)
+    k_out = k if inplace or k is None else _new(k)
     if tokens and heads:
         kt, kh, kot, koh = (*_strides(k), *_strides(k_out)) if k is not None else (0, 0, 0, 0)
         kp, kop, kn = (k.data_ptr(), k_out.data_ptr(), k.shape[1]) if k is not None else (None, None, 0)
-        dev = q.device
-        with ops._on(dev):
-            rc = ops.load_library().sngguf_rotary(table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, *_strides(q), q_out.data_ptr(),
-                                                  *_strides(q_out), kp, kn, kt, kh, kop, kot, koh, ops._stream(dev))
-        ops._check(rc, "sngguf_rotary")
+        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, *_strides(q), q_out.data_ptr(), *_strides(q_out),
+                kp, kn, kt, kh, kop, kot, koh)
     return q_out, k_out
 
 
@@ -211,11 +231,7 @@ class PagedKVCache:
         the last page are passed over)."""
         k, v, slots = self._rows(k, v, slots, "PagedKVCache.write")
         if k.shape[0]:
-            dev = k.device
-            with ops._on(dev):
-                rc = ops.load_library().sngguf_cache_write(self._address, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), k.shape[0],
-                                                           ops._stream(dev))
-            ops._check(rc, "sngguf_cache_write")
+            _launch(self._index, "sngguf_cache_write", self._address, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), k.shape[0])
 
     def write_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: RotaryTable, slots: torch.Tensor,
                      inplace: bool = False) -> torch.Tensor:
@@ -232,32 +248,26 @@ class PagedKVCache:
             raise SnGgufError(f"{what}: in place needs the elements of a head next to each other")
         positions = _numbers(positions, torch.int64, tokens, what, "positions")
         _same_device(what, self._index, q, positions, table.turns)
-        out = q if inplace else torch.empty(q.shape, dtype=_BF16, device=q.device)
+        out = q if inplace else _new(q)
         if tokens:
-            dev = q.device
-            with ops._on(dev):
-                rc = ops.load_library().sngguf_cache_write_rotary(
-                    self._address, table._address, positions.data_ptr(), q.data_ptr(), q.shape[1], *_strides(q), out.data_ptr(), *_strides(out),
-                    k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), tokens, ops._stream(dev))
-            ops._check(rc, "sngguf_cache_write_rotary")
+            _launch(self._index, "sngguf_cache_write_rotary", self._address, table._address, positions.data_ptr(), q.data_ptr(), q.shape[1], *_strides(q),
+                    out.data_ptr(), *_strides(out), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), tokens)
         return out
 
     def read(self, slots: torch.Tensor):
         """``(k, v)`` of ``slots`` (int64 [tokens]) as bf16 [tokens][kv_heads][dim]; a slot outside the cache gives zeros."""
         slots = _numbers(slots, torch.int64, None, "PagedKVCache.read", "slots")
         _same_device("PagedKVCache.read", self._index, slots)
-        dev = self.k.device
-        k, v = (torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=_BF16, device=dev) for _ in range(2))
+        k = torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=_BF16, device=self.k.device)
+        v = torch.empty_like(k)
         if slots.shape[0]:
-            with ops._on(dev):
-                rc = ops.load_library().sngguf_cache_read(self._address, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(), ops._stream(dev))
-            ops._check(rc, "sngguf_cache_read")
+            _launch(self._index, "sngguf_cache_read", self._address, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr())
         return k, v
 
 
 def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=_BF16, device=q.device)
+        return _new(q)
     if out.dtype != _BF16 or out.shape != q.shape or out.get_device() != q.get_device() or out.stride(2) != 1 or _pieces(out) is not out:
         raise SnGgufError(f"{what}: out must be bf16 {tuple(q.shape)} on q's device, its rows of whole 16-byte pieces")
     return out
@@ -301,15 +311,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
     out = _output(out, q, what)
     sequences = ends_q.shape[0] - 1
     if tokens and sequences:
-        dev = q.device
-        lib = ops.load_library()
-        nbytes = lib.sngguf_attention_workspace_bytes(tokens, k.shape[0], sequences, heads, k.shape[1], dim)
-        with ops._on(dev), ops._whole_call(dev):
-            ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
-            rc = lib.sngguf_attention(q.data_ptr(), tokens, heads, *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), k.shape[0],
-                                      k.shape[1], dim, ends_q.data_ptr(), ends_k.data_ptr(), sequences, scale, int(causal), window,
-                                      out.data_ptr(), *_strides(out), ops._ptr(ws), nbytes, ops._stream(dev))
-        ops._check(rc, "sngguf_attention")
+        nbytes = ops.load_library().sngguf_attention_workspace_bytes(tokens, k.shape[0], sequences, heads, k.shape[1], dim)
+        _launch_with_workspace(q.device, nbytes, "sngguf_attention", q.data_ptr(), tokens, heads, *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
+                               *_strides(v), k.shape[0], k.shape[1], dim, ends_q.data_ptr(), ends_k.data_ptr(), sequences, scale, int(causal), window,
+                               out.data_ptr(), *_strides(out))
     return out
 
 
@@ -345,15 +350,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     _same_device(what, cache._index, q, pages, lens, ends_q)
     out = _output(out, q, what)
     if tokens and sequences:
-        dev = q.device
-        lib = ops.load_library()
         if ends_q is None:
             max_new = 1
-        nbytes = lib.sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
-        with ops._on(dev), ops._whole_call(dev):
-            ws = ops.pooled_workspace(dev, nbytes) if nbytes else None
-            rc = lib.sngguf_paged_attention(q.data_ptr(), tokens, heads, *_strides(q), cache._address, pages.data_ptr(), pages.stride(0), width,
-                                            lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), *_strides(out),
-                                            ops._ptr(ws), nbytes, ops._stream(dev))
-        ops._check(rc, "sngguf_paged_attention")
+        nbytes = ops.load_library().sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
+        _launch_with_workspace(q.device, nbytes, "sngguf_paged_attention", q.data_ptr(), tokens, heads, *_strides(q), cache._address, pages.data_ptr(),
+                               pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), *_strides(out))
     return out

@@ -16,6 +16,8 @@
 //    rows, and instruction t takes element t of each.
 // An 8-bit cache is widened to fp16 (whole numbers are exact there, the product with the scale is rounded to 11 bits; values are
 // within fp16 by the format) and multiplied in fp16, with p scaled by 2^12: p down to 2^-36 of the largest still counts.
+#include <type_traits>
+
 #include "attention.hpp"
 
 namespace sngguf {
@@ -436,76 +438,101 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     }
 }
 
-// Joins the splits of rows: WIDE: a workgroup a row, its wavefronts taking every fourth pair of splits; else a wavefront a row.
-// Lanes: 32 along the row's elements, two splits at a time.
+// Joins the splits of rows.  WIDE: a workgroup a row; else a wavefront a row.  Half a wavefront lies along the row's elements and
+// takes some splits at a time, all of whose words are asked for before any is used (behind the last split, those of the first
+// again: a branch around a load would have the loads wait for each other): the launch is one latency long, and what it
+// reads is little.
 template <int ROWS, int KEYS, int DT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionArgs a) {
     constexpr int PER = DT / 32;            // elements of a lane
-    __shared__ float part[WIDE ? kWaves : 1][DT + 1];
-    __shared__ float tops[kWaves];
+    constexpr int TEAMS = WIDE ? 2 * kWaves : 2;
+    __shared__ float part[WIDE ? TEAMS : 1][DT + 2];
     const AttentionBlock b = attention_block<ROWS, KEYS, true>(a, blockIdx.x);
     if (!b.there || b.splits < 2) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int half = lane >> 5, e = PER * (lane & 31);
+    const int half = lane >> 5, e = PER * (lane & 31), team = WIDE ? 2 * wave + half : half;
     const float* stats = a.partial + a.grid * ROWS * DT;
     const int64_t r0 = (int64_t)b.row_tile * ROWS, left = (int64_t)b.s.lq * a.group - r0;
     const int rows = left < ROWS ? (int)left : ROWS;
     // (the launch has as many workgroups as the caller takes for the most rows; more rows are taken in turn)
     for (int row = WIDE ? blockIdx.y : blockIdx.y * kWaves + wave; row < rows; row += gridDim.y * (WIDE ? 1 : kWaves)) {
-        auto slot = [&](int s) { return (b.slot + (int64_t)s * a.kv_heads) * ROWS + row; };
-        float top = -__builtin_inff();
-        for (int s = WIDE ? threadIdx.x : lane; s < b.splits; s += WIDE ? kThreads : 64) top = fmaxf(top, stats[slot(s) * 2]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if constexpr (WIDE) {
-            if (lane == 0) tops[wave] = top;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) top = fmaxf(top, tops[w]);
-        }
-        float o[PER], l = 0.f;
+        float o[PER], l = 0.f, m = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < PER; t++) o[t] = 0.f;
-#pragma unroll 8
-        for (int s = WIDE ? 2 * wave + half : half; s < b.splits; s += WIDE ? 2 * kWaves : 2) {
-            const int64_t at = slot(s);
-            const float ms = stats[at * 2], ls = stats[at * 2 + 1];
-            // (a split in which the row sees nothing holds zeros)
-            const float w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - top);
-            l += ls * w;
-            const float* p = a.partial + at * DT + e;
-            if constexpr (PER == 2) {
-                const float2 x = *reinterpret_cast<const float2*>(p);
-                o[0] += x.x * w, o[1] += x.y * w;
-            } else {
+        auto join = [&](auto chunk_) {
+            constexpr int CHUNK = decltype(chunk_)::value;
+            for (int s0 = team; s0 < b.splits; s0 += CHUNK * TEAMS) {
+                float ms[CHUNK], ls[CHUNK], x[CHUNK][PER];
 #pragma unroll
-                for (int t = 0; t < PER; t += 4) {
-                    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + t);
+                for (int k = 0; k < CHUNK; k++) {
+                    const int s = s0 + TEAMS * k;
+                    const int64_t at = (b.slot + (int64_t)(s < b.splits ? s : s0) * a.kv_heads) * ROWS + row;
+                    const float2 st = *reinterpret_cast<const float2*>(stats + at * 2);
+                    ms[k] = s < b.splits ? st.x : -__builtin_inff();
+                    ls[k] = st.y;
+                    const float* p = a.partial + at * DT + e;
+                    if constexpr (PER == 2) {
+                        const float2 v = *reinterpret_cast<const float2*>(p);
+                        x[k][0] = v.x, x[k][1] = v.y;
+                    } else {
 #pragma unroll
-                    for (int y = 0; y < 4; y++) o[t + y] += x[y] * w;
+                        for (int t = 0; t < PER; t += 4) {
+                            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p + t);
+#pragma unroll
+                            for (int y = 0; y < 4; y++) x[k][t + y] = v[y];
+                        }
+                    }
+                }
+                float top = m;
+#pragma unroll
+                for (int k = 0; k < CHUNK; k++) top = fmaxf(top, ms[k]);
+                if (top == -__builtin_inff()) continue;       // (splits in which the row sees nothing)
+                const float keep = __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < PER; t++) o[t] *= keep;
+#pragma unroll
+                for (int k = 0; k < CHUNK; k++) {
+                    const float w = __builtin_amdgcn_exp2f(ms[k] - top);
+                    l += ls[k] * w;
+#pragma unroll
+                    for (int t = 0; t < PER; t++) o[t] += x[k][t] * w;
                 }
             }
-        }
-        l += __shfl_xor(l, 32);
-#pragma unroll
-        for (int t = 0; t < PER; t++) o[t] += __shfl_xor(o[t], 32);
+        };
+        if (!WIDE || b.splits <= 2 * TEAMS) join(std::integral_constant<int, 2>());
+        else join(std::integral_constant<int, DT == 256 ? 8 : 16>());
+        // the teams' results: in LDS, or the wavefront's two halves
         if constexpr (WIDE) {
-            if (half == 0) {
 #pragma unroll
-                for (int t = 0; t < PER; t++) part[wave][e + t] = o[t];
-                if (lane == 0) part[wave][DT] = l;
-            }
+            for (int t = 0; t < PER; t++) part[team][e + t] = o[t];
+            if ((lane & 31) == 0) part[team][DT] = m, part[team][DT + 1] = l;
             __syncthreads();
             if (wave == 0) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int w = 0; w < TEAMS; w++) top = fmaxf(top, part[w][DT]);
                 l = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWaves; w++) l += part[w][DT];
+                for (int t = 0; t < PER; t++) o[t] = 0.f;
 #pragma unroll
-                for (int t = 0; t < PER; t++) {
-                    o[t] = 0.f;
+                for (int w = 0; w < TEAMS; w++) {
+                    const float f = part[w][DT] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(part[w][DT] - top);
+                    l += part[w][DT + 1] * f;
 #pragma unroll
-                    for (int w = 0; w < kWaves; w++) o[t] += part[w][e + t];
+                    for (int t = 0; t < PER; t++) o[t] += part[w][e + t] * f;
                 }
+            }
+        } else {
+            const float other = __shfl_xor(m, 32), top = fmaxf(m, other);
+            const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            l *= f;
+            l += __shfl_xor(l, 32);
+#pragma unroll
+            for (int t = 0; t < PER; t++) {
+                o[t] *= f;
+                o[t] += __shfl_xor(o[t], 32);
             }
         }
         if ((!WIDE || wave == 0) && half == 0 && e < a.dim) {
@@ -518,7 +545,7 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
 #pragma unroll
             for (int t = 0; t < PER; t += 2) *reinterpret_cast<uint32_t*>(out + t) = pack_bf16(o[t] * inv, o[t + 1] * inv);
         }
-        if constexpr (WIDE) __syncthreads();       // (part and tops are written again)
+        if constexpr (WIDE) __syncthreads();       // (part is written again)
     }
 }
 
