@@ -552,11 +552,11 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
 // tiles: (row tile, head) pairs at most; most_rows: of a tile, as far as is known
 int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, int64_t most_rows, hipStream_t stream) {
     const unsigned count = (unsigned)(most_rows < rows ? most_rows : rows);
-    // few rows have many splits each
+    // few rows have many splits each; many rows few: four rows a wavefront, as finding its place costs a workgroup more than they do
 #define SNGGUF_GO(R, K, D)                                                                                              \
     if (rows == R && keys == K && dim == D) {                                                                           \
         constexpr bool kWide = R <= 64;                                                                                 \
-        attention_combine_kernel<R, K, D, kWide><<<dim3((unsigned)tiles, kWide ? count : (count + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a); \
+        attention_combine_kernel<R, K, D, kWide><<<dim3((unsigned)tiles, kWide ? count : (count + 4 * kWaves - 1) / (4 * kWaves)), kThreads, 0, stream>>>(a); \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
 #define SNGGUF_GO_DIM(R, K) SNGGUF_GO(R, K, 64) SNGGUF_GO(R, K, 128) SNGGUF_GO(R, K, 256)
