@@ -113,55 +113,6 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     attention_keys(a, b.s, r0, r1, lo, hi);
     const int32_t back = b.s.lk - b.s.lq;
 
-    // ---- this lane's rows: their queries as operand fragments, and the keys that they see --------------------------------
-    op_t qf[CT][KS];
-    float c[CT];
-    int32_t first[CT], last[CT];
-    int64_t row_of[CT];
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        row_of[n] = r0 + 32 * (CT * wave + n) + col;
-        const int64_t rr = row_of[n] < r1 ? row_of[n] : r1 - 1;
-        int32_t head;
-        const int32_t token = attention_token(a, rr, head);
-        head += b.kv_head * a.group;
-        const int32_t place = back + token;
-        last[n] = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
-        first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
-        c[n] = a.scale_log2;
-        const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
-        u32x4_t raw[KS];
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int e = 16 * i + 8 * h;
-            raw[i] = e < a.dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
-        }
-        if constexpr (Q8) {
-            // bf16 -> fp16: scaled by a power of two that brings the row's largest element into [1, 2)
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t x = raw[i][j] & 0x7F807F80u;
-                    top = max(top, max(x >> 16, x & 0xFFFFu));
-                }
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const int ex = top == 0 ? 0 : (int)(top >> 7) - 127;
-#pragma unroll
-            for (int i = 0; i < KS; i++) {
-                u32x4_t w;
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[j] = pack_f16(__builtin_ldexpf(bf16lo_to_f32(raw[i][j]), -ex), __builtin_ldexpf(bf16hi_to_f32(raw[i][j]), -ex));
-                qf[n][i] = __builtin_bit_cast(op_t, w);
-            }
-            c[n] = fmaxf(__builtin_ldexpf(c[n], ex), 1.2e-38f);
-        } else {
-#pragma unroll
-            for (int i = 0; i < KS; i++) qf[n][i] = __builtin_bit_cast(op_t, raw[i]);
-        }
-    }
-
     // ---- this split's tiles -------------------------------------------------------------------------------------------
     int32_t s0 = lo / kKeys, s1 = (hi + kKeys - 1) / kKeys;
     {
@@ -281,6 +232,64 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     };
     typedef std::integral_constant<int, 0> First;
     typedef std::integral_constant<int, 1> Second;
+
+    // The first tile's keys are asked for before the queries are read, nothing else before both are there.
+    int32_t page_k = 0, page_v = 0;
+    if (count > 0) {
+        page_k = page_v = page_of(s0);
+        aim(0, s0, page_k);
+#pragma unroll
+        for (int j = 0; j < REQ; j++) request(0, lds0, j);
+    }
+
+    // ---- this lane's rows: their queries as operand fragments, and the keys that they see --------------------------------
+    op_t qf[CT][KS];
+    float c[CT];
+    int32_t first[CT], last[CT];
+    int64_t row_of[CT];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        row_of[n] = r0 + 32 * (CT * wave + n) + col;
+        const int64_t rr = row_of[n] < r1 ? row_of[n] : r1 - 1;
+        int32_t head;
+        const int32_t token = attention_token(a, rr, head);
+        head += b.kv_head * a.group;
+        const int32_t place = back + token;
+        last[n] = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
+        first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
+        c[n] = a.scale_log2;
+        const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
+        u32x4_t raw[KS];
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int e = 16 * i + 8 * h;
+            raw[i] = e < a.dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
+        }
+        if constexpr (Q8) {
+            // bf16 -> fp16: scaled by a power of two that brings the row's largest element into [1, 2)
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t x = raw[i][j] & 0x7F807F80u;
+                    top = max(top, max(x >> 16, x & 0xFFFFu));
+                }
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+            const int ex = top == 0 ? 0 : (int)(top >> 7) - 127;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                u32x4_t w;
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = pack_f16(__builtin_ldexpf(bf16lo_to_f32(raw[i][j]), -ex), __builtin_ldexpf(bf16hi_to_f32(raw[i][j]), -ex));
+                qf[n][i] = __builtin_bit_cast(op_t, w);
+            }
+            c[n] = fmaxf(__builtin_ldexpf(c[n], ex), 1.2e-38f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < KS; i++) qf[n][i] = __builtin_bit_cast(op_t, raw[i]);
+        }
+    }
 
     // ---- fragments ---------------------------------------------------------------------------------------------------
     // keys: row 32 half + col, piece 2 ks + h; values: keys 32 half + 16 x + 8 y + 4 h + (lane % 16) / 4 (the rows of one transposing
@@ -458,7 +467,6 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ * (NS - 2)) : "memory");
             __syncthreads();
         };
-        int32_t page_k = page_of(s0), page_v = page_k;
         auto aim_stage = [&](int32_t i) {
             const int32_t tk = s0 + (i < count ? i : count - 1), tv = s0 + (i <= count ? i : count) - 1;
             page_v = page_k;
@@ -466,21 +474,18 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
             aim(0, tk, page_k);
             aim(1, tv, page_v);
         };
-        aim(0, s0, page_k);
-#pragma unroll
-        for (int j = 0; j < REQ; j++) request(0, lds0, j);
         if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < QN; i++) widen(0, lds0, i);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
 #pragma unroll
         for (int n = 1; n < NS; n++) {
             aim_stage(n);
 #pragma unroll
             for (int j = 0; j < 2 * REQ; j++) request(j / REQ, lds0 + n * kStage, j % REQ);
         }
-        if constexpr (!Q8) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ * (NS - 1)) : "memory");     // the keys of tile 0
-        __syncthreads();
         At at = at_stage(0);
         scores(sa, at, 0);
         scores(sb, at, 1);
@@ -538,10 +543,11 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
 
     // ---- out: acc[n][t][i]: row row_of[n], element 32 t + 8 (i / 4) + 4 h + i % 4 --------------------------------------------
 #pragma unroll
-    for (int n = 0; n < CT; n++) {
-        l[n] += other_half(l[n]);
-        if (row_of[n] >= r1) continue;
-        if (b.splits > 1) {
+    for (int n = 0; n < CT; n++) l[n] += other_half(l[n]);
+    if (b.splits > 1) {
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            if (row_of[n] >= r1) continue;
             const int64_t at = b.slot * ROWS + (row_of[n] - r0);
 #pragma unroll
             for (int t = 0; t < DTILES; t++)
@@ -553,22 +559,42 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
                 st[0] = m[n];
                 st[1] = l[n];
             }
-            continue;
         }
+        return;
+    }
+    // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
+    // each of its row's pieces
+    constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
+    static_assert(32 * W * OUT <= NS * 2 * TILE, "room");
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
         const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-        int32_t head;
-        const int32_t token = attention_token(a, row_of[n], head);
-        head += b.kv_head * a.group;
-        bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head;
+        uint8_t* to = lds + wave * 32 * OUT;
 #pragma unroll
         for (int t = 0; t < DTILES; t++)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int e = 32 * t + 2 * i + 4 * h;
-                if (e < a.dim)
-                    *reinterpret_cast<u32x2_t*>(out + e) =
-                        u32x2_t{pack_bf16(acc[n][t][i] * inv, acc[n][t][i + 1] * inv), pack_bf16(acc[n][t][i + 2] * inv, acc[n][t][i + 3] * inv)};
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<u32x2_t*>(to + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
+                    u32x2_t{pack_bf16(acc[n][t][i] * inv, acc[n][t][i + 1] * inv), pack_bf16(acc[n][t][i + 2] * inv, acc[n][t][i + 3] * inv)};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int LANES = DT / 8;                  // of a row
+        const int e = 8 * (lane % LANES);
+#pragma unroll
+        for (int i = 0; i < 32 / (64 / LANES); i++) {
+            const int row = lane / LANES + 64 / LANES * i;
+            const int64_t r = r0 + 32 * (CT * wave + n) + row;
+            if (r < r1 && e < a.dim) {
+                int32_t head;
+                const int32_t token = attention_token(a, r, head);
+                head += b.kv_head * a.group;
+                *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
+                    *reinterpret_cast<const u32x4_t*>(to + row * OUT + 2 * e);
             }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
