@@ -81,7 +81,7 @@ void set_table(RotaryCacheArgs& a, const sngguf_rotary_table* t, const int64_t* 
 constexpr int64_t kMostKeys = kMost - 65536;          // of a sequence: a few tiles more still have 32-bit numbers
 
 constexpr int kRowsLeast = 2, kRowsKeys = 128;        // key tiles that a split has at least; keys of a tile
-constexpr int kTilesLeast = 4, kTilesKeys = 64;
+constexpr int kTilesLeast = 16, kTilesKeys = 64;     // (a workgroup costs as much as five tiles before its first and behind its last)
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
@@ -102,7 +102,7 @@ Launch plan(int64_t tiles, int64_t keys, int dim, int rows, int want, int64_t le
     p.rows = rows;
     p.tiles = tiles;
     p.want = want;
-    const bool split = tiles < want && keys > least;
+    const bool split = tiles < want && keys >= 2 * least;
     p.grid = tiles + (split ? want : 0);
     p.partial_bytes = split ? p.grid * rows * (dim + 2) * 4 : 0;
     return p;
@@ -111,13 +111,17 @@ Launch plan(int64_t tiles, int64_t keys, int dim, int rows, int want, int64_t le
 // Row tiles of all sequences at most: every sequence's last one may hold a single row
 int64_t row_tiles(int64_t tokens, int64_t sequences, int64_t group, int rows) { return (tokens * group + sequences * (rows - 1)) / rows; }
 
-// The kernel for many rows: 256 a workgroup unless that leaves most of a sequence's only tile empty.  (Workgroups of equal work
-// that leave a last round nearly empty are not split: every workgroup costs some microseconds before its first tile and
-// behind its last, and 2500 queries over 3000 keys, 320 workgroups, took 193 us as 960 instead of 173.)
+// The kernel for many rows: 256 a workgroup (eight wavefronts that share tiles), or 128 where a sequence's only tile would be
+// mostly empty, or where 256-row workgroups leave two of five compute units idle and there are no keys to split (one prompt
+// of 1024 tokens and 8 heads of keys: 29 us against 33; of 1500: 43 against 42; of 4096: 150 against 135).
+// Workgroups of equal work that leave a last round nearly empty are not split: 2500 queries over 3000 keys, 320 workgroups, took 193 us
+// as 960 instead of 173.
 Launch plan_many(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
-    const int64_t group = heads / kv_heads;
-    const int rows = dim <= 128 && tokens * group >= 512 * sequences ? 256 : 128;
-    return plan(kv_heads * row_tiles(tokens, sequences, group, rows), keys / kTilesKeys + 1, dim, rows, many_at_a_time(rows, dim), kTilesLeast);
+    const int64_t group = heads / kv_heads, key_tiles = keys / kTilesKeys + 1;
+    const bool wide = dim <= 128 && tokens * group >= 512 * sequences &&
+                      (key_tiles >= 2 * kTilesLeast || kv_heads * row_tiles(tokens, sequences, group, 256) >= 160);
+    const int rows = wide ? 256 : 128;
+    return plan(kv_heads * row_tiles(tokens, sequences, group, rows), key_tiles, dim, rows, many_at_a_time(rows, dim), kTilesLeast);
 }
 
 struct PagedPlan {

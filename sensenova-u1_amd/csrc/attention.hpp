@@ -90,6 +90,18 @@ __device__ __forceinline__ void attention_tiles(const AttentionArgs& a, const At
     key_tiles = (uint32_t)(hi > lo ? hi - lo : 1);
 }
 
+// x of the lanes up to this one added up, in the vector unit (row shifts, then a row's last value handed on)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(x), 63); }
+
 struct AttentionBlock {
     AttentionSequence s;
     int32_t seq, row_tile, split, splits, kv_head;
@@ -116,13 +128,15 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
                 attention_tiles<ROWS, KEYS>(a, attention_sequence(a, base + lane), rt, kt);
                 mine = (uint64_t)rt * kt;
             }
+            // (64 numbers of 25 bits add up within 32)
+            if (__ballot(mine >> 25) == 0) {
+                mine = wave_total((uint32_t)mine);
+            } else {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                mine += __shfl_xor((unsigned long long)mine, o);
-                rt += __shfl_xor(rt, o);
+                for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor((unsigned long long)mine, o);
             }
             total += mine;
-            tiles += rt;
+            tiles += wave_total(rt);
         }
         // the last split of a row tile is half as long as the others on average: so many workgroups less, or the device would have
         // a few to do in a second round
@@ -144,15 +158,7 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
             if (splits < 1) splits = 1;
         }
         const uint32_t slots = rt * splits, mine = COMBINE ? rt : slots;
-        uint32_t sum = mine, sum_slots = slots;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(sum, o), y = __shfl_up(sum_slots, o);
-            if (lane >= o) {
-                sum += x;
-                sum_slots += y;
-            }
-        }
+        const uint32_t sum = wave_scan(mine), sum_slots = COMBINE ? wave_scan(slots) : sum;
         const uint64_t hit = __ballot(want >= before + sum - mine && want < before + sum);
         if (hit) {
             const int l = __builtin_ctzll(hit);
@@ -164,7 +170,9 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
             const uint32_t within = want - first;
             const uint32_t t = COMBINE ? within : within / (uint32_t)b.splits;
             b.split = COMBINE ? 0 : (int32_t)(within - t * (uint32_t)b.splits);
-            // the last rows of a causal sequence see the most keys: first
+            // the last rows of a causal sequence see the most keys: first.  (Sequences follow one another all the same: longest first over
+            // all of them was 8 % faster for four prompts of 1000 tokens and 10 % slower for eight of 300 to 1700, whose keys and values
+            // then no longer stay in an XCD's cache.)
             b.row_tile = (int32_t)(tiles - 1 - t);
             b.slot = ((int64_t)first_slot + (int64_t)t * b.splits + b.split) * a.kv_heads + b.kv_head;
             b.s.q0 = (uint32_t)__builtin_amdgcn_readlane((int)mine_s.q0, l);     // (both below 2^31)
