@@ -51,8 +51,9 @@ __device__ __forceinline__ f16x2_t whole_pair(uint32_t flipped) {
 
 }  // namespace
 
-// Workgroups that a compute unit takes at a time (as many wavefronts a SIMD: four a workgroup)
-constexpr int rows_workgroups(int dt, int nt) { return nt * dt <= 128 ? 3 : nt * dt <= 256 ? 2 : 1; }
+// Workgroups that a compute unit takes at a time (as many wavefronts a SIMD: four a workgroup).  Heads of 256 elements: one, as two
+// spill (32 single tokens over 4000 in bf16: 193 us against 297).
+constexpr int rows_workgroups(int dt, int nt) { return nt * dt <= 128 ? 3 : nt * dt <= 256 && dt < 256 ? 2 : 1; }
 
 // DT: elements of a head, rounded up (FULL: exactly).  NT: 16-row tiles.
 template <int DT, bool FULL, bool Q8, int NT>
