@@ -1,7 +1,7 @@
 // Attention of many rows: whole prompts over their own packed keys and values, and chunks of new tokens over a paged cache.
 //
-// A workgroup takes 128 CT rows of one sequence and key / value head (row = token x query heads of the group, so the heads that
-// share keys and values share their tiles), four wavefronts of 32 CT rows, and walks over tiles of 64 keys in a ring of LDS
+// A workgroup takes 128 or 256 rows of one sequence and key / value head (row = token x query heads of the group, so the heads
+// that share keys and values share their tiles), 32 for each wavefront, and walks over tiles of 64 keys in a ring of LDS
 // stages.  One pass with a running maximum m and sum l, in base 2.  Bound by the matrix instructions (32 x 32 x 16):
 //  * S^T = K Q^T: a lane holds sixteen of a row's 32 scores (row = lane % 32).  Register i of lane half h is key 8 (i / 4) +
 //    4 h + i % 4;
@@ -89,16 +89,16 @@ template <int DT> struct Tile {
 
 enum { kPacked = 0, kPaged = 1, kPagedQ8 = 2 };
 
-// W: wavefronts.  CT: 32-row tiles of each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
-template <int DT, int SOURCE, int W, int CT, int NS>
-__global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
+// W: wavefronts, of 32 rows each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
+template <int DT, int SOURCE, int W, int NS>
+__global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
-    constexpr int ROWS = 32 * W * CT;
+    constexpr int ROWS = 32 * W;
     constexpr int TILE = Tile<DT>::kBytes, RB = Tile<DT>::kRowBlock, PB = Tile<DT>::kBlocks;
     constexpr int KS = DT / 16, DTILES = DT / 32;
     constexpr int VF = 2 * DTILES, NF = VF + KS;       // operand fragments of a step: of values, in all
-    constexpr int NP = 8 * CT;                         // pairs of weights of a step that a lane forms
+    constexpr int NP = 8;                              // pairs of weights of a step that a lane forms
     constexpr float kLimit = Q8 ? 32768.f : 1e9f;      // (fp16 weights are scaled by 2^12)
     constexpr float kUp = Q8 ? 12.f : 0.f;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // [stage][keys, values]
@@ -126,18 +126,13 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     const int32_t all_last = a.causal && place0 < b.s.lk - 1 ? place0 : b.s.lk - 1;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
-    f32x16_t acc[CT][DTILES];
-    float m[CT], l[CT], nb[CT];      // nb: what is added to a scaled score, kUp - m
+    f32x16_t acc[DTILES];
 #pragma unroll
-    for (int n = 0; n < CT; n++) {
-        m[n] = -__builtin_inff();
-        nb[n] = __builtin_inff();    // nothing known yet: whatever is formed with it is set right
-        l[n] = 0.f;
+    for (int t = 0; t < DTILES; t++)
 #pragma unroll
-        for (int t = 0; t < DTILES; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) acc[n][t][i] = 0.f;
-    }
+        for (int i = 0; i < 16; i++) acc[t][i] = 0.f;
+    float m = -__builtin_inff(), l = 0.f;
+    float nb = __builtin_inff();     // what is added to a scaled score, kUp - m; nothing known yet: whatever is formed with it is set right
 
     // ---- tiles into LDS ------------------------------------------------------------------------------------------------
     // Rows behind the last key are the last key's: masked, but finite wherever the keys are.
@@ -145,8 +140,8 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     constexpr int LOAD = kKeys / W;                    // rows of a tile that a wavefront brings, 8 or 16
     constexpr int REQ = LOAD / 8 * PB;                 // requests for them: blocks
     constexpr int QP = DT / 16;                        // 8-bit: 16-byte pieces of a row
-    constexpr int QN = LOAD * QP / 64;                 // ... a lane has of each tile
-    static_assert(LOAD % 8 == 0 && (!Q8 || LOAD * QP % 64 == 0), "whole requests");
+    constexpr int QN = (LOAD * QP + 63) / 64;          // ... a lane has of each tile
+    static_assert(LOAD % 8 == 0, "whole requests");
     u32x4_t held[2][Q8 ? QN : 1];
     uint16_t held_scale[2][Q8 ? QN : 1];
     // this lane's part of a request: row and piece of a block
@@ -161,7 +156,7 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
         rows_there[half] = spare;
 #pragma unroll
         for (int j = 0; j < REQ; j++) {
-            const int i = j / PB, p = j % PB, row = 8 * i + crow < spare ? 8 * i + crow : spare;
+            const int i = j / PB, p = j % PB, at = 8 * i + crow, row = at < spare ? at : spare;
             // (pieces behind dim: the first, whose elements meet queries of zero, or are never stored)
             coff[half][j] = (uint32_t)(2 * row * (int32_t)(half ? v_stride : k_stride)) + (64 * p + 8 * cpiece < a.dim ? 128 * p + 16 * cpiece : 0);
         }
@@ -183,7 +178,7 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
         const int32_t base = tile * kKeys + LOAD * wave, lead = base < most ? base : most;
         const int32_t spare = most - lead;             // rows behind the first that there are
         if constexpr (SOURCE == kPacked) {
-            from[half] = uniform_ptr((half ? v_base : k_base) + 2 * lead * (half ? v_stride : k_stride));
+            from[half] = uniform_ptr((half ? v_base : k_base) + 2 * (int64_t)lead * (half ? v_stride : k_stride));
             set_offsets(half, spare);
         } else {
             const int64_t at_page = (int64_t)page * a.kv_heads + b.kv_head;
@@ -195,8 +190,10 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
                 const uint16_t* scales = (half ? a.v_scales : a.k_scales) + (at_page * (a.dim >> 5) << a.page_shift) + (lead & page_mask);
 #pragma unroll
                 for (int i = 0; i < QN; i++) {
-                    const int p = lane + 64 * i, row = p / QP < spare ? p / QP : spare;
-                    int piece = p % QP;
+                    // neighbouring lanes have neighbouring rows, which lie in different banks when they are written to LDS (piece by
+                    // piece they would all lie in the same ones: a chunk of 1024 over 30000 took 568 us instead of 540)
+                    const int p = lane + 64 * i, row = p % LOAD < spare ? p % LOAD : spare;
+                    int piece = p / LOAD;
                     piece = 16 * piece < a.dim ? piece : 0;
                     held[half][i] = *reinterpret_cast<const u32x4_t*>(from[half] + row * a.dim + 16 * piece);
                     held_scale[half][i] = scales[((piece >> 1) << a.page_shift) + row];
@@ -212,7 +209,8 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     // 8-bit tiles: widened from the registers that the request filled
     auto widen = [&](int half, uint32_t stage, int i) {
         if constexpr (Q8) {
-            const int p = lane + 64 * i, row = LOAD * wave + p / QP, piece = p % QP;
+            const int p = lane + 64 * i, row = LOAD * wave + p % LOAD, piece = p / LOAD;
+            if (LOAD * QP % 64 != 0 && piece >= QP) return;
             const u32x4_t w = held[half][i];
             const _Float16 d1 = __builtin_bit_cast(_Float16, held_scale[half][i]);
             const f16x2_t d = {d1, d1};
@@ -242,22 +240,18 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
         for (int j = 0; j < REQ; j++) request(0, lds0, j);
     }
 
-    // ---- this lane's rows: their queries as operand fragments, and the keys that they see --------------------------------
-    op_t qf[CT][KS];
-    float c[CT];
-    int32_t first[CT], last[CT];
-    int64_t row_of[CT];
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        row_of[n] = r0 + 32 * (CT * wave + n) + col;
-        const int64_t rr = row_of[n] < r1 ? row_of[n] : r1 - 1;
+    // ---- this lane's row: its query as operand fragments, and the keys that it sees --------------------------------
+    const int64_t my_row = r0 + 32 * wave + col;
+    op_t qf[KS];
+    float c = a.scale_log2;
+    int32_t first, last;
+    {
         int32_t head;
-        const int32_t token = attention_token(a, rr, head);
+        const int32_t token = attention_token(a, my_row < r1 ? my_row : r1 - 1, head);
         head += b.kv_head * a.group;
         const int32_t place = back + token;
-        last[n] = a.causal && place < b.s.lk - 1 ? place : b.s.lk - 1;
-        first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
-        c[n] = a.scale_log2;
+        last = a.causal && place < most ? place : most;
+        first = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
         const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
         u32x4_t raw[KS];
 #pragma unroll
@@ -282,12 +276,12 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
                 u32x4_t w;
 #pragma unroll
                 for (int j = 0; j < 4; j++) w[j] = pack_f16(__builtin_ldexpf(bf16lo_to_f32(raw[i][j]), -ex), __builtin_ldexpf(bf16hi_to_f32(raw[i][j]), -ex));
-                qf[n][i] = __builtin_bit_cast(op_t, w);
+                qf[i] = __builtin_bit_cast(op_t, w);
             }
-            c[n] = fmaxf(__builtin_ldexpf(c[n], ex), 1.2e-38f);
+            c = fmaxf(__builtin_ldexpf(c, ex), 1.2e-38f);
         } else {
 #pragma unroll
-            for (int i = 0; i < KS; i++) qf[n][i] = __builtin_bit_cast(op_t, raw[i]);
+            for (int i = 0; i < KS; i++) qf[i] = __builtin_bit_cast(op_t, raw[i]);
         }
     }
 
@@ -318,65 +312,48 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     };
 
     // ---- pieces of a step ----------------------------------------------------------------------------------------------
-    typedef f32x16_t scores_t[CT];
-    typedef uint32_t weights_t[CT][2][4];     // [16 keys][pair]
-    auto clear = [&](scores_t& s) {
-#pragma unroll
-        for (int n = 0; n < CT; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-    };
-    auto mask = [&](scores_t& s, int32_t key0) {
+    typedef uint32_t weights_t[2][4];     // [16 keys][pair]
+    auto mask = [&](f32x16_t& s, int32_t key0) {
         if (key0 + 31 > all_last || key0 < all_first) {
 #pragma unroll
-            for (int n = 0; n < CT; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int32_t key = key0 + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (key < first[n] || key > last[n]) s[n][i] = -__builtin_inff();
-                }
+            for (int i = 0; i < 16; i++) {
+                const int32_t key = key0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                if (key < first || key > last) s[i] = -__builtin_inff();
+            }
         }
     };
-    auto raise_pair = [&](const scores_t& s, const float (&add)[CT], int p, float& p0, float& p1) {
-        const int n = p / 8, i = 2 * (p % 8);
-        p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c[n], add[n]));
-        p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], c[n], add[n]));
+    auto raise_pair = [&](const f32x16_t& s, float add, int p, float& p0, float& p1) {
+        p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p], c, add));
+        p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p + 1], c, add));
     };
-    auto pack_pair = [&](weights_t& w, float (&sum)[CT], int p, float p0, float p1) {
-        const int n = p / 8, i = 2 * (p % 8);
+    auto pack_pair = [&](weights_t& w, float& sum, int p, float p0, float p1) {
         if constexpr (Q8) {
-            w[n][i / 8][(i / 2) % 4] = pack_f16(p0, p1);
-            sum[n] += p0 + p1;
+            w[p / 4][p % 4] = pack_f16(p0, p1);
+            sum += p0 + p1;
         } else {
             // the rounded weights are summed
             const uint32_t both = pack_bf16(p0, p1);
-            w[n][i / 8][(i / 2) % 4] = both;
-            sum[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), sum[n], false);
+            w[p / 4][p % 4] = both;
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), sum, false);
         }
     };
     // maximum, sums and weights from the scores
-    auto set_right = [&](const scores_t& s, weights_t& w, float (&sum)[CT]) {
-        float add[CT];
+    auto set_right = [&](const f32x16_t& s, weights_t& w, float& sum) {
+        float top = s[0];
 #pragma unroll
-        for (int n = 0; n < CT; n++) {
-            float top = s[n][0];
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        top = fmaxf(top, other_half(top));
+        top = fmaxf(top * c, m);
+        const bool none = top == -__builtin_inff();
+        const float base = none ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - base), add = kUp - base;
+        m = top;
+        nb = none ? __builtin_inff() : add;
+        l *= keep;
 #pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, s[n][i]);
-            top = fmaxf(top, other_half(top));
-            top = fmaxf(top * c[n], m[n]);
-            const bool none = top == -__builtin_inff();
-            const float base = none ? 0.f : top;
-            const float keep = __builtin_amdgcn_exp2f(m[n] - base);
-            m[n] = top;
-            add[n] = kUp - base;
-            nb[n] = none ? __builtin_inff() : add[n];
-            l[n] *= keep;
+        for (int t = 0; t < DTILES; t++)
 #pragma unroll
-            for (int t = 0; t < DTILES; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) acc[n][t][i] *= keep;
-            sum[n] = 0.f;
-        }
+            for (int i = 0; i < 16; i++) acc[t][i] *= keep;
+        sum = 0.f;
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             float p0, p1;
@@ -384,29 +361,18 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
             pack_pair(w, sum, p, p0, p1);
         }
     };
-    auto settle = [&](const scores_t& s, weights_t& w, float (&sum)[CT]) {
-        bool fine = true;
-#pragma unroll
-        for (int n = 0; n < CT; n++) fine = fine && sum[n] <= kLimit;
-        if (__any(!fine)) set_right(s, w, sum);
-#pragma unroll
-        for (int n = 0; n < CT; n++) l[n] += sum[n];
-    };
-    auto weights_operand = [&](const weights_t& w, int n, int x) -> op_t {
-        return __builtin_bit_cast(op_t, u32x4_t{w[n][x][0], w[n][x][1], w[n][x][2], w[n][x][3]});
-    };
+    auto weights_operand = [&](const weights_t& w, int x) -> op_t { return __builtin_bit_cast(op_t, u32x4_t{w[x][0], w[x][1], w[x][2], w[x][3]}); };
 
     op_t ring[4];
     // One step: values of keys 32 half ... of a stage times w0; weights of s into w1; scores of keys 32 half ... into s1.
     // The first three fragments are in the ring; the next step's are fetched by its end, from the same stage or from `next`, behind
     // the barrier that this needs.  beside(f): what else is done beside fragment f.
-    auto step = [&](scores_t& s, scores_t& s1, const weights_t& w0, weights_t& w1, const At& at, const At& next, int32_t key0, auto half_, auto beside) {
+    auto step = [&](f32x16_t& s, f32x16_t& s1, const weights_t& w0, weights_t& w1, const At& at, const At& next, int32_t key0, auto half_, auto beside) {
         constexpr int half = decltype(half_)::value;
         mask(s, key0);
-        clear(s1);
-        float sum[CT];
 #pragma unroll
-        for (int n = 0; n < CT; n++) sum[n] = 0.f;
+        for (int i = 0; i < 16; i++) s1[i] = 0.f;
+        float sum = 0.f;
         // (a pair is packed one fragment after it was raised: the exponential's result is a while coming)
         constexpr int PF = (NP + NF - 1) / NF;         // pairs of a fragment at most
         float up[2][PF][2];
@@ -422,11 +388,8 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
                 if constexpr (g < VF) ring[g & 3] = value_fragment(at, half, g % DTILES, g / DTILES);
                 else if constexpr (g < NF) ring[g & 3] = key_fragment(at, half, g - VF);
                 else ring[g & 3] = value_fragment(next, half ^ 1, (g - NF) % DTILES, (g - NF) / DTILES);
-#pragma unroll
-                for (int n = 0; n < CT; n++) {
-                    if constexpr (f < VF) acc[n][f % DTILES] = mfma(ring[f & 3], weights_operand(w0, n, f / DTILES), acc[n][f % DTILES]);
-                    else s1[n] = mfma(ring[f & 3], qf[n][f - VF], s1[n]);
-                }
+                if constexpr (f < VF) acc[f % DTILES] = mfma(ring[f & 3], weights_operand(w0, f / DTILES), acc[f % DTILES]);
+                else s1 = mfma(ring[f & 3], qf[f - VF], s1);
                 constexpr int p0 = f * NP / NF, p1 = (f + 1) * NP / NF;
 #pragma unroll
                 for (int p = p0; p < p1; p++) raise_pair(s, nb, p, up[f & 1][p - p0][0], up[f & 1][p - p0][1]);
@@ -434,30 +397,23 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
             },
             std::make_integer_sequence<int, NF>());
         pack_of(std::integral_constant<int, NF - 1>());
-        settle(s, w1, sum);
+        if (__any(!(sum <= kLimit))) set_right(s, w1, sum);
+        l += sum;
     };
-    auto scores = [&](scores_t& s, const At& at, int half) {
-        clear(s);
+    auto scores = [&](const At& at, int half) -> f32x16_t {
+        f32x16_t s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const op_t k = key_fragment(at, half, ks);
-#pragma unroll
-            for (int n = 0; n < CT; n++) s[n] = mfma(k, qf[n][ks], s[n]);
-        }
+        for (int ks = 0; ks < KS; ks++) s = mfma(key_fragment(at, half, ks), qf[ks], s);
+        return s;
     };
     auto values = [&](const weights_t& w, const At& at, int half) {
 #pragma unroll
-        for (int f = 0; f < VF; f++) {
-            const op_t v = value_fragment(at, half, f >> 1, f & 1);
-#pragma unroll
-            for (int n = 0; n < CT; n++) acc[n][f >> 1] = mfma(v, weights_operand(w, n, f & 1), acc[n][f >> 1]);
-        }
+        for (int f = 0; f < VF; f++) acc[f % DTILES] = mfma(value_fragment(at, half, f % DTILES, f / DTILES), weights_operand(w, f / DTILES), acc[f % DTILES]);
     };
 
     if (count > 0) {
-        scores_t sa, sb;
         weights_t wa, wb;
-        float sum[CT];
+        float sum;
         // A stage: keys of tile i, values of tile i - 1 (behind the last tile: of the last, read by nobody, so that the loop neither
         // asks whether there are more nor counts what is under way)
         constexpr uint32_t kStage = 2 * TILE, kRing = NS * kStage;
@@ -487,16 +443,14 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
             for (int j = 0; j < 2 * REQ; j++) request(j / REQ, lds0 + n * kStage, j % REQ);
         }
         At at = at_stage(0);
-        scores(sa, at, 0);
-        scores(sb, at, 1);
+        f32x16_t sa = scores(at, 0), sb = scores(at, 1);
         if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < 2 * QN; i++) widen(i / QN, lds0 + kStage, i % QN);
         }
         mask(sa, s0 * kKeys);
         set_right(sa, wa, sum);
-#pragma unroll
-        for (int n = 0; n < CT; n++) l[n] += sum[n];
+        l += sum;
         wait_stage();
         uint32_t stage = kStage;                       // of tile i's keys
         uint32_t ahead = NS == 2 ? 0u : after(kStage); // the last one asked for
@@ -535,29 +489,25 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
         values(wa, at, 0);
         mask(sb, (s1 - 1) * kKeys + 32);
         set_right(sb, wb, sum);
-#pragma unroll
-        for (int n = 0; n < CT; n++) l[n] += sum[n];
+        l += sum;
         values(wb, at, 1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no request outlives the workgroup's LDS
     }
 
-    // ---- out: acc[n][t][i]: row row_of[n], element 32 t + 8 (i / 4) + 4 h + i % 4 --------------------------------------------
-#pragma unroll
-    for (int n = 0; n < CT; n++) l[n] += other_half(l[n]);
+    // ---- out: acc[t][i]: this lane's row, element 32 t + 8 (i / 4) + 4 h + i % 4 ---------------------------------------------
+    l += other_half(l);
     if (b.splits > 1) {
-#pragma unroll
-        for (int n = 0; n < CT; n++) {
-            if (row_of[n] >= r1) continue;
-            const int64_t at = b.slot * ROWS + (row_of[n] - r0);
+        if (my_row < r1) {
+            const int64_t at = b.slot * ROWS + (my_row - r0);
 #pragma unroll
             for (int t = 0; t < DTILES; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4_t*>(a.partial + at * DT + 32 * t + 2 * i + 4 * h) = f32x4_t{acc[n][t][i], acc[n][t][i + 1], acc[n][t][i + 2], acc[n][t][i + 3]};
+                    *reinterpret_cast<f32x4_t*>(a.partial + at * DT + 32 * t + 2 * i + 4 * h) = f32x4_t{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
             if (h == 0) {
                 float* st = a.partial + a.grid * ROWS * DT + at * 2;
-                st[0] = m[n];
-                st[1] = l[n];
+                st[0] = m;
+                st[1] = l;
             }
         }
         return;
@@ -565,62 +515,52 @@ __global__ __launch_bounds__(64 * W, CT == 1 && DT <= 128 ? 2 : 1) void attentio
     // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
     // each of its row's pieces
     constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
-    static_assert(32 * W * OUT <= NS * 2 * TILE, "room");
+    static_assert(ROWS * OUT <= NS * 2 * TILE, "room");
     __syncthreads();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint8_t* room = lds + wave * 32 * OUT;
 #pragma unroll
-    for (int n = 0; n < CT; n++) {
-        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-        uint8_t* to = lds + wave * 32 * OUT;
+    for (int t = 0; t < DTILES; t++)
 #pragma unroll
-        for (int t = 0; t < DTILES; t++)
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<u32x2_t*>(room + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
+                u32x2_t{pack_bf16(acc[t][i] * inv, acc[t][i + 1] * inv), pack_bf16(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
+    __syncthreads();
+    constexpr int LANES = DT / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
+    const int e = 8 * (lane % LANES);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<u32x2_t*>(to + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
-                    u32x2_t{pack_bf16(acc[n][t][i] * inv, acc[n][t][i + 1] * inv), pack_bf16(acc[n][t][i + 2] * inv, acc[n][t][i + 3] * inv)};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
-        constexpr int LANES = DT / 8;                  // of a row
-        const int e = 8 * (lane % LANES);
-#pragma unroll
-        for (int i = 0; i < 32 / (64 / LANES); i++) {
-            const int row = lane / LANES + 64 / LANES * i;
-            const int64_t r = r0 + 32 * (CT * wave + n) + row;
-            if (r < r1 && e < a.dim) {
-                int32_t head;
-                const int32_t token = attention_token(a, r, head);
-                head += b.kv_head * a.group;
-                *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
-                    *reinterpret_cast<const u32x4_t*>(to + row * OUT + 2 * e);
-            }
+    for (int i = 0; i < 32 / AT_ONCE; i++) {
+        const int row = lane / LANES + AT_ONCE * i;
+        const int64_t r = r0 + 32 * wave + row;
+        if (r < r1 && e < a.dim) {
+            int32_t head;
+            const int32_t token = attention_token(a, r, head);
+            head += b.kv_head * a.group;
+            *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
+                *reinterpret_cast<const u32x4_t*>(room + row * OUT + 2 * e);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// rows: of a workgroup, 128 or (up to 128 elements) 256
+// dim: of the kernel, 64, 128 or 256; rows: of a workgroup, 128 or (up to 128 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
-#define SNGGUF_GO(D, S, W, C, N)                                                                                        \
-    if (dim == D && source == S && rows == 32 * W * C) {                                                                \
+#define SNGGUF_GO(D, S, W, N)                                                                                           \
+    if (dim == D && source == S && rows == 32 * W) {                                                                    \
         constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                   \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, C, N>), \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, N>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_tiles_kernel<D, S, W, C, N><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                     \
+        attention_tiles_kernel<D, S, W, N><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                        \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
-#define SNGGUF_GO_PLAIN(D, W, C, N) SNGGUF_GO(D, kPacked, W, C, N) SNGGUF_GO(D, kPaged, W, C, N)
-    SNGGUF_GO_PLAIN(64, 4, 1, 3)
-    SNGGUF_GO_PLAIN(64, 4, 2, 3)
-    SNGGUF_GO_PLAIN(128, 4, 1, 2)
-    SNGGUF_GO_PLAIN(128, 8, 1, 3)
-    SNGGUF_GO_PLAIN(256, 4, 1, 2)
-    SNGGUF_GO(64, kPagedQ8, 4, 1, 2)
-    SNGGUF_GO(64, kPagedQ8, 4, 2, 2)
-    SNGGUF_GO(128, kPagedQ8, 4, 1, 2)
-    SNGGUF_GO(128, kPagedQ8, 8, 1, 2)
-    SNGGUF_GO(256, kPagedQ8, 4, 1, 2)
-#undef SNGGUF_GO_PLAIN
+    // (three stages where a compute unit has room for them; 8-bit tiles pass through registers and need two)
+#define SNGGUF_GO_DIM(D, W, N) SNGGUF_GO(D, kPacked, W, N) SNGGUF_GO(D, kPaged, W, N) SNGGUF_GO(D, kPagedQ8, W, 2)
+    SNGGUF_GO_DIM(64, 4, 3)
+    SNGGUF_GO_DIM(64, 8, 3)
+    SNGGUF_GO_DIM(128, 4, 2)
+    SNGGUF_GO_DIM(128, 8, 3)
+    SNGGUF_GO_DIM(256, 4, 2)
+#undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
 }
