@@ -449,7 +449,8 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
     constexpr int TEAMS = WIDE ? 2 * kWaves : 2;
     __shared__ float part[WIDE ? TEAMS : 1][DT + 2];
     const AttentionBlock b = attention_block<ROWS, KEYS, true>(a, blockIdx.x);
-    if (!b.there || b.splits < 2) return;
+    // (lengths that are none can name more splits than there were workgroups)
+    if (!b.there || b.splits < 2 || b.slot + (int64_t)(b.splits - 1) * a.kv_heads >= a.grid) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int half = lane >> 5, e = PER * (lane & 31), team = WIDE ? 2 * wave + half : half;
     const float* stats = a.partial + a.grid * ROWS * DT;

@@ -22,8 +22,9 @@ def attention(q, k, v, causal=True, window=0, scale=None, operand=torch.bfloat16
     ``most`` bounds the error of a kernel that sums in 32 bits, rounds the weights (``operand`` float16: keys and values too) to
     ``operand`` and the result to bf16.  With A = sum_j p_j |v_j|, S = max_j scale sum_d |q_d k_jd| of a row, u = the operand's half
     step, e = 2^-24, n keys:
-    * a score is off by dim e S from the sum and 4 e S from its scaling (operand float16: u S more from its key), which changes
-      each weight by twice that at most (its own score and the normaliser's);
+    * a score is off by d = dim e S from the sum and 4 e S from its scaling (operand float16: u S more from its key).  A weight
+      p_j / sum_i p_i becomes p_j exp(d_j) / sum_i p_i exp(d_i), |d_j| <= d, so it changes by a factor between exp(-2 d) and
+      exp(2 d): by exp(2 d) - 1 of itself at most (2 d, to first order, where d is small, which it is not for scores of thousands);
     * exp2 is off by 2^-21, n-term sums of weights and products by n e, each weight's rounding by u (float16: the value's too, and
       2^-36 absolute of the largest weight for n weights below its smallest step);
     * the result is rounded to bf16: 2^-8 of its value."""
@@ -47,10 +48,10 @@ def attention(q, k, v, causal=True, window=0, scale=None, operand=torch.bfloat16
         spread = p @ vh.abs()
         size = (q[:, h].abs() @ kh.abs().T * scale).masked_fill(~seen, 0.0).amax(1, keepdim=True)
         n = seen.sum(1, keepdim=True)
-        off = 2 * (dim + 4) * e * size + 2.0 ** -21 + 2 * n * e + u
-        most[:, h] = off * spread
+        d = ((dim + 4) * e + (u if operand == torch.float16 else 0.0)) * size
+        most[:, h] = (torch.expm1(2 * d) + 2.0 ** -21 + 2 * n * e + u) * spread
         if operand == torch.float16:
-            most[:, h] += (2 * u * size + u) * spread + n * 2.0 ** -36 * vh.abs().amax()
+            most[:, h] += u * spread + n * 2.0 ** -36 * vh.abs().amax()
         most[:, h] = 1.01 * (most[:, h] + 2.0 ** -8 * (out[:, h].abs() + most[:, h])) + 1e-37
     return out, most
 

@@ -296,3 +296,223 @@ def test_calls_that_are_refused(dev):
         with pytest.raises(ops.SnGgufError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_lengths_that_are_none_where_keys_are_split(dev):
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = _values(gen, 30, 4, 64).to(dev), _values(gen, 6000, 2, 64).to(dev), _values(gen, 6000, 2, 64).to(dev)
+    for n in (1, 40):
+        ends_q, ends_k = torch.tensor([0, 30] * n, dtype=torch.int32, device=dev), torch.tensor([0, 6000] * n, dtype=torch.int32, device=dev)
+        assert prompt_attention(q, k, v, ends_q, ends_k).shape == q.shape
+    cache = PagedKVCache.empty(8, 2, 64, 64, ops.Q8_0, dev)
+    cache.write(k[:512], v[:512], torch.arange(512, device=dev))
+    table = torch.arange(8, dtype=torch.int32, device=dev).repeat(80, 8).contiguous()
+    ends = torch.tensor([0, 30] * 40 + [0], dtype=torch.int32, device=dev)
+    for max_new in (0, 1, 30):
+        assert paged_attention(q, cache, table, torch.full((80,), 4096, dtype=torch.int32, device=dev), ends, max_new=max_new).shape == q.shape
+    torch.cuda.synchronize()
+
+
+def test_no_keys_and_no_queries(dev):
+    q = torch.ones((3, 4, 64), dtype=torch.bfloat16, device=dev)
+    none = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=dev)
+    ends = torch.tensor([0, 1, 3], dtype=torch.int32, device=dev)
+    assert bool((prompt_attention(q, none, none, ends, torch.zeros(3, dtype=torch.int32, device=dev)) == 0).all())
+    assert prompt_attention(q[:0], none, none, torch.zeros(3, dtype=torch.int32, device=dev)).shape == (0, 4, 64)
+    assert prompt_attention(q, none, none, torch.zeros(1, dtype=torch.int32, device=dev)).shape == q.shape
+    cache = PagedKVCache.empty(2, 2, 16, 64, ops.BF16, dev)
+    lens = torch.zeros(3, dtype=torch.int32, device=dev)
+    assert bool((paged_attention(q, cache, torch.zeros((3, 0), dtype=torch.int32, device=dev), lens) == 0).all())
+    assert paged_attention(q[:0], cache, torch.zeros((0, 4), dtype=torch.int32, device=dev), lens[:0]).shape == (0, 4, 64)
+
+
+def test_paged_rows_behind_the_last_sequence_are_left(dev):
+    gen = torch.Generator().manual_seed(13)
+    for qt in (ops.Q8_0, ops.BF16):
+        cache = PagedKVCache.empty(4, 2, 16, 64, qt, dev)
+        cache.write(_values(gen, 64, 2, 64).to(dev), _values(gen, 64, 2, 64).to(dev), torch.arange(64, device=dev))
+        table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=dev)
+        lens = torch.tensor([20, 32], dtype=torch.int32, device=dev)
+        for new in (1, 18):
+            q = _values(gen, 2 * new + 5, 4, 64).to(dev)
+            out = torch.full_like(q, 9.0)
+            paged_attention(q, cache, table, lens, torch.tensor([0, new, 2 * new], dtype=torch.int32, device=dev), out=out)
+            assert bool((out[2 * new:] == 9).all()) and not bool((out[:2 * new] == 9).any(1).any(1).all())
+
+
+@BOTH
+def test_offsets_past_32_bits(dev, qt):
+    """A cache whose last pages lie behind 2^32 bytes (8 bits) or 2^33 (bf16) of each half."""
+    pages, page, heads, dim = 2 ** 17 + 3, 64, 4, 128
+    cache = PagedKVCache.empty(pages, heads, page, dim, qt, dev)
+    gen = torch.Generator().manual_seed(14)
+    k, v, q = _values(gen, 190, heads, dim), _values(gen, 190, heads, dim), _values(gen, 41, 8, dim)
+    table = torch.tensor([[pages - 1, 0, pages - 3, 7]], dtype=torch.int32)
+    t = torch.arange(190)
+    slots = (table[0].long()[t // page] * page + t % page).to(dev)
+    cache.write(k.to(dev), v.to(dev), slots)
+    got = cache.read(slots)
+    held = [ao.quantised(x)[2] if qt == ops.Q8_0 else x.double() for x in (k, v)]
+    assert all(torch.equal(a.double().cpu(), b.float().to(torch.bfloat16).double()) for a, b in zip(got, held))
+    for new in (1, 41):
+        out = paged_attention(q[:new].to(dev), cache, table.to(dev), torch.tensor([190], dtype=torch.int32, device=dev), torch.tensor([0, new], dtype=torch.int32, device=dev))
+        want, most = ao.attention(q[:new], *held, operand=torch.float16 if qt == ops.Q8_0 else torch.bfloat16)
+        _close(out, want, most)
+
+
+def test_long_strides_of_packed_keys(dev):
+    """Keys far apart: the last lies behind 2^32 bytes."""
+    apart = 2 ** 24
+    room = torch.zeros((200 * apart,), dtype=torch.bfloat16, device=dev)
+    gen = torch.Generator().manual_seed(15)
+    q, k, v = _values(gen, 200, 2, 64), _values(gen, 200, 1, 64), _values(gen, 200, 1, 64)
+    kd = room.as_strided((200, 1, 64), (apart, 64, 1)).copy_(k)
+    vd = room.as_strided((200, 1, 64), (apart, 64, 1), 128).copy_(v)
+    got = prompt_attention(q.to(dev), kd, vd, _ends([200], dev))
+    want, most = ao.attention(q, k, v)
+    _close(got, want, most)
+
+
+# ---- together, captured, on other streams ---------------------------------------------------------------------------------
+
+
+def _step(s, cache, table_of_angles):
+    from sensenova_u1_amd import rotary
+
+    q = cache.write_rotary(s["q"], s["k"], s["v"], s["positions"], table_of_angles, s["slots"])
+    out = paged_attention(q, cache, s["pages"], s["lens"], s["ends"], max_new=s["max_new"])
+    q2, k2 = rotary(s["q"], s["k"], s["positions"], table_of_angles)
+    own = prompt_attention(q2, k2, s["v"], s["ends"])
+    return out, own, cache.read(s["slots"])
+
+
+@BOTH
+@pytest.mark.parametrize("new,max_new", [([1] * 5, 1), ([1, 40, 1, 300, 7], 0)])
+def test_captured_steps_replay_with_new_lengths_pages_and_values(dev, qt, new, max_new):
+    """One captured step of a layer, replayed over growing contexts with the program's own work between the replays: every replay is what
+    the same calls give outside the graph."""
+    from sensenova_u1_amd import RotaryTable
+
+    gen = torch.Generator().manual_seed(16)
+    tokens, page, width = sum(new), 16, 160
+    angles = RotaryTable.for_model(128, 1e6, device=dev)
+    caches = [PagedKVCache.empty(5 * width, 2, page, 128, qt, dev) for _ in range(2)]
+    for c in caches:
+        for t in (c.k, c.v, c.k_scale, c.v_scale):
+            if t is not None:
+                t.zero_()
+    s = {"q": torch.zeros((tokens, 8, 128), dtype=torch.bfloat16, device=dev), "k": torch.zeros((tokens, 2, 128), dtype=torch.bfloat16, device=dev),
+         "v": torch.zeros((tokens, 2, 128), dtype=torch.bfloat16, device=dev), "positions": torch.zeros(tokens, dtype=torch.int64, device=dev),
+         "slots": torch.zeros(tokens, dtype=torch.int64, device=dev), "pages": torch.zeros((5, width), dtype=torch.int32, device=dev),
+         "lens": torch.ones(5, dtype=torch.int32, device=dev), "ends": _ends(new, dev), "max_new": max_new}
+    lens = torch.zeros(5, dtype=torch.int64)
+    _step(s, caches[0], angles)          # (kernels are loaded)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = _step(s, caches[0], angles)
+    for replay in range(4):
+        order = torch.randperm(5 * width, generator=gen).view(5, width) if replay == 0 else order
+        grown = torch.tensor(new) + (torch.randint(0, 200, (5,), generator=gen) if replay else 0)
+        at, pos, slots = 0, [], []
+        for i, n in enumerate(new):
+            first = int(lens[i] + grown[i]) - n
+            p = torch.arange(first, first + n)
+            pos.append(p)
+            slots.append(order[i][p // page] * page + p % page)
+        lens += grown
+        for name, value in (("positions", torch.cat(pos)), ("slots", torch.cat(slots)), ("pages", order.int()), ("lens", lens.int()),
+                            ("q", _values(gen, tokens, 8, 128)), ("k", _values(gen, tokens, 2, 128)), ("v", _values(gen, tokens, 2, 128))):
+            s[name].copy_(value)
+        graph.replay()
+        eager = _step(s, caches[1], angles)
+        torch.cuda.synchronize()
+        for a, b in zip((captured[0], captured[1], *captured[2]), (eager[0], eager[1], *eager[2])):
+            assert torch.equal(a, b), replay
+        for a, b in ((caches[0].k, caches[1].k), (caches[0].v_scale, caches[1].v_scale)):
+            assert a is None or torch.equal(a, b)
+
+
+def test_two_graphs_and_other_streams_do_not_share_scratch(dev):
+    """Splits of keys write partial results: of two graphs replayed on two streams, and of eager calls on a third."""
+    gen = torch.Generator().manual_seed(17)
+    work = []
+    for n in (9000, 7000, 5000):
+        q, k, v = _values(gen, 4, 8, 128).to(dev), _values(gen, n, 2, 128).to(dev), _values(gen, n, 2, 128).to(dev)
+        cache = PagedKVCache.empty(-(-n // 64), 2, 64, 128, ops.Q8_0, dev)
+        cache.write(k, v, torch.arange(n, device=dev))
+        pages = torch.arange(-(-n // 64), dtype=torch.int32, device=dev)[None]
+        args = (q, cache, pages, torch.tensor([n], dtype=torch.int32, device=dev), _ends([4], dev))
+        work.append((args, paged_attention(*args), (q, k, v, _ends([4], dev), _ends([n], dev)), prompt_attention(q, k, v, _ends([4], dev), _ends([n], dev))))
+    torch.cuda.synchronize()
+    graphs = []
+    for args, _, packed, _ in work[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = (paged_attention(*args), prompt_attention(*packed))
+        graphs.append((g, outs))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    eager = []
+    for _ in range(20):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager.append((paged_attention(*work[2][0]), prompt_attention(*work[2][2])))
+    torch.cuda.synchronize()
+    for (_, outs), (_, a, _, b) in zip(graphs, work):
+        assert torch.equal(outs[0], a) and torch.equal(outs[1], b)
+    assert all(torch.equal(x, work[2][1]) and torch.equal(y, work[2][3]) for x, y in eager)
+
+
+def test_results_do_not_change_from_call_to_call(dev):
+    gen = torch.Generator().manual_seed(18)
+    q, k, v = _values(gen, 700, 8, 128).to(dev), _values(gen, 700, 2, 128, True).to(dev), _values(gen, 700, 2, 128).to(dev)
+    first = prompt_attention(q, k, v, _ends([300, 400], dev))
+    assert all(torch.equal(prompt_attention(q, k, v, _ends([300, 400], dev)), first) for _ in range(10))
+
+
+def test_scores_that_rise_from_key_to_key(dev):
+    """The maximum is passed again and again, by little and by much: weights, sums and results are set right each time."""
+    gen = torch.Generator().manual_seed(19)
+    lk = 700
+    for rise in (0.05, 0.5, 5.0, -0.5):
+        k = (_values(gen, lk, 2, 128).float() * 0.1)
+        k[:, :, 0] = torch.arange(lk)[:, None] * rise
+        k = k.to(torch.bfloat16)
+        q = (_values(gen, lk, 4, 128).float() * 0.1)
+        q[:, :, 0] = 8.0
+        q, v = q.to(torch.bfloat16), _values(gen, lk, 2, 128)
+        got = prompt_attention(q.to(dev), k.to(dev), v.to(dev), _ends([lk], dev))
+        want, most = ao.attention(q, k, v)
+        _close(got, want, most, f"rise {rise}")
+        for qt in (ops.Q8_0, ops.BF16):
+            cache = PagedKVCache.empty(44, 2, 16, 128, qt, dev)
+            cache.write(k.to(dev), v.to(dev), torch.arange(lk, device=dev))
+            kk, vv = [ao.quantised(x)[2] if qt == ops.Q8_0 else x for x in (k, v)]
+            for new in (1, 200):
+                got = paged_attention(q[-new:].to(dev), cache, torch.arange(44, dtype=torch.int32, device=dev)[None], torch.tensor([lk], dtype=torch.int32, device=dev), _ends([new], dev))
+                want, most = ao.attention(q[-new:], kk, vv, operand=torch.float16 if qt == ops.Q8_0 else torch.bfloat16)
+                _close(got, want, most, f"rise {rise}, {new} new, type {qt}")
+
+
+def test_many_small_weights_beside_one_large(dev):
+    """30000 keys of weight about 2^-25 of the largest: together a thousandth of the sum, each below fp16's smallest step of it."""
+    gen = torch.Generator().manual_seed(20)
+    lk = 30000
+    k = torch.zeros((lk, 1, 64))
+    k[5, 0, 0] = 17.33 / 8.0
+    q = torch.zeros((1, 2, 64))
+    q[..., 0] = 8.0 * 8.0
+    v = torch.ones((lk, 1, 64))
+    v[5] = -1.0
+    q, k, v = (x.to(torch.bfloat16) for x in (q, k, v))
+    for qt in (ops.Q8_0, ops.BF16):
+        cache = PagedKVCache.empty(469, 1, 64, 64, qt, dev)
+        cache.write(k.to(dev), v.to(dev), torch.arange(lk, device=dev))
+        kk, vv = [ao.quantised(x)[2] if qt == ops.Q8_0 else x for x in (k, v)]
+        got = paged_attention(q.to(dev), cache, torch.arange(469, dtype=torch.int32, device=dev)[None], torch.tensor([lk], dtype=torch.int32, device=dev))
+        want, most = ao.attention(q, kk, vv, operand=torch.float16 if qt == ops.Q8_0 else torch.bfloat16)
+        _close(got, want, most)
