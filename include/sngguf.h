@@ -457,8 +457,8 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
  * `window` of them.  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, those of out not
  * written.  heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads).  dim: a multiple of 32 up to 256.
  * q, k, v, out: rows of whole 16-byte pieces.  Scores, maxima and sums are fp32, the weights are rounded to bf16 for the product
- * with v.  A key or value that is not finite reaches every query of its sequence that sees it, and may reach those that share
- * a tile of 64 keys with it; other sequences' never do.
+ * with v.  A key or value that is not finite reaches the queries that see it and no others (their rows are done a second time, key by key: slowly).
+ * out must not overlap q, k or v.
  * workspace (16-byte aligned) of sngguf_attention_workspace_bytes(...): partial results where few rows meet many keys; with
  * less, or NULL, such a call is slower.  Nothing in it outlives the call.
  */
@@ -475,7 +475,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
  * one query a sequence, in order.  Causal.  max_new: the most queries of any sequence as far as the caller knows, 0 if it does
  * not (a wrong value costs time only).  Lengths beyond the table's width count as its width; page numbers outside the cache are
  * read as the nearest page.  table: rows table_stride apart, table_width numbers each.  max_keys (of the workspace): table_width *
- * page_size, below 2^31 - 65536.  An 8-bit cache is multiplied in fp16,
+ * page_size, below 2^31 - 65536.  With a window, pages in front of every query's are not used.  An 8-bit cache is multiplied in fp16,
  * its values rounded to 11 bits.  Everything else as sngguf_attention.
  */
 int64_t sngguf_paged_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads, int64_t dim);

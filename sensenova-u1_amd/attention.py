@@ -90,6 +90,16 @@ def _strides(x: torch.Tensor):
     return (t if x.shape[0] > 1 else 0), (h if x.shape[1] > 1 else 0)
 
 
+def _apart(x: torch.Tensor) -> bool:
+    """Whether no two rows of ``x`` share an element (as they do in an expanded tensor)."""
+    reach = x.shape[2]
+    for stride, size in sorted((x.stride(i), x.shape[i]) for i in (0, 1) if x.shape[i] > 1):
+        if stride < reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
 def _numbers(x: torch.Tensor, dtype: torch.dtype, count: Optional[int], what: str, name: str) -> torch.Tensor:
     if x.dtype != dtype or x.dim() != 1 or (count is not None and x.shape[0] != count):
         raise SnGgufError(f"{what}: {name} must be {dtype} [{count if count is not None else 'n'}], got {x.dtype} {tuple(x.shape)}")
@@ -148,7 +158,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """Queries and keys turned by their positions: ``(q, k)``, new tensors or with ``inplace`` the given ones.
 
     q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None.  positions: int64 [tokens].  A model whose head
-    has parts with positions of their own calls it on views of the parts."""
+    has parts with positions of their own calls it on views of the parts.  In place, no two rows may share an element."""
     q0, k0 = q, k
     q = _heads(q, "rotary", "q")
     tokens, heads, dim = q.shape
@@ -161,6 +171,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             raise SnGgufError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
     if inplace and (q is not q0 or k is not k0):
         raise SnGgufError("rotary: in place needs the elements of a head next to each other")
+    if inplace and not (_apart(q) and (k is None or (_apart(k) and (k.data_ptr() != q.data_ptr() or not k.numel())))):
+        raise SnGgufError("rotary: in place needs rows that share no element")
     q_out = q if inplace else _new(q)
     k_out = k if inplace or k is None else _new(k)
     if tokens and heads:
@@ -244,8 +256,8 @@ class PagedKVCache:
         tokens = k.shape[0]
         if q.shape[0] != tokens or q.shape[2] != self.dim:
             raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
-        if inplace and q is not q0:
-            raise SnGgufError(f"{what}: in place needs the elements of a head next to each other")
+        if inplace and (q is not q0 or not _apart(q) or (q.data_ptr() in (k.data_ptr(), v.data_ptr()) and q.numel())):
+            raise SnGgufError(f"{what}: in place needs rows that share no element, the elements of a head next to each other")
         positions = _numbers(positions, torch.int64, tokens, what, "positions")
         _same_device(what, self._index, q, positions, table.turns)
         out = q if inplace else _new(q)
@@ -265,11 +277,13 @@ class PagedKVCache:
         return k, v
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str) -> torch.Tensor:
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, *others: torch.Tensor) -> torch.Tensor:
     if out is None:
         return _new(q)
     if out.dtype != _BF16 or out.shape != q.shape or out.get_device() != q.get_device() or out.stride(2) != 1 or _pieces(out) is not out:
         raise SnGgufError(f"{what}: out must be bf16 {tuple(q.shape)} on q's device, its rows of whole 16-byte pieces")
+    if out.numel() and (not _apart(out) or out.data_ptr() in [x.data_ptr() for x in (q, *others)]):
+        raise SnGgufError(f"{what}: out must not overlap itself or an input")
     return out
 
 
@@ -293,8 +307,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
 
     q [tokens][heads][dim], k and v [keys][kv_heads][dim], ``heads`` a multiple of ``kv_heads``, ``dim`` a multiple of 32 up to
     256.  Causal: the last query of a sequence stands at its last key, and none sees a key behind its own place; ``window`` > 0: only the last
-    ``window`` keys up to it.  A query that sees nothing gives zeros.  ``scale`` defaults to dim ** -0.5.  Rows of ``out`` behind
-    the last sequence are not written."""
+    ``window`` keys up to it.  A query that sees nothing gives zeros, and keys and values that a query does not see
+    have no part in its result, whatever they hold.  ``scale`` defaults to dim ** -0.5.  Rows of ``out`` behind the last sequence are not
+    written; ``out`` overlaps no input."""
     what = "prompt_attention"
     q, k, v = _pieces(_heads(q, what, "q")), _pieces(_heads(k, what, "k")), _pieces(_heads(v, what, "v"))
     tokens, heads, dim = q.shape
@@ -308,7 +323,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
     if ends_q.shape[0] < 1:
         raise SnGgufError(f"{what}: ends_q has no entry")
     _same_device(what, q.get_device(), k, v, ends_q, ends_k)
-    out = _output(out, q, what)
+    out = _output(out, q, what, k, v)
     sequences = ends_q.shape[0] - 1
     if tokens and sequences:
         nbytes = ops.load_library().sngguf_attention_workspace_bytes(tokens, k.shape[0], sequences, heads, k.shape[1], dim)
@@ -325,7 +340,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     pages: int32 [sequences][width], the pages of each sequence in order.  lens: int32 [sequences], its tokens in all.  The queries
     of sequence i are ``ends_q[i] : ends_q[i + 1]`` (int32 [sequences + 1]) and stand at its last places; without ``ends_q`` every
     sequence has one, in order.  ``max_new``: the most queries of any sequence, where the program knows it (0: unknown); it
-    decides which kernels are launched and never what they compute.  ``scale``, ``window``, ``out``: as ``prompt_attention``."""
+    decides which kernels are launched and never what they compute.  With a ``window``, the pages in front of it may be anyone's.
+    ``scale``, ``window``, ``out``: as ``prompt_attention``."""
     what = "paged_attention"
     q = _pieces(_heads(q, what, "q"))
     tokens, heads, dim = q.shape
@@ -348,7 +364,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     elif tokens != sequences:
         raise SnGgufError(f"{what}: {tokens} queries of {sequences} sequences need ends_q")
     _same_device(what, cache._index, q, pages, lens, ends_q)
-    out = _output(out, q, what)
+    out = _output(out, q, what, cache.k, cache.v)
     if tokens and sequences:
         if ends_q is None:
             max_new = 1

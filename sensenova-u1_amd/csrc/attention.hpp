@@ -210,6 +210,97 @@ __device__ __forceinline__ void attention_keys(const AttentionArgs& a, const Att
     }
 }
 
+enum { kPacked = 0, kPaged = 1, kPagedQ8 = 2 };       // where keys and values lie
+
+// Row r over the keys [lo, hi) again, key by key, by one wavefront, and its result to where it goes (a row of `out`, or of a split's
+// partial result for tiles of ROWS rows).  The matrix products multiply a value that a row does not see by a weight of zero,
+// which takes it away unless it is an infinity or a NaN; and their weights may be as large as the limit above which they are set
+// right, too much for values near the end of bf16.  So a row whose result is not finite is done again: what it sees counts, and
+// nothing else.  A lane has a key's score, then all lanes lie along the elements of one value after the other; weights are
+// scaled by 2^-31, so that no sum of values leaves fp32.  (UP: by which power of two the other splits' are.)
+template <int DT, int SOURCE, int ROWS, int UP>
+__device__ __forceinline__ void attention_row_again(const AttentionArgs& a, const AttentionBlock& b, int64_t r, int32_t lo, int32_t hi) {
+    constexpr int PER = DT / 64;            // elements of a lane: lane, lane + 64, ...
+    const int lane = threadIdx.x & 63;
+    int32_t head;
+    const int32_t token = attention_token(a, r, head), place = b.s.lk - b.s.lq + token;
+    head += b.kv_head * a.group;
+    const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
+    if (a.causal && place + 1 < hi) hi = place + 1;
+    if (a.window && place - a.window + 1 > lo) lo = (int32_t)(place - a.window + 1);
+    float m = -__builtin_inff(), l = 0.f, o[PER];
+#pragma unroll
+    for (int t = 0; t < PER; t++) o[t] = 0.f;
+    for (int64_t base = lo; base < hi; base += 64) {
+        const int count = hi - base < 64 ? (int)(hi - base) : 64;
+        const int64_t key = base + (lane < count ? lane : count - 1);
+        // elements in front of the key's and the value's first; 8-bit: also of the scales
+        int64_t k_at, v_at, scale_at = 0;
+        if constexpr (SOURCE == kPacked) {
+            k_at = (b.s.k0 + key) * a.k_token + (int64_t)b.kv_head * a.k_head;
+            v_at = (b.s.k0 + key) * a.v_token + (int64_t)b.kv_head * a.v_head;
+        } else {
+            int64_t page = a.table[(int64_t)b.seq * a.table_stride + (key >> a.page_shift)];
+            page = (page < 0 ? 0 : page >= a.pages ? a.pages - 1 : page) * a.kv_heads + b.kv_head;
+            const int64_t row = key & ((1 << a.page_shift) - 1);
+            k_at = v_at = ((page << a.page_shift) + row) * a.dim;
+            scale_at = (page * (a.dim >> 5) << a.page_shift) + row;
+        }
+        float s = 0.f;
+        for (int e = 0; e < a.dim; e++) {
+            float k;
+            if constexpr (SOURCE == kPagedQ8)
+                k = (float)static_cast<const int8_t*>(a.k_pages)[k_at + e] * f16_to_f32(a.k_scales[scale_at + ((int64_t)(e >> 5) << a.page_shift)]);
+            else
+                k = bf16_to_f32((SOURCE == kPacked ? a.k : static_cast<const bf16_t*>(a.k_pages))[k_at + e]);
+            s = __builtin_fmaf(k, bf16_to_f32(q[e]), s);
+        }
+        s = lane < count ? s * a.scale_log2 : -__builtin_inff();
+        float top = s;
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        top = fmaxf(top, m);
+        const float from = top == -__builtin_inff() ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - from);
+        m = top;
+        const float p = __builtin_amdgcn_exp2f(s - from - 31.f);
+        l = l * keep + p;                   // (of this lane's keys)
+#pragma unroll
+        for (int t = 0; t < PER; t++) o[t] *= keep;
+        for (int j = 0; j < count; j++) {
+            const float pj = __shfl(p, j);
+            const int64_t at = __shfl((long long)v_at, j), sc = SOURCE == kPagedQ8 ? __shfl((long long)scale_at, j) : 0;
+#pragma unroll
+            for (int t = 0; t < PER; t++) {
+                const int e = lane + 64 * t;
+                if (e >= a.dim) continue;
+                float v;
+                if constexpr (SOURCE == kPagedQ8)
+                    v = (float)static_cast<const int8_t*>(a.v_pages)[at + e] * f16_to_f32(a.v_scales[sc + ((int64_t)(e >> 5) << a.page_shift)]);
+                else
+                    v = bf16_to_f32((SOURCE == kPacked ? a.v : static_cast<const bf16_t*>(a.v_pages))[at + e]);
+                o[t] = __builtin_fmaf(pj, v, o[t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+    const int64_t part = b.slot * ROWS + r - (int64_t)b.row_tile * ROWS;
+    constexpr float kBack = (float)(1ull << (31 + UP));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int t = 0; t < PER; t++) {
+        const int e = lane + 64 * t;
+        if (e >= a.dim) continue;
+        if (b.splits > 1) a.partial[part * DT + e] = o[t] * kBack;
+        else a.out[(b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e] = f32_to_bf16(o[t] * inv);
+    }
+    if (b.splits > 1 && lane == 0) {
+        float* st = a.partial + a.grid * ROWS * DT + part * 2;
+        st[0] = m;
+        st[1] = l * kBack;
+    }
+}
+
 int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim, int64_t tiles, int64_t most_rows, hipStream_t stream);
 
 }  // namespace sngguf

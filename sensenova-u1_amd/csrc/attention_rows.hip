@@ -372,6 +372,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     }
 
     // ---- the four wavefronts' results --------------------------------------------------------------------------------
+    uint32_t again = 0;                     // this wavefront's rows that are not finite: four of each 16
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         l[n] += __shfl_xor(l[n], 16);
@@ -399,6 +400,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         // thread: row tid / 16 of the tile, elements VP (tid % 16) ...
         const int row = threadIdx.x >> 4, e = VP * (threadIdx.x & 15);
         const int64_t r = r0 + 16 * n + row;
+        float odd = 0.f;
         if (r < r1 && e < dim) {
             float o[VP];
 #pragma unroll
@@ -415,6 +417,9 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
                 const float wm = stats[(w * ROWS + 16 * n + row) * 2];
                 if (wm != -__builtin_inff()) rl += stats[(w * ROWS + 16 * n + row) * 2 + 1] * __builtin_amdgcn_exp2f(wm - rm);
             }
+            odd = rl * 0.f;
+#pragma unroll
+            for (int t = 0; t < VP; t++) odd = __builtin_fmaf(o[t], 0.f, odd);
             if (b.splits > 1) {
                 float* part = a.partial + (b.slot * ROWS + 16 * n + row) * DT + e;
 #pragma unroll
@@ -427,15 +432,24 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
             } else {
                 const float inv = rl == 0.f ? 0.f : 1.f / rl;
                 int32_t head;
-            const int32_t token = attention_token(a, r, head);
-            head += b.kv_head * a.group;
+                const int32_t token = attention_token(a, r, head);
+                head += b.kv_head * a.group;
                 bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e;
 #pragma unroll
                 for (int t = 0; t < VP; t += 4)
                     *reinterpret_cast<u32x2_t*>(out + t) = u32x2_t{pack_bf16(o[t] * inv, o[t + 1] * inv), pack_bf16(o[t + 2] * inv, o[t + 3] * inv)};
             }
         }
+        const uint64_t odd_lanes = __ballot(odd != 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) again |= (odd_lanes >> (16 * i) & 0xFFFFu) ? 1u << (4 * n + i) : 0u;
         __syncthreads();
+    }
+    // (this wavefront's stores above stay in front: these rows are written twice, and the second is what is left)
+    while (again) {
+        const int i = __builtin_ctz(again);
+        again &= again - 1;
+        attention_row_again<DT, Q8 ? kPagedQ8 : kPaged, ROWS, Q8 ? 12 : 0>(a, b, r0 + 16 * (i >> 2) + 4 * wave + (i & 3), s0 * kKeys, end);
     }
 }
 

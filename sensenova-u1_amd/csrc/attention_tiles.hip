@@ -87,8 +87,6 @@ template <int DT> struct Tile {
 
 }  // namespace
 
-enum { kPacked = 0, kPaged = 1, kPagedQ8 = 2 };
-
 // W: wavefronts, of 32 rows each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
 template <int DT, int SOURCE, int W, int NS>
 __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
@@ -496,6 +494,13 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
 
     // ---- out: acc[t][i]: this lane's row, element 32 t + 8 (i / 4) + 4 h + i % 4 ---------------------------------------------
     l += other_half(l);
+    float odd = l * 0.f;
+#pragma unroll
+    for (int t = 0; t < DTILES; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) odd = __builtin_fmaf(acc[t][i], 0.f, odd);
+    const uint64_t odd_lanes = __ballot(odd != 0.f && my_row < r1);
+    uint32_t again = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);      // the wavefront's rows that are not finite
     if (b.splits > 1) {
         if (my_row < r1) {
             const int64_t at = b.slot * ROWS + (my_row - r0);
@@ -510,35 +515,42 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
                 st[1] = l;
             }
         }
-        return;
-    }
-    // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
-    // each of its row's pieces
-    constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
-    static_assert(ROWS * OUT <= NS * 2 * TILE, "room");
-    __syncthreads();
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint8_t* room = lds + wave * 32 * OUT;
+    } else {
+        // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
+        // each of its row's pieces
+        constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
+        static_assert(ROWS * OUT <= NS * 2 * TILE, "room");
+        __syncthreads();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint8_t* room = lds + wave * 32 * OUT;
 #pragma unroll
-    for (int t = 0; t < DTILES; t++)
+        for (int t = 0; t < DTILES; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<u32x2_t*>(room + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
-                u32x2_t{pack_bf16(acc[t][i] * inv, acc[t][i + 1] * inv), pack_bf16(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
-    __syncthreads();
-    constexpr int LANES = DT / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
-    const int e = 8 * (lane % LANES);
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<u32x2_t*>(room + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
+                    u32x2_t{pack_bf16(acc[t][i] * inv, acc[t][i + 1] * inv), pack_bf16(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
+        __syncthreads();
+        constexpr int LANES = DT / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
+        const int e = 8 * (lane % LANES);
 #pragma unroll
-    for (int i = 0; i < 32 / AT_ONCE; i++) {
-        const int row = lane / LANES + AT_ONCE * i;
-        const int64_t r = r0 + 32 * wave + row;
-        if (r < r1 && e < a.dim) {
-            int32_t head;
-            const int32_t token = attention_token(a, r, head);
-            head += b.kv_head * a.group;
-            *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
-                *reinterpret_cast<const u32x4_t*>(room + row * OUT + 2 * e);
+        for (int i = 0; i < 32 / AT_ONCE; i++) {
+            const int row = lane / LANES + AT_ONCE * i;
+            const int64_t r = r0 + 32 * wave + row;
+            if (r < r1 && e < a.dim) {
+                int32_t head;
+                const int32_t token = attention_token(a, r, head);
+                head += b.kv_head * a.group;
+                *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
+                    *reinterpret_cast<const u32x4_t*>(room + row * OUT + 2 * e);
+            }
         }
+    }
+    // (this wavefront's stores above stay in front: these rows are written twice, and the second is what is left)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    while (again) {
+        const int i = __builtin_ctz(again);
+        again &= again - 1;
+        attention_row_again<DT, SOURCE, ROWS, Q8 ? 12 : 0>(a, b, r0 + 32 * wave + i, s0 * kKeys, s1 * kKeys < hi ? s1 * kKeys : hi);
     }
 }
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from sensenova_u1_amd import PagedKVCache, ops, paged_attention, prompt_attention
+from sensenova_u1_amd import PagedKVCache, RotaryTable, ops, paged_attention, prompt_attention, rotary
 
 from . import attention_oracle as ao
 
@@ -516,3 +516,28 @@ def test_many_small_weights_beside_one_large(dev):
         got = paged_attention(q.to(dev), cache, torch.arange(469, dtype=torch.int32, device=dev)[None], torch.tensor([lk], dtype=torch.int32, device=dev))
         want, most = ao.attention(q, kk, vv, operand=torch.float16 if qt == ops.Q8_0 else torch.bfloat16)
         _close(got, want, most)
+
+
+def test_overlapping_outputs_are_refused(dev):
+    x = torch.zeros((8, 6, 64), dtype=torch.bfloat16, device=dev)
+    q, k, v = x.split([2, 2, 2], 1)
+    ends = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    prompt_attention(q, k, v, ends, out=torch.empty((2, 8, 64), dtype=q.dtype, device=dev).transpose(0, 1))
+    cache = PagedKVCache.empty(4, 2, 16, 64, ops.BF16, dev)
+    pages, lens = torch.zeros((1, 4), dtype=torch.int32, device=dev), torch.tensor([8], dtype=torch.int32, device=dev)
+    turns, positions = RotaryTable.for_model(64, device=dev), torch.arange(8, device=dev)
+    wide = torch.zeros((8, 1, 64), dtype=torch.bfloat16, device=dev).expand(8, 2, 64)
+    for out in (q, k, v, wide):
+        with pytest.raises(ops.SnGgufError):
+            prompt_attention(q, k, v, ends, out=out)
+    for out in (q, wide):
+        with pytest.raises(ops.SnGgufError):
+            paged_attention(q, cache, pages, lens, ends, out=out)
+    for a, b in ((wide, k), (q, wide), (q, q), (wide, None), (wide.transpose(0, 1)[:1].expand(8, 8, 64), None)):
+        with pytest.raises(ops.SnGgufError):
+            rotary(a, b, positions, turns, inplace=True)
+        rotary(a, b, positions, turns)
+    for a, b in ((wide, k), (k, k)):
+        with pytest.raises(ops.SnGgufError):
+            cache.write_rotary(a, b, v, positions, turns, positions, inplace=True)
+    rotary(q, k, positions, turns, inplace=True)
