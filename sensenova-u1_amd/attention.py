@@ -15,6 +15,7 @@ A layer's attention for new tokens of sequences that lie in a cache::
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -40,23 +41,38 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
+def _stream(index: int) -> int:
+    return ops._raw_stream(index) if ops._raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def _launch(index: int, name: str, *args) -> None:
     """``lib.<name>(*args, current stream)`` with device ``index`` current."""
     fn = getattr(ops.load_library(), name)
     if index == ops._current_device():
-        rc = fn(*args, ops._stream(torch.device("cuda", index)) if ops._raw_stream is None else ops._raw_stream(index))
+        rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, _stream(index))
     if rc:
         ops._check(rc, name)
 
 
-def _launch_with_workspace(dev: torch.device, nbytes: int, name: str, *args) -> None:
+@functools.lru_cache(1024)
+def _prompt_workspace(*sizes: int) -> int:
+    return ops.load_library().sngguf_attention_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(1024)
+def _paged_workspace(*sizes: int) -> int:
+    return ops.load_library().sngguf_paged_attention_workspace_bytes(*sizes)
+
+
+def _launch_with_workspace(index: int, nbytes: int, name: str, *args) -> None:
     if not nbytes:
-        return _launch(dev.index, name, *args, None, 0)
+        return _launch(index, name, *args, None, 0)
+    dev = torch.device("cuda", index)
     with ops._on(dev), ops._whole_call(dev):
-        _launch(dev.index, name, *args, ops.pooled_workspace(dev, nbytes).data_ptr(), nbytes)
+        _launch(index, name, *args, ops.pooled_workspace(dev, nbytes).data_ptr(), nbytes)
 
 
 def _same_device(what: str, index: int, *tensors: Optional[torch.Tensor]) -> None:
@@ -65,29 +81,25 @@ def _same_device(what: str, index: int, *tensors: Optional[torch.Tensor]) -> Non
             raise SnGgufError(f"{what}: tensors on different devices (or on the host; there is no CPU implementation)")
 
 
-def _heads(x: torch.Tensor, what: str, name: str) -> torch.Tensor:
-    """``x`` as [tokens][heads][dim] rows whose elements are neighbours."""
+def _heads(x: torch.Tensor, what: str, name: str, pieces: bool = False):
+    """``x`` as [tokens][heads][dim] rows whose elements are neighbours (``pieces``: each at a 16-byte boundary), copied where it is not,
+    and its (token, head) strides; those of an axis of one entry are never stepped over and count as 0."""
     if not x.is_cuda:
         raise SnGgufError(f"sn_gguf ops run on a HIP device only, got {name} on '{x.device}'; there is no CPU implementation")
-    if x.dtype != _BF16 or x.dim() != 3:
-        raise SnGgufError(f"{what}: {name} must be bf16 [tokens][heads][dim], got {x.dtype} {tuple(x.shape)}")
+    shape = x.shape
+    if x.dtype != _BF16 or len(shape) != 3:
+        raise SnGgufError(f"{what}: {name} must be bf16 [tokens][heads][dim], got {x.dtype} {tuple(shape)}")
     if x.requires_grad and torch.is_grad_enabled():
         raise SnGgufError(f"{what}: forward only, but {name} requires a gradient")
-    return x if x.stride(2) == 1 or x.numel() == 0 else x.contiguous()
-
-
-def _pieces(x: torch.Tensor) -> torch.Tensor:
-    """``x`` with every row at a 16-byte boundary (copied where it is not; strides of one row or none do not count)."""
-    t, h, _ = x.stride()
-    if (t % 8 == 0 or x.shape[0] < 2) and (h % 8 == 0 or x.shape[1] < 2) and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _strides(x: torch.Tensor):
-    """(token, head) strides; those of an axis of one entry are never stepped over and count as whole pieces."""
-    t, h, _ = x.stride()
-    return (t if x.shape[0] > 1 else 0), (h if x.shape[1] > 1 else 0)
+    tokens, heads, dim = shape
+    t, h, e = x.stride()
+    if tokens < 2:
+        t = 0
+    if heads < 2:
+        h = 0
+    if (e != 1 and x.numel()) or (pieces and (t % 8 or h % 8 or x.data_ptr() % 16)):
+        return x.clone(memory_format=torch.contiguous_format), heads * dim, dim
+    return x, t, h
 
 
 def _apart(x: torch.Tensor) -> bool:
@@ -160,26 +172,27 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None.  positions: int64 [tokens].  A model whose head
     has parts with positions of their own calls it on views of the parts.  In place, no two rows may share an element."""
     q0, k0 = q, k
-    q = _heads(q, "rotary", "q")
+    q, qt, qh = _heads(q, "rotary", "q")
     tokens, heads, dim = q.shape
     index = q.get_device()
     positions = _numbers(positions, torch.int64, tokens, "rotary", "positions")
     _same_device("rotary", index, k, positions, table.turns)
     if k is not None:
-        k = _heads(k, "rotary", "k")
+        k, kt, kh = _heads(k, "rotary", "k")
         if k.shape[0] != tokens or k.shape[2] != dim:
             raise SnGgufError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
     if inplace and (q is not q0 or k is not k0):
         raise SnGgufError("rotary: in place needs the elements of a head next to each other")
     if inplace and not (_apart(q) and (k is None or (_apart(k) and (k.data_ptr() != q.data_ptr() or not k.numel())))):
         raise SnGgufError("rotary: in place needs rows that share no element")
-    q_out = q if inplace else _new(q)
+    q_out, qot, qoh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
     k_out = k if inplace or k is None else _new(k)
     if tokens and heads:
-        kt, kh, kot, koh = (*_strides(k), *_strides(k_out)) if k is not None else (0, 0, 0, 0)
-        kp, kop, kn = (k.data_ptr(), k_out.data_ptr(), k.shape[1]) if k is not None else (None, None, 0)
-        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, *_strides(q), q_out.data_ptr(), *_strides(q_out),
-                kp, kn, kt, kh, kop, kot, koh)
+        if k is None:
+            rest = (None, 0, 0, 0, None, 0, 0)
+        else:
+            rest = (k.data_ptr(), k.shape[1], kt, kh, k_out.data_ptr(), *((kt, kh) if inplace else (k.shape[1] * dim, dim)))
+        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, qt, qh, q_out.data_ptr(), qot, qoh, *rest)
     return q_out, k_out
 
 
@@ -231,19 +244,19 @@ class PagedKVCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
     def _rows(self, k, v, slots, what):
-        k, v = _heads(k, what, "k"), _heads(v, what, "v")
+        (k, kt, kh), (v, vt, vh) = _heads(k, what, "k"), _heads(v, what, "v")
         if k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[2] != self.dim:
             raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with a cache of {self.kv_heads} heads of {self.dim}")
         slots = _numbers(slots, torch.int64, k.shape[0], what, "slots")
         _same_device(what, self._index, k, v, slots)
-        return k, v, slots
+        return k, v, slots, (k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), k.shape[0])
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Keys and values [tokens][kv_heads][dim] into ``slots`` (int64 [tokens], different ones; negative ones and those behind
         the last page are passed over)."""
-        k, v, slots = self._rows(k, v, slots, "PagedKVCache.write")
+        k, v, slots, rows = self._rows(k, v, slots, "PagedKVCache.write")
         if k.shape[0]:
-            _launch(self._index, "sngguf_cache_write", self._address, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), k.shape[0])
+            _launch(self._index, "sngguf_cache_write", self._address, *rows)
 
     def write_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: RotaryTable, slots: torch.Tensor,
                      inplace: bool = False) -> torch.Tensor:
@@ -251,19 +264,19 @@ class PagedKVCache:
         q's own memory; k is left as it is)."""
         what = "PagedKVCache.write_rotary"
         q0 = q
-        q = _heads(q, what, "q")
-        k, v, slots = self._rows(k, v, slots, what)
-        tokens = k.shape[0]
-        if q.shape[0] != tokens or q.shape[2] != self.dim:
+        q, qt, qh = _heads(q, what, "q")
+        k, v, slots, rows = self._rows(k, v, slots, what)
+        tokens, heads, dim = q.shape
+        if k.shape[0] != tokens or dim != self.dim:
             raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
         if inplace and (q is not q0 or not _apart(q) or (q.data_ptr() in (k.data_ptr(), v.data_ptr()) and q.numel())):
             raise SnGgufError(f"{what}: in place needs rows that share no element, the elements of a head next to each other")
         positions = _numbers(positions, torch.int64, tokens, what, "positions")
         _same_device(what, self._index, q, positions, table.turns)
-        out = q if inplace else _new(q)
+        out, ot, oh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
         if tokens:
-            _launch(self._index, "sngguf_cache_write_rotary", self._address, table._address, positions.data_ptr(), q.data_ptr(), q.shape[1], *_strides(q),
-                    out.data_ptr(), *_strides(out), k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), slots.data_ptr(), tokens)
+            _launch(self._index, "sngguf_cache_write_rotary", self._address, table._address, positions.data_ptr(), q.data_ptr(), heads, qt, qh, out.data_ptr(),
+                    ot, oh, *rows)
         return out
 
     def read(self, slots: torch.Tensor):
@@ -277,14 +290,19 @@ class PagedKVCache:
         return k, v
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, *others: torch.Tensor) -> torch.Tensor:
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, *others: torch.Tensor):
+    """(out, its token and head strides)"""
+    tokens, heads, dim = q.shape
     if out is None:
-        return _new(q)
-    if out.dtype != _BF16 or out.shape != q.shape or out.get_device() != q.get_device() or out.stride(2) != 1 or _pieces(out) is not out:
-        raise SnGgufError(f"{what}: out must be bf16 {tuple(q.shape)} on q's device, its rows of whole 16-byte pieces")
+        return _new(q), heads * dim, dim
+    if out.dtype != _BF16 or out.shape != q.shape or out.get_device() != q.get_device():
+        raise SnGgufError(f"{what}: out must be bf16 {tuple(q.shape)} on q's device")
+    rows, t, h = _heads(out, what, "out", True)
+    if rows is not out:
+        raise SnGgufError(f"{what}: out must have rows of whole 16-byte pieces")
     if out.numel() and (not _apart(out) or out.data_ptr() in [x.data_ptr() for x in (q, *others)]):
         raise SnGgufError(f"{what}: out must not overlap itself or an input")
-    return out
+    return out, t, h
 
 
 def _check_options(what: str, heads: int, kv_heads: int, dim: int, scale: Optional[float], window: int) -> float:
@@ -311,25 +329,26 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
     have no part in its result, whatever they hold.  ``scale`` defaults to dim ** -0.5.  Rows of ``out`` behind the last sequence are not
     written; ``out`` overlaps no input."""
     what = "prompt_attention"
-    q, k, v = _pieces(_heads(q, what, "q")), _pieces(_heads(k, what, "k")), _pieces(_heads(v, what, "v"))
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = _heads(q, what, "q", True), _heads(k, what, "k", True), _heads(v, what, "v", True)
     tokens, heads, dim = q.shape
     if k.shape != v.shape or k.shape[2] != dim:
         raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
-    scale = _check_options(what, heads, k.shape[1], dim, scale, window)
+    keys, kv_heads = k.shape[0], k.shape[1]
+    scale = _check_options(what, heads, kv_heads, dim, scale, window)
     if window and not causal:
         raise SnGgufError(f"{what}: a window needs causal attention")
     ends_q = _numbers(ends_q, torch.int32, None, what, "ends_q")
     ends_k = ends_q if ends_k is None else _numbers(ends_k, torch.int32, ends_q.shape[0], what, "ends_k")
     if ends_q.shape[0] < 1:
         raise SnGgufError(f"{what}: ends_q has no entry")
-    _same_device(what, q.get_device(), k, v, ends_q, ends_k)
-    out = _output(out, q, what, k, v)
+    index = q.get_device()
+    _same_device(what, index, k, v, ends_q, ends_k)
+    out, ot, oh = _output(out, q, what, k, v)
     sequences = ends_q.shape[0] - 1
     if tokens and sequences:
-        nbytes = ops.load_library().sngguf_attention_workspace_bytes(tokens, k.shape[0], sequences, heads, k.shape[1], dim)
-        _launch_with_workspace(q.device, nbytes, "sngguf_attention", q.data_ptr(), tokens, heads, *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
-                               *_strides(v), k.shape[0], k.shape[1], dim, ends_q.data_ptr(), ends_k.data_ptr(), sequences, scale, int(causal), window,
-                               out.data_ptr(), *_strides(out))
+        nbytes = _prompt_workspace(tokens, keys, sequences, heads, kv_heads, dim)
+        _launch_with_workspace(index, nbytes, "sngguf_attention", q.data_ptr(), tokens, heads, qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, keys,
+                               kv_heads, dim, ends_q.data_ptr(), ends_k.data_ptr(), sequences, scale, int(causal), window, out.data_ptr(), ot, oh)
     return out
 
 
@@ -343,7 +362,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     decides which kernels are launched and never what they compute.  With a ``window``, the pages in front of it may be anyone's.
     ``scale``, ``window``, ``out``: as ``prompt_attention``."""
     what = "paged_attention"
-    q = _pieces(_heads(q, what, "q"))
+    q, qt, qh = _heads(q, what, "q", True)
     tokens, heads, dim = q.shape
     if dim != cache.dim:
         raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with a cache of heads of {cache.dim}")
@@ -364,11 +383,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     elif tokens != sequences:
         raise SnGgufError(f"{what}: {tokens} queries of {sequences} sequences need ends_q")
     _same_device(what, cache._index, q, pages, lens, ends_q)
-    out = _output(out, q, what, cache.k, cache.v)
+    out, ot, oh = _output(out, q, what, cache.k, cache.v)
     if tokens and sequences:
         if ends_q is None:
             max_new = 1
-        nbytes = ops.load_library().sngguf_paged_attention_workspace_bytes(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
-        _launch_with_workspace(q.device, nbytes, "sngguf_paged_attention", q.data_ptr(), tokens, heads, *_strides(q), cache._address, pages.data_ptr(),
-                               pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), *_strides(out))
+        nbytes = _paged_workspace(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
+        _launch_with_workspace(cache._index, nbytes, "sngguf_paged_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
+                               pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), ot, oh)
     return out
