@@ -84,6 +84,8 @@ constexpr int kRowsLeast = 2, kRowsKeys = 128;        // key tiles that a split 
 constexpr int kTilesLeast = 16, kTilesKeys = 64;     // (a workgroup costs as much as five tiles before its first and behind its last)
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// The kernel for many rows, bound by its arithmetic, has two more
+int many_dim(int64_t dim) { return dim > 64 && dim <= 96 ? 96 : dim > 128 && dim <= 192 ? 192 : kernel_dim(dim); }
 
 // Workgroups that the device's 256 compute units take at a time, by the registers of the kernels
 int few_at_a_time(int rows, int dim) { return rows * dim <= 16 * 128 ? 768 : rows * dim <= 16 * 256 && dim < 256 ? 512 : 256; }
@@ -162,7 +164,7 @@ int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* p
     a.want = p.want;
     a.least = kTilesLeast;
     a.grid = partial ? p.grid : p.tiles;
-    const int rc = sngguf::launch_attention_tiles(a, p.rows, dim, source, stream);
+    const int rc = sngguf::launch_attention_tiles(a, p.rows, many_dim(a.dim), source, stream);
     if (rc != SNGGUF_OK || !partial) return rc;
     return sngguf::launch_attention_combine(a, p.rows, kTilesKeys, dim, p.tiles, most_rows, stream);
 }

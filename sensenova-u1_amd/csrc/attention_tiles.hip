@@ -80,7 +80,7 @@ __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
 __device__ __forceinline__ int block_place(int row, int piece) { return 8 * (piece & 7) + ((row & 7) ^ (4 * ((piece >> 1) & 1))); }
 
 template <int DT> struct Tile {
-    static constexpr int kBlocks = DT / 64;                    // of eight rows
+    static constexpr int kBlocks = (DT + 63) / 64;             // of eight rows
     static constexpr int kRowBlock = kBlocks * 1024 + 128;     // bytes from eight rows to the next
     static constexpr int kBytes = kKeys / 8 * kRowBlock;
 };
@@ -95,6 +95,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
     constexpr int ROWS = 32 * W;
     constexpr int TILE = Tile<DT>::kBytes, RB = Tile<DT>::kRowBlock, PB = Tile<DT>::kBlocks;
     constexpr int KS = DT / 16, DTILES = DT / 32;
+    constexpr int DP = DT <= 64 ? 64 : DT <= 128 ? 128 : 256;   // elements of a row of a partial result
     constexpr int VF = 2 * DTILES, NF = VF + KS;       // operand fragments of a step: of values, in all
     constexpr int NP = 8;                              // pairs of weights of a step that a lane forms
     constexpr float kLimit = Q8 ? 32768.f : 1e9f;      // (fp16 weights are scaled by 2^12)
@@ -508,9 +509,9 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
             for (int t = 0; t < DTILES; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4_t*>(a.partial + at * DT + 32 * t + 2 * i + 4 * h) = f32x4_t{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
+                    *reinterpret_cast<f32x4_t*>(a.partial + at * DP + 32 * t + 2 * i + 4 * h) = f32x4_t{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
             if (h == 0) {
-                float* st = a.partial + a.grid * ROWS * DT + at * 2;
+                float* st = a.partial + a.grid * ROWS * DP + at * 2;
                 st[0] = m;
                 st[1] = l;
             }
@@ -518,7 +519,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
     } else {
         // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
         // each of its row's pieces
-        constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
+        constexpr int OUT = 2 * DP + 16;                   // bytes of a row there; the padding spreads rows over the banks
         static_assert(ROWS * OUT <= NS * 2 * TILE, "room");
         __syncthreads();
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
                 *reinterpret_cast<u32x2_t*>(room + col * OUT + 2 * (32 * t + 2 * i + 4 * h)) =
                     u32x2_t{pack_bf16(acc[t][i] * inv, acc[t][i + 1] * inv), pack_bf16(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
         __syncthreads();
-        constexpr int LANES = DT / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
+        constexpr int LANES = DP / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
         const int e = 8 * (lane % LANES);
 #pragma unroll
         for (int i = 0; i < 32 / AT_ONCE; i++) {
@@ -550,11 +551,11 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
     while (again) {
         const int i = __builtin_ctz(again);
         again &= again - 1;
-        attention_row_again<DT, SOURCE, ROWS, Q8 ? 12 : 0>(a, b, r0 + 32 * wave + i, s0 * kKeys, s1 * kKeys < hi ? s1 * kKeys : hi);
+        attention_row_again<DP, SOURCE, ROWS, Q8 ? 12 : 0>(a, b, r0 + 32 * wave + i, s0 * kKeys, s1 * kKeys < hi ? s1 * kKeys : hi);
     }
 }
 
-// dim: of the kernel, 64, 128 or 256; rows: of a workgroup, 128 or (up to 128 elements) 256
+// dim: of the kernel, 64, 96, 128, 192 or 256; rows: of a workgroup, 128 or (up to 128 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
 #define SNGGUF_GO(D, S, W, N)                                                                                           \
     if (dim == D && source == S && rows == 32 * W) {                                                                    \
@@ -569,8 +570,11 @@ int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source
 #define SNGGUF_GO_DIM(D, W, N) SNGGUF_GO(D, kPacked, W, N) SNGGUF_GO(D, kPaged, W, N) SNGGUF_GO(D, kPagedQ8, W, 2)
     SNGGUF_GO_DIM(64, 4, 3)
     SNGGUF_GO_DIM(64, 8, 3)
+    SNGGUF_GO_DIM(96, 4, 2)
+    SNGGUF_GO_DIM(96, 8, 3)
     SNGGUF_GO_DIM(128, 4, 2)
     SNGGUF_GO_DIM(128, 8, 3)
+    SNGGUF_GO_DIM(192, 4, 2)
     SNGGUF_GO_DIM(256, 4, 2)
 #undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
