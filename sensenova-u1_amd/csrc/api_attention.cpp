@@ -118,12 +118,13 @@ int64_t row_tiles(int64_t tokens, int64_t sequences, int64_t group, int rows) { 
 // of 1024 tokens and 8 heads of keys: 29 us against 33; of 1500: 43 against 42; of 4096: 150 against 135).
 // Workgroups of equal work that leave a last round nearly empty are not split: 2500 queries over 3000 keys, 320 workgroups, took 193 us
 // as 960 instead of 173.
-Launch plan_many(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
+Launch plan_many(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
+    const int d = kernel_dim(dim);
     const int64_t group = heads / kv_heads, key_tiles = keys / kTilesKeys + 1;
-    const bool wide = dim <= 128 && tokens * group >= 512 * sequences &&
+    const bool wide = many_dim(dim) <= 192 && tokens * group >= 512 * sequences &&
                       (key_tiles >= 2 * kTilesLeast || kv_heads * row_tiles(tokens, sequences, group, 256) >= 160);
     const int rows = wide ? 256 : 128;
-    return plan(kv_heads * row_tiles(tokens, sequences, group, rows), key_tiles, dim, rows, many_at_a_time(rows, dim), kTilesLeast);
+    return plan(kv_heads * row_tiles(tokens, sequences, group, rows), key_tiles, d, rows, many_at_a_time(rows, d), kTilesLeast);
 }
 
 struct PagedPlan {
@@ -150,7 +151,7 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t
     p.most_rows = most < rows ? most : rows;
     const int64_t tiles = kv_heads * (p.many ? sequences : row_tiles(tokens, sequences, group, rows));
     p.a = plan(tiles, keys / kRowsKeys + 1, d, rows, few_at_a_time(rows, d), kRowsLeast);
-    p.b = plan_many(tokens, keys, sequences, heads, kv_heads, d);
+    p.b = plan_many(tokens, keys, sequences, heads, kv_heads, dim);
     return p;
 }
 
@@ -268,7 +269,7 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
 int64_t sngguf_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim) {
     if (tokens_q <= 0 || tokens_q >= kMost || tokens_k < 0 || tokens_k > kMostKeys || sequences <= 0 || sequences >= kMost || !heads_fit(heads, kv_heads, dim))
         return 0;
-    return plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, kernel_dim(dim)).partial_bytes;
+    return plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, dim).partial_bytes;
 }
 
 int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const void* k,
@@ -286,7 +287,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
         !whole_pieces(out, out_token, out_head) || !aligned(ends_q, 4) || !aligned(ends_k, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
     const int d = kernel_dim(dim);
-    const Launch p = plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, d);
+    const Launch p = plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, dim);
     if (p.grid >= kMost) return SNGGUF_E_BADSHAPE;
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);

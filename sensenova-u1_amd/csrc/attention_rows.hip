@@ -582,6 +582,7 @@ int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim
     SNGGUF_GO_DIM(128, 64)
     SNGGUF_GO(256, 64, 64)
     SNGGUF_GO(256, 64, 128)
+    SNGGUF_GO(256, 64, 256)
 #undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;

@@ -89,7 +89,7 @@ template <int DT> struct Tile {
 
 // W: wavefronts, of 32 rows each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
 template <int DT, int SOURCE, int W, int NS>
-__global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
     constexpr int ROWS = 32 * W;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
     } else {
         // through LDS (each wavefront its own rows, in the room of the stages), so that whole rows are written: a lane has eight bytes of
         // each of its row's pieces
-        constexpr int OUT = 2 * DP + 16;                   // bytes of a row there; the padding spreads rows over the banks
+        constexpr int OUT = 2 * DT + 16;                   // bytes of a row there; the padding spreads rows over the banks
         static_assert(ROWS * OUT <= NS * 2 * TILE, "room");
         __syncthreads();
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 ? 2 : 1) void attention_tiles_ker
     }
 }
 
-// dim: of the kernel, 64, 96, 128, 192 or 256; rows: of a workgroup, 128 or (up to 128 elements) 256
+// dim: of the kernel, 64, 96, 128, 192 or 256; rows: of a workgroup, 128 or (up to 192 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
 #define SNGGUF_GO(D, S, W, N)                                                                                           \
     if (dim == D && source == S && rows == 32 * W) {                                                                    \
@@ -575,6 +575,7 @@ int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source
     SNGGUF_GO_DIM(128, 4, 2)
     SNGGUF_GO_DIM(128, 8, 3)
     SNGGUF_GO_DIM(192, 4, 2)
+    SNGGUF_GO_DIM(192, 8, 2)
     SNGGUF_GO_DIM(256, 4, 2)
 #undef SNGGUF_GO_DIM
 #undef SNGGUF_GO
