@@ -6,10 +6,12 @@
 // the bytes of the cache, so a workgroup's wavefronts read keys and values straight into registers, in the order in which
 // the matrix instructions want them, and never through LDS; each wavefront takes every fourth run of 32 keys with a maximum
 // and a sum of its own, and the four are joined at the end.  Sequences are split over workgroups where there are few.
+// Measured, 32 query and 8 key / value heads of 128: 24 tokens over 37 .. 9996 in 8 bits 46.7 us, 5.6 TB/s; one over 131071 in bf16
+// 94 us, 5.7 TB/s; the join 6 to 7 us more.
 //
 // Per run of 32 keys and 16 rows (columns of the 16 x 16 x 32 instructions, lane % 16; lane group g = lane / 16):
-//  * scores: K (16 keys x dim) times Q^T.  The order in which dim is summed is free: lane group g takes elements
-//    [g DT / 4, (g + 1) DT / 4) of its key's row, which are contiguous.  Matrix row 4 g + i of the first instruction is key
+//  * scores: K (16 keys x dim) times Q^T.  The order in which dim is summed is free: in 8 bits lane group g takes elements
+//    [g DT / 4, (g + 1) DT / 4) of its key's row, in bf16 eight of every 32.  Matrix row 4 g + i of the first instruction is key
 //    8 g + i, of the second key 8 g + 4 + i;
 //  * so a lane's eight scores are of keys 8 g .. 8 g + 7, which is how the second product wants them: V^T (16 elements x 32
 //    keys) times P^T, where lane group g holds keys 8 g .. 8 g + 7.  A lane reads DT / 16 neighbouring elements of those eight

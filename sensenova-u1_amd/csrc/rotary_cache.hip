@@ -11,7 +11,9 @@
 // +-65024.  A run with a NaN is held as NaN.
 //
 // All of it is bound by memory.  A workgroup takes a few tokens: its threads first make one (cosine, sine) pair each, in LDS,
-// then work through the tokens' heads in pieces of 16 bytes.
+// then work through the tokens' heads in pieces of 16 bytes.  8192 tokens of 40 heads of 128: 35.7 us, 4.7 TB/s; 5003 tokens of 32 query
+// and 8 + 8 heads, keys and values written in 8 bits: 27 us, 4.2 TB/s; 40000 tokens read back: 42 us, 5.9 TB/s (61.6 where nothing of
+// it is in the last-level cache; nontemporal stores: 43 and 65).
 #include "rotary_cache.hpp"
 
 namespace sngguf {
