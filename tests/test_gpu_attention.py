@@ -541,3 +541,18 @@ def test_overlapping_outputs_are_refused(dev):
         with pytest.raises(ops.SnGgufError):
             cache.write_rotary(a, b, v, positions, turns, positions, inplace=True)
     rotary(q, k, positions, turns, inplace=True)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_many_rows_of_all_dims(dev, dim):
+    """Workgroups of 256 rows where the dim has them: with the keys of few tiles split, and without."""
+    _prompt(dev, [290], [2100], 4, 2, dim, seed=dim)
+    _prompt(dev, [1300], [1300], 32, 32, dim, seed=dim)
+    _prompt(dev, [700, 31, 520], [700, 90, 600], 32, 16, dim, False, seed=dim)
+
+
+@BOTH
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_many_rows_of_all_dims_over_the_cache(dev, qt, dim):
+    _paged(dev, [290], [2100], 4, 2, dim, 64, qt, seed=dim)
+    _paged(dev, [1300], [1311], 32, 32, dim, 32, qt, seed=dim)

@@ -135,3 +135,13 @@ def test_values_at_the_end_of_the_range(dev):
     got = paged_attention(q[129:].to(dev), cache, table, torch.tensor([130], dtype=torch.int32, device=dev))
     want, most = ao.attention(q[129:], k, big)
     assert bool(((got.double().cpu() - want).abs() <= most).all())
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+def test_many_rows(dev, dim):
+    gen = torch.Generator().manual_seed(dim)
+    q, k, v = _values(gen, 1300, 16, dim), _values(gen, 1300, 16, dim), _values(gen, 1300, 16, dim)
+    bad = v.clone()
+    bad[[700, 1290], :, 3] = torch.tensor([INF, NAN], dtype=v.dtype)[:, None]
+    got = prompt_attention(q.to(dev), k.to(dev), bad.to(dev), _ends([1300], dev))
+    _check(got, q, k, v, [], [700, 1290], True, 0)
