@@ -310,7 +310,7 @@ def _check_options(what: str, heads: int, kv_heads: int, dim: int, scale: Option
         raise SnGgufError(f"{what}: {heads} query heads cannot share {kv_heads} key / value heads")
     if dim % 32 or not 32 <= dim <= 256:
         raise SnGgufError(f"{what}: heads of {dim} elements (a multiple of 32 up to 256 is needed)")
-    if window < 0:
+    if not 0 <= window < 1 << 63:
         raise SnGgufError(f"{what}: a window of {window} tokens")
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 1e-30 <= scale <= 1e30:
@@ -367,7 +367,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     if dim != cache.dim:
         raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with a cache of heads of {cache.dim}")
     scale = _check_options(what, heads, cache.kv_heads, dim, scale, window)
-    if max_new < 0:
+    if not 0 <= max_new < 1 << 63:
         raise SnGgufError(f"{what}: max_new is {max_new}")
     lens = _numbers(lens, torch.int32, None, what, "lens")
     sequences = lens.shape[0]

@@ -307,7 +307,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
     a.dim = (int32_t)dim;
     a.scale_log2 = scale * 1.44269504088896341f;
     a.causal = causal != 0;
-    a.window = window;
+    a.window = window < kMost ? window : 0;     // (no sequence is that long, and places less the window stay within 64 bits)
     a.min_rows = 1;
     a.max_rows = (int32_t)(kMost - 1);
     float* partial = p.partial_bytes && workspace && workspace_bytes >= p.partial_bytes ? static_cast<float*>(workspace) : nullptr;
@@ -364,7 +364,7 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
     a.dim = (int32_t)cache->dim;
     a.scale_log2 = scale * 1.44269504088896341f;
     a.causal = 1;
-    a.window = window;
+    a.window = window < kMost ? window : 0;
     const int64_t need = (p.few ? p.a.partial_bytes : 0) + (p.many ? p.b.partial_bytes : 0);
     float* partial = workspace && workspace_bytes >= need ? static_cast<float*>(workspace) : nullptr;
     const hipStream_t s = static_cast<hipStream_t>(stream);

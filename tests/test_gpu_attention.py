@@ -556,3 +556,56 @@ def test_many_rows_of_all_dims(dev, dim):
 def test_many_rows_of_all_dims_over_the_cache(dev, qt, dim):
     _paged(dev, [290], [2100], 4, 2, dim, 64, qt, seed=dim)
     _paged(dev, [1300], [1311], 32, 32, dim, 32, qt, seed=dim)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 62, 2 ** 63 - 1])
+def test_windows_wider_than_any_sequence(dev, window):
+    gen = torch.Generator().manual_seed(11)
+    q, k, v = _values(gen, 90, 4, 64).to(dev), _values(gen, 50, 2, 64).to(dev), _values(gen, 50, 2, 64).to(dev)
+    for n in (1, 9, 90):
+        ends, ends_k = _ends([n], dev), _ends([50], dev)
+        assert torch.equal(prompt_attention(q[:n], k, v, ends, ends_k, window=window), prompt_attention(q[:n], k, v, ends, ends_k))
+    cache = PagedKVCache.empty(4, 2, 16, 64, ops.BF16, dev)
+    cache.write(k, v, torch.arange(50, device=dev))
+    pages, lens = torch.arange(4, dtype=torch.int32, device=dev)[None], torch.tensor([50], dtype=torch.int32, device=dev)
+    for n in (1, 9, 90):
+        assert torch.equal(paged_attention(q[:n], cache, pages, lens, _ends([n], dev), window=window), paged_attention(q[:n], cache, pages, lens, _ends([n], dev)))
+    for bad in (dict(window=2 ** 63), dict(window=2 ** 64 + 3), dict(max_new=2 ** 63)):
+        with pytest.raises(ops.SnGgufError):
+            paged_attention(q[:1], cache, pages, lens, **bad)
+
+
+@BOTH
+def test_without_a_workspace(dev, qt):
+    """Through the C entry points: keys are not split then, and a workspace that is too small is as none."""
+    lib = ops.load_library()
+    gen = torch.Generator().manual_seed(12)
+    heads, kv_heads, dim, keys, page = 8, 2, 128, 5000, 64
+    k, v = _values(gen, keys, kv_heads, dim, True), _values(gen, keys, kv_heads, dim)
+    cache = PagedKVCache.empty(keys // page + 1, kv_heads, page, dim, qt, dev)
+    kd, vd = k.to(dev), v.to(dev)
+    cache.write(kd, vd, torch.arange(keys, device=dev))
+    pages = torch.arange(cache.pages, dtype=torch.int32, device=dev)[None].repeat(2, 1)
+    lens = torch.tensor([keys, 900], dtype=torch.int32, device=dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(1 << 16, dtype=torch.uint8, device=dev)
+    held = (ao.quantised(k)[2], ao.quantised(v)[2]) if qt == ops.Q8_0 else (k, v)
+    for new in (1, 200):
+        q = _values(gen, 2 * new, heads, dim)
+        qd, ends = q.to(dev), _ends([new, new], dev)
+        need = lib.sngguf_paged_attention_workspace_bytes(2 * new, 2, new, pages.shape[1] * page, heads, kv_heads, dim)
+        assert need > ws.numel()
+        for given, nbytes in ((None, 0), (ws.data_ptr(), ws.numel())):
+            out = torch.empty_like(qd)
+            assert lib.sngguf_paged_attention(qd.data_ptr(), 2 * new, heads, heads * dim, dim, cache._address, pages.data_ptr(), pages.shape[1], pages.shape[1],
+                                              lens.data_ptr(), ends.data_ptr(), 2, new, dim ** -0.5, 0, out.data_ptr(), heads * dim, dim, given, nbytes, stream) == 0
+            for i, n in enumerate((keys, 900)):
+                want, most = ao.attention(q[i * new:(i + 1) * new], held[0][:n], held[1][:n], True, 0, None, torch.float16 if qt == ops.Q8_0 else torch.bfloat16)
+                _close(out[i * new:(i + 1) * new], want, most, f"{new} new of {n}")
+        if qt == ops.BF16:
+            out = torch.empty_like(qd)
+            ends_k = _ends([keys - 900, 900], dev)
+            assert lib.sngguf_attention(qd.data_ptr(), 2 * new, heads, heads * dim, dim, kd.data_ptr(), kv_heads * dim, dim, vd.data_ptr(), kv_heads * dim, dim, keys,
+                                        kv_heads, dim, ends.data_ptr(), ends_k.data_ptr(), 2, dim ** -0.5, 1, 0, out.data_ptr(), heads * dim, dim, None, 0, stream) == 0
+            want, most = ao.attention(q[:new], k[:keys - 900], v[:keys - 900])
+            _close(out[:new], want, most)
