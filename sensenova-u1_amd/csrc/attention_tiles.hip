@@ -75,11 +75,29 @@ __device__ __forceinline__ void copy_request(uint32_t lds, uint32_t off, const v
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
+// the same from an address of each lane's own
+__device__ __forceinline__ void copy_request(uint32_t lds, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+
 // f(0), f(1), ... f(N - 1), each number a constant (an unrolled loop of this size is given up by the compiler)
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>()), ...);
 }
+
+// From a row to the one `step` behind it: token and head of the group, without a division for each
+struct RowWalk {
+    uint32_t group, heads;
+    int64_t hop, wrap;
+    __device__ __forceinline__ RowWalk(uint32_t group, uint32_t step, int64_t token, int64_t head)
+        : group(group), heads(step % group), hop((int64_t)(step / group) * token + (int64_t)(step % group) * head), wrap(token - (int64_t)group * head) {}
+    template <typename P> __device__ __forceinline__ void next(P*& at, uint32_t& head) const {
+        at += hop;
+        head += heads;
+        if (head >= group) at += wrap, head -= group;
+    }
+};
 
 // Place of (row % 8, piece % 8) in its block, in pieces.
 __device__ __forceinline__ int block_place(int row, int piece) { return 8 * (piece & 7) + ((row & 7) ^ (4 * ((piece >> 1) & 1))); }
@@ -235,17 +253,42 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     typedef std::integral_constant<int, 0> First;
     typedef std::integral_constant<int, 1> Second;
 
-    // The first tile's keys are asked for before the queries are read, nothing else before both are there.
-    int32_t page_k = 0, page_v = 0;
-    if (count > 0) {
-        page_k = page_v = page_of(s0);
-        aim(0, s0, page_k);
+    // ---- fragments ---------------------------------------------------------------------------------------------------
+    // keys: row 32 half + col, piece 2 ks + h; values: keys 32 half + 16 x + 8 y + 4 h + (lane % 16) / 4 (the rows of one transposing
+    // read are four keys), elements 32 t + 16 ((lane % 32) / 16) + 4 (lane % 4) ...
+    const uint32_t k_at[2] = {lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, h)), lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, 2 + h))};
+    const uint32_t v_at = lds0 + (uint32_t)(TILE + 16 * block_place(4 * h + ((lane & 15) >> 2), 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1)) + 8 * (lane & 1));
+    // one lane's addresses in a stage; everything else is an immediate offset
+    struct At {
+        uint32_t k[2], v;
+    };
+    auto at_stage = [&](uint32_t stage) -> At {
+        At x = {{k_at[0] + stage, k_at[1] + stage}, v_at + stage};
+        asm volatile("" : "+v"(x.k[0]), "+v"(x.k[1]), "+v"(x.v));     // (or every address would be formed by itself)
+        return x;
+    };
+    auto key_fragment = [&](const At& x, int half, int ks) -> op_t {
+        return *(const __attribute__((address_space(3))) op_t*)(uintptr_t)(x.k[ks & 1] + 4 * half * RB + (ks >> 2) * 1024 + ((ks & 2) ? 512 : 0));
+    };
+    auto value_fragment = [&](const At& x, int half, int t, int y) -> op_t {
+        u32x2_t part[2];
 #pragma unroll
-        for (int j = 0; j < REQ; j++) request(0, lds0, j);
-    }
+        for (int z = 0; z < 2; z++)
+            part[z] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)(
+                x.v + (4 * half + 2 * y + z) * RB + (t >> 1) * 1024 + (t & 1) * 512)));
+        return __builtin_bit_cast(op_t, u32x4_t{part[0][0], part[0][1], part[1][0], part[1][1]});
+    };
 
-    // ---- this lane's row: its query as operand fragments, and the keys that it sees --------------------------------
+    // ---- the first tile's keys, this lane's row: its query as operand fragments, and the keys that it sees -----------------------
+    // Queries are asked for as tiles are, whole lines at a time (a lane that reads its own row takes a quarter of each line: 2.6 us until they
+    // were there, of a workgroup's 9 beside its tiles), each wavefront its own rows, into the room of the stages behind the
+    // first; or of all, if keys come through registers.  Nothing else is asked for before both are there.
     const int64_t my_row = r0 + 32 * wave + col;
+    constexpr uint32_t kStage = 2 * TILE, kRing = NS * kStage;   // a stage: keys of tile i, values of tile i - 1
+    constexpr bool QLDS = DT < 256 && (Q8 || (NS - 1) * kStage >= 4 * W * RB);
+    constexpr uint32_t QROOM = Q8 ? 0 : kStage;
+    const uint32_t group = (uint32_t)a.group, token0 = (uint32_t)r0 / group;
+    int32_t page_k = 0, page_v = 0;
     op_t qf[KS];
     float c = a.scale_log2;
     int32_t first, last;
@@ -256,12 +299,44 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
         const int32_t place = back + token;
         last = a.causal && place < most ? place : most;
         first = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
-        const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
-        u32x4_t raw[KS];
+        u32x4_t raw[KS] = {};
+        if (count > 0) {
+            page_k = page_v = page_of(s0);
+            aim(0, s0, page_k);
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int e = 16 * i + 8 * h;
-            raw[i] = e < a.dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
+            for (int j = 0; j < REQ; j++) request(0, lds0, j);
+            if constexpr (QLDS) {
+                // row 32 wave + 8 i + crow of the tile; rows behind the last are its first
+                const bf16_t* row0 = a.q + (b.s.q0 + token0) * a.q_token + (int64_t)(b.kv_head * a.group + (uint32_t)r0 - token0 * group) * a.q_head;
+                const uint32_t r = (uint32_t)r0 + 32 * wave + crow;
+                const uint32_t t = r / group;
+                uint32_t g = r - t * group;
+                const RowWalk walk(group, 8, a.q_token, a.q_head);
+                const bf16_t* from = a.q + (b.s.q0 + t) * a.q_token + (int64_t)(b.kv_head * group + g) * a.q_head;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bf16_t* row = r + 8 * i < r1 ? from : row0;
+#pragma unroll
+                    for (int p = 0; p < PB; p++)
+                        copy_request(lds0 + QROOM + (4 * wave + i) * RB + p * 1024, row + (64 * p + 8 * cpiece < a.dim ? 64 * p + 8 * cpiece : 0));
+                    walk.next(from, g);
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                const At at = at_stage(QROOM + 4 * wave * RB);
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    raw[i] = __builtin_bit_cast(u32x4_t, key_fragment(at, 0, i));
+                    if (16 * i + 8 * h >= a.dim) raw[i] = u32x4_t{0u, 0u, 0u, 0u};
+                }
+            }
+        }
+        if constexpr (!QLDS) {
+            const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                const int e = 16 * i + 8 * h;
+                raw[i] = e < a.dim ? *reinterpret_cast<const u32x4_t*>(q + e) : u32x4_t{0u, 0u, 0u, 0u};
+            }
         }
         if constexpr (Q8) {
             // bf16 -> fp16: scaled by a power of two that brings the row's largest element into [1, 2)
@@ -288,32 +363,6 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
             for (int i = 0; i < KS; i++) qf[i] = __builtin_bit_cast(op_t, raw[i]);
         }
     }
-
-    // ---- fragments ---------------------------------------------------------------------------------------------------
-    // keys: row 32 half + col, piece 2 ks + h; values: keys 32 half + 16 x + 8 y + 4 h + (lane % 16) / 4 (the rows of one transposing
-    // read are four keys), elements 32 t + 16 ((lane % 32) / 16) + 4 (lane % 4) ...
-    const uint32_t k_at[2] = {lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, h)), lds0 + (uint32_t)((col >> 3) * RB + 16 * block_place(col, 2 + h))};
-    const uint32_t v_at = lds0 + (uint32_t)(TILE + 16 * block_place(4 * h + ((lane & 15) >> 2), 2 * ((lane & 31) >> 4) + ((lane & 3) >> 1)) + 8 * (lane & 1));
-    // one lane's addresses in a stage; everything else is an immediate offset
-    struct At {
-        uint32_t k[2], v;
-    };
-    auto at_stage = [&](uint32_t stage) -> At {
-        At x = {{k_at[0] + stage, k_at[1] + stage}, v_at + stage};
-        asm volatile("" : "+v"(x.k[0]), "+v"(x.k[1]), "+v"(x.v));     // (or every address would be formed by itself)
-        return x;
-    };
-    auto key_fragment = [&](const At& x, int half, int ks) -> op_t {
-        return *(const __attribute__((address_space(3))) op_t*)(uintptr_t)(x.k[ks & 1] + 4 * half * RB + (ks >> 2) * 1024 + ((ks & 2) ? 512 : 0));
-    };
-    auto value_fragment = [&](const At& x, int half, int t, int y) -> op_t {
-        u32x2_t part[2];
-#pragma unroll
-        for (int z = 0; z < 2; z++)
-            part[z] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)(
-                x.v + (4 * half + 2 * y + z) * RB + (t >> 1) * 1024 + (t & 1) * 512)));
-        return __builtin_bit_cast(op_t, u32x4_t{part[0][0], part[0][1], part[1][0], part[1][1]});
-    };
 
     // ---- pieces of a step ----------------------------------------------------------------------------------------------
     typedef uint32_t weights_t[2][4];     // [16 keys][pair]
@@ -418,9 +467,8 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     if (count > 0) {
         weights_t wa, wb;
         float sum;
-        // A stage: keys of tile i, values of tile i - 1 (behind the last tile: of the last, read by nobody, so that the loop neither
-        // asks whether there are more nor counts what is under way)
-        constexpr uint32_t kStage = 2 * TILE, kRing = NS * kStage;
+        // (behind the last tile: of the last, read by nobody, so that the loop neither asks whether there are more nor counts what is
+        // under way)
         auto after = [&](uint32_t stage) { return stage + kStage < kRing ? stage + kStage : 0u; };
         // the requests of all stages but the NS - 2 last asked for have arrived, from every wavefront
         auto wait_stage = [&] {
@@ -435,6 +483,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
             aim(1, tv, page_v);
         };
         if constexpr (Q8) {
+            __syncthreads();       // (every wavefront has its queries)
 #pragma unroll
             for (int i = 0; i < QN; i++) widen(0, lds0, i);
         }
@@ -538,17 +587,15 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
         __syncthreads();
         constexpr int LANES = DP / 8, AT_ONCE = 64 / LANES;   // lanes of a row, rows of an instruction
         const int e = 8 * (lane % LANES);
+        uint32_t row = lane / LANES;
+        const uint32_t r = (uint32_t)r0 + 32 * wave + row, t = r / group;
+        uint32_t g = r - t * group;
+        bf16_t* to = a.out + (b.s.q0 + t) * a.out_token + (int64_t)(b.kv_head * group + g) * a.out_head + e;
+        const RowWalk walk(group, AT_ONCE, a.out_token, a.out_head);
 #pragma unroll
         for (int i = 0; i < 32 / AT_ONCE; i++) {
-            const int row = lane / LANES + AT_ONCE * i;
-            const int64_t r = r0 + 32 * wave + row;
-            if (r < r1 && e < a.dim) {
-                int32_t head;
-                const int32_t token = attention_token(a, r, head);
-                head += b.kv_head * a.group;
-                *reinterpret_cast<u32x4_t*>(a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e) =
-                    *reinterpret_cast<const u32x4_t*>(room + row * OUT + 2 * e);
-            }
+            if (r + AT_ONCE * i < r1 && e < a.dim) *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(room + (row + AT_ONCE * i) * OUT + 2 * e);
+            walk.next(to, g);
         }
     }
     // (this wavefront's stores above stay in front: these rows are written twice, and the second is what is left)
