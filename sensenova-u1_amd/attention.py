@@ -283,10 +283,11 @@ class PagedKVCache:
         """``(k, v)`` of ``slots`` (int64 [tokens]) as bf16 [tokens][kv_heads][dim]; a slot outside the cache gives zeros."""
         slots = _numbers(slots, torch.int64, None, "PagedKVCache.read", "slots")
         _same_device("PagedKVCache.read", self._index, slots)
-        k = torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=_BF16, device=self.k.device)
+        tokens = slots.shape[0]
+        k = self.k.new_empty((tokens, self.kv_heads, self.dim), dtype=_BF16)
         v = torch.empty_like(k)
-        if slots.shape[0]:
-            _launch(self._index, "sngguf_cache_read", self._address, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr())
+        if tokens:
+            _launch(self._index, "sngguf_cache_read", self._address, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
         return k, v
 
 

@@ -22,8 +22,8 @@
 //
 // Measured, 32 query and 8 key / value heads of 128: a prompt of 16384 tokens 1.85 .. 1.94 ms, 1.13 .. 1.19 PFLOP/s (matrix cores busy 59 % of
 // the cycles at 1.85 GHz; a large library product reaches 1.40 PFLOP/s); 1024 new tokens over 30000 in 8 bits 0.55 ms, 0.9 PFLOP/s.  A
-// workgroup costs 9 us beside its tiles, 1.8 us each.  Level or slower: 64 rows a wavefront (half the LDS reads), eight fragments
-// in the ring, a barrier that drains no reads, the two products in turn, 128 rows a workgroup (2.17 ms).
+// workgroup costs 8 us beside its tiles, 1.4 to 1.8 us each.  Level or slower: 64 rows a wavefront (half the LDS reads), eight
+// fragments in the ring, a barrier that drains no reads, the two products in turn, 128 rows a workgroup (2.17 ms).
 #include <type_traits>
 #include <utility>
 
@@ -280,9 +280,10 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     };
 
     // ---- the first tile's keys, this lane's row: its query as operand fragments, and the keys that it sees -----------------------
-    // Queries are asked for as tiles are, whole lines at a time (a lane that reads its own row takes a quarter of each line: 2.6 us until they
-    // were there, of a workgroup's 9 beside its tiles), each wavefront its own rows, into the room of the stages behind the
-    // first; or of all, if keys come through registers.  Nothing else is asked for before both are there.
+    // Queries are asked for as tiles are, whole lines at a time, each wavefront its own rows, into the room of the stages behind the first, or of
+    // all if keys come through registers (a lane that reads its own row takes a quarter of each line: seven prompts of 1 to 2047 tokens, 78.7 us, took
+    // 80.9).  Read by lanes where the room is too small, and for heads of 256, whose loop then took 4 % longer.  Nothing else is asked for
+    // before both are there.
     const int64_t my_row = r0 + 32 * wave + col;
     constexpr uint32_t kStage = 2 * TILE, kRing = NS * kStage;   // a stage: keys of tile i, values of tile i - 1
     constexpr bool QLDS = DT < 256 && (Q8 || (NS - 1) * kStage >= 4 * W * RB);
