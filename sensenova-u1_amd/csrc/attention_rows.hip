@@ -6,8 +6,8 @@
 // the bytes of the cache, so a workgroup's wavefronts read keys and values straight into registers, in the order in which
 // the matrix instructions want them, and never through LDS; each wavefront takes every fourth run of 32 keys with a maximum
 // and a sum of its own, and the four are joined at the end.  Sequences are split over workgroups where there are few.
-// Measured, 32 query and 8 key / value heads of 128: 24 tokens over 37 .. 9996 in 8 bits 46.7 us, 5.6 TB/s; one over 131071 in bf16
-// 94 us, 5.7 TB/s; the join 6 to 7 us more.
+// Measured, 32 query and 8 key / value heads of 128: 24 tokens over 37 .. 9996 in 8 bits 52 us, 5.0 TB/s; one over 131071 in bf16
+// 85 us, 6.3 TB/s (a kernel that only reads: 6.5); the join 5 to 6 us more.
 //
 // Per run of 32 keys and 16 rows (columns of the 16 x 16 x 32 instructions, lane % 16; lane group g = lane / 16):
 //  * scores: K (16 keys x dim) times Q^T.  The order in which dim is summed is free: in 8 bits lane group g takes elements

@@ -12,8 +12,7 @@
 //
 // All of it is bound by memory.  A workgroup takes a few tokens: its threads first make one (cosine, sine) pair each, in LDS,
 // then work through the tokens' heads in pieces of 16 bytes.  8192 tokens of 40 heads of 128: 35.7 us, 4.7 TB/s; 5003 tokens of 32 query
-// and 8 + 8 heads, keys and values written in 8 bits: 27 us, 4.2 TB/s; 40000 tokens read back: 42 us, 5.9 TB/s (61.6 where nothing of
-// it is in the last-level cache; nontemporal stores: 43 and 65).
+// and 8 + 8 heads, keys and values written in 8 bits: 27 us, 4.2 TB/s; 40000 tokens read back: 53 us, 4.7 TB/s (nontemporal stores: 58).
 #include "rotary_cache.hpp"
 
 namespace sngguf {
@@ -262,7 +261,8 @@ __global__ __launch_bounds__(kThreads) void rotary_cache_kernel(RotaryCacheArgs 
     }
 }
 
-// Slots of the cache as bf16 rows [tokens][kv_heads][dim]; a slot outside the cache gives zeros.
+// Slots of the cache as bf16 rows [tokens][kv_heads][dim]; a slot outside the cache gives zeros.  The cache with the read-once hint: 40000
+// tokens in 8 bits, another cache each pass, 53 us against 55 (the same one again at once, 55 against 48).
 template <bool Q8>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(RotaryCacheArgs a) {
     const int pieces = a.dim >> 3;
@@ -281,14 +281,14 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(RotaryCacheArgs a)
         u32x4_t v = {0u, 0u, 0u, 0u};
         if (slot >= 0 && slot < a.slot_count) {
             if constexpr (Q8) {
-                const u32x2_t q = *reinterpret_cast<const u32x2_t*>(static_cast<const int8_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e);
+                const u32x2_t q = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(static_cast<const int8_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e));
                 const float d = f16_to_f32(scales[((at * (a.dim >> 5) + (e >> 5)) << a.page_shift) + row]);
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = d * (float)(int8_t)(q[j >> 2] >> (8 * (j & 3)));
                 v = pack8(x);
             } else {
-                v = *reinterpret_cast<const u32x4_t*>(static_cast<const bf16_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e);
+                v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const bf16_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e));
             }
         }
         *reinterpret_cast<u32x4_t*>(out) = v;
