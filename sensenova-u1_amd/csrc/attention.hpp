@@ -295,8 +295,9 @@ __device__ __forceinline__ void attention_row_again(const AttentionArgs& a, cons
         else a.out[(b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e] = f32_to_bf16(o[t] * inv);
     }
     if (b.splits > 1 && lane == 0) {
+        // (a row whose scores are NaN has no maximum, and the join passes over splits without one: any number, so that the sum gets there)
         float* st = a.partial + a.grid * ROWS * DT + part * 2;
-        st[0] = m;
+        st[0] = l != l ? 0.f : m;
         st[1] = l * kBack;
     }
 }
