@@ -522,10 +522,12 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
                 for (int t = 0; t < PER; t++) o[t] *= keep;
 #pragma unroll
                 for (int k = 0; k < CHUNK; k++) {
+                    // (nothing is added for a slot behind the last split: what was read there may be an infinity, which a weight of zero makes NaN)
+                    const bool there = s0 + TEAMS * k < b.splits;
                     const float w = __builtin_amdgcn_exp2f(ms[k] - top);
-                    l += ls[k] * w;
+                    l += there ? ls[k] * w : 0.f;
 #pragma unroll
-                    for (int t = 0; t < PER; t++) o[t] += x[k][t] * w;
+                    for (int t = 0; t < PER; t++) o[t] += there ? x[k][t] * w : 0.f;
                 }
             }
         };

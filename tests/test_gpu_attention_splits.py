@@ -1,4 +1,4 @@
-"""Rows whose keys are split over workgroups: queries and keys that are not finite."""
+"""Rows whose keys are split over workgroups against the same rows in one: infinities with their signs, queries and keys that are not finite."""
 import pytest
 import torch
 
@@ -32,6 +32,54 @@ def _paged(dev, q, k, v, qt=ops.BF16, **options):
     cache.write(k.to(dev), v.to(dev), torch.arange(len(k), device=dev))
     pages = torch.arange(cache.pages, dtype=torch.int32, device=dev)[None]
     return paged_attention(q.to(dev), cache, pages, torch.tensor([len(k)], dtype=torch.int32, device=dev), _ends(len(q), dev), max_new=len(q), **options)
+
+
+def _unsplit(dev, q, k, v):
+    """Through the C entry point without a workspace."""
+    qd, kd, vd, ends_q, ends_k = q.to(dev), k.to(dev), v.to(dev), _ends(len(q), dev), _ends(len(k), dev)
+    out = torch.empty_like(qd)
+    assert ops.load_library().sngguf_attention(qd.data_ptr(), len(q), HEADS, HEADS * DIM, DIM, kd.data_ptr(), KV * DIM, DIM, vd.data_ptr(), KV * DIM, DIM, len(k), KV, DIM,
+                                               ends_q.data_ptr(), ends_k.data_ptr(), 1, DIM ** -0.5, 1, 0, out.data_ptr(), HEADS * DIM, DIM, None, 0,
+                                               torch.cuda.current_stream().cuda_stream) == 0
+    return out
+
+
+def _all_split(new):
+    lib = ops.load_library()
+    assert lib.sngguf_attention_workspace_bytes(new, KEYS, 1, HEADS, KV, DIM) > 0
+    assert lib.sngguf_paged_attention_workspace_bytes(new, 1, new, -(-KEYS // PAGE) * PAGE, HEADS, KV, DIM) > 0
+
+
+def _classes(q, k, v):
+    """1, -1 and 2 where the result is +infinity, -infinity and NaN: a value's weight is more than nothing wherever it is seen."""
+    seen = ao.visible(len(q), len(k), True, 0)
+    out = torch.zeros(q.shape, dtype=torch.int64)
+    for h in range(HEADS):
+        x = v[:, h // (HEADS // KV)]
+        up, down, none = ((seen.double() @ hit.double()) > 0 for hit in (x == INF, x == -INF, torch.isnan(x)))
+        out[:, h] = torch.where(none | (up & down), 2, up.long() - down.long())
+    return out
+
+
+@pytest.mark.parametrize("new", [1, 9, 30, 200])
+def test_infinities_keep_their_signs(dev, new):
+    """One in the first split, in a middle one, in the last, and some that only the last rows see."""
+    _all_split(new)
+    gen = torch.Generator().manual_seed(new)
+    q, k, v = _values(gen, new, HEADS), _values(gen, KEYS, KV), _values(gen, KEYS, KV)
+    bad = v.clone()
+    bad[5, :, 3], bad[4444, :, 4], bad[KEYS - 1, :, 5], bad[KEYS - 1, :, 6] = INF, -INF, INF, -INF
+    bad[100, :, 7], bad[8000, :, 7] = INF, -INF
+    bad[200, :, 8] = NAN
+    want, most = ao.attention(q, k, v)
+    classes = _classes(q, k, bad)
+    assert {1, -1, 2} <= set(classes.unique().tolist())
+    for name, call in (("unsplit", _unsplit), ("packed", _packed), ("paged", _paged)):
+        got = call(dev, q, k, bad).double().cpu()
+        found = torch.where(torch.isnan(got), 2, (got == INF).long() - (got == -INF).long())
+        assert torch.equal(found, classes), f"{name}: elements {(found != classes).any(0).any(0).nonzero().flatten().tolist()}"
+        fine = classes == 0
+        assert bool(((got - want).abs() <= most)[fine].all()), name
 
 
 @pytest.mark.parametrize("keys", [40, KEYS])
