@@ -285,20 +285,27 @@ __device__ __forceinline__ void attention_row_again(const AttentionArgs& a, cons
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
     const int64_t part = b.slot * ROWS + r - (int64_t)b.row_tile * ROWS;
+    // A partial result is in the scale of the other splits', or, where an element would leave fp32 there, as it is with a maximum higher by
+    // as much.
     constexpr float kBack = (float)(1ull << (31 + UP));
+    bool far = false;
+#pragma unroll
+    for (int t = 0; t < PER; t++) far |= __builtin_isfinite(o[t]) && !__builtin_isfinite(o[t] * kBack);
+    far = __any(far);
+    const float back = far ? 1.f : kBack;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int t = 0; t < PER; t++) {
         const int e = lane + 64 * t;
         if (e >= a.dim) continue;
-        if (b.splits > 1) a.partial[part * DT + e] = o[t] * kBack;
+        if (b.splits > 1) a.partial[part * DT + e] = o[t] * back;
         else a.out[(b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e] = f32_to_bf16(o[t] * inv);
     }
     if (b.splits > 1 && lane == 0) {
         // (a row whose scores are NaN has no maximum, and the join passes over splits without one: any number, so that the sum gets there)
         float* st = a.partial + a.grid * ROWS * DT + part * 2;
-        st[0] = l != l ? 0.f : m;
-        st[1] = l * kBack;
+        st[0] = l != l ? 0.f : far ? m + (31 + UP) : m;
+        st[1] = l * back;
     }
 }
 

@@ -484,16 +484,19 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
     const int rows = left < ROWS ? (int)left : ROWS;
     // (the launch has as many workgroups as the caller takes for the most rows; more rows are taken in turn)
     for (int row = WIDE ? blockIdx.y : blockIdx.y * kWaves + wave; row < rows; row += gridDim.y * (WIDE ? 1 : kWaves)) {
-        float o[PER], l = 0.f, m = -__builtin_inff();
+        float o[PER], l, m;
+        // splits first, first + step ..., their weights scaled by `down`
+        auto join = [&](auto chunk_, int first, auto step_, float down) {
+            constexpr int CHUNK = decltype(chunk_)::value, STEP = decltype(step_)::value;
+            l = 0.f;
+            m = -__builtin_inff();
 #pragma unroll
-        for (int t = 0; t < PER; t++) o[t] = 0.f;
-        auto join = [&](auto chunk_) {
-            constexpr int CHUNK = decltype(chunk_)::value;
-            for (int s0 = team; s0 < b.splits; s0 += CHUNK * TEAMS) {
+            for (int t = 0; t < PER; t++) o[t] = 0.f;
+            for (int s0 = first; s0 < b.splits; s0 += CHUNK * STEP) {
                 float ms[CHUNK], ls[CHUNK], x[CHUNK][PER];
 #pragma unroll
                 for (int k = 0; k < CHUNK; k++) {
-                    const int s = s0 + TEAMS * k;
+                    const int s = s0 + STEP * k;
                     const int64_t at = (b.slot + (int64_t)(s < b.splits ? s : s0) * a.kv_heads) * ROWS + row;
                     const float2 st = *reinterpret_cast<const float2*>(stats + at * 2);
                     ms[k] = s < b.splits ? st.x : -__builtin_inff();
@@ -523,17 +526,30 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
 #pragma unroll
                 for (int k = 0; k < CHUNK; k++) {
                     // (nothing is added for a slot behind the last split: what was read there may be an infinity, which a weight of zero makes NaN)
-                    const bool there = s0 + TEAMS * k < b.splits;
-                    const float w = __builtin_amdgcn_exp2f(ms[k] - top);
+                    const bool there = s0 + STEP * k < b.splits;
+                    const float w = __builtin_amdgcn_exp2f(ms[k] - top) * down;
                     l += there ? ls[k] * w : 0.f;
 #pragma unroll
                     for (int t = 0; t < PER; t++) o[t] += there ? x[k][t] * w : 0.f;
                 }
             }
         };
-        if (!WIDE || b.splits <= 2 * TEAMS) join(std::integral_constant<int, 2>());
-        else join(std::integral_constant<int, DT == 256 ? 8 : 16>());
-        // the teams' results: in LDS, or the wavefront's two halves
+        // the wavefront's two halves
+        auto join_halves = [&] {
+            const float other = __shfl_xor(m, 32), top = fmaxf(m, other);
+            const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            l *= f;
+            l += __shfl_xor(l, 32);
+#pragma unroll
+            for (int t = 0; t < PER; t++) {
+                o[t] *= f;
+                o[t] += __shfl_xor(o[t], 32);
+            }
+        };
+        typedef std::integral_constant<int, TEAMS> Teams;
+        if (!WIDE || b.splits <= 2 * TEAMS) join(std::integral_constant<int, 2>(), team, Teams(), 1.f);
+        else join(std::integral_constant<int, DT == 256 ? 8 : 16>(), team, Teams(), 1.f);
+        // the teams' results: in LDS, or the halves
         if constexpr (WIDE) {
 #pragma unroll
             for (int t = 0; t < PER; t++) part[team][e + t] = o[t];
@@ -555,14 +571,17 @@ __global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionAr
                 }
             }
         } else {
-            const float other = __shfl_xor(m, 32), top = fmaxf(m, other);
-            const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            l *= f;
-            l += __shfl_xor(l, 32);
+            join_halves();
+        }
+        // Splits whose sums are within fp32 can have one together that is not: a row that is not finite is joined again, by one wavefront, with
+        // weights so small that the sums of all splits (at most as many as there are workgroups, below 2^16) stay there.
+        if (!WIDE || wave == 0) {
+            float odd = l * 0.f;
 #pragma unroll
-            for (int t = 0; t < PER; t++) {
-                o[t] *= f;
-                o[t] += __shfl_xor(o[t], 32);
+            for (int t = 0; t < PER; t++) odd = __builtin_fmaf(o[t], 0.f, odd);
+            if (__any(odd != 0.f && e < a.dim)) {
+                join(std::integral_constant<int, 2>(), half, std::integral_constant<int, 2>(), 0x1p-16f);
+                join_halves();
             }
         }
         if ((!WIDE || wave == 0) && half == 0 && e < a.dim) {

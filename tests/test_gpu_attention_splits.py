@@ -1,4 +1,5 @@
-"""Rows whose keys are split over workgroups against the same rows in one: infinities with their signs, queries and keys that are not finite."""
+"""Rows whose keys are split over workgroups against the same rows in one: sums beyond fp32 whose averages are not, infinities with their
+signs, and queries that are not finite."""
 import pytest
 import torch
 
@@ -48,6 +49,20 @@ def _all_split(new):
     lib = ops.load_library()
     assert lib.sngguf_attention_workspace_bytes(new, KEYS, 1, HEADS, KV, DIM) > 0
     assert lib.sngguf_paged_attention_workspace_bytes(new, 1, new, -(-KEYS // PAGE) * PAGE, HEADS, KV, DIM) > 0
+
+
+@pytest.mark.parametrize("new", [1, 9, 30, 200])
+@pytest.mark.parametrize("power", [127, 117])
+def test_sums_beyond_fp32(dev, new, power):
+    """Weights that are nearly equal: with values near 2^127 a split's own sum leaves fp32, with values near 2^117 only that of all splits does."""
+    _all_split(new)
+    gen = torch.Generator().manual_seed(new)
+    q, k = (_values(gen, new, HEADS).float() * 0.1).to(torch.bfloat16), _values(gen, KEYS, KV)
+    v = (_values(gen, KEYS, KV).float().abs().clamp(0.5, 1) * 2.0 ** power).to(torch.bfloat16)
+    want, most = ao.attention(q, k, v)
+    for name, call in (("unsplit", _unsplit), ("packed", _packed), ("paged", _paged)):
+        off = (call(dev, q, k, v).double().cpu() - want).abs()
+        assert bool((off <= most).all()), f"{name}: {int((~(off <= most)).sum())} of {off.numel()} values are off"
 
 
 def _classes(q, k, v):
