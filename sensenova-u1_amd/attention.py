@@ -169,7 +169,7 @@ class RotaryTable:
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: RotaryTable, inplace: bool = False):
     """Queries and keys turned by their positions: ``(q, k)``, new tensors or with ``inplace`` the given ones.
 
-    q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None.  positions: int64 [tokens].  A model whose head
+    q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None, either may have no heads.  positions: int64 [tokens].  A model whose head
     has parts with positions of their own calls it on views of the parts.  In place, no two rows may share an element."""
     q0, k0 = q, k
     q, qt, qh = _heads(q, "rotary", "q")
@@ -187,12 +187,15 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         raise SnGgufError("rotary: in place needs rows that share no element")
     q_out, qot, qoh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
     k_out = k if inplace or k is None else _new(k)
+    if k is None or not k.shape[1]:
+        rest = (None, 0, 0, 0, None, 0, 0)
+    else:
+        rest = (k.data_ptr(), k.shape[1], kt, kh, k_out.data_ptr(), *((kt, kh) if inplace else (k.shape[1] * dim, dim)))
+    first = (q.data_ptr(), heads, qt, qh, q_out.data_ptr(), qot, qoh)
+    if not heads:                       # keys alone: in the queries' place
+        first, rest, heads = rest, (None, 0, 0, 0, None, 0, 0), rest[1]
     if tokens and heads:
-        if k is None:
-            rest = (None, 0, 0, 0, None, 0, 0)
-        else:
-            rest = (k.data_ptr(), k.shape[1], kt, kh, k_out.data_ptr(), *((kt, kh) if inplace else (k.shape[1] * dim, dim)))
-        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, q.data_ptr(), heads, qt, qh, q_out.data_ptr(), qot, qoh, *rest)
+        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, *first, *rest)
     return q_out, k_out
 
 
