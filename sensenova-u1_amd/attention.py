@@ -112,6 +112,59 @@ def _apart(x: torch.Tensor) -> bool:
     return True
 
 
+def _places(x: torch.Tensor):
+    """Where the rows of ``x`` [tokens][heads][dim] lie: (address, ((count, stride) of each axis), length of a row), in bytes."""
+    size = x.element_size()
+    return x.data_ptr(), [(x.shape[i], x.stride(i) * size) for i in (0, 1) if x.shape[i] > 1 and x.stride(i)], x.shape[2] * size
+
+
+def _whole(x: torch.Tensor):
+    """The same of a contiguous tensor: one row."""
+    return x.data_ptr(), [], x.numel() * x.element_size()
+
+
+def _share(a, b) -> bool:
+    """Whether a row of ``a`` and one of ``b`` (of ``_places``) have a byte in common."""
+    (a_at, a_axes, a_row), (b_at, b_axes, b_row) = a, b
+    off = b_at - a_at
+
+    def reach(axes, row):
+        return sum((n - 1) * s for n, s in axes) + row
+
+    if off >= reach(a_axes, a_row) or -off >= reach(b_axes, b_row):
+        return False
+    # interleaved, as the parts of a stacked projection are: what lies within some strides repeats at every multiple of what divides the longer ones
+    for least in sorted({s for _, s in a_axes + b_axes}):
+        every = math.gcd(*(s for _, s in a_axes + b_axes if s >= least))
+        a_reach, b_reach = (reach([x for x in axes if x[1] < least], row) for axes, row in ((a_axes, a_row), (b_axes, b_row)))
+        if a_reach <= off % every <= every - b_reach:
+            return False
+    # row by row
+    starts = []
+    for at, axes in ((0, a_axes), (off, b_axes)):
+        rows = torch.tensor([at], dtype=torch.int64)
+        for n, s in axes:
+            rows = (rows[:, None] + torch.arange(n, dtype=torch.int64) * s).flatten()
+        starts.append(rows)
+    rows = starts[0].sort().values
+    behind = torch.searchsorted(rows, starts[1], right=True)
+    before = rows[(behind - 1).clamp(min=0)]
+    after = rows[behind.clamp(max=len(rows) - 1)]
+    return bool((((behind > 0) & (starts[1] - before < a_row)) | ((behind < len(rows)) & (after - starts[1] < b_row))).any())
+
+
+def _rows_share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows of two bf16 [tokens][heads][dim] share an element."""
+    (n, heads, dim), (t, h, _), (_, b_heads, b_dim), (b_t, b_h, _) = a.shape, a.stride(), b.shape, b.stride()
+    if not n or t != b_t or n != b.shape[0]:
+        return _share(_places(a), _places(b))
+    # the usual case, parts of one projection's output, without the rest (11 us, as much as a call)
+    off, reach, b_reach = (b.data_ptr() - a.data_ptr()) // 2, (heads - 1) * h + dim, (b_heads - 1) * b_h + b_dim
+    if off >= (n - 1) * t + reach or -off >= (n - 1) * t + b_reach or (t and reach <= off % t <= t - b_reach):
+        return False
+    return _share(_places(a), _places(b))
+
+
 def _numbers(x: torch.Tensor, dtype: torch.dtype, count: Optional[int], what: str, name: str) -> torch.Tensor:
     if x.dtype != dtype or x.dim() != 1 or (count is not None and x.shape[0] != count):
         raise SnGgufError(f"{what}: {name} must be {dtype} [{count if count is not None else 'n'}], got {x.dtype} {tuple(x.shape)}")
@@ -183,7 +236,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             raise SnGgufError(f"rotary: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
     if inplace and (q is not q0 or k is not k0):
         raise SnGgufError("rotary: in place needs the elements of a head next to each other")
-    if inplace and not (_apart(q) and (k is None or (_apart(k) and (k.data_ptr() != q.data_ptr() or not k.numel())))):
+    if inplace and not (_apart(q) and (k is None or (_apart(k) and not (q.numel() and k.numel() and _rows_share(q, k))))):
         raise SnGgufError("rotary: in place needs rows that share no element")
     q_out, qot, qoh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
     k_out = k if inplace or k is None else _new(k)
@@ -272,7 +325,7 @@ class PagedKVCache:
         tokens, heads, dim = q.shape
         if k.shape[0] != tokens or dim != self.dim:
             raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
-        if inplace and (q is not q0 or not _apart(q) or (q.data_ptr() in (k.data_ptr(), v.data_ptr()) and q.numel())):
+        if inplace and (q is not q0 or not _apart(q) or (q.numel() and (_rows_share(q, k) or _rows_share(q, v)))):
             raise SnGgufError(f"{what}: in place needs rows that share no element, the elements of a head next to each other")
         positions = _numbers(positions, torch.int64, tokens, what, "positions")
         _same_device(what, self._index, q, positions, table.turns)
@@ -294,8 +347,8 @@ class PagedKVCache:
         return k, v
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, *others: torch.Tensor):
-    """(out, its token and head strides)"""
+def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, k: torch.Tensor, v: torch.Tensor, *scales: Optional[torch.Tensor]):
+    """(out, its token and head strides); k, v: packed rows, or the halves of a cache"""
     tokens, heads, dim = q.shape
     if out is None:
         return _new(q), heads * dim, dim
@@ -304,8 +357,9 @@ def _output(out: Optional[torch.Tensor], q: torch.Tensor, what: str, *others: to
     rows, t, h = _heads(out, what, "out", True)
     if rows is not out:
         raise SnGgufError(f"{what}: out must have rows of whole 16-byte pieces")
-    if out.numel() and (not _apart(out) or out.data_ptr() in [x.data_ptr() for x in (q, *others)]):
-        raise SnGgufError(f"{what}: out must not overlap itself or an input")
+    if out.numel():
+        if not _apart(out) or any(_rows_share(out, x) if len(x.shape) == 3 else _share(_places(out), _whole(x)) for x in (q, k, v, *scales) if x is not None and x.numel()):
+            raise SnGgufError(f"{what}: out must not overlap itself or an input")
     return out, t, h
 
 
@@ -387,7 +441,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     elif tokens != sequences:
         raise SnGgufError(f"{what}: {tokens} queries of {sequences} sequences need ends_q")
     _same_device(what, cache._index, q, pages, lens, ends_q)
-    out, ot, oh = _output(out, q, what, cache.k, cache.v)
+    out, ot, oh = _output(out, q, what, cache.k, cache.v, cache.k_scale, cache.v_scale)
     if tokens and sequences:
         if ends_q is None:
             max_new = 1
