@@ -51,7 +51,7 @@ __device__ __forceinline__ f16x2_t whole_pair(uint32_t flipped) {
     return __builtin_bit_cast(f16x2_t, w) + f16x2_t{(_Float16)-1152.f, (_Float16)-1152.f};
 }
 
-// Words of the cache that a workgroup reads once, and no other does
+// Words of the cache; ONCE: that one workgroup reads once, and no other does
 template <bool ONCE, typename T> __device__ __forceinline__ T word_at(const uint8_t* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
     else return *reinterpret_cast<const T*>(p);
@@ -75,10 +75,14 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     constexpr int KR = DT / 128 > 0 ? DT / 128 : 1;   // scales of a key
     constexpr int VW = Q8 ? VP / 4 : VP / 2;          // dwords of a value
     constexpr int E = Q8 ? 1 : 2;           // bytes of an element
-    // With the read-once hint where a line is not asked for again much later (wider heads take a line in four requests, heads between two
-    // kernels read pieces in place of those behind them).  16 tokens over 8000, each over a cache of its own: 128 elements in bf16 94 us
-    // against 103, in 8 bits 59 against 64; 96 in bf16 84 against 81, 256 in 8 bits 134 against 112.
-    constexpr bool ONCE = FULL && DT <= 128;
+    // Pages that no other sequence has are read with the read-once hint, where a line is not asked for again much later (wider heads take a line
+    // in four requests, heads between two kernels read pieces in place of those behind them).  16 tokens over 8000, each over a cache of
+    // its own: 128 elements in bf16 92 us against 101, in 8 bits 59 against 62; 96 in bf16 84 against 81, 256 in 8 bits 134 against
+    // 112.  Pages that sequences share come from a cache but for the first time: with the hint 8 sequences with 32768 tokens in common took
+    // 141 us instead of 91 (8 bits 87, 70).  Who shares is asked only by tiles of 16 rows: a loop with both kinds of loads has four new
+    // tokens each over 8000 2 to 5 % slower (60 us instead of 76 with the 8000 in common), eight new ones, in 32 rows, 6 to 12 %.  Heads of 64 in
+    // 8 bits do not ask, which lose as much as they gain (16 over 8000 34.8 us, asking 37.4; 8 with 32768 in common 50.0, 48.0).
+    constexpr bool HINT = FULL && DT <= 128, ASK = HINT && NT == 1 && !(Q8 && DT == 64);
     constexpr float kUp = Q8 ? 12.f : 0.f;
     constexpr float kLimit = Q8 ? 32768.f : 1e9f;
     extern __shared__ __attribute__((aligned(16))) float lds[];   // [wave][16][DT] sums, then [wave][ROWS][2]
@@ -122,7 +126,8 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     uint16_t k_scale[2][KR];
     uint32_t v_raw[8][VW];
     u32x4_t v_scale;
-    auto load_keys = [&](int32_t key0, int32_t page) {
+    auto load_keys_as = [&](auto once_, int32_t key0, int32_t page) {
+        constexpr bool ONCE = decltype(once_)::value;
         const int64_t at = (int64_t)page * a.kv_heads + b.kv_head;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -137,7 +142,8 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
             }
         }
     };
-    auto load_values = [&](int32_t key0, int32_t page) {
+    auto load_values_as = [&](auto once_, int32_t key0, int32_t page) {
+        constexpr bool ONCE = decltype(once_)::value;
         const int64_t at = (int64_t)page * a.kv_heads + b.kv_head;
         const int32_t lead = key0 + v_key < most ? key0 + v_key : most, row = lead & page_mask & ~7;
         const uint8_t* p = static_cast<const uint8_t*>(a.v_pages) + ((at << a.page_shift) + row) * (dim * E) + E * v_e;
@@ -168,11 +174,42 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         }
         if constexpr (Q8) v_scale = *reinterpret_cast<const u32x4_t*>(a.v_scales + ((at * (dim >> 5) + (v_e >> 5)) << a.page_shift) + row);
     };
+    typedef std::integral_constant<bool, false> Often;
+    typedef std::integral_constant<bool, true> Once;
+    bool once = false;
+    // (the marks keep the compiler from making one load without the hint of the two)
+    auto load_keys = [&](int32_t key0, int32_t page) {
+        if constexpr (!ASK) {
+            load_keys_as(std::integral_constant<bool, HINT>(), key0, page);
+        } else if (once) {
+            load_keys_as(Once(), key0, page);
+            asm volatile("; once");
+        } else {
+            load_keys_as(Often(), key0, page);
+        }
+    };
+    auto load_values = [&](int32_t key0, int32_t page) {
+        if constexpr (!ASK) {
+            load_values_as(std::integral_constant<bool, HINT>(), key0, page);
+        } else if (once) {
+            load_values_as(Once(), key0, page);
+            asm volatile("; once");
+        } else {
+            load_values_as(Often(), key0, page);
+        }
+    };
     int32_t key0 = s0 * kKeys + wave * kRun;
     int32_t page_k = 0, page_v = 0;
     if (key0 < end) {
         page_k = page_of(key0 + (k_key & ~7));
         page_v = page_of(key0 + v_key);
+        if constexpr (ASK) {
+            // this split's first page, and what up to 63 other sequences have in its place: a common prompt is at the same place in all tables
+            const int32_t other = (b.seq & ~63) + lane, at = (s0 * kKeys) >> a.page_shift;
+            const bool there = other < a.sequences && other != b.seq;
+            const int32_t mine = table[at], theirs = a.table[(int64_t)(there ? other : b.seq) * a.table_stride + at];
+            once = __ballot(there && theirs == mine) == 0;
+        }
         load_keys(key0, page_k);
         load_values(key0, page_v);
         page_k = page_of(key0 + kKeys + (k_key & ~7));
