@@ -502,13 +502,36 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     }
 }
 
+// A lane's elements of a row that is not finite again, split by split: what was read for a split behind the last may be an infinity, which a
+// weight of zero makes NaN, and splits whose sums are within fp32 can have one together that is not, unless all weights are that
+// much smaller (there are at most as many splits as workgroups, below 2^16).  A function of its own: in line it takes registers from the
+// loads under way (three workgroups a compute unit instead of four: 16 sequences of 8 new tokens over 8000 84 us instead of 79).
+template <int PER>
+__device__ __attribute__((noinline)) void join_row_again(const float* stats, const float* part, int step, int dim, int splits, bf16_t* out) {
+    float o[PER], l = 0.f, m = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < PER; t++) o[t] = 0.f;
+    for (int s = 0; s < splits; s++) {
+        const int64_t at = (int64_t)s * step;
+        const float ms = stats[at * 2], ls = stats[at * 2 + 1], top = fmaxf(m, ms);
+        if (top == -__builtin_inff()) continue;
+        const float keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(ms - top) * 0x1p-16f;
+        m = top;
+        l = l * keep + ls * w;
+#pragma unroll
+        for (int t = 0; t < PER; t++) o[t] = o[t] * keep + part[at * dim + t] * w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int t = 0; t < PER; t += 2) *reinterpret_cast<uint32_t*>(out + t) = pack_bf16(o[t] * inv, o[t + 1] * inv);
+}
+
 // Joins the splits of rows.  WIDE: a workgroup a row; else a wavefront a row.  Half a wavefront lies along the row's elements and
 // takes some splits at a time, all of whose words are asked for before any is used (behind the last split, those of the first
 // again: a branch around a load would have the loads wait for each other): the launch is one latency long, and what it
 // reads is little.
-// (Three workgroups a compute unit instead of four: 16 sequences of 8 new tokens 84 us against 79.)
 template <int ROWS, int KEYS, int DT, bool WIDE>
-__global__ __launch_bounds__(kThreads, 4) void attention_combine_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kThreads) void attention_combine_kernel(AttentionArgs a) {
     constexpr int PER = DT / 32;            // elements of a lane
     constexpr int TEAMS = WIDE ? 2 * kWaves : 2;
     __shared__ float part[WIDE ? TEAMS : 1][DT + 2];
@@ -567,21 +590,9 @@ __global__ __launch_bounds__(kThreads, 4) void attention_combine_kernel(Attentio
                 }
             }
         };
-        // the wavefront's two halves
-        auto join_halves = [&] {
-            const float other = __shfl_xor(m, 32), top = fmaxf(m, other);
-            const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            l *= f;
-            l += __shfl_xor(l, 32);
-#pragma unroll
-            for (int t = 0; t < PER; t++) {
-                o[t] *= f;
-                o[t] += __shfl_xor(o[t], 32);
-            }
-        };
         if (!WIDE || b.splits <= 2 * TEAMS) join(std::integral_constant<int, 2>());
         else join(std::integral_constant<int, DT == 256 ? 8 : 16>());
-        // the teams' results: in LDS, or the halves
+        // the teams' results: in LDS, or the wavefront's two halves
         if constexpr (WIDE) {
 #pragma unroll
             for (int t = 0; t < PER; t++) part[team][e + t] = o[t];
@@ -603,35 +614,19 @@ __global__ __launch_bounds__(kThreads, 4) void attention_combine_kernel(Attentio
                 }
             }
         } else {
-            join_halves();
-        }
-        // A row that is not finite is joined again, by one wavefront, split by split: what was read for a split behind the last may be an
-        // infinity, which a weight of zero makes NaN, and splits whose sums are within fp32 can have one together that is not, unless all weights
-        // are that much smaller (there are at most as many splits as workgroups, below 2^16).
-        if (!WIDE || wave == 0) {
-            float odd = l * 0.f;
+            const float other = __shfl_xor(m, 32), top = fmaxf(m, other);
+            const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            l *= f;
+            l += __shfl_xor(l, 32);
 #pragma unroll
-            for (int t = 0; t < PER; t++) odd = __builtin_fmaf(o[t], 0.f, odd);
-            if (__any(odd != 0.f && e < a.dim)) {
-                l = 0.f;
-                m = -__builtin_inff();
-#pragma unroll
-                for (int t = 0; t < PER; t++) o[t] = 0.f;
-                int here = lane;
-                asm volatile("" : "+v"(here));     // (or what this needs is formed in front of every row and held in registers)
-                for (int s = here >> 5; s < b.splits; s += 2) {
-                    const int64_t at = (b.slot + (int64_t)s * a.kv_heads) * ROWS + row;
-                    const float ms = stats[at * 2], ls = stats[at * 2 + 1], top = fmaxf(m, ms);
-                    if (top == -__builtin_inff()) continue;
-                    const float keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(ms - top) * 0x1p-16f;
-                    m = top;
-                    l = l * keep + ls * w;
-#pragma unroll
-                    for (int t = 0; t < PER; t++) o[t] = o[t] * keep + a.partial[at * DT + PER * (here & 31) + t] * w;
-                }
-                join_halves();
+            for (int t = 0; t < PER; t++) {
+                o[t] *= f;
+                o[t] += __shfl_xor(o[t], 32);
             }
         }
+        float odd = l * 0.f;
+#pragma unroll
+        for (int t = 0; t < PER; t++) odd = __builtin_fmaf(o[t], 0.f, odd);
         if ((!WIDE || wave == 0) && half == 0 && e < a.dim) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t r = r0 + row;
@@ -641,6 +636,8 @@ __global__ __launch_bounds__(kThreads, 4) void attention_combine_kernel(Attentio
             bf16_t* out = a.out + (b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e;
 #pragma unroll
             for (int t = 0; t < PER; t += 2) *reinterpret_cast<uint32_t*>(out + t) = pack_bf16(o[t] * inv, o[t + 1] * inv);
+            if (odd != 0.f)
+                join_row_again<PER>(stats + (b.slot * ROWS + row) * 2, a.partial + (b.slot * ROWS + row) * DT + e, a.kv_heads * ROWS, DT, b.splits, out);
         }
         if constexpr (WIDE) __syncthreads();       // (part is written again)
     }
