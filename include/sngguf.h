@@ -454,8 +454,8 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
  * Attention of packed sequences: sequence i has the queries [ends_q[i], ends_q[i + 1]) and the keys [ends_k[i], ends_k[i + 1])
  * (device, [sequences + 1], not decreasing).  out = softmax(scale q . k) v, each query over the keys that it sees: all, or
  * with causal != 0 those up to its own place, the last query standing at the last key; with window > 0 (causal only) the last
- * `window` of them.  A query that sees no key gives zeros.  Rows of q behind the last sequence are not read, those of out not
- * written.  heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads).  dim: a multiple of 32 up to 256.
+ * `window` of them.  A query that sees no key, or only keys whose scores are minus infinity, gives zeros.  Rows of q behind
+ * the last sequence are not read, those of out not written.  heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads).  dim: a multiple of 32 up to 256.
  * q, k, v, out: rows of whole 16-byte pieces.  Scores, maxima and sums are fp32, the weights are rounded to bf16 for the product
  * with v.  A key or value that is not finite reaches the queries that see it and no others (their rows are done a second time, key by key: slowly).
  * out must not overlap q, k or v.

@@ -3,8 +3,9 @@
 Every case goes through the entry points a user's program calls: the module that a checkpoint's Linear becomes
 (``GGUFLinear``), a decoder layer as the loader leaves it (q / k / v on one stacked weight, the fused MLP forward), the
 helpers that fold norms and residual adds in, the launcher for mixed text and image rows, the greedy token step on the
-vocabulary projection, and the standalone decoder.  Attention, rope and sampling belong to the model that uses the
-framework and are not here; streaming layers from host memory is bound by the host link and is not here either.
+vocabulary projection, and the standalone decoder.  Rotary positions, the paged cache and attention are timed in
+``operators.py``; sampling belongs to the model that uses the framework and is not here; streaming layers from host memory
+is bound by the host link and is not here either.
 
 Kinds of case
 * ``linear``     one projection, ``rows`` activation rows, with or without bias;

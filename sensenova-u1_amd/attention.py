@@ -8,6 +8,7 @@ stacked projection's output go in as they are.  Forward only: nothing here recor
 A layer's attention for new tokens of sequences that lie in a cache::
 
     q, k, v = (y.view(tokens, -1, dim) for y in qkv(hidden, norm_weight, eps))     # FusedProjections
+    q, k = q_norm(q), k_norm(k)          # the model's own, where it norms single heads: nothing here does
     q = cache.write_rotary(q, k, v, positions, table, slots)
     out = paged_attention(q, cache, pages, lens, ends)                              # [tokens][heads][dim]
     hidden = o_proj.forward_residual(out.view(tokens, -1), hidden)
@@ -383,7 +384,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
 
     q [tokens][heads][dim], k and v [keys][kv_heads][dim], ``heads`` a multiple of ``kv_heads``, ``dim`` a multiple of 32 up to
     256.  Causal: the last query of a sequence stands at its last key, and none sees a key behind its own place; ``window`` > 0: only the last
-    ``window`` keys up to it.  A query that sees nothing gives zeros, and keys and values that a query does not see
+    ``window`` keys up to it.  A query that sees nothing, or only scores of minus infinity, gives zeros, and keys and values that a query does not see
     have no part in its result, whatever they hold.  ``scale`` defaults to dim ** -0.5.  Rows of ``out`` behind the last sequence are not
     written; ``out`` overlaps no input."""
     what = "prompt_attention"

@@ -139,8 +139,8 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t max_new, int64_t
     const int64_t group = heads / kv_heads;
     const int64_t most = (max_new > 0 && max_new < tokens ? max_new : tokens) * group;
     // a tile of 64 rows leaves a SIMD one wavefront: it pays where sequences are few and their keys split finer than the other kernel's
-    // (16 new tokens of 4 heads a group: one sequence of 30000 in bf16 39 us against 66, four of 8000 47 against 48, 16 of
-    // 8000 147 against 120)
+    // (16 new tokens of 4 heads a group, caches in turn, 8 bits / bf16: one sequence of 30000 45 / 44 us against 73 / 74, four of 8000
+    // 53 / 52 against 56 / 55, eight 82 / 83 against 72 / 73, sixteen 142 / 149 against 118 / 121)
     const int d = kernel_dim(dim), widest = d == 256 || sequences * kv_heads > 32 ? 32 : 64;
     // one kernel where no sequence has more rows than its tile; else single tokens and chunks each have their own
     const int64_t r = most <= widest ? most : group;

@@ -6,8 +6,10 @@
 // the bytes of the cache, so a workgroup's wavefronts read keys and values straight into registers, in the order in which
 // the matrix instructions want them, and never through LDS; each wavefront takes every fourth run of 32 keys with a maximum
 // and a sum of its own, and the four are joined at the end.  Sequences are split over workgroups where there are few.
-// Measured, 32 query and 8 key / value heads of 128: 24 tokens over 37 .. 9996 in 8 bits 52 us, 5.0 TB/s; one over 131071 in bf16
-// 85 us, 6.3 TB/s (a kernel that only reads: 6.5); the join 5 to 6 us more.
+// Measured, 32 query and 8 key / value heads of 128: 24 tokens over 37 .. 9996 in 8 bits 49.5 us, 5.3 TB/s; one over 131071 in bf16
+// 80 us, 6.6 TB/s (the same cache each time, which stays in the last-level cache in part; a kernel that only reads: 6.5); the join 6 to 7
+// us more.  Short runs of new tokens are bound by their arithmetic, which one or two wavefronts a SIMD do not overlap: 8 new tokens each of 16
+// sequences of 8000 in 8 bits 3.5 TB/s, 16 of 4 1.3.
 //
 // Per run of 32 keys and 16 rows (columns of the 16 x 16 x 32 instructions, lane % 16; lane group g = lane / 16):
 //  * scores: K (16 keys x dim) times Q^T.  The order in which dim is summed is free: in 8 bits lane group g takes elements
@@ -16,8 +18,13 @@
 //  * so a lane's eight scores are of keys 8 g .. 8 g + 7, which is how the second product wants them: V^T (16 elements x 32
 //    keys) times P^T, where lane group g holds keys 8 g .. 8 g + 7.  A lane reads DT / 16 neighbouring elements of those eight
 //    rows, and instruction t takes element t of each.
-// An 8-bit cache is widened to fp16 (whole numbers are exact there, the product with the scale is rounded to 11 bits; values are
-// within fp16 by the format) and multiplied in fp16, with p scaled by 2^12: p down to 2^-36 of the largest still counts.
+// What is rounded: in bf16 the weights, to bf16, for the product with the values (the matrix instructions take both operands in one type;
+// weights in two parts would be twice the instructions).  It is most of the error: one token over 131071 is off by 0.0023 of its norm from the
+// definition, where fp32 weights and a result in bf16 are off by 0.0017.  An 8-bit cache is widened to fp16 (whole numbers are
+// exact there, the product with the scale is rounded to 11 bits; values are within fp16 by the format) and multiplied in fp16, queries scaled
+// into it by a power of two, with p scaled by 2^12: p down to 2^-36 of the largest still counts, and 11 bits are enough: 0.0017.
+// The sum of a row's weights is of the fp32 ones: their roundings are to the nearest and cancel in a long sum, and the sum is done while the
+// rounded ones are still being packed.  Scores, maxima, sums and the values' sums are fp32.
 #include <type_traits>
 
 #include "attention.hpp"

@@ -127,3 +127,21 @@ def test_keys_that_are_all_nan(dev, keys, new):
     for call in (_packed, _paged):
         got = call(dev, q, k, v).cpu()
         assert bool(torch.isnan(got[:, 2:]).all()) and bool(torch.isfinite(got[:, :2].float()).all())
+
+
+@pytest.mark.parametrize("keys", [40, KEYS])
+@pytest.mark.parametrize("new", [1, 30])
+def test_scores_of_minus_infinity(dev, keys, new):
+    """They have no weight: a row with one other key is that key's value, a row without any is zeros."""
+    gen = torch.Generator().manual_seed(new)
+    q, k, v = _values(gen, new, HEADS), _values(gen, keys, KV), _values(gen, keys, KV)
+    q[:, :, 2] = q[:, :, 2].abs() + 1
+    k[:, :, 2] = -INF
+    for one in (False, True):
+        if one:
+            k[3, 1] = 0.5
+        want = torch.zeros_like(q)
+        want[:, 2:] = v[3, 1] if one else 0
+        for name, call in (("unsplit", _unsplit), ("packed", _packed), ("paged", _paged)):
+            got = call(dev, q, k, v).cpu()
+            assert bool(((got.double() - want.double()).abs() <= 2.0 ** -8 * want.double().abs()).all()), (name, one)
