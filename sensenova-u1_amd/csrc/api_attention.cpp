@@ -21,6 +21,9 @@ using sngguf::RotaryCacheArgs;
 constexpr int64_t kMost = (int64_t)1 << 31;           // tokens, heads, pages: numbered with 32 bits
 constexpr int64_t kMostStride = (int64_t)1 << 26;     // elements between tokens: sixteen rows within 32-bit byte offsets
 
+// Threads of a launch are numbered with 32 bits.
+bool launch_fits(int64_t workgroups, int64_t threads) { return workgroups < kMost && workgroups * threads < (int64_t)1 << 32; }
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 int check_cache(const sngguf_kv_cache* c) {
@@ -251,8 +254,8 @@ int sngguf_cache_write_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_
 int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream) {
     const int rc = check_cache(cache);
     if (rc != SNGGUF_OK) return rc;
-    // (one thread for eight elements, workgroups of 256 numbered with 31 bits)
-    if (tokens < 0 || tokens >= kMost || tokens * cache->kv_heads * (cache->dim / 8) >= kMost * 256) return SNGGUF_E_BADSHAPE;
+    // (one thread for eight elements; kv_heads and dim / 8 together below 2^21)
+    if (tokens < 0 || tokens >= kMost || !launch_fits((tokens * cache->kv_heads * (cache->dim / 8) + 255) / 256, 256)) return SNGGUF_E_BADSHAPE;
     if (tokens == 0) return SNGGUF_OK;
     if (!slots || !k_out || !v_out) return SNGGUF_E_NULLPTR;
     if (!aligned(slots, 8) || !aligned(k_out, 16) || !aligned(v_out, 16)) return SNGGUF_E_ALIGN;
@@ -288,7 +291,7 @@ int sngguf_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_t
         return SNGGUF_E_ALIGN;
     const int d = kernel_dim(dim);
     const Launch p = plan_many(tokens_q, tokens_k, sequences, heads, kv_heads, dim);
-    if (p.grid >= kMost) return SNGGUF_E_BADSHAPE;
+    if (!launch_fits(p.grid, 2 * p.rows)) return SNGGUF_E_BADSHAPE;       // (a wavefront for 32 rows)
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);
     a.k = static_cast<const bf16_t*>(k);
@@ -340,7 +343,7 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
     const int d = kernel_dim(cache->dim);
     const bool q8 = cache->qtype == SNGGUF_TYPE_Q8_0;
     const PagedPlan p = paged_plan(tokens_q, sequences, ends_q ? max_new : 1, table_width * cache->page_size, heads, kv_heads, cache->dim);
-    if (p.a.grid >= kMost || p.b.grid >= kMost) return SNGGUF_E_BADSHAPE;
+    if ((p.few && !launch_fits(p.a.grid, 256)) || (p.many && !launch_fits(p.b.grid, 2 * p.b.rows))) return SNGGUF_E_BADSHAPE;
     AttentionArgs a = {};
     a.q = static_cast<const bf16_t*>(q);
     a.out = static_cast<bf16_t*>(out);

@@ -301,7 +301,9 @@ int launch_rotary_cache(const RotaryCacheArgs& a0, int cache, hipStream_t stream
     // less than one unit for each thread
     const int64_t units = (int64_t)(a.q_heads + (cache ? 2 * a.kv_heads : a.k_heads)) * (a.dim >> 3);
     a.tokens_per_block = units >= kThreads ? 1 : units * 8 <= kThreads ? 8 : (int32_t)(kThreads / units);
-    const dim3 grid((unsigned)((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block));
+    const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+    if (blocks * kThreads >= (int64_t)1 << 32) return SNGGUF_E_BADSHAPE;     // (threads of a launch are numbered with 32 bits)
+    const dim3 grid((unsigned)blocks);
     const size_t lds = (size_t)a.tokens_per_block * a.pairs * sizeof(float2);
     if (a.turns) {
         if (cache == 0) rotary_cache_kernel<true, 0><<<grid, kThreads, lds, stream>>>(a);
