@@ -259,11 +259,12 @@ class PagedKVCache:
     bf16: ``k`` and ``v`` are bf16 ``[pages][kv_heads][page_size][dim]``.  8 bits: int8 of that shape, with fp16 ``k_scale`` and
     ``v_scale`` ``[pages][kv_heads][dim / 32][page_size]``; 32 elements of a token share a scale, as in a Q8_0 block (magnitudes
     beyond 65024 saturate, a NaN makes its 32 elements NaN).  ``page_size`` is a power of two from 16 to 4096, ``dim`` a multiple
-    of 32 up to 256.  ``PagedKVCache.empty`` allocates one; the constructor takes tensors that are there.
+    of 32 up to 256.  ``PagedKVCache.empty`` allocates one; the constructor takes tensors that are there (keys and values that share memory
+    can be read, not written).
 
     Token t of a sequence lies at slot ``page_of_the_sequence[t // page_size] * page_size + t % page_size``."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index", "_shared")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
         if not k.is_cuda:
@@ -283,8 +284,10 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.quant_type = ops.Q8_0 if q8 else ops.BF16
         self.pages, self.kv_heads, self.page_size, self.dim, self._index = pages, kv_heads, page, dim, index
-        self._struct = _CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None, pages, page,
-                                    kv_heads, dim, self.quant_type)
+        at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None)
+        self._struct = _CacheStruct(*at, pages, page, kv_heads, dim, self.quant_type)
+        count = pages * kv_heads * page * dim
+        self._shared = abs(at[0] - at[1]) < (count if q8 else 2 * count) or (q8 and abs(at[2] - at[3]) < count // 16)
         self._address = ctypes.addressof(self._struct)
 
     @classmethod
@@ -301,6 +304,8 @@ class PagedKVCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
     def _rows(self, k, v, slots, what):
+        if self._shared:
+            raise SnGgufError(f"{what}: the cache's keys and values share memory")
         (k, kt, kh), (v, vt, vh) = _heads(k, what, "k"), _heads(v, what, "v")
         if k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[2] != self.dim:
             raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with a cache of {self.kv_heads} heads of {self.dim}")
@@ -310,7 +315,7 @@ class PagedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Keys and values [tokens][kv_heads][dim] into ``slots`` (int64 [tokens], different ones; negative ones and those behind
-        the last page are passed over)."""
+        the last page are passed over).  k and v may be views of the cache itself, of other slots."""
         k, v, slots, rows = self._rows(k, v, slots, "PagedKVCache.write")
         if k.shape[0]:
             _launch(self._index, "sngguf_cache_write", self._address, *rows)
