@@ -416,6 +416,31 @@ typedef struct sngguf_rotary_table {
     int32_t interleaved;
 } sngguf_rotary_table;
 
+/* Rotation of a head's pairs by several positions of its token (time, row and column of a picture): pair i at the positions p[axes]
+ * turns by 2 pi p[axis[i]] turns[i].  The first 2 * pairs elements of a head are cut into `parts` parts of part[] elements (even,
+ * 1 .. 4 of them); pairs of a part of n elements are (i, i + n / 2) of it, or neighbours with interleaved != 0, and follow one
+ * another from part to part.  Everything else as sngguf_rotary_table, which is one part and one axis. */
+typedef struct sngguf_rotary_axes {
+    const double* turns;  /* device, [pairs]                                                                      */
+    const int32_t* axis;  /* device, [pairs]; NULL: all pairs by the first.  A number that is no axis counts as the nearest */
+    int64_t pairs;        /* 1 .. dim / 2                                                                         */
+    double magnitude;
+    int32_t interleaved;
+    int32_t parts;
+    int32_t part[4];
+} sngguf_rotary_axes;
+
+/* Norm of single heads: `parts` parts (1 .. 4) of elements[] elements each (multiples of 8, together a whole head), y = weight x /
+ * sqrt(mean of the part's x^2 + eps) in fp32.  weight[]: device, [elements] of one type, 16-byte aligned: bf16 (weight_type 2) or
+ * fp32 (weight_type 0). */
+typedef struct sngguf_head_norm {
+    const void* weight[4];
+    int32_t elements[4];
+    int32_t parts;
+    int32_t weight_type;
+    float eps;
+} sngguf_head_norm;
+
 /* Keys and values of `pages` * `page_size` tokens.  qtype SNGGUF_TYPE_BF16: k, v are bf16 [pages][kv_heads][page_size][dim].
  * SNGGUF_TYPE_Q8_0: k, v are int8 of that shape and k_scale, v_scale fp16 [pages][kv_heads][dim / 32][page_size]; 32 elements
  * of a token share a scale d = fp16(max |x| / 127), at most 512, and are held as rint(x / d), at most 127 in magnitude (the
@@ -445,6 +470,21 @@ int sngguf_cache_write_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_
                               const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head,
                               const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                               const int64_t* slots, int64_t tokens, void* stream);
+
+/* q_out = q normed by q_norm and turned, and the same for k (k_heads = 0: q alone) with k_norm; a norm that is NULL leaves its heads as they are.
+ * positions: axis i of token t at positions[i * axis_stride + t], i < axes.  Norm and rotation in fp32, rounded to bf16 once.
+ * dim % 8 == 0, up to 512; outputs and alignment as sngguf_rotary. */
+int sngguf_head_rotary(const sngguf_rotary_axes* table, const int64_t* positions, int64_t axes, int64_t axis_stride, int64_t tokens, int64_t dim,
+                       const sngguf_head_norm* q_norm, const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out,
+                       int64_t q_out_token, int64_t q_out_head, const sngguf_head_norm* k_norm, const void* k, int64_t k_heads, int64_t k_token,
+                       int64_t k_head, void* k_out, int64_t k_out_token, int64_t k_out_head, void* stream);
+
+/* sngguf_head_rotary of q, and sngguf_cache_write of the normed and turned k (rounded to bf16) and of v, in one launch. */
+int sngguf_cache_write_head_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_axes* table, const int64_t* positions, int64_t axes,
+                                   int64_t axis_stride, const sngguf_head_norm* q_norm, const void* q, int64_t q_heads, int64_t q_token,
+                                   int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head, const sngguf_head_norm* k_norm,
+                                   const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                                   const int64_t* slots, int64_t tokens, void* stream);
 
 /* The cache's slots as bf16 rows: k_out, v_out [tokens][kv_heads][dim], contiguous, 16-byte aligned.  Slots outside the cache
  * give zeros. */

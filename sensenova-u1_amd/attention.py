@@ -8,8 +8,7 @@ stacked projection's output go in as they are.  Forward only: nothing here recor
 A layer's attention for new tokens of sequences that lie in a cache::
 
     q, k, v = (y.view(tokens, -1, dim) for y in qkv(hidden, norm_weight, eps))     # FusedProjections
-    q, k = q_norm(q), k_norm(k)          # the model's own, where it norms single heads: nothing here does
-    q = cache.write_rotary(q, k, v, positions, table, slots)
+    q = cache.write_rotary(q, k, v, positions, table, slots, q_norm=q_norm, k_norm=k_norm)      # HeadNorm, where the model norms single heads
     out = paged_attention(q, cache, pages, lens, ends)                              # [tokens][heads][dim]
     hidden = o_proj.forward_residual(out.view(tokens, -1), hidden)
 """
@@ -18,7 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Optional
+from typing import Optional, Sequence, Union
 
 import torch
 
@@ -30,6 +29,16 @@ _BF16 = torch.bfloat16
 
 class _TableStruct(ctypes.Structure):
     _fields_ = [("turns", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double), ("interleaved", ctypes.c_int32)]
+
+
+class _AxesStruct(ctypes.Structure):
+    _fields_ = [("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double),
+                ("interleaved", ctypes.c_int32), ("parts", ctypes.c_int32), ("part", ctypes.c_int32 * 4)]
+
+
+class _NormStruct(ctypes.Structure):
+    _fields_ = [("weight", ctypes.c_void_p * 4), ("elements", ctypes.c_int32 * 4), ("parts", ctypes.c_int32), ("weight_type", ctypes.c_int32),
+                ("eps", ctypes.c_float)]
 
 
 class _CacheStruct(ctypes.Structure):
@@ -178,7 +187,7 @@ class RotaryTable:
     ``turns``: float64 on the device, one for each pair; pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with
     ``interleaved``; elements behind the 2 * pairs first are left as they are.  ``for_model`` makes it of a checkpoint's settings."""
 
-    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address")
+    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes", "_axes_address")
 
     def __init__(self, turns: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -189,6 +198,9 @@ class RotaryTable:
         self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
         self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self.magnitude, self.interleaved)
         self._address = ctypes.addressof(self._struct)
+        # (the same as a table of one axis and one part, where heads are normed as well)
+        self._axes = _AxesStruct(turns.data_ptr(), None, turns.shape[0], self.magnitude, self.interleaved, 1, (2 * turns.shape[0], 0, 0, 0))
+        self._axes_address = ctypes.addressof(self._axes)
 
     @classmethod
     def for_model(cls, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_context: int = 0,
@@ -220,16 +232,114 @@ class RotaryTable:
         return cls(turns.to(device), interleaved, size if magnitude is None else magnitude)
 
 
-def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: RotaryTable, inplace: bool = False):
+class RotaryAxes:
+    """How the pairs of a head turn by several positions of their token: pair i by ``turns[i]`` turns (of 2 pi) a position of axis
+    ``axis[i]`` (time, row, column of a picture ...), and the result scaled by ``magnitude``.
+
+    ``turns``: float64, ``axis``: int32, both on the device, one entry for each pair.  ``parts``: elements of the stretches, one to four, into
+    which the first 2 * pairs elements of a head are cut; the pairs of one of n elements are (i, i + n / 2) of it, and pairs are
+    counted from part to part (default: one part).  With ``interleaved`` pairs are (2 i, 2 i + 1) throughout.  Elements behind are
+    left as they are.  An axis that positions do not have counts as the nearest that they have."""
+
+    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes", "_axes_address")
+
+    def __init__(self, turns: torch.Tensor, axis: torch.Tensor, parts: Optional[Sequence[int]] = None, interleaved: bool = False, magnitude: float = 1.0) -> None:
+        if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
+            raise SnGgufError(f"RotaryAxes: turns must be float64 [pairs] on a HIP device, got {turns.dtype} {tuple(turns.shape)} on '{turns.device}'")
+        pairs = turns.shape[0]
+        axis = _numbers(axis, torch.int32, pairs, "RotaryAxes", "axis")
+        _same_device("RotaryAxes", turns.get_device(), axis)
+        self.parts = parts = (2 * pairs,) if parts is None else tuple(int(n) for n in parts)
+        if not 1 <= len(parts) <= 4 or any(n < 2 or n % 2 for n in parts) or sum(parts) != 2 * pairs:
+            raise SnGgufError(f"RotaryAxes: parts of {parts} elements (one to four, even) do not hold {pairs} pairs")
+        if not math.isfinite(magnitude):
+            raise SnGgufError("RotaryAxes: the magnitude is not finite")
+        self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
+        self.axis, self.interleaved, self.magnitude = axis, bool(interleaved), float(magnitude)
+        self._axes = _AxesStruct(turns.data_ptr(), axis.data_ptr(), pairs, self.magnitude, self.interleaved, len(parts), parts + (0,) * (4 - len(parts)))
+        self._axes_address = ctypes.addressof(self._axes)
+
+    @classmethod
+    def for_model(cls, parts: Sequence[tuple], interleaved: bool = False, device="cuda") -> "RotaryAxes":
+        """The table of a head whose parts turn by an axis each: ``parts`` holds (elements, axis, base) of each part, with wavelengths
+        from 2 pi to 2 pi ``base`` positions.  ``[(64, 0, 5e6), (32, 1, 1e4), (32, 2, 1e4)]``: half a head of 128 by the place in the
+        text, a quarter each by row and column."""
+        if not parts or any(n < 2 or n % 2 or not base > 1 for n, _, base in parts):
+            raise SnGgufError(f"RotaryAxes: parts {parts} (elements, axis, base) are not known")
+        turns = torch.cat([float(base) ** (-torch.arange(n // 2, dtype=torch.float64) / (n // 2)) / (2 * math.pi) for n, _, base in parts])
+        axis = torch.cat([torch.full((n // 2,), int(a), dtype=torch.int32) for n, a, _ in parts])
+        return cls(turns.to(device), axis.to(device), [n for n, _, _ in parts], interleaved)
+
+
+class HeadNorm:
+    """The norm of single heads in front of the rotation: y = weight * x / sqrt(mean(x^2) + eps), in 32 bits.
+
+    ``weights``: one to four tensors [elements] on the device, bf16 or fp32, for the consecutive parts of a head that are normed each by
+    itself (one: the whole head); their elements, multiples of 8, are a head's together.  Their memory is read at every call: a change in place counts, a tensor
+    put in a module's place does not."""
+
+    __slots__ = ("weights", "eps", "dim", "_struct", "_address", "_index")
+
+    def __init__(self, *weights: torch.Tensor, eps: float = 1e-6) -> None:
+        if not 1 <= len(weights) <= 4:
+            raise SnGgufError(f"HeadNorm: {len(weights)} parts (one to four are possible)")
+        for w in weights:
+            if w.dtype not in (_BF16, torch.float32) or w.dtype != weights[0].dtype or w.dim() != 1 or w.shape[0] < 8 or w.shape[0] % 8 or not w.is_cuda:
+                raise SnGgufError("HeadNorm: weights must be bf16 or fp32 [a multiple of 8] on a HIP device, of one type, "
+                                  f"got {[(str(w.dtype), tuple(w.shape), str(w.device)) for w in weights]}")
+            if w.requires_grad and torch.is_grad_enabled():
+                raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
+        if not (math.isfinite(eps) and eps >= 0):
+            raise SnGgufError(f"HeadNorm: eps is {eps}")
+        self._index = weights[0].get_device()
+        _same_device("HeadNorm", self._index, *weights)
+        # (detached: what a parameter's .data is set to later does not take this memory away)
+        weights = [w.detach() for w in weights]
+        self.weights = weights = tuple(w if (w.stride(0) == 1 and w.data_ptr() % 16 == 0) else w.clone(memory_format=torch.contiguous_format) for w in weights)
+        self.eps, self.dim = float(eps), sum(w.shape[0] for w in weights)
+        rest = (0,) * (4 - len(weights))
+        self._struct = _NormStruct(tuple(w.data_ptr() for w in weights) + rest, tuple(w.shape[0] for w in weights) + rest, len(weights),
+                                   ops._OUT_CODE[weights[0].dtype], self.eps)
+        self._address = ctypes.addressof(self._struct)
+
+
+def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tensor, table, q_norm: Optional[HeadNorm], k_norm: Optional[HeadNorm]):
+    """(positions, their axes, elements from one axis to the next) where heads are normed or turned by several positions, and the norms' addresses"""
+    if isinstance(table, RotaryAxes):
+        if positions.dtype != torch.int64 or positions.dim() != 2 or positions.shape[1] != tokens or positions.shape[0] < 1:
+            raise SnGgufError(f"{what}: positions must be torch.int64 [axes][{tokens}], got {positions.dtype} {tuple(positions.shape)}")
+        if positions.stride(1) != 1 and tokens > 1:
+            positions = positions.contiguous()
+        axes, stride = positions.shape[0], positions.stride(0)
+        if 2 * table.turns.shape[0] > dim:
+            raise SnGgufError(f"{what}: {table.turns.shape[0]} pairs do not fit heads of {dim} elements")
+        _same_device(what, index, table.axis)
+    else:
+        positions, axes, stride = _numbers(positions, torch.int64, tokens, what, "positions"), 1, 0
+    for norm in (q_norm, k_norm):
+        if norm is not None and (norm.dim != dim or norm._index != index):
+            raise SnGgufError(f"{what}: a norm of {norm.dim} elements on device {norm._index} does not go with heads of {dim} on device {index}")
+    if dim > 512:
+        raise SnGgufError(f"{what}: heads of {dim} elements (up to 512 are normed or turned by several positions)")
+    return positions, (positions.data_ptr(), axes, stride), q_norm and q_norm._address, k_norm and k_norm._address
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: Union[RotaryTable, RotaryAxes], inplace: bool = False,
+           q_norm: Optional[HeadNorm] = None, k_norm: Optional[HeadNorm] = None):
     """Queries and keys turned by their positions: ``(q, k)``, new tensors or with ``inplace`` the given ones.
 
-    q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None, either may have no heads.  positions: int64 [tokens].  A model whose head
-    has parts with positions of their own calls it on views of the parts.  In place, no two rows may share an element."""
+    q, k: bf16 [tokens][heads][dim], ``dim`` a multiple of 8; ``k`` may be None, either may have no heads.  positions: int64 [tokens], or [axes][tokens] with
+    ``RotaryAxes``.  ``q_norm``, ``k_norm``: the norm of each head in front of the rotation, in the same launch; norm and rotation are
+    in 32 bits and rounded once.  ``dim`` is up to 1024, up to 512 with a norm or several axes.  In place, no two rows may share an element."""
     q0, k0 = q, k
     q, qt, qh = _heads(q, "rotary", "q")
     tokens, heads, dim = q.shape
     index = q.get_device()
-    positions = _numbers(positions, torch.int64, tokens, "rotary", "positions")
+    wide = q_norm is not None or k_norm is not None or isinstance(table, RotaryAxes)
+    if wide:
+        positions, at, q_at, k_at = _axes_of("rotary", index, tokens, dim, positions, table, q_norm, k_norm)
+    else:
+        positions = _numbers(positions, torch.int64, tokens, "rotary", "positions")
     _same_device("rotary", index, k, positions, table.turns)
     if k is not None:
         k, kt, kh = _heads(k, "rotary", "k")
@@ -248,8 +358,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     first = (q.data_ptr(), heads, qt, qh, q_out.data_ptr(), qot, qoh)
     if not heads:                       # keys alone: in the queries' place
         first, rest, heads = rest, (None, 0, 0, 0, None, 0, 0), rest[1]
+        if wide:
+            q_at, k_at = k_at, None
     if tokens and heads:
-        _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, *first, *rest)
+        if wide:
+            _launch(index, "sngguf_head_rotary", table._axes_address, *at, tokens, dim, q_at, *first, k_at, *rest)
+        else:
+            _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, *first, *rest)
     return q_out, k_out
 
 
@@ -320,10 +435,10 @@ class PagedKVCache:
         if k.shape[0]:
             _launch(self._index, "sngguf_cache_write", self._address, *rows)
 
-    def write_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: RotaryTable, slots: torch.Tensor,
-                     inplace: bool = False) -> torch.Tensor:
-        """``rotary`` of q and k, then ``write`` of the turned k and of v, in one launch; returns the turned q (with ``inplace`` in
-        q's own memory; k is left as it is)."""
+    def write_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: Union[RotaryTable, RotaryAxes],
+                     slots: torch.Tensor, inplace: bool = False, q_norm: Optional[HeadNorm] = None, k_norm: Optional[HeadNorm] = None) -> torch.Tensor:
+        """``rotary`` of q and k (with their norms, if given), then ``write`` of the turned k and of v, in one launch; returns the turned q
+        (with ``inplace`` in q's own memory; k is left as it is)."""
         what = "PagedKVCache.write_rotary"
         q0 = q
         q, qt, qh = _heads(q, what, "q")
@@ -333,10 +448,17 @@ class PagedKVCache:
             raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
         if inplace and (q is not q0 or not _apart(q) or (q.numel() and (_rows_share(q, k) or _rows_share(q, v)))):
             raise SnGgufError(f"{what}: in place needs rows that share no element, the elements of a head next to each other")
-        positions = _numbers(positions, torch.int64, tokens, what, "positions")
+        wide = q_norm is not None or k_norm is not None or isinstance(table, RotaryAxes)
+        if wide:
+            positions, at, q_at, k_at = _axes_of(what, self._index, tokens, dim, positions, table, q_norm, k_norm)
+        else:
+            positions = _numbers(positions, torch.int64, tokens, what, "positions")
         _same_device(what, self._index, q, positions, table.turns)
         out, ot, oh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
-        if tokens:
+        if tokens and wide:
+            _launch(self._index, "sngguf_cache_write_head_rotary", self._address, table._axes_address, *at, q_at, q.data_ptr(), heads, qt, qh, out.data_ptr(),
+                    ot, oh, k_at, *rows)
+        elif tokens:
             _launch(self._index, "sngguf_cache_write_rotary", self._address, table._address, positions.data_ptr(), q.data_ptr(), heads, qt, qh, out.data_ptr(),
                     ot, oh, *rows)
         return out

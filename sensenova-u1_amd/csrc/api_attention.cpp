@@ -5,7 +5,7 @@
 #include <stdint.h>
 
 #include "attention.hpp"
-#include "rotary_cache.hpp"
+#include "head_rotary.hpp"
 
 namespace sngguf {
 int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream);
@@ -77,6 +77,66 @@ void set_table(RotaryCacheArgs& a, const sngguf_rotary_table* t, const int64_t* 
     a.positions = positions;
     a.pairs = (int32_t)t->pairs;
     a.interleaved = t->interleaved != 0;
+}
+
+int check_axes(const sngguf_rotary_axes* t, const int64_t* positions, int64_t axes, int64_t tokens, int64_t dim, int64_t heads) {
+    if (!t) return SNGGUF_E_NULLPTR;
+    if (tokens < 0 || tokens >= kMost || dim < 8 || dim > 512 || dim % 8 != 0 || heads < 1 || heads > 65535 || t->pairs < 1 || 2 * t->pairs > dim ||
+        !isfinite(t->magnitude) || t->parts < 1 || t->parts > sngguf::kMostParts || axes < 1 || axes >= kMost)
+        return SNGGUF_E_BADSHAPE;
+    int64_t elements = 0;
+    for (int p = 0; p < t->parts; p++) {
+        if (t->part[p] < 2 || t->part[p] > dim || t->part[p] % 2 != 0) return SNGGUF_E_BADSHAPE;
+        elements += t->part[p];
+    }
+    if (elements != 2 * t->pairs) return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!t->turns || !positions) return SNGGUF_E_NULLPTR;
+    if (!aligned(t->turns, 8) || !aligned(positions, 8) || !aligned(t->axis, 4)) return SNGGUF_E_ALIGN;
+    return SNGGUF_OK;
+}
+
+int check_norm(const sngguf_head_norm* n, int64_t dim) {
+    if (!n) return SNGGUF_OK;
+    if (n->weight_type != 0 && n->weight_type != 2) return SNGGUF_E_BADTYPE;
+    if (n->parts < 1 || n->parts > sngguf::kMostParts || !(n->eps >= 0.f) || !isfinite(n->eps)) return SNGGUF_E_BADSHAPE;
+    int64_t elements = 0;
+    for (int p = 0; p < n->parts; p++) {
+        if (n->elements[p] < 8 || n->elements[p] > dim || n->elements[p] % 8 != 0) return SNGGUF_E_BADSHAPE;
+        elements += n->elements[p];
+    }
+    if (elements != dim) return SNGGUF_E_BADSHAPE;
+    for (int p = 0; p < n->parts; p++) {
+        if (!n->weight[p]) return SNGGUF_E_NULLPTR;
+        if (!aligned(n->weight[p], 16)) return SNGGUF_E_ALIGN;
+    }
+    return SNGGUF_OK;
+}
+
+void set_norm(sngguf::HeadNormArgs& a, const sngguf_head_norm* n) {
+    if (!n) return;
+    a.parts = n->parts;
+    a.bf16 = n->weight_type == 2;
+    a.eps = n->eps;
+    a.group = n->elements[0] / 8;
+    for (int p = 0; p < n->parts; p++) {
+        a.weight[p] = n->weight[p];
+        a.elements[p] = n->elements[p];
+        if (n->elements[p] != n->elements[0] || (a.group & (a.group - 1)) != 0) a.group = 0;
+    }
+}
+
+void set_axes(sngguf::HeadRotaryArgs& a, const sngguf_rotary_axes* t, const int64_t* positions, int64_t axes, int64_t axis_stride) {
+    a.turns = t->turns;
+    a.axis = t->axis;
+    a.magnitude = t->magnitude;
+    a.positions = positions;
+    a.axes = (int32_t)axes;
+    a.axis_stride = axis_stride;
+    a.pairs = (int32_t)t->pairs;
+    a.interleaved = t->interleaved != 0;
+    a.parts = t->parts;
+    for (int p = 0; p < t->parts; p++) a.part[p] = t->part[p];
 }
 
 // ---- attention: how much is launched ----------------------------------------------------------------------------------
@@ -249,6 +309,70 @@ int sngguf_cache_write_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_
     a.wide = whole_pieces(q, q_token, q_head) && whole_pieces(q_out, q_out_token, q_out_head) && whole_pieces(k, k_token, k_head) &&
              whole_pieces(v, v_token, v_head);
     return sngguf::launch_rotary_cache(a, cache->qtype == SNGGUF_TYPE_Q8_0 ? 2 : 1, static_cast<hipStream_t>(stream));
+}
+
+int sngguf_head_rotary(const sngguf_rotary_axes* table, const int64_t* positions, int64_t axes, int64_t axis_stride, int64_t tokens, int64_t dim,
+                       const sngguf_head_norm* q_norm, const void* q, int64_t q_heads, int64_t q_token, int64_t q_head, void* q_out,
+                       int64_t q_out_token, int64_t q_out_head, const sngguf_head_norm* k_norm, const void* k, int64_t k_heads, int64_t k_token,
+                       int64_t k_head, void* k_out, int64_t k_out_token, int64_t k_out_head, void* stream) {
+    int rc = check_axes(table, positions, axes, tokens, dim, q_heads);
+    if (rc == SNGGUF_OK) rc = check_norm(q_norm, dim);
+    if (rc == SNGGUF_OK) rc = check_norm(k_norm, dim);
+    if (rc != SNGGUF_OK) return rc;
+    if (k_heads < 0 || k_heads > 65535) return SNGGUF_E_BADSHAPE;
+    if (tokens == 0) return SNGGUF_OK;
+    if (!q || !q_out || (k_heads && (!k || !k_out))) return SNGGUF_E_NULLPTR;
+    if (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(k, 2) || !aligned(k_out, 2)) return SNGGUF_E_ALIGN;
+    sngguf::HeadRotaryArgs a = {};
+    set_axes(a, table, positions, axes, axis_stride);
+    set_norm(a.q_norm, q_norm);
+    if (k_heads) set_norm(a.k_norm, k_norm);
+    a.q = static_cast<const bf16_t*>(q);
+    a.q_out = static_cast<bf16_t*>(q_out);
+    a.k = static_cast<const bf16_t*>(k);
+    a.k_out = static_cast<bf16_t*>(k_out);
+    a.q_token = q_token, a.q_head = q_head, a.q_out_token = q_out_token, a.q_out_head = q_out_head;
+    a.k_token = k_token, a.k_head = k_head, a.k_out_token = k_out_token, a.k_out_head = k_out_head;
+    a.tokens = tokens;
+    a.dim = (int32_t)dim;
+    a.q_heads = (int32_t)q_heads;
+    a.k_heads = (int32_t)k_heads;
+    a.wide = whole_pieces(q, q_token, q_head) && whole_pieces(q_out, q_out_token, q_out_head) &&
+             (!k_heads || (whole_pieces(k, k_token, k_head) && whole_pieces(k_out, k_out_token, k_out_head)));
+    return sngguf::launch_head_rotary(a, 0, static_cast<hipStream_t>(stream));
+}
+
+int sngguf_cache_write_head_rotary(const sngguf_kv_cache* cache, const sngguf_rotary_axes* table, const int64_t* positions, int64_t axes,
+                                   int64_t axis_stride, const sngguf_head_norm* q_norm, const void* q, int64_t q_heads, int64_t q_token,
+                                   int64_t q_head, void* q_out, int64_t q_out_token, int64_t q_out_head, const sngguf_head_norm* k_norm,
+                                   const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                                   const int64_t* slots, int64_t tokens, void* stream) {
+    int rc = check_cache(cache);
+    if (rc == SNGGUF_OK) rc = check_axes(table, positions, axes, tokens, cache->dim, q_heads);
+    if (rc == SNGGUF_OK) rc = check_norm(q_norm, cache->dim);
+    if (rc == SNGGUF_OK) rc = check_norm(k_norm, cache->dim);
+    if (rc != SNGGUF_OK || tokens == 0) return rc;
+    if (!q || !q_out || !k || !v || !slots) return SNGGUF_E_NULLPTR;
+    if (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return SNGGUF_E_ALIGN;
+    sngguf::HeadRotaryArgs a = {};
+    set_cache(a, cache);
+    set_axes(a, table, positions, axes, axis_stride);
+    set_norm(a.q_norm, q_norm);
+    set_norm(a.k_norm, k_norm);
+    if (cache->qtype != SNGGUF_TYPE_Q8_0) a.k_scales = a.v_scales = nullptr;
+    a.q = static_cast<const bf16_t*>(q);
+    a.q_out = static_cast<bf16_t*>(q_out);
+    a.k = static_cast<const bf16_t*>(k);
+    a.v = static_cast<const bf16_t*>(v);
+    a.q_token = q_token, a.q_head = q_head, a.q_out_token = q_out_token, a.q_out_head = q_out_head;
+    a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+    a.slots = slots;
+    a.tokens = tokens;
+    a.dim = (int32_t)cache->dim;
+    a.q_heads = (int32_t)q_heads;
+    a.wide = whole_pieces(q, q_token, q_head) && whole_pieces(q_out, q_out_token, q_out_head) && whole_pieces(k, k_token, k_head) &&
+             whole_pieces(v, v_token, v_head);
+    return sngguf::launch_head_rotary(a, 1, static_cast<hipStream_t>(stream));
 }
 
 int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream) {
