@@ -491,6 +491,37 @@ int sngguf_cache_write_head_rotary(const sngguf_kv_cache* cache, const sngguf_ro
 int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out, void* stream);
 
 /*
+ * The tables of many sequences over a paged cache, all in device memory: pages [sequences][width], the pages of each sequence in order;
+ * lens [sequences], its tokens; held [sequences] (NULL: none), leading pages of a row that belong to another sequence; free
+ * [ring], page numbers in a ring of which those from cursor[0] (taken so far) up to cursor[1] (given so far) are there, the c-th
+ * at place c mod ring.  page_size as in a cache; width * page_size below 2^31 - 65536, sequences below 2^24.
+ */
+typedef struct sngguf_page_tables {
+    int32_t *pages, *lens, *held, *free;
+    int64_t* cursor;
+    int64_t sequences, width, ring, page_size;
+} sngguf_page_tables;
+
+/* A step in which sequence i gets added[i] new tokens (fewer than 0 count as 0), packed one sequence after the other into `tokens` rows:
+ * ends [sequences + 1] where each one's rows start and end (cut at `tokens`), positions and slots [tokens] of each row (0 and -1 behind the last), lens_out
+ * [sequences] and cursor_out [2] what lens and cursor are behind the step (they may be the tables' own), and pages filled in for
+ * sequences that outgrow theirs, taken from the ring in the order of the sequences.  Tokens for which there is no page, or
+ * whose row of pages is full, have slot -1 and no part in lens_out; missing[0] counts them.  workspace (16-byte aligned) of
+ * sngguf_page_append_workspace_bytes(sequences, tokens) bytes, NULL where that is 0. */
+int64_t sngguf_page_append_workspace_bytes(int64_t sequences, int64_t tokens);
+int sngguf_page_append(const sngguf_page_tables* tables, const int32_t* added, int64_t tokens, int32_t* ends, int32_t* lens_out, int64_t* cursor_out,
+                       int64_t* positions, int64_t* slots, int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Sequences with done[i] != 0 end: their own pages go back to the ring, in the order of the sequences, lens and held become 0.  Pages
+ * for which the ring has no room (more than there are in all) are dropped. */
+int sngguf_page_release(const sngguf_page_tables* tables, const uint8_t* done, void* stream);
+
+/* Sequence i with parent[i] >= 0 starts with the first common[i] tokens of that one, rounded down to whole pages (at most what the parent
+ * has), which it holds and the parent owns: a parent is released behind its children.  Nothing happens to a sequence that has tokens already, or
+ * whose parent is no sequence, itself, or one that has a parent in the same call. */
+int sngguf_page_fork(const sngguf_page_tables* tables, const int32_t* parent, const int32_t* common, void* stream);
+
+/*
  * Attention of packed sequences: sequence i has the queries [ends_q[i], ends_q[i + 1]) and the keys [ends_k[i], ends_k[i + 1])
  * (device, [sequences + 1], not decreasing).  out = softmax(scale q . k) v, each query over the keys that it sees: all, or
  * with causal != 0 those up to its own place, the last query standing at the last key; with window > 0 (causal only) the last

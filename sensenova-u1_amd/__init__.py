@@ -4,6 +4,7 @@ from .attention import HeadNorm, PagedKVCache, RotaryAxes, RotaryTable, paged_at
 from .gguf_file import GGML_QUANT_SIZES, GGMLQuantizationType, GGUFReader, GGUFWriter, NativeGGUFReader
 from .gguf_loader import count_gguf_linear, load_gguf_checkpoint, load_gguf_model, match_state_dict, set_gguf2meta_model
 from .layer_offload import LayerOffloadWrapper, LayerStreamer, PackedLayerStore
+from .page_tables import PageStep, PageTables
 from .modality import FusedProjections, SharedInputStack, find_mot_pairs, stack_shared_input_projections, fuse_gated_mlps, gated_mlp, grouped_linear, unfuse_gated_mlps
 from .quantized_linear import (
     SUPPORTED_GGUF_QUANT_TYPES,
@@ -19,5 +20,5 @@ __all__ = [
     "GGUFLinear", "GGUFParameter", "SUPPORTED_GGUF_QUANT_TYPES", "dequantize_gguf_tensor",
     "grouped_linear", "find_mot_pairs", "gated_mlp", "fuse_gated_mlps", "unfuse_gated_mlps", "FusedProjections", "SharedInputStack", "stack_shared_input_projections", "NativeGGUFReader",
     "LayerOffloadWrapper", "PackedLayerStore", "LayerStreamer", "set_decode_layout",
-    "RotaryTable", "RotaryAxes", "HeadNorm", "rotary", "PagedKVCache", "prompt_attention", "paged_attention",
+    "RotaryTable", "RotaryAxes", "HeadNorm", "rotary", "PagedKVCache", "PageTables", "PageStep", "prompt_attention", "paged_attention",
 ]

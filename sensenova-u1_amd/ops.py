@@ -41,7 +41,8 @@ EXPORTED_SYMBOLS = (
     "sngguf_rmsnorm_linear_tiled", "sngguf_rmsnorm_gate_up_silu_tiled",
     "sngguf_mlp_decode_workspace_bytes", "sngguf_mlp_decode_status_offset", "sngguf_mlp_decode_fits", "sngguf_mlp_decode",
     "sngguf_probe_stream_read_out_bytes", "sngguf_probe_stream_read",
-    "sngguf_rotary", "sngguf_cache_write", "sngguf_cache_write_rotary", "sngguf_head_rotary", "sngguf_cache_write_head_rotary", "sngguf_cache_read", "sngguf_attention_workspace_bytes", "sngguf_attention",
+    "sngguf_rotary", "sngguf_cache_write", "sngguf_cache_write_rotary", "sngguf_head_rotary", "sngguf_cache_write_head_rotary", "sngguf_cache_read",
+    "sngguf_page_append_workspace_bytes", "sngguf_page_append", "sngguf_page_release", "sngguf_page_fork", "sngguf_attention_workspace_bytes", "sngguf_attention",
     "sngguf_paged_attention_workspace_bytes", "sngguf_paged_attention",
     "sngguf_file_open", "sngguf_file_close", "sngguf_file_version", "sngguf_file_alignment", "sngguf_file_tensor_count",
     "sngguf_file_tensor", "sngguf_file_metadata_count", "sngguf_file_metadata", "sngguf_file_read_tensors",
@@ -164,6 +165,14 @@ def load_library() -> ctypes.CDLL:
     lib.sngguf_cache_write_head_rotary.restype = ci
     lib.sngguf_cache_read.argtypes = [vp, vp, i64, vp, vp, vp]
     lib.sngguf_cache_read.restype = ci
+    lib.sngguf_page_append_workspace_bytes.argtypes = [i64, i64]
+    lib.sngguf_page_append_workspace_bytes.restype = i64
+    lib.sngguf_page_append.argtypes = [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.sngguf_page_append.restype = ci
+    lib.sngguf_page_release.argtypes = [vp, vp, vp]
+    lib.sngguf_page_release.restype = ci
+    lib.sngguf_page_fork.argtypes = [vp, vp, vp, vp]
+    lib.sngguf_page_fork.restype = ci
     lib.sngguf_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
     lib.sngguf_attention_workspace_bytes.restype = i64
     lib.sngguf_attention.argtypes = [vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, i64, i64, i64, i64, vp, vp, i64, cf, ci, i64, vp, i64, i64,

@@ -1,0 +1,59 @@
+"""What the entry points of the page tables refuse, before anything touches a device (so this runs on a CPU host)."""
+import ctypes
+
+import pytest
+import torch
+
+from sensenova_u1_amd import PageTables, ops
+from sensenova_u1_amd.page_tables import _TablesStruct
+
+E_SHAPE, E_NULL, E_ALIGN = -2, -3, -4
+_BUF = ctypes.create_string_buffer(4096 + 64)
+P = (ctypes.addressof(_BUF) + 63) // 64 * 64
+
+
+def _tables(pages=P, lens=P, held=P, free=P, cursor=P, sequences=4, width=4, ring=8, page=16):
+    return _TablesStruct(pages, lens, held, free, cursor, sequences, width, ring, page)
+
+
+def _at(s):
+    return None if s is None else ctypes.addressof(s)
+
+
+def _append(tables=_tables(), added=P, tokens=4, ends=P, lens=P, cursor=P, positions=P, slots=P, missing=P, ws=None, nbytes=0):
+    return ops.load_library().sngguf_page_append(_at(tables), added, tokens, ends, lens, cursor, positions, slots, missing, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("bad,code", [(dict(sequences=-1), E_SHAPE), (dict(sequences=1 << 24), E_SHAPE), (dict(width=0), E_SHAPE), (dict(width=1 << 27), E_SHAPE), (dict(ring=0), E_SHAPE),
+                                      (dict(ring=1 << 31), E_SHAPE), (dict(page=8), E_SHAPE), (dict(page=24), E_SHAPE), (dict(page=8192), E_SHAPE), (dict(pages=None), E_NULL),
+                                      (dict(lens=None), E_NULL), (dict(free=None), E_NULL), (dict(cursor=None), E_NULL), (dict(pages=P + 2), E_ALIGN), (dict(cursor=P + 4), E_ALIGN),
+                                      (dict(held=P + 1), E_ALIGN)])
+def test_tables(bad, code):
+    lib = ops.load_library()
+    t = _tables(**bad)
+    assert _append(tables=t) == code and lib.sngguf_page_release(_at(t), P, None) == code and lib.sngguf_page_fork(_at(t), P, P, None) == code
+
+
+def test_calls():
+    lib = ops.load_library()
+    t = _tables()
+    assert _append(tables=None) == E_NULL and lib.sngguf_page_release(None, P, None) == E_NULL and lib.sngguf_page_fork(None, P, P, None) == E_NULL
+    for bad in (dict(added=None), dict(ends=None), dict(lens=None), dict(cursor=None), dict(positions=None), dict(slots=None), dict(missing=None), dict(tokens=8193)):
+        assert _append(**bad) == E_NULL, bad
+    for bad in (dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=8193, ws=P, nbytes=63)):
+        assert _append(**bad) == E_SHAPE, bad
+    for bad in (dict(added=P + 2), dict(positions=P + 4), dict(cursor=P + 4), dict(tokens=8193, ws=P + 8, nbytes=64)):
+        assert _append(**bad) == E_ALIGN, bad
+    assert lib.sngguf_page_release(_at(t), None, None) == E_NULL
+    assert lib.sngguf_page_fork(_at(t), None, P, None) == E_NULL and lib.sngguf_page_fork(_at(_tables(held=None)), P, P, None) == E_NULL
+    none = _tables(sequences=0, pages=None, lens=None, held=None, free=None, cursor=None)
+    assert _append(tables=none, added=None) == 0 and lib.sngguf_page_release(_at(none), None, None) == 0 and lib.sngguf_page_fork(_at(none), None, None, None) == 0
+    for sequences, tokens, nbytes in ((1024, 8192, 0), (1025, 1, 1025 * 16), (4, 8193, 64), (0, 9000, 0), (-1, 9000, 0), (4, -1, 0)):
+        assert lib.sngguf_page_append_workspace_bytes(sequences, tokens) == nbytes
+
+
+def test_host_tensors():
+    for call in (lambda: PageTables.empty(4, 4, 8, 16, device="cpu"), lambda: PageTables.empty(-1, 4, 8, 16, device="cpu"), lambda: PageTables.empty(4, 0, 8, 16, device="cpu"),
+                 lambda: PageTables.empty(4, 4, 0, 16, device="cpu")):
+        with pytest.raises(ops.SnGgufError):
+            call()
