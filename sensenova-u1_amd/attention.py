@@ -77,6 +77,11 @@ def _paged_workspace(*sizes: int) -> int:
     return ops.load_library().sngguf_paged_attention_workspace_bytes(*sizes)
 
 
+@functools.lru_cache(1024)
+def _shared_workspace(*sizes: int) -> int:
+    return ops.load_library().sngguf_shared_attention_workspace_bytes(*sizes)
+
+
 def _launch_with_workspace(index: int, nbytes: int, name: str, *args) -> None:
     if not nbytes:
         return _launch(index, name, *args, None, 0)
@@ -538,16 +543,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ends_q: 
     return out
 
 
-def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, lens: torch.Tensor, ends_q: Optional[torch.Tensor] = None,
-                    max_new: int = 0, scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Causal attention of new tokens over sequences in a paged cache, their own keys and values already written.
-
-    pages: int32 [sequences][width], the pages of each sequence in order.  lens: int32 [sequences], its tokens in all.  The queries
-    of sequence i are ``ends_q[i] : ends_q[i + 1]`` (int32 [sequences + 1]) and stand at its last places; without ``ends_q`` every
-    sequence has one, in order.  ``max_new``: the most queries of any sequence, where the program knows it (0: unknown); it
-    decides which kernels are launched and never what they compute.  With a ``window``, the pages in front of it may be anyone's.
-    ``scale``, ``window``, ``out``: as ``prompt_attention``."""
-    what = "paged_attention"
+def _paged(what: str, q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, lens: torch.Tensor, ends_q: Optional[torch.Tensor], max_new: int,
+           scale: Optional[float], window: int):
+    """The checked arguments of a call over a cache: (q, its token and head strides, pages, lens, ends_q, scale)"""
     q, qt, qh = _heads(q, what, "q", True)
     tokens, heads, dim = q.shape
     if dim != cache.dim:
@@ -569,6 +567,21 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     elif tokens != sequences:
         raise SnGgufError(f"{what}: {tokens} queries of {sequences} sequences need ends_q")
     _same_device(what, cache._index, q, pages, lens, ends_q)
+    return q, qt, qh, pages, lens, ends_q, scale
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, lens: torch.Tensor, ends_q: Optional[torch.Tensor] = None,
+                    max_new: int = 0, scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of new tokens over sequences in a paged cache, their own keys and values already written.
+
+    pages: int32 [sequences][width], the pages of each sequence in order.  lens: int32 [sequences], its tokens in all.  The queries
+    of sequence i are ``ends_q[i] : ends_q[i + 1]`` (int32 [sequences + 1]) and stand at its last places; without ``ends_q`` every
+    sequence has one, in order.  ``max_new``: the most queries of any sequence, where the program knows it (0: unknown); it
+    decides which kernels are launched and never what they compute.  With a ``window``, the pages in front of it may be anyone's.
+    ``scale``, ``window``, ``out``: as ``prompt_attention``."""
+    what = "paged_attention"
+    q, qt, qh, pages, lens, ends_q, scale = _paged(what, q, cache, pages, lens, ends_q, max_new, scale, window)
+    (tokens, heads, dim), (sequences, width) = q.shape, pages.shape
     out, ot, oh = _output(out, q, what, cache.k, cache.v, cache.k_scale, cache.v_scale)
     if tokens and sequences:
         if ends_q is None:
@@ -576,4 +589,35 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
         nbytes = _paged_workspace(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
         _launch_with_workspace(cache._index, nbytes, "sngguf_paged_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
                                pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), ot, oh)
+    return out
+
+
+def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, lens: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor,
+                            ends_q: Optional[torch.Tensor] = None, max_new: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attention`` of sequences that begin alike, as answers to one prompt do: what a group has in common is read once for all of it.
+
+    Group g is the sequences ``groups[g] : groups[g + 1]`` (int32 [groups + 1], not decreasing), whose first ``shared[g]`` tokens (int32 [groups])
+    lie in the pages of the first of them that has queries.  The other ones' pages hold the same there (``PageTables.fork`` makes them the same pages),
+    and are not read as far as whole multiples of 128 tokens go.  No more counts as common than every sequence of the group with queries has in front of its
+    new tokens; sequences of no group, or of a group of one, have nothing in common.  The result is that of ``paged_attention`` but for the order of its
+    sums; everything else is as there."""
+    what = "shared_prefix_attention"
+    q, qt, qh, pages, lens, ends_q, scale = _paged(what, q, cache, pages, lens, ends_q, max_new, scale, 0)
+    (tokens, heads, dim), (sequences, width) = q.shape, pages.shape
+    groups = _numbers(groups, torch.int32, None, what, "groups")
+    if groups.shape[0] < 1:
+        raise SnGgufError(f"{what}: groups has no entry")
+    count = groups.shape[0] - 1
+    shared = _numbers(shared, torch.int32, count, what, "shared")
+    _same_device(what, cache._index, groups, shared)
+    if not count:
+        return paged_attention(q, cache, pages, lens, ends_q, max_new, scale, out=out)
+    out, ot, oh = _output(out, q, what, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    if tokens and sequences:
+        if ends_q is None:
+            max_new = 1
+        nbytes = _shared_workspace(tokens, sequences, count, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
+        _launch_with_workspace(cache._index, nbytes, "sngguf_shared_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
+                               pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, groups.data_ptr(), shared.data_ptr(), count, max_new, scale,
+                               out.data_ptr(), ot, oh)
     return out

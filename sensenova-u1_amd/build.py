@@ -16,8 +16,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libsngguf.so")
 SOURCES = ["api.cpp", "gguf_reader.cpp", "dequantize.hip", "plain_bf16.hip", "rmsnorm.hip", "gemv.hip", "gemv_q8_mfma.hip", "gemv_kq_mfma.hip", "gemv_q8_tiled.hip", "gemm.hip", "gemm_tiles.hip", "gemm_dense4.hip", "gemm_mid_plan.hip", "gemm_mid.hip", "static_scratch.hip", "stream_probe.hip",
-           "api_attention.cpp", "rotary_cache.hip", "head_rotary.hip", "api_pages.cpp", "page_tables.hip", "attention_rows.hip", "attention_tiles.hip"]
-HEADERS = ["sngguf_common.hpp", "gemm_args.hpp", "gemm_mid.hpp", "kq_decode.hpp", "attention.hpp", "rotary_cache.hpp", "rotary_cache_device.hpp", "head_rotary.hpp", "page_tables.hpp"]
+           "api_attention.cpp", "rotary_cache.hip", "head_rotary.hip", "api_pages.cpp", "page_tables.hip", "attention_rows.hip", "attention_tiles.hip", "attention_shared.hip"]
+HEADERS = ["sngguf_common.hpp", "gemm_args.hpp", "gemm_mid.hpp", "kq_decode.hpp", "attention.hpp", "rotary_cache.hpp", "rotary_cache_device.hpp", "head_rotary.hpp", "page_tables.hpp", "attention_shared.hpp"]
 
 # packed-fp32 VALU forms are switched off for every device compile of this library
 HIP_FLAGS = [

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "attention.hpp"
+#include "attention_shared.hpp"
 #include "head_rotary.hpp"
 
 namespace sngguf {
@@ -145,6 +146,7 @@ constexpr int64_t kMostKeys = kMost - 65536;          // of a sequence: a few ti
 
 constexpr int kRowsLeast = 2, kRowsKeys = 128;        // key tiles that a split has at least; keys of a tile
 constexpr int kTilesLeast = 16, kTilesKeys = 64;     // (a workgroup costs as much as five tiles before its first and behind its last)
+constexpr int kCommonLeast = 4;                       // the same for keys that sequences have in common, whose rows have no other work
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // The kernel for many rows, bound by its arithmetic, has two more
@@ -231,6 +233,59 @@ int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* p
     const int rc = sngguf::launch_attention_tiles(a, p.rows, many_dim(a.dim), source, stream);
     if (rc != SNGGUF_OK || !partial) return rc;
     return sngguf::launch_attention_combine(a, p.rows, kTilesKeys, dim, p.tiles, most_rows, stream);
+}
+
+// ---- sequences that begin alike ----------------------------------------------------------------------------------------
+
+// The three launches of partial results, and where everything lies in the workspace
+struct SharedPlan {
+    Launch launch[sngguf::kSharedLaunches];
+    bool few_common;       // the common keys go to the kernel for few rows
+    int32_t few_rows;      // sequences of at most so many rows go to that kernel
+    int64_t entries, group_of, sequence_of, map[sngguf::kSharedLaunches], partial[sngguf::kSharedLaunches], bytes;
+};
+
+SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_t max_new, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    SharedPlan p = {};
+    const int64_t group = heads / kv_heads;
+    const int d = kernel_dim(dim);
+    // (one more for what a quotient leaves)
+    auto planned = [&](int64_t tiles, int rows, int want, int64_t key_tiles, int64_t least) {
+        Launch x;
+        x.rows = rows;
+        x.tiles = tiles;
+        x.want = key_tiles >= 2 * least ? want : 0;
+        x.grid = (tiles + (x.want + kv_heads - 1) / kv_heads) * kv_heads;     // (tiles here: of a key / value head)
+        x.partial_bytes = x.grid * rows * (d + 2) * 4;
+        return x;
+    };
+    // all queries of a group are rows of its common keys
+    const int64_t mean = tokens * group / groups;
+    const int widest = d == 256 ? 32 : 64;
+    p.few_common = mean <= widest;
+    const int rows = p.few_common ? (mean <= 16 ? 16 : mean <= 32 ? 32 : widest) : many_dim(dim) <= 192 && mean > 128 ? 256 : 128;
+    p.launch[0] = planned(row_tiles(tokens, groups, group, rows), rows, p.few_common ? few_at_a_time(rows, d) : many_at_a_time(rows, d),
+                          keys / (p.few_common ? kRowsKeys : kTilesKeys), p.few_common ? kRowsLeast : kCommonLeast);
+    const PagedPlan own = paged_plan(tokens, sequences, max_new, keys, heads, kv_heads, dim);
+    p.few_rows = (int32_t)own.few_rows;
+    if (own.few)
+        p.launch[1] = planned(own.many ? sequences : row_tiles(tokens, sequences, group, own.a.rows), own.a.rows, own.a.want, keys / kRowsKeys + 1, kRowsLeast);
+    if (own.many) p.launch[2] = planned(row_tiles(tokens, sequences, group, own.b.rows), own.b.rows, own.b.want, keys / kTilesKeys + 1, kTilesLeast);
+    auto room = [&](int64_t bytes) {
+        const int64_t at = p.bytes;
+        p.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    p.entries = room((groups + sequences) * (int64_t)sizeof(sngguf::AttentionEntry));
+    p.group_of = room(sequences * 4);
+    p.sequence_of = room(tokens * 4);
+    for (int l = 0; l < sngguf::kSharedLaunches; l++) p.map[l] = room(p.launch[l].grid / kv_heads * 4);
+    for (int l = 0; l < sngguf::kSharedLaunches; l++) p.partial[l] = room(p.launch[l].partial_bytes);
+    return p;
+}
+
+bool shared_sizes_fit(int64_t tokens, int64_t sequences, int64_t groups, int64_t max_new, int64_t keys) {
+    return tokens > 0 && tokens < kMost && sequences > 0 && groups > 0 && sequences + groups < kMost / 64 && max_new >= 0 && keys >= 0 && keys <= kMostKeys;
 }
 
 }  // namespace
@@ -514,6 +569,94 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
         return launch_many(a, p.b, d, q8 ? 2 : 1, rest, s);
     }
     return SNGGUF_OK;
+}
+
+int64_t sngguf_shared_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t groups, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads,
+                                                int64_t dim) {
+    if (!shared_sizes_fit(tokens_q, sequences, groups, max_new, max_keys) || !heads_fit(heads, kv_heads, dim)) return 0;
+    return shared_plan(tokens_q, sequences, groups, max_new, max_keys, heads, kv_heads, dim).bytes;
+}
+
+int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
+                            const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* lens, const int32_t* ends_q,
+                            int64_t sequences, const int32_t* groups, const int32_t* shared, int64_t group_count, int64_t max_new, float scale,
+                            void* out, int64_t out_token, int64_t out_head, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = check_cache(cache);
+    if (rc != SNGGUF_OK) return rc;
+    if (tokens_q < 0 || tokens_q >= kMost || sequences < 0 || sequences >= kMost || group_count < 1 || !heads_fit(heads, cache->kv_heads, cache->dim) ||
+        tokens_q * (heads / cache->kv_heads) >= kMost || max_new < 0 || !(scale >= 1e-30f) || scale > 1e30f || table_width < 0 ||
+        table_width > kMostKeys / cache->page_size || (sequences > 1 && table_stride < table_width) || (!ends_q && tokens_q < sequences))
+        return SNGGUF_E_BADSHAPE;
+    if (tokens_q == 0 || sequences == 0) return SNGGUF_OK;
+    const int64_t kv_heads = cache->kv_heads, keys = table_width * cache->page_size;
+    if (!ends_q) max_new = 1;
+    if (!shared_sizes_fit(tokens_q, sequences, group_count, max_new, keys)) return SNGGUF_E_BADSHAPE;
+    if (!q || !out || !lens || (table_width && !table) || !groups || !shared || !workspace) return SNGGUF_E_NULLPTR;
+    if (!whole_pieces(q, q_token, q_head) || !whole_pieces(out, out_token, out_head) || !aligned(table, 4) || !aligned(lens, 4) ||
+        !aligned(ends_q, 4) || !aligned(groups, 4) || !aligned(shared, 4) || !aligned(workspace, 16))
+        return SNGGUF_E_ALIGN;
+    const int d = kernel_dim(cache->dim);
+    const bool q8 = cache->qtype == SNGGUF_TYPE_Q8_0;
+    const SharedPlan p = shared_plan(tokens_q, sequences, group_count, max_new, keys, heads, kv_heads, cache->dim);
+    if (workspace_bytes < p.bytes || !launch_fits((tokens_q * heads + 3) / 4, 256)) return SNGGUF_E_BADSHAPE;
+    for (int l = 0; l < sngguf::kSharedLaunches; l++)
+        if (!launch_fits(p.launch[l].grid, l == 1 || (l == 0 && p.few_common) ? 256 : 2 * p.launch[l].rows)) return SNGGUF_E_BADSHAPE;
+    sngguf::SharedArgs s = {};
+    AttentionArgs& a = s.a;
+    a.q = static_cast<const bf16_t*>(q);
+    a.out = static_cast<bf16_t*>(out);
+    a.q_token = q_token, a.q_head = q_head, a.out_token = out_token, a.out_head = out_head;
+    a.k_pages = cache->k;
+    a.v_pages = cache->v;
+    a.k_scales = static_cast<const uint16_t*>(cache->k_scale);
+    a.v_scales = static_cast<const uint16_t*>(cache->v_scale);
+    a.table = table;
+    a.lens = lens;
+    a.table_stride = table_stride;
+    a.table_width = (int32_t)table_width;
+    a.pages = (int32_t)cache->pages;
+    a.page_shift = log2_of(cache->page_size);
+    a.ends_q = ends_q;
+    a.sequences = (int32_t)sequences;
+    a.tokens_q = tokens_q;
+    a.heads = (int32_t)heads;
+    a.kv_heads = (int32_t)kv_heads;
+    a.group = (int32_t)(heads / kv_heads);
+    a.dim = (int32_t)cache->dim;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    uint8_t* room = static_cast<uint8_t*>(workspace);
+    s.groups = groups;
+    s.shared = shared;
+    s.group_count = (int32_t)group_count;
+    s.entries = reinterpret_cast<sngguf::AttentionEntry*>(room + p.entries);
+    s.group_of = reinterpret_cast<int32_t*>(room + p.group_of);
+    s.sequence_of = ends_q ? reinterpret_cast<int32_t*>(room + p.sequence_of) : nullptr;
+    for (int l = 0; l < sngguf::kSharedLaunches; l++) {
+        sngguf::SharedLaunch& x = s.launch[l];
+        const bool few = l == 1 || (l == 0 && p.few_common);
+        x.rows = p.launch[l].rows;
+        x.keys = few ? kRowsKeys : kTilesKeys;
+        x.min_rows = l == 2 && x.rows ? p.few_rows + 1 : 1;
+        x.max_rows = l == 1 ? p.few_rows : (int32_t)(kMost - 1);
+        x.want = p.launch[l].want;
+        x.least = few ? kRowsLeast : l == 0 ? kCommonLeast : kTilesLeast;
+        x.split = x.want > 0;
+        x.slots = (int32_t)(p.launch[l].grid / kv_heads);
+        x.map = reinterpret_cast<int32_t*>(room + p.map[l]);
+        x.partial = reinterpret_cast<float*>(room + p.partial[l]);
+    }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    int r = sngguf::launch_shared_plan(s, st);
+    a.entries = s.entries;
+    for (int l = 0; l < sngguf::kSharedLaunches && r == SNGGUF_OK; l++) {
+        if (!p.launch[l].grid) continue;
+        a.map = s.launch[l].map;
+        a.partial = s.launch[l].partial;
+        a.grid = p.launch[l].grid;
+        r = l == 1 || (l == 0 && p.few_common) ? sngguf::launch_attention_rows(a, p.launch[l].rows, d, q8, st)
+                                               : sngguf::launch_attention_tiles(a, p.launch[l].rows, many_dim(cache->dim), q8 ? 2 : 1, st);
+    }
+    return r == SNGGUF_OK ? sngguf::launch_shared_join(s, d, st) : r;
 }
 
 }  // extern "C"

@@ -12,6 +12,17 @@
 
 namespace sngguf {
 
+// Where a launch's sequences and workgroups are planned by a kernel in front of it (attention_shared.hip): a sequence, or the tokens that a
+// group of sequences has in common as one whose queries are all of the group's.
+struct AttentionEntry {
+    int32_t q0, lq;         // its queries
+    int32_t k0, lk;         // its keys: places [k0, lk), k0 a multiple of every kernel's key tile
+    int32_t row;            // of the table of pages
+    int32_t splits, first;  // workgroups (of a key / value head) of each row tile, number of the first one
+    int32_t flags;
+};
+enum { kEntryCausal = 1, kEntryPartial = 2, kEntryOnce = 4 };
+
 struct AttentionArgs {
     const bf16_t* q;        // [tokens_q][heads][dim]
     bf16_t* out;
@@ -40,15 +51,20 @@ struct AttentionArgs {
     int32_t want;           // workgroups that fill the device
     int32_t least;          // key tiles of a split at least
     int64_t grid;           // workgroups of the main launch
+    // planned launches (NULL: every workgroup finds its own place)
+    const AttentionEntry* entries;
+    const int32_t* map;     // [workgroups / kv_heads]: entry of each, or -1
 };
 
 struct AttentionSequence {
     int64_t q0, k0;
     int32_t lq, lk;
+    int32_t from;           // first key that counts, a multiple of the key tile
 };
 
 __device__ __forceinline__ AttentionSequence attention_sequence(const AttentionArgs& a, int i) {
     AttentionSequence s;
+    s.from = 0;
     if (a.ends_q) {
         // (values that are no cumulative lengths stay within the tensors)
         int64_t e0 = a.ends_q[i], e1 = a.ends_q[i + 1];
@@ -107,14 +123,47 @@ struct AttentionBlock {
     int32_t seq, row_tile, split, splits, kv_head;
     int64_t slot;           // number of this workgroup's (combining: of split 0's) partial result; splits lie kv_heads apart
     bool there;
+    bool causal, partial;   // partial: its result goes to be joined
+    bool once;              // planned launches: nobody else reads its pages
 };
+
+// A planned workgroup's place
+template <int ROWS>
+__device__ __forceinline__ AttentionBlock attention_planned_block(const AttentionArgs& a, uint32_t id) {
+    AttentionBlock b;
+    b.kv_head = id % (uint32_t)a.kv_heads;
+    const uint32_t want = id / (uint32_t)a.kv_heads;
+    const int32_t at = __builtin_amdgcn_readfirstlane(a.map[want]);
+    b.there = at >= 0;
+    if (!b.there) return b;
+    const AttentionEntry e = a.entries[at];
+    b.s.q0 = (uint32_t)__builtin_amdgcn_readfirstlane(e.q0);
+    b.s.lq = __builtin_amdgcn_readfirstlane(e.lq);
+    b.s.k0 = 0;
+    b.s.lk = __builtin_amdgcn_readfirstlane(e.lk);
+    b.s.from = __builtin_amdgcn_readfirstlane(e.k0);
+    b.seq = __builtin_amdgcn_readfirstlane(e.row);
+    b.splits = __builtin_amdgcn_readfirstlane(e.splits);
+    const int32_t flags = __builtin_amdgcn_readfirstlane(e.flags);
+    b.causal = flags & kEntryCausal;
+    b.partial = flags & kEntryPartial;
+    b.once = flags & kEntryOnce;
+    const uint32_t within = want - (uint32_t)__builtin_amdgcn_readfirstlane(e.first), t = within / (uint32_t)b.splits;
+    b.split = (int32_t)(within - t * (uint32_t)b.splits);
+    b.row_tile = (int32_t)(((uint32_t)b.s.lq * (uint32_t)a.group + ROWS - 1) / ROWS - 1 - t);
+    b.slot = id;
+    return b;
+}
 
 // COMBINE: `id` counts (row tile, head) pairs and not (row tile, split, head) triples.
 template <int ROWS, int KEYS, bool COMBINE>
 __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a, uint32_t id) {
+    if (!COMBINE && a.entries) return attention_planned_block<ROWS>(a, id);
     const int lane = threadIdx.x & 63;
     AttentionBlock b;
     b.there = false;
+    b.causal = a.causal;
+    b.once = false;
     // heads of one row tile are neighbours: with 8 key / value heads each XCD keeps to one head's keys and values
     b.kv_head = id % (uint32_t)a.kv_heads;
     const uint32_t want = id / (uint32_t)a.kv_heads;
@@ -179,6 +228,8 @@ __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a
             b.s.k0 = (uint32_t)__builtin_amdgcn_readlane((int)mine_s.k0, l);
             b.s.lq = __builtin_amdgcn_readlane(mine_s.lq, l);
             b.s.lk = __builtin_amdgcn_readlane(mine_s.lk, l);
+            b.s.from = 0;
+            b.partial = b.splits > 1;
             b.there = true;
             return b;
         }
@@ -196,17 +247,18 @@ __device__ __forceinline__ int32_t attention_token(const AttentionArgs& a, int64
 }
 
 // Keys [lo, hi) that some row of rows [r0, r1) of a sequence sees.
-__device__ __forceinline__ void attention_keys(const AttentionArgs& a, const AttentionSequence& s, int64_t r0, int64_t r1, int32_t& lo, int32_t& hi) {
+__device__ __forceinline__ void attention_keys(const AttentionArgs& a, const AttentionBlock& b, int64_t r0, int64_t r1, int32_t& lo, int32_t& hi) {
+    const AttentionSequence& s = b.s;
     const int64_t back = (int64_t)s.lk - s.lq;
-    lo = 0;
+    lo = s.from;
     hi = s.lk;
-    if (a.causal) {
+    if (b.causal) {
         const int64_t last = back + (uint32_t)(r1 - 1) / (uint32_t)a.group + 1;
         if (last < hi) hi = (int32_t)(last < 0 ? 0 : last);
     }
     if (a.window) {
         const int64_t first = back + (uint32_t)r0 / (uint32_t)a.group - a.window + 1;
-        if (first > 0) lo = (int32_t)(first < hi ? first : hi);
+        if (first > lo) lo = (int32_t)(first < hi ? first : hi);
     }
 }
 
@@ -228,7 +280,7 @@ __device__ __forceinline__ void attention_row_again(const AttentionArgs& a, cons
     const int32_t token = attention_token(a, r, head), place = b.s.lk - b.s.lq + token;
     head += b.kv_head * a.group;
     const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
-    if (a.causal && place + 1 < hi) hi = place + 1;
+    if (b.causal && place + 1 < hi) hi = place + 1;
     if (a.window && place - a.window + 1 > lo) lo = (int32_t)(place - a.window + 1);
     float m = -__builtin_inff(), l = 0.f, o[PER];
 #pragma unroll
@@ -310,10 +362,10 @@ __device__ __forceinline__ void attention_row_again(const AttentionArgs& a, cons
     for (int t = 0; t < PER; t++) {
         const int e = lane + 64 * t;
         if (e >= a.dim) continue;
-        if (b.splits > 1) a.partial[part * DT + e] = o[t] * back;
+        if (b.partial) a.partial[part * DT + e] = o[t] * back;
         else a.out[(b.s.q0 + token) * a.out_token + (int64_t)head * a.out_head + e] = f32_to_bf16(o[t] * inv);
     }
-    if (b.splits > 1 && lane == 0) {
+    if (b.partial && lane == 0) {
         // (a row whose scores are NaN has no maximum, and the join passes over splits without one: any number, so that the sum gets there)
         float* st = a.partial + a.grid * ROWS * DT + part * 2;
         st[0] = l != l ? 0.f : far ? m + (31 + UP) : m;

@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     const int64_t rows = (int64_t)b.s.lq * a.group;
     const int64_t r0 = (int64_t)b.row_tile * ROWS, r1 = r0 + ROWS < rows ? r0 + ROWS : rows;
     int32_t lo, hi;
-    attention_keys(a, b.s, r0, r1, lo, hi);
+    attention_keys(a, b, r0, r1, lo, hi);
     const int32_t back = b.s.lk - b.s.lq, most = b.s.lk - 1;
 
     // ---- this split's runs, and the cache's words of a run -----------------------------------------------------------------
@@ -212,10 +212,14 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         page_v = page_of(key0 + v_key);
         if constexpr (ASK) {
             // this split's first page, and what up to 63 other sequences have in its place: a common prompt is at the same place in all tables
-            const int32_t other = (b.seq & ~63) + lane, at = (s0 * kKeys) >> a.page_shift;
-            const bool there = other < a.sequences && other != b.seq;
-            const int32_t mine = table[at], theirs = a.table[(int64_t)(there ? other : b.seq) * a.table_stride + at];
-            once = __ballot(there && theirs == mine) == 0;
+            if (a.entries) {
+                once = b.once;
+            } else {
+                const int32_t other = (b.seq & ~63) + lane, at = (s0 * kKeys) >> a.page_shift;
+                const bool there = other < a.sequences && other != b.seq;
+                const int32_t mine = table[at], theirs = a.table[(int64_t)(there ? other : b.seq) * a.table_stride + at];
+                once = __ballot(there && theirs == mine) == 0;
+            }
         }
         load_keys(key0, page_k);
         load_values(key0, page_v);
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         head += b.kv_head * a.group;
         const bf16_t* q = a.q + (b.s.q0 + token) * a.q_token + (int64_t)head * a.q_head;
         const int32_t place = back + token;
-        last[n] = a.causal && place < most ? place : most;
+        last[n] = b.causal && place < most ? place : most;
         first[n] = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
         u32x4_t raw[KC];
 #pragma unroll
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     }
     // keys that every row of the tile sees
     const int32_t place0 = back + (int32_t)((uint32_t)r0 / (uint32_t)a.group), place1 = back + (int32_t)((uint32_t)(r1 - 1) / (uint32_t)a.group);
-    const int32_t all_last = a.causal && place0 < most ? place0 : most;
+    const int32_t all_last = b.causal && place0 < most ? place0 : most;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
     f32x4_t acc[NT][VP];
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
             odd = rl * 0.f;
 #pragma unroll
             for (int t = 0; t < VP; t++) odd = __builtin_fmaf(o[t], 0.f, odd);
-            if (b.splits > 1) {
+            if (b.partial) {
                 float* part = a.partial + (b.slot * ROWS + 16 * n + row) * DT + e;
 #pragma unroll
                 for (int t = 0; t < VP; t += 4) *reinterpret_cast<f32x4_t*>(part + t) = f32x4_t{o[t], o[t + 1], o[t + 2], o[t + 3]};

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     const int64_t rows = (int64_t)b.s.lq * a.group;
     const int64_t r0 = (int64_t)b.row_tile * ROWS, r1 = r0 + ROWS < rows ? r0 + ROWS : rows;
     int32_t lo, hi;
-    attention_keys(a, b.s, r0, r1, lo, hi);
+    attention_keys(a, b, r0, r1, lo, hi);
     const int32_t back = b.s.lk - b.s.lq;
 
     // ---- this split's tiles -------------------------------------------------------------------------------------------
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     const int32_t count = s1 - s0;
     // rows whose visible keys are the fewest: tiles inside these bounds need no mask
     const int32_t place0 = back + (int32_t)((uint32_t)r0 / (uint32_t)a.group), place1 = back + (int32_t)((uint32_t)(r1 - 1) / (uint32_t)a.group);
-    const int32_t all_last = a.causal && place0 < b.s.lk - 1 ? place0 : b.s.lk - 1;
+    const int32_t all_last = b.causal && place0 < b.s.lk - 1 ? place0 : b.s.lk - 1;
     const int32_t all_first = a.window && place1 - a.window + 1 > 0 ? (int32_t)(place1 - a.window + 1) : 0;
 
     f32x16_t acc[DTILES];
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
         const int32_t token = attention_token(a, my_row < r1 ? my_row : r1 - 1, head);
         head += b.kv_head * a.group;
         const int32_t place = back + token;
-        last = a.causal && place < most ? place : most;
+        last = b.causal && place < most ? place : most;
         first = a.window && place - a.window + 1 > 0 ? (int32_t)(place - a.window + 1) : 0;
         u32x4_t raw[KS] = {};
         if (count > 0) {
@@ -560,7 +560,7 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
         for (int i = 0; i < 16; i++) odd = __builtin_fmaf(acc[t][i], 0.f, odd);
     const uint64_t odd_lanes = __ballot(odd != 0.f && my_row < r1);
     uint32_t again = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);      // the wavefront's rows that are not finite
-    if (b.splits > 1) {
+    if (b.partial) {
         if (my_row < r1) {
             const int64_t at = b.slot * ROWS + (my_row - r0);
 #pragma unroll

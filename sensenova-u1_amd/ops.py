@@ -43,7 +43,7 @@ EXPORTED_SYMBOLS = (
     "sngguf_probe_stream_read_out_bytes", "sngguf_probe_stream_read",
     "sngguf_rotary", "sngguf_cache_write", "sngguf_cache_write_rotary", "sngguf_head_rotary", "sngguf_cache_write_head_rotary", "sngguf_cache_read",
     "sngguf_page_append_workspace_bytes", "sngguf_page_append", "sngguf_page_release", "sngguf_page_fork", "sngguf_attention_workspace_bytes", "sngguf_attention",
-    "sngguf_paged_attention_workspace_bytes", "sngguf_paged_attention",
+    "sngguf_paged_attention_workspace_bytes", "sngguf_paged_attention", "sngguf_shared_attention_workspace_bytes", "sngguf_shared_attention",
     "sngguf_file_open", "sngguf_file_close", "sngguf_file_version", "sngguf_file_alignment", "sngguf_file_tensor_count",
     "sngguf_file_tensor", "sngguf_file_metadata_count", "sngguf_file_metadata", "sngguf_file_read_tensors",
 )
@@ -182,6 +182,10 @@ def load_library() -> ctypes.CDLL:
     lib.sngguf_paged_attention_workspace_bytes.restype = i64
     lib.sngguf_paged_attention.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, cf, i64, vp, i64, i64, vp, i64, vp]
     lib.sngguf_paged_attention.restype = ci
+    lib.sngguf_shared_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i64, i64]
+    lib.sngguf_shared_attention_workspace_bytes.restype = i64
+    lib.sngguf_shared_attention.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64, vp, vp, i64, i64, cf, vp, i64, i64, vp, i64, vp]
+    lib.sngguf_shared_attention.restype = ci
     # host-only GGUF container reader
     cp = ctypes.c_char_p
     lib.sngguf_file_open.argtypes = [cp, ctypes.POINTER(vp), cp, i64]
