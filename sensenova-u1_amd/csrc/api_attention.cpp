@@ -119,11 +119,10 @@ void set_norm(sngguf::HeadNormArgs& a, const sngguf_head_norm* n) {
     a.parts = n->parts;
     a.bf16 = n->weight_type == 2;
     a.eps = n->eps;
-    a.group = n->elements[0] / 8;
     for (int p = 0; p < n->parts; p++) {
         a.weight[p] = n->weight[p];
         a.elements[p] = n->elements[p];
-        if (n->elements[p] != n->elements[0] || (a.group & (a.group - 1)) != 0) a.group = 0;
+        a.one_over[p] = 1.f / (float)n->elements[p];
     }
 }
 
@@ -242,7 +241,7 @@ struct SharedPlan {
     Launch launch[sngguf::kSharedLaunches];
     bool few_common;       // the common keys go to the kernel for few rows
     int32_t few_rows;      // sequences of at most so many rows go to that kernel
-    int64_t entries, group_of, sequence_of, map[sngguf::kSharedLaunches], partial[sngguf::kSharedLaunches], bytes;
+    int64_t entries, sequence_of, map[sngguf::kSharedLaunches], partial[sngguf::kSharedLaunches], bytes;
 };
 
 SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_t max_new, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
@@ -277,9 +276,8 @@ SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_
         return at;
     };
     p.entries = room((groups + sequences) * (int64_t)sizeof(sngguf::AttentionEntry));
-    p.group_of = room(sequences * 4);
     p.sequence_of = room(tokens * 4);
-    for (int l = 0; l < sngguf::kSharedLaunches; l++) p.map[l] = room(p.launch[l].grid / kv_heads * 4);
+    for (int l = 0; l < sngguf::kSharedLaunches; l++) p.map[l] = room(p.launch[l].grid / kv_heads * (int64_t)sizeof(sngguf::AttentionEntry));
     for (int l = 0; l < sngguf::kSharedLaunches; l++) p.partial[l] = room(p.launch[l].partial_bytes);
     return p;
 }
@@ -629,25 +627,21 @@ int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int6
     s.shared = shared;
     s.group_count = (int32_t)group_count;
     s.entries = reinterpret_cast<sngguf::AttentionEntry*>(room + p.entries);
-    s.group_of = reinterpret_cast<int32_t*>(room + p.group_of);
     s.sequence_of = ends_q ? reinterpret_cast<int32_t*>(room + p.sequence_of) : nullptr;
     for (int l = 0; l < sngguf::kSharedLaunches; l++) {
         sngguf::SharedLaunch& x = s.launch[l];
         const bool few = l == 1 || (l == 0 && p.few_common);
-        x.rows = p.launch[l].rows;
-        x.keys = few ? kRowsKeys : kTilesKeys;
-        x.min_rows = l == 2 && x.rows ? p.few_rows + 1 : 1;
-        x.max_rows = l == 1 ? p.few_rows : (int32_t)(kMost - 1);
+        x.row_shift = log2_of(p.launch[l].rows);
+        x.key_shift = log2_of(few ? kRowsKeys : kTilesKeys);
+        x.max_rows = p.few_rows;
         x.want = p.launch[l].want;
         x.least = few ? kRowsLeast : l == 0 ? kCommonLeast : kTilesLeast;
-        x.split = x.want > 0;
         x.slots = (int32_t)(p.launch[l].grid / kv_heads);
-        x.map = reinterpret_cast<int32_t*>(room + p.map[l]);
+        x.map = reinterpret_cast<sngguf::AttentionEntry*>(room + p.map[l]);
         x.partial = reinterpret_cast<float*>(room + p.partial[l]);
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     int r = sngguf::launch_shared_plan(s, st);
-    a.entries = s.entries;
     for (int l = 0; l < sngguf::kSharedLaunches && r == SNGGUF_OK; l++) {
         if (!p.launch[l].grid) continue;
         a.map = s.launch[l].map;

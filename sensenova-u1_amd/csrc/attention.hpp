@@ -52,8 +52,7 @@ struct AttentionArgs {
     int32_t least;          // key tiles of a split at least
     int64_t grid;           // workgroups of the main launch
     // planned launches (NULL: every workgroup finds its own place)
-    const AttentionEntry* entries;
-    const int32_t* map;     // [workgroups / kv_heads]: entry of each, or -1
+    const AttentionEntry* map;   // [workgroups / kv_heads]: what each does; nothing where there are no queries
 };
 
 struct AttentionSequence {
@@ -133,12 +132,11 @@ __device__ __forceinline__ AttentionBlock attention_planned_block(const Attentio
     AttentionBlock b;
     b.kv_head = id % (uint32_t)a.kv_heads;
     const uint32_t want = id / (uint32_t)a.kv_heads;
-    const int32_t at = __builtin_amdgcn_readfirstlane(a.map[want]);
-    b.there = at >= 0;
-    if (!b.there) return b;
-    const AttentionEntry e = a.entries[at];
-    b.s.q0 = (uint32_t)__builtin_amdgcn_readfirstlane(e.q0);
+    const AttentionEntry e = a.map[want];
     b.s.lq = __builtin_amdgcn_readfirstlane(e.lq);
+    b.there = b.s.lq != 0;
+    if (!b.there) return b;
+    b.s.q0 = (uint32_t)__builtin_amdgcn_readfirstlane(e.q0);
     b.s.k0 = 0;
     b.s.lk = __builtin_amdgcn_readfirstlane(e.lk);
     b.s.from = __builtin_amdgcn_readfirstlane(e.k0);
@@ -158,7 +156,6 @@ __device__ __forceinline__ AttentionBlock attention_planned_block(const Attentio
 // COMBINE: `id` counts (row tile, head) pairs and not (row tile, split, head) triples.
 template <int ROWS, int KEYS, bool COMBINE>
 __device__ __forceinline__ AttentionBlock attention_block(const AttentionArgs& a, uint32_t id) {
-    if (!COMBINE && a.entries) return attention_planned_block<ROWS>(a, id);
     const int lane = threadIdx.x & 63;
     AttentionBlock b;
     b.there = false;

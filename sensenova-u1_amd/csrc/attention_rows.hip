@@ -70,8 +70,8 @@ template <bool ONCE, typename T> __device__ __forceinline__ T word_at(const uint
 // spill (32 single tokens over 4000 in bf16: 193 us against 297).
 constexpr int rows_workgroups(int dt, int nt) { return nt * dt <= 128 ? 3 : nt * dt <= 256 && dt < 256 ? 2 : 1; }
 
-// DT: elements of a head, rounded up (FULL: exactly).  NT: 16-row tiles.
-template <int DT, bool FULL, bool Q8, int NT>
+// DT: elements of a head, rounded up (FULL: exactly).  NT: 16-row tiles.  PLANNED: a kernel in front of this one dealt the work.
+template <int DT, bool FULL, bool Q8, int NT, bool PLANNED>
 __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_rows_kernel(AttentionArgs a) {
     typedef typename Operand<Q8>::T op_t;
     constexpr int ROWS = 16 * NT;
@@ -95,7 +95,9 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
     extern __shared__ __attribute__((aligned(16))) float lds[];   // [wave][16][DT] sums, then [wave][ROWS][2]
     float* stats = lds + kWaves * 16 * DT;
 
-    const AttentionBlock b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
+    AttentionBlock b;
+    if constexpr (PLANNED) b = attention_planned_block<ROWS>(a, blockIdx.x);
+    else b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
     if (!b.there) return;
     const int dim = FULL ? DT : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(kThreads, rows_workgroups(DT, NT)) void attention_r
         page_v = page_of(key0 + v_key);
         if constexpr (ASK) {
             // this split's first page, and what up to 63 other sequences have in its place: a common prompt is at the same place in all tables
-            if (a.entries) {
+            if constexpr (PLANNED) {
                 once = b.once;
             } else {
                 const int32_t other = (b.seq & ~63) + lane, at = (s0 * kKeys) >> a.page_shift;
@@ -678,14 +680,15 @@ int launch_attention_combine(const AttentionArgs& a, int rows, int keys, int dim
 }
 
 // dim: of the kernel, 64, 128 or 256; rows: of a tile, 16, 32 or (up to 128 elements) 64
-int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream) {
+template <bool PLANNED>
+static int launch_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream) {
 #define SNGGUF_GO(D, F, Q, N)                                                                                           \
     if (dim == D && (a.dim == D) == F && q8 == Q && rows == 16 * N) {                                                   \
         constexpr int kLds = (kWaves * 16 * D + kWaves * 16 * N * 2) * 4;                                               \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_rows_kernel<D, F, Q, N>), \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_rows_kernel<D, F, Q, N, PLANNED>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_rows_kernel<D, F, Q, N><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);                       \
+        attention_rows_kernel<D, F, Q, N, PLANNED><<<dim3((unsigned)a.grid), kThreads, kLds, stream>>>(a);              \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
 #define SNGGUF_GO_TYPES(D, N) SNGGUF_GO(D, true, false, N) SNGGUF_GO(D, false, false, N) SNGGUF_GO(D, true, true, N) SNGGUF_GO(D, false, true, N)
@@ -700,6 +703,10 @@ int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hi
 #undef SNGGUF_GO_TYPES
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
+}
+
+int launch_attention_rows(const AttentionArgs& a, int rows, int dim, bool q8, hipStream_t stream) {
+    return a.map ? launch_rows<true>(a, rows, dim, q8, stream) : launch_rows<false>(a, rows, dim, q8, stream);
 }
 
 }  // namespace sngguf

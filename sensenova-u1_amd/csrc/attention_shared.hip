@@ -19,184 +19,295 @@ namespace sngguf {
 
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kThreads = 256;
+constexpr int32_t kOwn = 16;            // so many numbers a lane writes by itself, more all lanes of the wavefront
+constexpr float kNever = 1e9f;
 
+// The least of the wavefront's numbers (row shifts, then a row's last value handed on; lanes without a partner keep theirs)
 __device__ __forceinline__ int32_t wave_min(int32_t x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o));
-    return x;
-}
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor((unsigned long long)x, o);
-    return x;
+#define SNGGUF_STEP(CONTROL, ROWS) x = min(x, __builtin_amdgcn_update_dpp(x, x, CONTROL, ROWS, 0xF, false));
+    SNGGUF_STEP(0x111, 0xF)
+    SNGGUF_STEP(0x112, 0xF)
+    SNGGUF_STEP(0x114, 0xF)
+    SNGGUF_STEP(0x118, 0xF)
+    SNGGUF_STEP(0x142, 0xA)
+    SNGGUF_STEP(0x143, 0xC)
+#undef SNGGUF_STEP
+    return __builtin_amdgcn_readlane(x, 63);
 }
 
-// Which launch takes an entry, its row tiles and key tiles
-__device__ __forceinline__ int entry_tiles(const SharedArgs& s, const AttentionEntry& e, bool common, uint32_t& row_tiles, uint32_t& key_tiles) {
-    const uint32_t rows = (uint32_t)e.lq * (uint32_t)s.a.group;
-    row_tiles = key_tiles = 0;
-    if (rows == 0 || (common && e.lk == 0)) return -1;
-#pragma unroll
-    for (int l = 0; l < kSharedLaunches; l++) {
-        const SharedLaunch& x = s.launch[l];
-        if ((l == 0) != common || x.slots == 0 || (int32_t)rows < x.min_rows || (int32_t)rows > x.max_rows) continue;
-        row_tiles = (rows + (uint32_t)x.rows - 1) / (uint32_t)x.rows;
-        const int32_t lo = e.k0 / x.keys, hi = (int32_t)(((int64_t)e.lk + x.keys - 1) / x.keys);
-        key_tiles = hi > lo ? hi - lo : 1;
-        return l;
-    }
-    return -1;
+// Sum over the wavefront, in all lanes
+__device__ __forceinline__ float wave_total(float x) {
+#define SNGGUF_STEP(CONTROL, ROWS) x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CONTROL, ROWS, 0xF, false));
+    SNGGUF_STEP(0x111, 0xF)
+    SNGGUF_STEP(0x112, 0xF)
+    SNGGUF_STEP(0x114, 0xF)
+    SNGGUF_STEP(0x118, 0xF)
+    SNGGUF_STEP(0x142, 0xA)
+    SNGGUF_STEP(0x143, 0xC)
+#undef SNGGUF_STEP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// Choices for the key tiles of a split: what fills all workgroups that run at once, to the sixteenth, as splits are whole; where
+// none of them does, what does in any case
+constexpr int kTries = 3;
+__device__ __forceinline__ float choice(float fill, int i) { return __builtin_ceilf(fill * (1.f + i / 16.f)); }
+
+// An entry's launch (-1: none), its row tiles and key tiles, and how many workgroups of a head it would take by each choice
+struct Entry {
+    int launch;
+    uint32_t row_tiles, key_tiles;
+};
+__device__ __forceinline__ Entry entry_of(const SharedLaunch* launch, const AttentionEntry& e, int group, bool common) {
+    const uint32_t rows = (uint32_t)e.lq * (uint32_t)group;
+    Entry x = {-1, 0, 0};
+    if (rows == 0 || (common && e.lk == 0)) return x;
+    const int l = common ? 0 : (int32_t)rows > launch[1].max_rows || launch[1].slots == 0 ? 2 : 1;
+    if (launch[l].slots == 0) return x;
+    const int row_shift = launch[l].row_shift, key_shift = launch[l].key_shift;
+    x.launch = l;
+    x.row_tiles = (rows + (1u << row_shift) - 1) >> row_shift;
+    const int32_t lo = e.k0 >> key_shift, hi = (int32_t)(((int64_t)e.lk + (1 << key_shift) - 1) >> key_shift);
+    x.key_tiles = hi > lo ? hi - lo : 1;
+    return x;
 }
 
 }  // namespace
 
-__global__ __launch_bounds__(kPlanThreads) void attention_shared_plan_kernel(SharedArgs s) {
-    __shared__ uint64_t sums[kPlanWaves][2 * kSharedLaunches];
-    __shared__ uint32_t ups[kPlanWaves][kSharedLaunches];
-    __shared__ int32_t firsts[kPlanThreads], counts[kPlanThreads];
+// W wavefronts.  ONE: there are no more entries than threads, and what a phase hands to the next stays in LDS and registers.
+// The kernel runs through once, on one compute unit, and its code comes from memory as it goes: what is done for each launch is a
+// loop that is not unrolled, and what is done once for each of them is done by as many lanes.
+template <int W, bool ONE>
+__global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArgs s) {
+    constexpr int T = 64 * W;
+    touch_arguments(s);
+    __shared__ AttentionEntry held[ONE ? T : 1];
+    __shared__ SharedLaunch launch[kSharedLaunches];
+    __shared__ float work_of[W][kSharedLaunches];
+    __shared__ uint32_t tiles_of[W][kSharedLaunches], tried[W][kSharedLaunches][kTries], ups[W][kSharedLaunches];
     const AttentionArgs& a = s.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t groups = s.group_count, sequences = a.sequences;
     const int64_t all = (int64_t)groups + sequences;
+    AttentionEntry* entries = ONE ? held : s.entries;         // groups, then sequences; `row` of a sequence: its group with common keys, or -1
 
-    for (int64_t i = tid; i < sequences; i += kPlanThreads) {
-        const AttentionSequence q = attention_sequence(a, (int)i);
-        s.entries[groups + i] = {(int32_t)q.q0, q.lq, 0, q.lk, (int32_t)i, 1, -1, 0};
-        s.group_of[i] = -1;
+    // (the first group's numbers are on their way while lengths are)
+    int32_t group_0 = 0, group_1 = 0, group_shared = 0;
+    if (wave < groups) group_0 = s.groups[wave], group_1 = s.groups[wave + 1], group_shared = s.shared[wave];
+    if (tid < kSharedLaunches) launch[tid] = s.launch[tid];
+#pragma unroll 1
+    for (int64_t base = 0; base < sequences; base += T) {
+        const int64_t i = base + tid;
+        AttentionSequence q = {0, 0, 0, 0, 0};
+        if (i < sequences) {
+            q = attention_sequence(a, (int)i);
+            entries[groups + i] = {(int32_t)q.q0, q.lq, 0, q.lk, -1, 1, -1, 0};
+        }
+        // (tokens of no sequence keep any number, and the join sees that they are not that one's)
+        if (!s.sequence_of) continue;
+        if (q.lq <= kOwn)
+            for (int32_t j = 0; j < q.lq; j++) s.sequence_of[q.q0 + j] = (int32_t)i;
+        for (uint64_t many = __ballot(q.lq > kOwn); many; many &= many - 1) {
+            const int m = __builtin_ctzll(many);
+            const int32_t q0 = __builtin_amdgcn_readlane((int)q.q0, m), lq = __builtin_amdgcn_readlane(q.lq, m), of = __builtin_amdgcn_readlane((int)i, m);
+            for (int32_t j = lane; j < lq; j += 64) s.sequence_of[q0 + j] = of;
+        }
     }
-    if (s.sequence_of)
-        for (int64_t t = tid; t < a.tokens_q; t += kPlanThreads) s.sequence_of[t] = -1;
-#pragma unroll
-    for (int l = 0; l < kSharedLaunches; l++)
-        for (int32_t i = tid; i < s.launch[l].slots; i += kPlanThreads) s.launch[l].map[i] = -1;
     __syncthreads();
 
     // ---- what a group has in common: a wavefront a group -------------------------------------------------------------------
-    for (int64_t g = wave; g < groups; g += kPlanWaves) {
+#pragma unroll 1
+    for (int64_t g = wave; g < groups; g += W) {
         // (numbers that are no cumulative counts stay within the tensors)
-        int32_t e0 = s.groups[g], e1 = s.groups[g + 1];
+        int32_t e0 = group_0, e1 = group_1;
+        const int32_t said = group_shared;
+        if (g + W < groups) group_0 = s.groups[g + W], group_1 = s.groups[g + W + 1], group_shared = s.shared[g + W];
         e0 = e0 < 0 ? 0 : e0 > sequences ? sequences : e0;
         e1 = e1 < e0 ? e0 : e1 > sequences ? sequences : e1;
         // sequences without new tokens have no say
-        int32_t least = 0x7FFFFFFF, row = 0x7FFFFFFF, q0 = 0x7FFFFFFF, q1 = 0, count = 0;
+        int32_t least = 0x7FFFFFFF, row = 0x7FFFFFFF, q0 = 0x7FFFFFFF, q1 = 0, row_again = 0x7FFFFFFF;
+#pragma unroll 1
         for (int64_t i = (int64_t)e0 + lane; i < e1; i += 64) {
-            const AttentionEntry e = s.entries[groups + i];
+            const AttentionEntry e = entries[groups + i];
             if (e.lq == 0) continue;
             least = min(least, e.lk - e.lq);
+            row_again = min(row_again, max(row, (int32_t)i));
             row = min(row, (int32_t)i);
             q0 = min(q0, e.q0);
             q1 = max(q1, e.q0 + e.lq);
-            count++;
         }
+        // (two with queries: one lane has two, or two lanes have one)
+        const bool two = __any(row_again != 0x7FFFFFFF) || __builtin_popcountll(__ballot(row != 0x7FFFFFFF)) > 1;
         least = wave_min(least);
         row = wave_min(row);
         q0 = wave_min(q0);
         q1 = -wave_min(-q1);
-        const int32_t said = s.shared[g];
         int32_t common = said < least ? said : least;
-        common = common < 0 ? 0 : common / kSharedUnit * kSharedUnit;
-        if (wave_total((uint32_t)count) < 2) common = 0;
-        if (lane == 0) s.entries[g] = {q0, common ? q1 - q0 : 0, 0, common, row, 1, -1, 0};
+        common = common < 0 || !two ? 0 : common / kSharedUnit * kSharedUnit;
+        if (lane == 0) entries[g] = {q0, common ? q1 - q0 : 0, 0, common, row, 1, -1, 0};
         if (common)
+#pragma unroll 1
             for (int64_t i = (int64_t)e0 + lane; i < e1; i += 64) {
-                s.entries[groups + i].k0 = common;
-                s.group_of[i] = (int32_t)g;
+                entries[groups + i].k0 = common;
+                entries[groups + i].row = (int32_t)g;
             }
     }
-    if (s.sequence_of)
-        for (int64_t i = wave; i < sequences; i += kPlanWaves) {
-            const AttentionEntry e = s.entries[groups + i];
-            for (int32_t j = lane; j < e.lq; j += 64) s.sequence_of[e.q0 + j] = (int32_t)i;
-        }
     __syncthreads();
 
-    // ---- all work of each launch, and how many key tiles of it a workgroup takes ---------------------------------------------
-    uint64_t sum[2 * kSharedLaunches] = {};
-    for (int64_t v = tid; v < all; v += kPlanThreads) {
-        uint32_t rt, kt;
-        const int mine = entry_tiles(s, s.entries[v], v < groups, rt, kt);
-#pragma unroll
-        for (int l = 0; l < kSharedLaunches; l++)
-            if (l == mine) sum[2 * l] += (uint64_t)rt * kt, sum[2 * l + 1] += rt;
+    // f(entry, its launch and tiles) for this thread's entries, then the wavefront's sums of what f returns, by launch
+    AttentionEntry e = {};
+    Entry x = {-1, 0, 0};
+    if (ONE && tid < all) {
+        e = entries[tid];
+        x = entry_of(launch, e, a.group, tid < groups);
     }
+    // ---- all work of each launch, and how many key tiles of it a workgroup takes ---------------------------------------------
+    {
+        float work[kSharedLaunches] = {};
+        uint32_t tiles[kSharedLaunches] = {};
+        auto add = [&](const Entry& y) {
 #pragma unroll
-    for (int x = 0; x < 2 * kSharedLaunches; x++) {
-        const uint64_t t = wave_sum64(sum[x]);
-        if (lane == 0) sums[wave][x] = t;
+            for (int l = 0; l < kSharedLaunches; l++)
+                if (l == y.launch) work[l] += (float)y.row_tiles * (float)y.key_tiles, tiles[l] += y.row_tiles;
+        };
+        if constexpr (ONE) add(x);
+        else
+            for (int64_t v = tid; v < all; v += T) add(entry_of(launch, entries[v], a.group, v < groups));
+#pragma unroll 1
+        for (int l = 0; l < kSharedLaunches; l++) {
+            const uint32_t n = l == 0 ? tiles[0] : l == 1 ? tiles[1] : tiles[2];
+            const float w = l == 0 ? work[0] : l == 1 ? work[1] : work[2];
+            const uint32_t count = wave_total(n);
+            const float sum = wave_total(w);
+            if (lane == 0) work_of[wave][l] = sum, tiles_of[wave][l] = count;
+        }
     }
     __syncthreads();
-    uint32_t chunk[kSharedLaunches];
+    // (lane l has launch l's) key tiles that fill all workgroups, and those with which n splits of whole numbers of tiles, which are at most one
+    // more than their fraction for each row tile, do in any case
+    float fill = kNever, safe = kNever;
+    if (lane < kSharedLaunches) {
+        float sum = 0.f, count = 0.f;
 #pragma unroll
-    for (int l = 0; l < kSharedLaunches; l++) {
-        uint64_t work = 0, tiles = 0;
+        for (int w = 0; w < W; w++) sum += work_of[w][lane], count += (float)tiles_of[w][lane];
+        const float want = (float)launch[lane].want, least = (float)launch[lane].least;
+        const float all_work = sum * (float)a.kv_heads, left = want - count * (float)a.kv_heads;
+        if (want > 0.f) fill = fmaxf(all_work * __builtin_amdgcn_rcpf(want), least);
+        if (left > 0.f) safe = fmaxf(all_work * __builtin_amdgcn_rcpf(left) * 1.0001f, least);
+    }
+    uint32_t counts[kSharedLaunches][kTries] = {};
+    auto add_tries = [&](const Entry& y) {
+        const float base = __shfl(fill, y.launch < 0 ? 0 : y.launch);
 #pragma unroll
-        for (int w = 0; w < kPlanWaves; w++) work += sums[w][2 * l], tiles += sums[w][2 * l + 1];
-        // the last split of a row tile is half as long as the others on average: so many workgroups less
-        const SharedLaunch& x = s.launch[l];
-        const uint64_t cut = tiles * a.kv_heads / 2, most = x.want;
-        const uint64_t target = cut < most / 2 ? most - cut : most / 2 > 0 ? most / 2 : 1;
-        const double exact = (double)(work * a.kv_heads) / (double)target;
-        chunk[l] = !x.split || exact >= 2147483646.0 ? 0x7FFFFFFFu : (uint32_t)exact + 1;
-        if (chunk[l] < (uint32_t)x.least) chunk[l] = x.least;
+        for (int i = 0; i < kTries; i++) {
+            const uint32_t n = y.row_tiles * (uint32_t)__builtin_ceilf((float)y.key_tiles * __builtin_amdgcn_rcpf(choice(base, i)) * 0.99999f);
+#pragma unroll
+            for (int l = 0; l < kSharedLaunches; l++)
+                if (l == y.launch) counts[l][i] += n;
+        }
+    };
+    if constexpr (ONE) add_tries(x);
+    else
+        for (int64_t base = 0; base < all; base += T) {
+            const int64_t v = base + tid;
+            add_tries(v < all ? entry_of(launch, entries[v], a.group, v < groups) : Entry{-1, 0, 0});
+        }
+#pragma unroll 1
+    for (int l = 0; l < kSharedLaunches; l++)
+#pragma unroll
+        for (int i = 0; i < kTries; i++) {
+            const uint32_t n = wave_total(l == 0 ? counts[0][i] : l == 1 ? counts[1][i] : counts[2][i]);
+            if (lane == 0) tried[wave][l][i] = n;
+        }
+    __syncthreads();
+    // (a lane for each launch and choice)
+    uint64_t hits;
+    {
+        const int l = lane / kTries, i = lane % kTries;
+        const bool listed = l < kSharedLaunches;
+        uint64_t n = 0;
+#pragma unroll
+        for (int w = 0; w < W; w++) n += listed ? tried[w][l][i] : 0;
+        hits = __ballot(listed && n * (uint32_t)a.kv_heads <= (uint64_t)(listed ? launch[l].want : 0));
     }
 
     // ---- which workgroups take an entry ------------------------------------------------------------------------------------
     uint32_t before[kSharedLaunches] = {};
-    for (int64_t base = 0; base < all; base += kPlanThreads) {
+#pragma unroll 1
+    for (int64_t base = 0; base < all; base += T) {
         const int64_t v = base + tid;
-        uint32_t rt = 0, kt = 0, splits = 1, up[kSharedLaunches] = {};
-        int mine = -1;
-        AttentionEntry e = {};
+        if (base) __syncthreads();                               // (the counts of the turn before are read)
+        if constexpr (!ONE) {
+            x = {-1, 0, 0};
+            if (v < all) {
+                e = entries[v];
+                x = entry_of(launch, e, a.group, v < groups);
+            }
+        }
+        const int mine = x.launch < 0 ? 0 : x.launch;
+        const uint32_t hit = (uint32_t)(hits >> (kTries * mine)) & ((1u << kTries) - 1);
+        const float by_choice = choice(__shfl(fill, mine), __builtin_ctz(hit | 1u << kTries)), in_any_case = __builtin_ceilf(__shfl(safe, mine));
+        const float c = hit ? by_choice : in_any_case;
+        const uint32_t chunk = c < kNever ? (uint32_t)c : 0x7FFFFFFFu;
+        const uint32_t splits = x.key_tiles > chunk ? (x.key_tiles + chunk - 1) / chunk : 1;
+        const uint32_t slots = x.row_tiles * splits;             // (no launch: none)
+        uint32_t up = 0;
+#pragma unroll 1
+        for (int l = 0; l < kSharedLaunches; l++) {
+            const uint32_t sum = wave_scan(l == x.launch ? slots : 0);
+            if (l == x.launch) up = sum;
+            if (lane == 63) ups[wave][l] = sum;
+        }
+        __syncthreads();
+        uint32_t in_front = mine == 0 ? before[0] : mine == 1 ? before[1] : before[2];
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            if (w < wave) in_front += ups[w][mine];
+#pragma unroll
+            for (int l = 0; l < kSharedLaunches; l++) before[l] += ups[w][l];
+        }
+        int32_t count = 0, first = -1;
         if (v < all) {
-            e = s.entries[v];
-            mine = entry_tiles(s, e, v < groups, rt, kt);
-        }
-#pragma unroll
-        for (int l = 0; l < kSharedLaunches; l++) {
-            if (l == mine) {
-                splits = (kt + chunk[l] - 1) / chunk[l];
-                if (splits < 1) splits = 1;
-            }
-            up[l] = wave_scan(l == mine ? rt * splits : 0);
-            if (lane == 63) ups[wave][l] = up[l];
-        }
-        __syncthreads();
-        int32_t first = -1, count = 0;
-#pragma unroll
-        for (int l = 0; l < kSharedLaunches; l++) {
-            uint32_t in_front = before[l];
-            for (int w = 0; w < kPlanWaves; w++) {
-                if (w < wave) in_front += ups[w][l];
-                before[l] += ups[w][l];
-            }
-            if (l == mine) {
-                count = (int32_t)(rt * splits);
-                first = (int32_t)(in_front + up[l]) - count;
-                // (lengths that are none can need more workgroups than there are)
-                if (first < 0 || (int64_t)first + count > s.launch[l].slots) first = -1, count = 0;
-            }
-        }
-        if (mine >= 0) {
             const bool common = v < groups;
+            const int32_t room = launch[mine].slots;
+            count = (int32_t)slots;
+            first = (int32_t)(in_front + up) - count;
             e.splits = (int32_t)splits;
-            e.first = first;
-            e.flags = mine << 8 | (common ? kEntryPartial | (rt == 1 ? kEntryOnce : 0)
-                                          : kEntryCausal | kEntryOnce | (splits > 1 || s.group_of[v - groups] >= 0 ? kEntryPartial : 0));
+            e.flags = x.launch < 0 ? 0
+                                   : mine << 8 | (common ? kEntryPartial | (x.row_tiles == 1 ? kEntryOnce : 0)
+                                                         : kEntryCausal | kEntryOnce | (splits > 1 || e.row >= 0 ? kEntryPartial : 0));
+            // (lengths that are none can need more workgroups than there are: the join passes over them)
+            e.first = x.launch < 0 || first < 0 || (int64_t)first + count > room ? -1 : first;
             s.entries[v] = e;
+            e.first = first;
+            if (!common) e.row = (int32_t)(v - groups);
+            if (first < 0 || first >= room) count = 0;
+            else if ((int64_t)first + count > room) count = room - first;
+            if (count <= kOwn) {
+                AttentionEntry* map = launch[mine].map + first;
+#pragma unroll 1
+                for (int32_t k = 0; k < count; k++) map[k] = e;
+            }
         }
-        firsts[tid] = first;
-        counts[tid] = mine < 0 ? 0 : count << 2 | mine;
-        __syncthreads();
-        for (int i = wave; i < kPlanThreads && base + i < all; i += kPlanWaves) {
-            const int32_t n = counts[i] >> 2, f = firsts[i];
-            int32_t* map = s.launch[0].map;
-            if ((counts[i] & 3) == 1) map = s.launch[1].map;
-            if ((counts[i] & 3) == 2) map = s.launch[2].map;
-            for (int32_t j = lane; j < n; j += 64) map[f + j] = (int32_t)(base + i);
+#pragma unroll 1
+        for (uint64_t many = __ballot(count > kOwn); many; many &= many - 1) {
+            const int m = __builtin_ctzll(many), l = __builtin_amdgcn_readlane(mine, m), n = __builtin_amdgcn_readlane(count, m);
+            const int32_t f = __builtin_amdgcn_readlane(first, m);
+            const AttentionEntry y = {__builtin_amdgcn_readlane(e.q0, m),  __builtin_amdgcn_readlane(e.lq, m),     __builtin_amdgcn_readlane(e.k0, m),    __builtin_amdgcn_readlane(e.lk, m),
+                                      __builtin_amdgcn_readlane(e.row, m), __builtin_amdgcn_readlane(e.splits, m), __builtin_amdgcn_readlane(e.first, m), __builtin_amdgcn_readlane(e.flags, m)};
+            AttentionEntry* map = launch[l].map + f;
+#pragma unroll 1
+            for (int32_t k = lane; k < n; k += 64) map[k] = y;
         }
-        __syncthreads();
+    }
+    // workgroups beyond the last: entries without queries
+#pragma unroll 1
+    for (int l = 0; l < kSharedLaunches; l++) {
+        const int32_t room = launch[l].slots;
+        AttentionEntry* map = launch[l].map;
+#pragma unroll 1
+        for (int64_t i = (int64_t)(l == 0 ? before[0] : l == 1 ? before[1] : before[2]) + tid; i < room; i += T) map[i].lq = 0;
     }
 }
 
@@ -206,6 +317,7 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedA
     constexpr int PER = DT / 32;             // elements of a lane
     constexpr int CHUNK = 4;                 // partial results that a team asks for at once
     __shared__ float room[TEAMS > 2 ? TEAMS : 1][DT + 2];
+    touch_arguments(s);
     const AttentionArgs& a = s.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, e = PER * (lane & 31);
     const int team = TEAMS > 2 ? (threadIdx.x >> 5) : half;
@@ -215,12 +327,11 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedA
     const int32_t seq = s.sequence_of ? s.sequence_of[token] : (int32_t)token;
     if (seq < 0 || seq >= a.sequences) return;
     const AttentionEntry own = s.entries[s.group_count + seq];
-    const int32_t g = s.group_of[seq];
-    if (!(own.flags & kEntryPartial)) return;
+    if (!(own.flags & kEntryPartial) || token - (uint32_t)own.q0 >= (uint32_t)own.lq) return;
     const uint32_t kv = head / (uint32_t)a.group, place = head - kv * (uint32_t)a.group;
     AttentionEntry common = {};
     common.first = -1;
-    if (g >= 0) common = s.entries[g];
+    if (own.row >= 0) common = s.entries[own.row];
 
     // this query's row of an entry: its partial results are `step` apart
     struct Part {
@@ -232,12 +343,12 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedA
         if (x.first < 0) return {nullptr, nullptr, 0, 0};
         const int l = x.flags >> 8;
         const SharedLaunch& y = l == 0 ? s.launch[0] : l == 1 ? s.launch[1] : s.launch[2];
-        const uint32_t row = (token - (uint32_t)x.q0) * (uint32_t)a.group + place, tile = row / (uint32_t)y.rows;
-        const uint32_t tiles = ((uint32_t)x.lq * (uint32_t)a.group + (uint32_t)y.rows - 1) / (uint32_t)y.rows;
+        const uint32_t row = (token - (uint32_t)x.q0) * (uint32_t)a.group + place, tile = row >> y.row_shift;
+        const uint32_t tiles = ((uint32_t)x.lq * (uint32_t)a.group + (1u << y.row_shift) - 1) >> y.row_shift;
         // (the last row tile comes first)
         const int64_t slot = ((int64_t)x.first + (int64_t)(tiles - 1 - tile) * x.splits) * a.kv_heads + kv;
-        const int64_t at = slot * y.rows + (row - tile * (uint32_t)y.rows);
-        return {y.partial + at * DT, y.partial + (int64_t)y.slots * a.kv_heads * y.rows * DT + at * 2, x.splits, (int64_t)a.kv_heads * y.rows};
+        const int64_t at = (slot << y.row_shift) + (row - (tile << y.row_shift));
+        return {y.partial + at * DT, y.partial + (((int64_t)y.slots * a.kv_heads) << y.row_shift) * DT + at * 2, x.splits, (int64_t)a.kv_heads << y.row_shift};
     };
     const Part c = part_of(common), w = part_of(own);
     const int32_t parts = c.splits + w.splits;
@@ -327,7 +438,9 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedA
 }
 
 int launch_shared_plan(const SharedArgs& s, hipStream_t stream) {
-    attention_shared_plan_kernel<<<1, kPlanThreads, 0, stream>>>(s);
+    const int64_t entries = (int64_t)s.group_count + s.a.sequences;
+    if (entries <= 256) attention_shared_plan_kernel<4, true><<<1, 256, 0, stream>>>(s);
+    else attention_shared_plan_kernel<16, false><<<1, 1024, 0, stream>>>(s);
     return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;
 }
 

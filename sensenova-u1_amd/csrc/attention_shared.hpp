@@ -9,12 +9,11 @@ constexpr int kSharedUnit = 128;     // common keys are taken in multiples of ev
 
 // One of the launches that compute partial results: the common keys', the single tokens', the chunks'
 struct SharedLaunch {
-    int32_t rows, keys;              // of a tile
-    int32_t min_rows, max_rows;      // of the sequences that it takes
-    int32_t want, least;             // workgroups aimed at where keys are split; key tiles of a split at least
-    int32_t split;
+    int32_t row_shift, key_shift;    // 2^row_shift rows and 2^key_shift keys of a tile
+    int32_t max_rows;                // of the sequences that the second takes; the third takes the others
+    int32_t want, least;             // workgroups that run at once (0: keys are not split); key tiles of a split at least
     int32_t slots;                   // workgroups of a key / value head
-    int32_t* map;                    // [slots]
+    AttentionEntry* map;             // [slots]: what each does
     float* partial;
 };
 constexpr int kSharedLaunches = 3;
@@ -25,7 +24,6 @@ struct SharedArgs {
     const int32_t* shared;           // [group_count]
     int32_t group_count;
     AttentionEntry* entries;         // [groups, then sequences]
-    int32_t* group_of;               // [sequences]: group with common keys, or -1
     int32_t* sequence_of;            // [tokens_q], or NULL: token t is sequence t
     SharedLaunch launch[kSharedLaunches];
 };

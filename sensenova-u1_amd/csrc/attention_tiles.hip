@@ -113,8 +113,9 @@ template <int DT> struct Tile {
 
 }  // namespace
 
-// W: wavefronts, of 32 rows each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.
-template <int DT, int SOURCE, int W, int NS>
+// W: wavefronts, of 32 rows each.  NS: LDS stages; stage i holds the keys of tile i and the values of tile i - 1.  PLANNED: a kernel in
+// front of this one dealt the work.
+template <int DT, int SOURCE, int W, int NS, bool PLANNED>
 __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a) {
     constexpr bool Q8 = SOURCE == kPagedQ8;
     typedef typename Operand<Q8>::T op_t;
@@ -128,7 +129,9 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
     constexpr float kUp = Q8 ? 12.f : 0.f;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // [stage][keys, values]
 
-    const AttentionBlock b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
+    AttentionBlock b;
+    if constexpr (PLANNED) b = attention_planned_block<ROWS>(a, blockIdx.x);
+    else b = attention_block<ROWS, kKeys, false>(a, blockIdx.x);
     if (!b.there) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
@@ -613,17 +616,19 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
 
 // dim: of the kernel, 64, 96, 128, 192 or 256; rows: of a workgroup, 128 or (up to 192 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
-#define SNGGUF_GO(D, S, W, N)                                                                                           \
-    if (dim == D && source == S && rows == 32 * W) {                                                                    \
+    const bool planned = a.map != nullptr;
+#define SNGGUF_GO(D, S, W, N, P)                                                                                         \
+    if (dim == D && source == S && rows == 32 * W && planned == P) {                                                                    \
         constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                   \
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, N>), \
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, N, P>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_tiles_kernel<D, S, W, N><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                        \
+        attention_tiles_kernel<D, S, W, N, P><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                        \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
     // (three stages where a compute unit has room for them; 8-bit tiles pass through registers and need two)
-#define SNGGUF_GO_DIM(D, W, N) SNGGUF_GO(D, kPacked, W, N) SNGGUF_GO(D, kPaged, W, N) SNGGUF_GO(D, kPagedQ8, W, 2)
+#define SNGGUF_GO_PAGED(D, W, N, P) SNGGUF_GO(D, kPaged, W, N, P) SNGGUF_GO(D, kPagedQ8, W, 2, P)
+#define SNGGUF_GO_DIM(D, W, N) SNGGUF_GO(D, kPacked, W, N, false) SNGGUF_GO_PAGED(D, W, N, false) SNGGUF_GO_PAGED(D, W, N, true)
     SNGGUF_GO_DIM(64, 4, 3)
     SNGGUF_GO_DIM(64, 8, 3)
     SNGGUF_GO_DIM(96, 4, 2)
@@ -634,6 +639,7 @@ int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source
     SNGGUF_GO_DIM(192, 8, 2)
     SNGGUF_GO_DIM(256, 4, 2)
 #undef SNGGUF_GO_DIM
+#undef SNGGUF_GO_PAGED
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
 }

@@ -8,11 +8,12 @@
 // bits and reduced to the nearest whole turn there; everything else is fp32, rounded to bf16 once (norm, weight and rotation
 // by themselves would round three times, and be off by 1.7 times as much).
 //
-// Bound by memory: an element is two bytes in and two out, for some ten operations.  2^lane_shift neighbouring lanes have a head,
-// 16 bytes each: its sums of squares are added up across them in the vector unit, and a lane gets its pairs' other elements from
-// the lane that has them (parts that are no multiple of 16 elements: from memory, where they were just read).  All of a head is
-// read before any of it is written, so a call may work in place.  A workgroup's lanes keep to the same elements of
-// all heads, so weights, cosines and sines are fetched once for a token.
+// Bound by memory: an element is two bytes in and two out, for some ten operations.  Neighbouring lanes have a head between them, its
+// sums of squares are added up across them in the vector unit, and all of it is read before any of it is written, so a call may work
+// in place.  A lane keeps to the same elements of all heads, so weights, cosines and sines are fetched once for a token.
+//  * head_pairs_kernel, pairs half a part apart in parts of multiples of 16 elements: a lane has eight pairs, both of their elements.
+//  * head_rotary_kernel, neighbouring pairs, any parts or rows: a lane has eight elements; those that they are turned with, where they are not among
+//    the eight, are read beside them.  Shapes for which the other is no form, so it is kept simple.
 #include "head_rotary.hpp"
 #include "rotary_cache_device.hpp"
 
@@ -21,9 +22,10 @@ namespace sngguf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;                                // heads of a lane that are asked for at once
+constexpr int kAhead = 2;                                // heads of a lane that head_rotary_kernel asks for at once
 
-enum { kHalves = 0, kNeighbours = 1, kAnyHalves = 2 };   // parts of multiples of 16 elements; pairs next to each other; any parts
+enum { kNeighbours = 0, kAnyHalves = 1 };
+enum { kNormNone = 0, kNormHalf = 1, kNormWide = 2 };     // weights: none, bf16, fp32
 
 template <int CONTROL>
 __device__ __forceinline__ float dpp(float x) {
@@ -41,7 +43,14 @@ __device__ __forceinline__ float lanes_sum(float x, int shift) {
     return x;
 }
 
-__device__ __forceinline__ float rstd_of(float sum, int elements, float eps) { return 1.0f / sqrtf(sum / (float)elements + eps); }
+// 1 / sqrt of the mean of squares: the instruction is off by a step at most; numbers below the smallest normal one, which it takes for zero, are
+// scaled into its range
+__device__ __forceinline__ float rstd_of(float sum, float one_over, float eps) {
+    const float mean = __builtin_fmaf(sum, one_over, eps);
+    const bool tiny = mean < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p64f : mean);
+    return tiny ? r * 0x1p32f : r;
+}
 
 // Part of the norm that element e belongs to, and where it starts
 __device__ __forceinline__ int norm_part(const HeadNormArgs& n, int e, int& start) {
@@ -53,12 +62,27 @@ __device__ __forceinline__ int norm_part(const HeadNormArgs& n, int e, int& star
     return p;
 }
 __device__ __forceinline__ const void* norm_weight(const HeadNormArgs& n, int p) { return p == 0 ? n.weight[0] : p == 1 ? n.weight[1] : p == 2 ? n.weight[2] : n.weight[3]; }
-__device__ __forceinline__ int norm_elements(const HeadNormArgs& n, int p) { return p == 0 ? n.elements[0] : p == 1 ? n.elements[1] : p == 2 ? n.elements[2] : n.elements[3]; }
+__device__ __forceinline__ float norm_one_over(const HeadNormArgs& n, int p) { return p == 0 ? n.one_over[0] : p == 1 ? n.one_over[1] : p == 2 ? n.one_over[2] : n.one_over[3]; }
+
+// Position of a token that turns a pair.  Up to four axes: all of the token's positions are asked for beside the pair's axis.
+__device__ __forceinline__ int64_t position_of(const HeadRotaryArgs& a, int pair, int64_t token) {
+    const int64_t* at = a.positions + token;
+    if (!a.axis || a.axes == 1) return at[0];
+    int axis = a.axis[pair];
+    if (a.axes <= 4) {
+        int64_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = at[(i < a.axes ? i : a.axes - 1) * a.axis_stride];
+        return axis <= 0 ? p[0] : axis == 1 ? p[1] : axis == 2 ? p[2] : p[3];
+    }
+    axis = axis < 0 ? 0 : axis >= a.axes ? a.axes - 1 : axis;
+    return at[axis * a.axis_stride];
+}
 
 // What a lane keeps of a norm: weights of its eight elements and of their pairs' others, and the parts that they belong to
 struct LaneNorm {
     float g[8], gz[8];
-    int part, elements;
+    int part;
     uint32_t z_parts;                                    // four bits each
 };
 
@@ -110,27 +134,9 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
     load_k(0);
 
     // ---- which pairs this lane's elements belong to ----------------------------------------------------------------------
-    // kHalves: pairs from `pair` on, the others in the lane `away` further; kAnyHalves: each element by itself
-    int pair = 0, away = 0;
-    bool second = false, rotates = there && e < turned;
     int z_at[8], pairs_of[8];
     uint32_t seconds = 0, rotated = 0;
-    if constexpr (LAYOUT == kHalves) {
-        int start = 0, first = 0;
-#pragma unroll
-        for (int p = 0; p < kMostParts; p++) {
-            const int n = p < a.parts ? a.part[p] : 0;
-            if (e >= start && e < start + n) {
-                second = e - start >= n / 2;
-                pair = first + (second ? e - start - n / 2 : e - start);
-                away = second ? -(n / 16) : n / 16;
-            }
-            start += n;
-            first += n / 2;
-        }
-    } else if constexpr (LAYOUT == kNeighbours) {
-        pair = e >> 1;
-    } else {
+    if constexpr (LAYOUT == kAnyHalves) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             int start = 0, first = 0;
@@ -151,14 +157,12 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
             }
         }
     }
-    const int z_lane = (tid & 63) + away;                // (a part lies in one head, and a head in one wavefront)
 
     // ---- weights -------------------------------------------------------------------------------------------------------
     auto weights = [&](const HeadNormArgs& n) -> LaneNorm {
         LaneNorm w;
         int start;
         w.part = norm_part(n, there ? e : 0, start);
-        w.elements = norm_elements(n, w.part);
         w.z_parts = 0;
         const void* at = norm_weight(n, w.part);
         const int off = (there ? e : 0) - start;
@@ -177,11 +181,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
                 for (int y = 0; y < 4; y++) w.g[j + y] = v[y];
             }
         }
-        if constexpr (LAYOUT == kHalves) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) w.gz[j] = __shfl(w.g[j], z_lane);
-            w.z_parts = (uint32_t)__shfl(w.part, z_lane);
-        } else if constexpr (LAYOUT == kNeighbours) {
+        if constexpr (LAYOUT == kNeighbours) {
 #pragma unroll
             for (int j = 0; j < 8; j++) w.gz[j] = w.g[j ^ 1];
             w.z_parts = (uint32_t)w.part;
@@ -206,9 +206,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
     // ---- angles ----------------------------------------------------------------------------------------------------------
     for (int i = tid; i < count * a.pairs; i += kThreads) {
         const int t = single ? 0 : i / a.pairs, p = i - t * a.pairs;
-        int axis = a.axis ? a.axis[p] : 0;
-        axis = axis < 0 ? 0 : axis >= a.axes ? a.axes - 1 : axis;
-        cs_all[i] = cos_sin(a.turns, p, a.positions[axis * a.axis_stride + t0 + t], a.magnitude);
+        cs_all[i] = cos_sin(a.turns, p, position_of(a, p, t0 + t), a.magnitude);
     }
     __syncthreads();
     float c[8], s[8];                                    // of token `t_of`; an element is y c + z s
@@ -220,10 +218,8 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             c[j] = 1.f, s[j] = -0.f;                     // (not turned: x + -0 is x, also where x is a zero of either sign)
-            if constexpr (LAYOUT == kHalves) {
-                if (rotates) c[j] = cs[pair + j].x, s[j] = second ? cs[pair + j].y : -cs[pair + j].y;
-            } else if constexpr (LAYOUT == kNeighbours) {
-                if (there && e + j < turned) c[j] = cs[pair + j / 2].x, s[j] = (j & 1) ? cs[pair + j / 2].y : -cs[pair + j / 2].y;
+            if constexpr (LAYOUT == kNeighbours) {
+                if (there && e + j < turned) c[j] = cs[(e + j) >> 1].x, s[j] = (j & 1) ? cs[(e + j) >> 1].y : -cs[(e + j) >> 1].y;
             } else {
                 if (rotated >> j & 1) c[j] = cs[pairs_of[j]].x, s[j] = (seconds >> j & 1) ? cs[pairs_of[j]].y : -cs[pairs_of[j]].y;
             }
@@ -234,16 +230,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
     auto turned8 = [&](u32x4_t raw, const bf16_t* row, const HeadNormArgs& n, const LaneNorm& w) -> u32x4_t {
         float x[8], z[8];
         unpack8(raw, x);
-        if constexpr (LAYOUT == kHalves) {
-            u32x4_t other;
-#pragma unroll
-            for (int i = 0; i < 4; i++) other[i] = (uint32_t)__shfl((int)raw[i], z_lane);
-            unpack8(other, z);
-            if (!rotates) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) z[j] = 0.f;
-            }
-        } else if constexpr (LAYOUT == kNeighbours) {
+        if constexpr (LAYOUT == kNeighbours) {
 #pragma unroll
             for (int j = 0; j < 8; j++) z[j] = there && e + j < turned ? x[j ^ 1] : 0.f;
         } else {
@@ -256,32 +243,21 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
 #pragma unroll
                 for (int j = 0; j < 8; j++) ss += x[j] * x[j];
                 float r = 0.f, rz[LAYOUT == kAnyHalves ? 8 : 1] = {};
-                if (LAYOUT != kAnyHalves && n.group) {
-                    r = rstd_of(lanes_sum(ss, __builtin_ctz(n.group)), w.elements, n.eps);
-                    if (n.parts == 1 || LAYOUT == kNeighbours) rz[0] = r;
-                    else rz[0] = __shfl(r, z_lane);
-                } else {
-                    for (int p = 0; p < n.parts; p++) {
-                        const float rp = rstd_of(lanes_sum(there && w.part == p ? ss : 0.f, a.lane_shift), norm_elements(n, p), n.eps);
-                        if (w.part == p) r = rp;
+                for (int p = 0; p < n.parts; p++) {
+                    const float rp = rstd_of(lanes_sum(there && w.part == p ? ss : 0.f, a.lane_shift), norm_one_over(n, p), n.eps);
+                    if (w.part == p) r = rp;
 #pragma unroll
-                        for (int j = 0; j < (LAYOUT == kAnyHalves ? 8 : 1); j++)
-                            if ((w.z_parts >> (4 * j) & 15u) == (uint32_t)p) rz[j] = rp;
-                    }
+                    for (int j = 0; j < (LAYOUT == kAnyHalves ? 8 : 1); j++)
+                        if ((w.z_parts >> (4 * j) & 15u) == (uint32_t)p) rz[j] = rp;
                 }
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     x[j] = x[j] * r * w.g[j];
                     z[j] = z[j] * rz[LAYOUT == kAnyHalves ? j : 0] * w.gz[j];
                 }
-                if (LAYOUT == kHalves && !rotates) {     // (weights that are not finite)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) z[j] = 0.f;
-                } else if (LAYOUT != kHalves) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (LAYOUT == kNeighbours ? e + j >= turned : !(rotated >> j & 1)) z[j] = 0.f;
-                }
+                for (int j = 0; j < 8; j++)              // (weights that are not finite)
+                    if (LAYOUT == kNeighbours ? e + j >= turned : !(rotated >> j & 1)) z[j] = 0.f;
             }
         }
         float y[8];
@@ -323,29 +299,257 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
     }
 }
 
+// Eight pairs a lane: pieces a and b of eight elements each, (a_j, b_j) the pairs; elements behind the turned ones as pairs that are not turned.
+// Rows start at 16-byte boundaries.
+__device__ __forceinline__ u32x4_t piece_at(const bf16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+
+template <bool CACHE, int NORM>
+__global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float2 cs_all[];    // [token][pair], then (CACHE) [team][dim] bf16
+    touch_arguments(a);
+    const int tid = threadIdx.x, lanes = 1 << a.lane_shift, teams = kThreads >> a.lane_shift;
+    const int team = tid >> a.lane_shift, unit = tid & (lanes - 1);
+    const bool there = 16 * unit < a.dim;
+    const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_block;
+    const int count = (int)(a.tokens - t0 < a.tokens_per_block ? a.tokens - t0 : a.tokens_per_block);
+    const int turned = 2 * a.pairs;
+
+    // ---- this lane's pieces --------------------------------------------------------------------------------------------------
+    int ea, eb, pair = 0;
+    const bool rotates = there && 8 * unit < a.pairs;
+    ea = there ? turned + 16 * (unit - (a.pairs >> 3)) : 0;
+    eb = ea + 8;
+    {
+        int start = 0, first = 0;
+#pragma unroll
+        for (int p = 0; p < kMostParts; p++) {
+            const int n = p < a.parts ? a.part[p] : 0, at = 8 * unit - first;
+            if (rotates && at >= 0 && at < n / 2) {
+                ea = start + at;
+                eb = ea + n / 2;
+                pair = 8 * unit;
+            }
+            start += n;
+            first += n / 2;
+        }
+    }
+
+    // ---- items: (token, head) pairs dealt over the teams, a lane's next kAhead on their way -----------------------------------
+    struct Item {
+        int t, h;
+    };
+    auto first_item = [&](int heads) -> Item {
+        const int t = (int)((uint32_t)team / (uint32_t)heads);
+        return {t, team - t * heads};
+    };
+    const int others = CACHE ? 2 * a.kv_heads : a.k_heads;
+    const int q_hop = teams / a.q_heads, q_rest = teams - q_hop * a.q_heads, k_hop = others ? teams / others : 0, k_rest = teams - k_hop * others;
+    auto next_item = [](const Item& x, int hop, int rest, int heads) -> Item {
+        const int h = x.h + rest;
+        return h >= heads ? Item{x.t + hop + 1, h - heads} : Item{x.t + hop, h};
+    };
+    struct Words {
+        u32x4_t a, b;
+    };
+    const int q_items = count * a.q_heads, k_items = count * others;
+    auto load_q = [&](const Item& x) -> Words {
+        Words w = {u32x4_t{0u, 0u, 0u, 0u}, u32x4_t{0u, 0u, 0u, 0u}};
+        if (x.t < count && there) {
+            const bf16_t* p = a.q + (t0 + x.t) * a.q_token + x.h * a.q_head;
+            w = {piece_at(p + ea), piece_at(p + eb)};
+        }
+        return w;
+    };
+    // values go to the cache as they are: pieces `unit` and `unit` + lanes
+    auto load_k = [&](const Item& x, int64_t& slot) -> Words {
+        Words w = {u32x4_t{0u, 0u, 0u, 0u}, u32x4_t{0u, 0u, 0u, 0u}};
+        slot = -1;
+        if (x.t >= count) return w;
+        if (CACHE) slot = a.slots[t0 + x.t];
+        if (CACHE && x.h >= a.kv_heads) {
+            const bf16_t* p = a.v + (t0 + x.t) * a.v_token + (x.h - a.kv_heads) * a.v_head;
+            if (8 * unit < a.dim) w.a = piece_at(p + 8 * unit);
+            if (8 * (unit + lanes) < a.dim) w.b = piece_at(p + 8 * (unit + lanes));
+        } else if (there) {
+            const bf16_t* p = a.k + (t0 + x.t) * a.k_token + x.h * a.k_head;
+            w = {piece_at(p + ea), piece_at(p + eb)};
+        }
+        return w;
+    };
+    Item x = first_item(a.q_heads), y = others ? first_item(others) : Item{count, 0};
+    int64_t slot;
+    Words q_raw = load_q(x), k_raw = load_k(y, slot);
+
+    // ---- weights: asked for here, used behind the angles -----------------------------------------------------------------------
+    struct Weights {
+        u32x4_t word[NORM == kNormWide ? 4 : 2];         // pieces a and b
+        int part_a, part_b;
+    };
+    auto ask_weights = [&](const HeadNormArgs& n) -> Weights {
+        Weights w;
+        int start_a, start_b;
+        w.part_a = norm_part(n, there ? ea : 0, start_a);
+        w.part_b = norm_part(n, there ? eb : 0, start_b);
+        if (NORM == kNormNone || n.parts == 0) return w;
+        const int at_a = (there ? ea : 0) - start_a, at_b = (there ? eb : 0) - start_b;
+        if constexpr (NORM == kNormWide) {
+            const u32x4_t* pa = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, w.part_a)) + at_a);
+            const u32x4_t* pb = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, w.part_b)) + at_b);
+            w.word[0] = pa[0], w.word[1] = pa[1], w.word[2] = pb[0], w.word[3] = pb[1];
+        } else {
+            w.word[0] = piece_at(static_cast<const bf16_t*>(norm_weight(n, w.part_a)) + at_a);
+            w.word[1] = piece_at(static_cast<const bf16_t*>(norm_weight(n, w.part_b)) + at_b);
+        }
+        return w;
+    };
+    auto weight_of = [](const Weights& w, int piece, int j) -> float {
+        if constexpr (NORM == kNormWide) return __builtin_bit_cast(float, (uint32_t)w.word[2 * piece + j / 4][j & 3]);
+        else return (j & 1) ? bf16hi_to_f32(w.word[piece][j / 2]) : bf16lo_to_f32(w.word[piece][j / 2]);
+    };
+    const Weights qw = ask_weights(a.q_norm), kw = ask_weights(a.k_norm);
+
+    // ---- angles ----------------------------------------------------------------------------------------------------------------
+    for (int i = tid; i < count * a.pairs; i += kThreads) {
+        const int t = count == 1 ? 0 : i / a.pairs, p = i - t * a.pairs;
+        cs_all[i] = cos_sin(a.turns, p, position_of(a, p, t0 + t), a.magnitude);
+    }
+    __syncthreads();
+
+    // Both pieces normed and turned (all lanes of a wavefront come here together)
+    auto turn = [&](Words raw, int t, const HeadNormArgs& n, const Weights& w) -> Words {
+        float u[8], v[8];
+        unpack8(raw.a, u);
+        unpack8(raw.b, v);
+        if (NORM && n.parts) {
+            float sa = 0.f, sb = 0.f, ra = 0.f, rb = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) sa = __builtin_fmaf(u[j], u[j], sa), sb = __builtin_fmaf(v[j], v[j], sb);
+#pragma unroll 1
+            for (int p = 0; p < n.parts; p++) {
+                const float mine = (w.part_a == p ? sa : 0.f) + (w.part_b == p ? sb : 0.f);
+                const float r = rstd_of(lanes_sum(mine, a.lane_shift), norm_one_over(n, p), n.eps);
+                if (w.part_a == p) ra = r;
+                if (w.part_b == p) rb = r;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) u[j] = u[j] * ra * weight_of(w, 0, j), v[j] = v[j] * rb * weight_of(w, 1, j);
+            if (!rotates) return {pack8(u), pack8(v)};
+        } else if (!rotates) {
+            return raw;
+        }
+        const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(cs_all + t * a.pairs + pair);
+        float p[8], q[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const f32x4_t w2 = cs[j / 2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float c = w2[2 * i], s = w2[2 * i + 1];
+                if constexpr (NORM) {
+                    p[j + i] = __builtin_fmaf(u[j + i], c, -(v[j + i] * s));
+                    q[j + i] = __builtin_fmaf(v[j + i], c, u[j + i] * s);
+                } else {                                 // (as the rotation by one position has it, to the bit)
+                    p[j + i] = u[j + i] * c - v[j + i] * s;
+                    q[j + i] = v[j + i] * c + u[j + i] * s;
+                }
+            }
+        }
+        return {pack8(p), pack8(q)};
+    };
+
+    for (int i0 = 0; i0 < q_items; i0 += teams) {
+        const Item next = next_item(x, q_hop, q_rest, a.q_heads);
+        const Words ahead = load_q(next);
+        const Words out = turn(q_raw, x.t, a.q_norm, qw);
+        if (x.t < count && there) {
+            bf16_t* p = a.q_out + (t0 + x.t) * a.q_out_token + x.h * a.q_out_head;
+            *reinterpret_cast<u32x4_t*>(p + ea) = out.a;
+            *reinterpret_cast<u32x4_t*>(p + eb) = out.b;
+        }
+        x = next;
+        q_raw = ahead;
+    }
+    bf16_t* room = reinterpret_cast<bf16_t*>(cs_all + a.tokens_per_block * a.pairs) + team * a.dim;
+    for (int i0 = 0; i0 < k_items; i0 += teams) {
+        const Item next = next_item(y, k_hop, k_rest, others);
+        int64_t slot_ahead;
+        const Words ahead = load_k(next, slot_ahead);
+        const bool value = CACHE && y.h >= a.kv_heads;
+        Words out = k_raw;
+        if (!CACHE || __any(!value)) out = turn(k_raw, y.t, a.k_norm, kw);
+        if constexpr (!CACHE) {
+            if (y.t < count && there) {
+                bf16_t* p = a.k_out + (t0 + y.t) * a.k_out_token + y.h * a.k_out_head;
+                *reinterpret_cast<u32x4_t*>(p + ea) = out.a;
+                *reinterpret_cast<u32x4_t*>(p + eb) = out.b;
+            }
+        } else {
+            // through LDS, so that four neighbouring lanes have a run of 32 elements (a head's lanes are one wavefront's)
+            if (there && !value) {
+                *reinterpret_cast<u32x4_t*>(room + ea) = out.a;
+                *reinterpret_cast<u32x4_t*>(room + eb) = out.b;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int h = value ? y.h - a.kv_heads : y.h;
+            // slots outside the cache (padding is marked by negative ones) are passed over; the lanes of a run agree
+            if (slot >= 0 && slot < a.slot_count) {
+                void* pages = value ? a.v_pages : a.k_pages;
+                uint16_t* scales = value ? a.v_scales : a.k_scales;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int e = 8 * (unit + half * lanes);
+                    if (e >= a.dim) continue;
+                    const u32x4_t held = value ? (half ? k_raw.b : k_raw.a) : *reinterpret_cast<const u32x4_t*>(room + e);
+                    if (scales) cache_piece<true>(pages, scales, a, slot, h, e, held);
+                    else cache_piece<false>(pages, scales, a, slot, h, e, held);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();             // (the room is written again)
+        }
+        y = next;
+        k_raw = ahead;
+        slot = slot_ahead;
+    }
+}
+
 int launch_head_rotary(const HeadRotaryArgs& a0, int cache, hipStream_t stream) {
     HeadRotaryArgs a = a0;
-    while ((8 << a.lane_shift) < a.dim) a.lane_shift++;
+    bool pairs = !a.interleaved && a.wide && a.dim % 16 == 0;
+    for (int p = 0; p < a.parts; p++) pairs = pairs && a.part[p] % 16 == 0;
+    if (a.q_norm.parts && a.k_norm.parts && a.q_norm.bf16 != a.k_norm.bf16) pairs = false;       // (weights of two types: the simple one)
+    const int elements = pairs ? 16 : 8;                 // of a lane
+    while ((elements << a.lane_shift) < a.dim) a.lane_shift++;
+    if (pairs && cache && a.lane_shift < 2) a.lane_shift = 2;        // (four lanes for a run of the 8-bit cache)
     const int teams = kThreads >> a.lane_shift;
     const int64_t heads = (int64_t)a.q_heads + (cache ? 2 * a.kv_heads : a.k_heads);
-    a.tokens_per_block = heads >= teams ? 1 : heads * 8 <= teams ? 8 : (int32_t)(teams / heads);
+    // as many tokens as give each team a head; where there are tokens enough for four workgroups a compute unit, up to four times as many, as
+    // finding its elements and weights costs a workgroup as much as two heads do (4096 tokens of 40 normed heads, 1 / 2 / 4 / 8 tokens a workgroup:
+    // 31.5 / 25.0 / 20.3 / 22.4 us)
+    const int64_t fill = heads * 8 <= teams ? 8 : heads < teams ? teams / heads : 1;
+    const int64_t spare = a.tokens / (1024 * fill);
+    const int64_t tokens = fill * (spare < 1 ? 1 : spare > 4 ? 4 : spare), room = 2048 / a.pairs;       // (16 KB of cosines and sines)
+    a.tokens_per_block = (int32_t)(tokens < room ? tokens : room);
     const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
     if (blocks * kThreads >= (int64_t)1 << 32) return SNGGUF_E_BADSHAPE;     // (threads of a launch are numbered with 32 bits)
-    bool halves = !a.interleaved;
-    for (int p = 0; p < a.parts; p++) halves = halves && a.part[p] % 16 == 0;
-    const int layout = a.interleaved ? kNeighbours : halves ? kHalves : kAnyHalves;
     const bool norm = a.q_norm.parts || a.k_norm.parts;
-    const size_t lds = (size_t)a.tokens_per_block * a.pairs * sizeof(float2);
-#define SNGGUF_GO(L, C, N)                                                                                              \
-    if (layout == L && (cache != 0) == C && norm == N) {                                                                \
-        head_rotary_kernel<L, C, N><<<dim3((unsigned)blocks), kThreads, lds, stream>>>(a);                              \
+    const size_t lds = (size_t)a.tokens_per_block * a.pairs * sizeof(float2) + (pairs && cache ? (size_t)teams * a.dim * 2 : 0);
+    const dim3 grid((unsigned)blocks);
+    const HeadNormArgs& one = a.q_norm.parts ? a.q_norm : a.k_norm;
+    const int kind = !norm ? kNormNone : one.bf16 ? kNormHalf : kNormWide;
+#define SNGGUF_GO(C)                                                                                                    \
+    if ((cache != 0) == C) {                                                                                            \
+        if (pairs && kind == kNormNone) head_pairs_kernel<C, kNormNone><<<grid, kThreads, lds, stream>>>(a);            \
+        else if (pairs && kind == kNormHalf) head_pairs_kernel<C, kNormHalf><<<grid, kThreads, lds, stream>>>(a);       \
+        else if (pairs) head_pairs_kernel<C, kNormWide><<<grid, kThreads, lds, stream>>>(a);                            \
+        else if (a.interleaved && norm) head_rotary_kernel<kNeighbours, C, true><<<grid, kThreads, lds, stream>>>(a);   \
+        else if (a.interleaved) head_rotary_kernel<kNeighbours, C, false><<<grid, kThreads, lds, stream>>>(a);          \
+        else if (norm) head_rotary_kernel<kAnyHalves, C, true><<<grid, kThreads, lds, stream>>>(a);                     \
+        else head_rotary_kernel<kAnyHalves, C, false><<<grid, kThreads, lds, stream>>>(a);                              \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
-#define SNGGUF_GO_ALL(L) SNGGUF_GO(L, false, false) SNGGUF_GO(L, false, true) SNGGUF_GO(L, true, false) SNGGUF_GO(L, true, true)
-    SNGGUF_GO_ALL(kHalves)
-    SNGGUF_GO_ALL(kNeighbours)
-    SNGGUF_GO_ALL(kAnyHalves)
-#undef SNGGUF_GO_ALL
+    SNGGUF_GO(false)
+    SNGGUF_GO(true)
 #undef SNGGUF_GO
     return SNGGUF_E_BADSHAPE;
 }

@@ -11,10 +11,10 @@ constexpr int kMostParts = 4;
 struct HeadNormArgs {
     const void* weight[kMostParts];      // 16-byte aligned
     int32_t elements[kMostParts];        // multiples of 8; behind the last part: 0
+    float one_over[kMostParts];          // 1 / elements
     int32_t parts;                       // 0: none
     int32_t bf16;                        // weights are bf16, else fp32
     float eps;
-    int32_t group;                       // lanes of a part where all parts are one power of two, else 0
 };
 
 struct HeadRotaryArgs : RotaryCacheArgs {
@@ -22,7 +22,7 @@ struct HeadRotaryArgs : RotaryCacheArgs {
     int32_t axes;
     int64_t axis_stride;                 // from a token's position to its next one
     int32_t parts, part[kMostParts];     // elements, together 2 x pairs
-    int32_t lane_shift;                  // 2^lane_shift lanes have a head, eight elements each
+    int32_t lane_shift;                  // 2^lane_shift lanes have a head
     HeadNormArgs q_norm, k_norm;
 };
 

@@ -45,34 +45,50 @@ __device__ __forceinline__ void store8(bf16_t* p, u32x4_t v, bool wide) {
 }
 
 // Eight elements into a run: four neighbouring lanes hold it.  Returns the whole numbers, and the scale for the run.
+//
+// q = rint(x / d) without a division for each: with r = 1 / d to a step, t = x r is off by less than 2^-15, and q = rint(t) can
+// be wrong only if x / d is that near to a half.  It then is one: x has 8 significant bits and d at most 11, so |x / d - (n + 1/2)|, a multiple
+// of 2^-12 at least for numbers in reach, is 0 or more than that.  x - q d is exact, so 2 |x - q d| = d tells, and the even one is taken.
+// (Largest magnitudes are compared as whole numbers, which bf16 without its sign is ordered as, NaN above all.)
 __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
-    float x[8];
-    unpack8(p, x);
-    float top = 0.f;
-    bool bad = false;
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t m = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        top = fmaxf(top, __builtin_fabsf(x[i]));
-        bad |= x[i] != x[i];
+    for (int i = 0; i < 4; i++) {
+        const uint32_t magnitude = p[i] & 0x7FFF7FFFu;
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, magnitude));
     }
-    if (bad) top = __builtin_nanf("");
+    uint32_t top_bits = m[0] > m[1] ? m[0] : m[1];
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        const float t = __shfl_xor(top, o);
-        top = (top != top || t != t) ? __builtin_nanf("") : fmaxf(top, t);
+        const uint32_t other = o == 1 ? (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top_bits, 0xB1, 0xF, 0xF, false)
+                                      : (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top_bits, 0x4E, 0xF, 0xF, false);
+        top_bits = top_bits > other ? top_bits : other;
     }
+    const float top = top_bits > 0x7F80u ? __builtin_nanf("") : __builtin_bit_cast(float, top_bits << 16);
     float d = top / 127.f;
     if (d > 512.f) d = 512.f;
     scale = f32_to_f16(d);
     d = f16_to_f32(scale);
     u32x2_t out = {0u, 0u};
     if (d > 0.f) {
+        constexpr float kWhole = 12582912.f;           // 1.5 x 2^23: added to a small number, it rounds it to a whole one in its low bits
+        const float r = __builtin_amdgcn_rcpf(d), most = 127.f * d;
+        float x[8];
+        unpack8(p, x);
+        uint32_t q[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float q = __builtin_rintf(x[i] / d);
-            q = q > 127.f ? 127.f : q < -127.f ? -127.f : q;
-            out[i >> 2] |= ((uint32_t)(int)q & 0xFFu) << (8 * (i & 3));
+            const float within = __builtin_amdgcn_fmed3f(x[i], -most, most);
+            const float u = within * r + kWhole;
+            const float off = __builtin_fmaf(-(u - kWhole), d, within);
+            q[i] = __builtin_bit_cast(uint32_t, u);
+            if (2.f * __builtin_fabsf(off) == d && (q[i] & 1u)) q[i] += off > 0.f ? 1u : 0xFFFFFFFFu;
         }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            out[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * i + 3], q[4 * i + 2], 0x0C0C0400u),
+                                           __builtin_amdgcn_perm(q[4 * i + 1], q[4 * i], 0x0C0C0400u), 0x05040100u);
     }
     return out;
 }

@@ -522,4 +522,13 @@ struct MlpCtl {
 };
 constexpr int64_t kMlpCtlBytes = 8192;   // the tagged activation words [M][inter / 2] follow at this offset
 
+// A kernel's arguments lie in memory, and a line of them that is read late is waited for late: this asks for all of their lines at once.
+template <typename Args>
+__device__ __forceinline__ void touch_arguments(const Args& a) {
+    uint32_t all = 0;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(Args); i += 64) all |= *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(&a) + i);
+    asm volatile("" ::"s"(all));
+}
+
 }  // namespace sngguf

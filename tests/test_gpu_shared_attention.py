@@ -160,6 +160,14 @@ def test_long_own_parts_are_split(dev, qt):
     b.check(b())
 
 
+@pytest.mark.parametrize("counts", [[127, 127], [200, 150], [3] * 90, [1100, 5], [0] * 300 + [2] * 20])
+def test_many_sequences_and_groups(dev, counts):
+    """Up to 256 of them are planned in one go, more in turns."""
+    n = sum(counts)
+    b = Batch(dev, counts, [256 + 16 * (i % 3) for i in range(len(counts))], [1] * n, [1 + i % 40 for i in range(n)], 2, 1, 64, 16, ops.BF16, n)
+    b.check(b(), only=set(range(0, n, 7)) | {n - 1})
+
+
 @BOTH
 def test_every_sequence_one_token_without_ends(dev, qt):
     b = Batch(dev, [4, 3], [260, 900], [1] * 7, [1, 2, 3, 4, 5, 6, 700], 8, 2, 128, 16, qt)
