@@ -558,13 +558,14 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
 /*
  * sngguf_paged_attention (without a window) of sequences that begin alike: what a group has in common is read once for all of it.
  * Group g is the sequences [groups[g], groups[g + 1]) (int32, device, [group_count + 1], not decreasing), whose first shared[g] tokens lie in the
- * pages of the first of them that has queries: the other ones' pages hold the same there, and are not read as far as whole multiples of 128 tokens go.
- * No more counts as common than every sequence of the group with queries has in front of its new tokens; sequences in no group have nothing in
- * common.  The result is sngguf_paged_attention's but for the order of its sums.  workspace (16-byte aligned) of
- * sngguf_shared_attention_workspace_bytes(..., max_keys = table_width * page_size, ...) bytes is needed; without ends_q, max_new there is 1.
+ * pages of the first of them that has queries; the other ones' pages hold the same there.  No more counts as common than every sequence of the
+ * group with queries has in front of its new tokens; sequences in no group have nothing in common.  The result is sngguf_paged_attention's
+ * but for the order of its sums, and where nothing would be gained (few keys, or many new tokens of each sequence) it is what runs.  workspace (16-byte
+ * aligned) of sngguf_shared_attention_workspace_bytes(..., max_keys = table_width * page_size, ..., the cache's qtype) bytes is needed where
+ * that is not sngguf_paged_attention's; without ends_q, max_new there is 1.
  */
 int64_t sngguf_shared_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t groups, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads,
-                                                int64_t dim);
+                                                int64_t dim, int qtype);
 int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
                             const int32_t* table, int64_t table_stride, int64_t table_width, const int32_t* lens, const int32_t* ends_q,
                             int64_t sequences, const int32_t* groups, const int32_t* shared, int64_t group_count, int64_t max_new, float scale,

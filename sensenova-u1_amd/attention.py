@@ -597,10 +597,10 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.T
     """``paged_attention`` of sequences that begin alike, as answers to one prompt do: what a group has in common is read once for all of it.
 
     Group g is the sequences ``groups[g] : groups[g + 1]`` (int32 [groups + 1], not decreasing), whose first ``shared[g]`` tokens (int32 [groups])
-    lie in the pages of the first of them that has queries.  The other ones' pages hold the same there (``PageTables.fork`` makes them the same pages),
-    and are not read as far as whole multiples of 128 tokens go.  No more counts as common than every sequence of the group with queries has in front of its
-    new tokens; sequences of no group, or of a group of one, have nothing in common.  The result is that of ``paged_attention`` but for the order of its
-    sums; everything else is as there."""
+    lie in the pages of the first of them that has queries; the other ones' pages hold the same there (``PageTables.fork`` makes them the same pages).
+    No more counts as common than every sequence of the group with queries has in front of its new tokens; sequences of no group, or of a group of
+    one, have nothing in common.  The result is that of ``paged_attention`` but for the order of its sums; everything else is as there, and where
+    nothing would be gained (few keys, or many new tokens of each sequence) it is what runs."""
     what = "shared_prefix_attention"
     q, qt, qh, pages, lens, ends_q, scale = _paged(what, q, cache, pages, lens, ends_q, max_new, scale, 0)
     (tokens, heads, dim), (sequences, width) = q.shape, pages.shape
@@ -616,7 +616,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.T
     if tokens and sequences:
         if ends_q is None:
             max_new = 1
-        nbytes = _shared_workspace(tokens, sequences, count, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
+        nbytes = _shared_workspace(tokens, sequences, count, max_new, width * cache.page_size, heads, cache.kv_heads, dim, cache.quant_type)
         _launch_with_workspace(cache._index, nbytes, "sngguf_shared_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
                                pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, groups.data_ptr(), shared.data_ptr(), count, max_new, scale,
                                out.data_ptr(), ot, oh)

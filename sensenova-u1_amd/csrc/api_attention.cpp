@@ -236,15 +236,23 @@ int launch_many(AttentionArgs& a, const Launch& p, int dim, int source, float* p
 
 // ---- sequences that begin alike ----------------------------------------------------------------------------------------
 
-// The three launches of partial results, and where everything lies in the workspace
+// The launches of partial results (common keys that many rows see; few rows; many rows), and where everything lies in the workspace
 struct SharedPlan {
     Launch launch[sngguf::kSharedLaunches];
-    bool few_common;       // the common keys go to the kernel for few rows
     int32_t few_rows;      // sequences of at most so many rows go to that kernel
     int64_t entries, sequence_of, map[sngguf::kSharedLaunches], partial[sngguf::kSharedLaunches], bytes;
 };
 
-SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_t max_new, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+// Whether what sequences have in common is left to each of them, as by sngguf_paged_attention:
+//  * where they can have few keys together, the plan and the join cost more than reading the common ones again from the caches (32 / 8 heads of
+//    128, bf16, 8 sequences of 4300 keys at most 23.5 us against 22.2, 32 of 1250 22.8 against 25.9, 64 of 700 25.0 against 26.7; 8 bits, 8 of 4300
+//    23.4 against 21.5, 4 of 16600 30.1 against 30.8);
+//  * where they have 256 rows each on average, whose tiles are full already (two of 256 tokens and four of one, 6016 keys in common: 107 us against 96).
+bool shared_alone(int64_t tokens, int64_t sequences, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+    return (double)sequences * (double)keys * (double)(kv_heads * dim) < (double)(40 << 20) || tokens * (heads / kv_heads) >= 256 * sequences;
+}
+
+SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_t max_new, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim, bool q8) {
     SharedPlan p = {};
     const int64_t group = heads / kv_heads;
     const int d = kernel_dim(dim);
@@ -258,18 +266,24 @@ SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_
         x.partial_bytes = x.grid * rows * (d + 2) * 4;
         return x;
     };
-    // all queries of a group are rows of its common keys
-    const int64_t mean = tokens * group / groups;
-    const int widest = d == 256 ? 32 : 64;
-    p.few_common = mean <= widest;
-    const int rows = p.few_common ? (mean <= 16 ? 16 : mean <= 32 ? 32 : widest) : many_dim(dim) <= 192 && mean > 128 ? 256 : 128;
-    p.launch[0] = planned(row_tiles(tokens, groups, group, rows), rows, p.few_common ? few_at_a_time(rows, d) : many_at_a_time(rows, d),
-                          keys / (p.few_common ? kRowsKeys : kTilesKeys), p.few_common ? kRowsLeast : kCommonLeast);
+    // All queries of a group are rows of its common keys.  While rows x keys are few, these go to the kernel for few rows, in one launch and in the
+    // same tiles as what sequences have of their own: tiles read the common keys again, from the caches, but there is a launch less, and more
+    // wavefronts than with larger tiles.  bf16, 16 sequences of 4 heads a group over 8192 / 16384 / 32768 common keys 31.7 / 44.6 / 75.9 us
+    // against 36.4 / 43.3 / 56.2, 64 over 512 / 2048 25.0 / 40.8 against 37.9 / 41.4; 8 bits, 16 over 16384 / 32768 39.2 / 54.6 against 45.1 /
+    // 54.6, 32 over 8192 / 16384 40.1 / 55.3 against 43.9 / 51.4.
     const PagedPlan own = paged_plan(tokens, sequences, max_new, keys, heads, kv_heads, dim);
+    const int64_t mean = tokens * group / groups;
+    const bool few_common = own.few && (double)mean * (double)keys <= (q8 ? 1.5 : 0.875) * (double)(1 << 20);
     p.few_rows = (int32_t)own.few_rows;
+    const int rows = own.a.rows;
     if (own.few)
-        p.launch[1] = planned(own.many ? sequences : row_tiles(tokens, sequences, group, own.a.rows), own.a.rows, own.a.want, keys / kRowsKeys + 1, kRowsLeast);
+        p.launch[1] = planned((own.many ? sequences : row_tiles(tokens, sequences, group, rows)) + (few_common ? row_tiles(tokens, groups, group, rows) : 0), rows, own.a.want,
+                              keys / kRowsKeys + 1, kRowsLeast);
     if (own.many) p.launch[2] = planned(row_tiles(tokens, sequences, group, own.b.rows), own.b.rows, own.b.want, keys / kTilesKeys + 1, kTilesLeast);
+    if (!few_common) {
+        const int many = many_dim(dim) <= 192 && mean > 128 ? 256 : 128;
+        p.launch[0] = planned(row_tiles(tokens, groups, group, many), many, many_at_a_time(many, d), keys / kTilesKeys, kCommonLeast);
+    }
     auto room = [&](int64_t bytes) {
         const int64_t at = p.bytes;
         p.bytes += (bytes + 255) / 256 * 256;
@@ -570,9 +584,11 @@ int sngguf_paged_attention(const void* q, int64_t tokens_q, int64_t heads, int64
 }
 
 int64_t sngguf_shared_attention_workspace_bytes(int64_t tokens_q, int64_t sequences, int64_t groups, int64_t max_new, int64_t max_keys, int64_t heads, int64_t kv_heads,
-                                                int64_t dim) {
+                                                int64_t dim, int qtype) {
     if (!shared_sizes_fit(tokens_q, sequences, groups, max_new, max_keys) || !heads_fit(heads, kv_heads, dim)) return 0;
-    return shared_plan(tokens_q, sequences, groups, max_new, max_keys, heads, kv_heads, dim).bytes;
+    if (shared_alone(tokens_q, sequences, max_keys, heads, kv_heads, dim))
+        return sngguf_paged_attention_workspace_bytes(tokens_q, sequences, max_new, max_keys, heads, kv_heads, dim);
+    return shared_plan(tokens_q, sequences, groups, max_new, max_keys, heads, kv_heads, dim, qtype == SNGGUF_TYPE_Q8_0).bytes;
 }
 
 int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int64_t q_token, int64_t q_head, const sngguf_kv_cache* cache,
@@ -589,16 +605,20 @@ int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int6
     const int64_t kv_heads = cache->kv_heads, keys = table_width * cache->page_size;
     if (!ends_q) max_new = 1;
     if (!shared_sizes_fit(tokens_q, sequences, group_count, max_new, keys)) return SNGGUF_E_BADSHAPE;
-    if (!q || !out || !lens || (table_width && !table) || !groups || !shared || !workspace) return SNGGUF_E_NULLPTR;
+    const bool alone = shared_alone(tokens_q, sequences, keys, heads, kv_heads, cache->dim);
+    if (!q || !out || !lens || (table_width && !table) || !groups || !shared || (!workspace && !alone)) return SNGGUF_E_NULLPTR;
     if (!whole_pieces(q, q_token, q_head) || !whole_pieces(out, out_token, out_head) || !aligned(table, 4) || !aligned(lens, 4) ||
         !aligned(ends_q, 4) || !aligned(groups, 4) || !aligned(shared, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
+    if (alone)
+        return sngguf_paged_attention(q, tokens_q, heads, q_token, q_head, cache, table, table_stride, table_width, lens, ends_q, sequences, max_new, scale, 0, out, out_token,
+                                      out_head, workspace, workspace_bytes, stream);
     const int d = kernel_dim(cache->dim);
     const bool q8 = cache->qtype == SNGGUF_TYPE_Q8_0;
-    const SharedPlan p = shared_plan(tokens_q, sequences, group_count, max_new, keys, heads, kv_heads, cache->dim);
+    const SharedPlan p = shared_plan(tokens_q, sequences, group_count, max_new, keys, heads, kv_heads, cache->dim, q8);
     if (workspace_bytes < p.bytes || !launch_fits((tokens_q * heads + 3) / 4, 256)) return SNGGUF_E_BADSHAPE;
     for (int l = 0; l < sngguf::kSharedLaunches; l++)
-        if (!launch_fits(p.launch[l].grid, l == 1 || (l == 0 && p.few_common) ? 256 : 2 * p.launch[l].rows)) return SNGGUF_E_BADSHAPE;
+        if (!launch_fits(p.launch[l].grid, l == 1 ? 256 : 2 * p.launch[l].rows)) return SNGGUF_E_BADSHAPE;
     sngguf::SharedArgs s = {};
     AttentionArgs& a = s.a;
     a.q = static_cast<const bf16_t*>(q);
@@ -630,12 +650,11 @@ int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int6
     s.sequence_of = ends_q ? reinterpret_cast<int32_t*>(room + p.sequence_of) : nullptr;
     for (int l = 0; l < sngguf::kSharedLaunches; l++) {
         sngguf::SharedLaunch& x = s.launch[l];
-        const bool few = l == 1 || (l == 0 && p.few_common);
         x.row_shift = log2_of(p.launch[l].rows);
-        x.key_shift = log2_of(few ? kRowsKeys : kTilesKeys);
+        x.key_shift = log2_of(l == 1 ? kRowsKeys : kTilesKeys);
         x.max_rows = p.few_rows;
         x.want = p.launch[l].want;
-        x.least = few ? kRowsLeast : l == 0 ? kCommonLeast : kTilesLeast;
+        x.least = l == 1 ? kRowsLeast : l == 0 ? kCommonLeast : kTilesLeast;
         x.slots = (int32_t)(p.launch[l].grid / kv_heads);
         x.map = reinterpret_cast<sngguf::AttentionEntry*>(room + p.map[l]);
         x.partial = reinterpret_cast<float*>(room + p.partial[l]);
@@ -647,8 +666,8 @@ int sngguf_shared_attention(const void* q, int64_t tokens_q, int64_t heads, int6
         a.map = s.launch[l].map;
         a.partial = s.launch[l].partial;
         a.grid = p.launch[l].grid;
-        r = l == 1 || (l == 0 && p.few_common) ? sngguf::launch_attention_rows(a, p.launch[l].rows, d, q8, st)
-                                               : sngguf::launch_attention_tiles(a, p.launch[l].rows, many_dim(cache->dim), q8 ? 2 : 1, st);
+        r = l == 1 ? sngguf::launch_attention_rows(a, p.launch[l].rows, d, q8, st)
+                   : sngguf::launch_attention_tiles(a, p.launch[l].rows, many_dim(cache->dim), q8 ? 2 : 1, st);
     }
     return r == SNGGUF_OK ? sngguf::launch_shared_join(s, d, st) : r;
 }

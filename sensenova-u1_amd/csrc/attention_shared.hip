@@ -63,7 +63,7 @@ __device__ __forceinline__ Entry entry_of(const SharedLaunch* launch, const Atte
     const uint32_t rows = (uint32_t)e.lq * (uint32_t)group;
     Entry x = {-1, 0, 0};
     if (rows == 0 || (common && e.lk == 0)) return x;
-    const int l = common ? 0 : (int32_t)rows > launch[1].max_rows || launch[1].slots == 0 ? 2 : 1;
+    const int l = common ? (launch[0].slots ? 0 : 1) : (int32_t)rows > launch[1].max_rows || launch[1].slots == 0 ? 2 : 1;
     if (launch[l].slots == 0) return x;
     const int row_shift = launch[l].row_shift, key_shift = launch[l].key_shift;
     x.launch = l;

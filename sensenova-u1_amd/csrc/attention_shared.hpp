@@ -7,7 +7,8 @@ namespace sngguf {
 
 constexpr int kSharedUnit = 128;     // common keys are taken in multiples of every kernel's key tile
 
-// One of the launches that compute partial results: the common keys', the single tokens', the chunks'
+// One of the launches that compute partial results: common keys of many rows; few rows, of common keys (where there is no first) and of
+// sequences; many rows of sequences
 struct SharedLaunch {
     int32_t row_shift, key_shift;    // 2^row_shift rows and 2^key_shift keys of a tile
     int32_t max_rows;                // of the sequences that the second takes; the third takes the others

@@ -182,7 +182,7 @@ def load_library() -> ctypes.CDLL:
     lib.sngguf_paged_attention_workspace_bytes.restype = i64
     lib.sngguf_paged_attention.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, cf, i64, vp, i64, i64, vp, i64, vp]
     lib.sngguf_paged_attention.restype = ci
-    lib.sngguf_shared_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i64, i64]
+    lib.sngguf_shared_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i64, i64, ci]
     lib.sngguf_shared_attention_workspace_bytes.restype = i64
     lib.sngguf_shared_attention.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, i64, vp, vp, i64, i64, cf, vp, i64, i64, vp, i64, vp]
     lib.sngguf_shared_attention.restype = ci

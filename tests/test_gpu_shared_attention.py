@@ -12,6 +12,8 @@ from . import attention_oracle as ao
 pytestmark = pytest.mark.gpu
 
 UNIT = 128          # what is common is taken in multiples of so many tokens
+KEYS = 50 << 20     # elements of keys that sequences could have, by the width of their tables, for the groups to count
+FEW, MANY = "few", "many"     # which kernel takes the common keys, by rows x keys of a group
 
 
 def _values(gen, tokens, heads, dim, wide=False):
@@ -32,9 +34,10 @@ def _close(got, want, most, what):
 
 
 class Batch:
-    """Sequences of some groups in a cache; pages that nobody may read for what is common hold NaN."""
+    """Sequences of some groups in a cache, in tables so wide that the groups count (``kernel``: as wide as that kernel needs; None: as narrow as the
+    sequences are); where they do, pages that nobody reads for what is common hold NaN."""
 
-    def __init__(self, dev, counts, shared, new, own, heads, kv_heads, dim, page, qt, seed=0, outside=0):
+    def __init__(self, dev, counts, shared, new, own, heads, kv_heads, dim, page, qt, seed=0, outside=0, kernel=FEW):
         gen = torch.Generator().manual_seed(seed)
         self.dev, self.new = dev, new
         group = [g for g, n in enumerate(counts) for _ in range(n)] + [None] * outside
@@ -49,6 +52,11 @@ class Batch:
         order = torch.randperm(total, generator=gen).tolist()
         nan_page = order.pop()
         width = max(-(-n // page) for n in self.lens) + 1
+        group_rows = sum(new) * (heads // kv_heads) // len(counts)
+        if kernel is not None:
+            width = max(width, -(-KEYS // (len(new) * kv_heads * dim * page)))
+        if kernel == MANY:
+            width = max(width, -(-(2 << 20) // (max(group_rows, 1) * page)))
         self.cache = PagedKVCache.empty(total, kv_heads, page, dim, qt, dev)
         for t in (self.cache.k, self.cache.v):
             t.fill_(-128 if qt == ops.Q8_0 else float("nan"))
@@ -64,11 +72,14 @@ class Batch:
             slots = torch.tensor(mine, dtype=torch.int64)[torch.arange(n) // page] * page + torch.arange(n) % page
             self.cache.write(self.kv[i][0].to(dev), self.kv[i][1].to(dev), slots.to(dev))
         self.whole = _ints(rows, dev)
+        lib = ops.load_library()
+        sizes = (sum(new), len(new), len(counts), max(new), width * page, heads, kv_heads, dim, qt)
+        self.counts = lib.sngguf_shared_attention_workspace_bytes(*sizes) != lib.sngguf_paged_attention_workspace_bytes(*sizes[:2], *sizes[3:8])
         # what is common, and who need not have it
-        first, hidden = {}, [list(r) for r in rows]
+        hidden = [list(r) for r in rows]
         for g, (a, n) in enumerate(zip(itertools.accumulate([0] + counts), counts)):
             live = [i for i in range(a, a + n) if new[i]]
-            common = max(0, min([shared[g]] + [self.lens[i] - new[i] for i in live])) // UNIT * UNIT if len(live) > 1 else 0
+            common = max(0, min([shared[g]] + [self.lens[i] - new[i] for i in live])) // UNIT * UNIT if len(live) > 1 and self.counts else 0
             for i in range(a, a + n):
                 if not live or i == live[0]:
                     continue
@@ -100,10 +111,15 @@ class Batch:
 BOTH = pytest.mark.parametrize("qt", [ops.BF16, ops.Q8_0])
 
 
+KERNELS = pytest.mark.parametrize("kernel", [FEW, MANY])
+
+
 @BOTH
+@pytest.mark.parametrize("kernel", [FEW, MANY, None])
 @pytest.mark.parametrize("shared", [0, 1, 16, 127, 128, 129, 255, 256, 300, 1000, 2048])
-def test_lengths_of_what_is_common(dev, shared, qt):
-    b = Batch(dev, [5], [shared], [1] * 5, [1, 3, 40, 129, 200], 8, 2, 128, 16, qt, shared)
+def test_lengths_of_what_is_common(dev, shared, kernel, qt):
+    b = Batch(dev, [5], [shared], [1] * 5, [1, 3, 40, 129, 200], 8, 2, 128, 16, qt, shared, kernel=kernel)
+    assert b.counts == (kernel is not None)
     b.check(b())
     assert torch.equal(b(), b())
 
@@ -111,29 +127,34 @@ def test_lengths_of_what_is_common(dev, shared, qt):
 @BOTH
 @pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (1, 1, 64), (4, 4, 64), (28, 4, 128), (5, 1, 96), (12, 1, 128), (16, 2, 32), (6, 2, 160), (4, 2, 192), (6, 2, 256), (40, 8, 64), (130, 1, 64)])
 @pytest.mark.parametrize("count", [2, 9, 40])
-def test_head_layouts_and_row_counts(dev, heads, kv_heads, dim, count, qt):
+@KERNELS
+def test_head_layouts_and_row_counts(dev, heads, kv_heads, dim, count, kernel, qt):
     rng = random.Random(count)
-    b = Batch(dev, [count], [640], [1] * count, [rng.randint(1, 70) for _ in range(count)], heads, kv_heads, dim, 32, qt, dim + count)
+    b = Batch(dev, [count], [640], [1] * count, [rng.randint(1, 70) for _ in range(count)], heads, kv_heads, dim, 32, qt, dim + count, kernel=kernel)
+    assert b.counts
     b.check(b())
 
 
 @BOTH
 @pytest.mark.parametrize("page", [16, 64, 256, 4096])
-def test_groups_that_differ(dev, page, qt):
+@KERNELS
+def test_groups_that_differ(dev, page, kernel, qt):
     counts, shared = [3, 1, 0, 6, 2], [300, 700, 5000, 1500, 0]
     new, own = [1] * 12, [5, 1, 100, 30, 1, 2, 3, 400, 5, 6, 77, 1]
-    b = Batch(dev, counts, shared, new, own, 8, 2, 64, page, qt, page)
+    b = Batch(dev, counts, shared, new, own, 8, 2, 64, page, qt, page, kernel=kernel)
     b.check(b())
-    b = Batch(dev, counts, shared, new + [1, 1], own + [300, 1], 8, 2, 64, page, qt, page, outside=2)      # sequences of no group
+    b = Batch(dev, counts, shared, new + [1, 1], own + [300, 1], 8, 2, 64, page, qt, page, outside=2, kernel=kernel)      # sequences of no group
     b.check(b())
 
 
 @BOTH
 @pytest.mark.parametrize("new", [[2, 3, 1], [7, 1, 5], [16, 16, 16], [1, 64, 3], [200, 1, 1], [300, 129, 257], [0, 4, 9], [0, 0, 5], [1, 1, 700]])
 @pytest.mark.parametrize("known", [True, False])
-def test_runs_of_new_tokens(dev, new, known, qt):
+@KERNELS
+def test_runs_of_new_tokens(dev, new, known, kernel, qt):
     own = [n + 20 * i for i, n in enumerate(new)]
-    b = Batch(dev, [3], [520], new, own, 8, 2, 128, 32, qt, sum(new))
+    b = Batch(dev, [3], [520], new, own, 8, 2, 128, 32, qt, sum(new), kernel=kernel)
+    assert b.counts == (sum(new) * 4 < 256 * 3)
     b.check(b(max_new=max(new) if known else 0))
 
 
@@ -148,9 +169,10 @@ def test_new_tokens_that_reach_into_what_is_said_to_be_common(dev, qt):
 
 @BOTH
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_long_common_parts_are_split(dev, dim, qt):
+@KERNELS
+def test_long_common_parts_are_split(dev, dim, kernel, qt):
     for count, shared in ((2, 20000), (20, 6000), (70, 2500)):
-        b = Batch(dev, [count], [shared], [1] * count, [1 + i % 50 for i in range(count)], 4, 1, dim, 64, qt, count)
+        b = Batch(dev, [count], [shared], [1] * count, [1 + i % 50 for i in range(count)], 4, 1, dim, 64, qt, count, kernel=kernel)
         b.check(b(), only={0, 1, count - 1})
 
 
@@ -220,17 +242,18 @@ def test_rows_behind_the_last_sequence_are_left_and_outputs_of_any_layout(dev):
     stacked[:, 3:11] = b.q.to(dev)
     assert torch.equal(shared_prefix_attention(stacked[:, 3:11], b.cache, b.pages, b.lens_dev, b.groups, b.shared, b.ends), want)
     # tables whose rows lie apart
-    wide = torch.zeros((3, 40), dtype=torch.int32, device=dev)
+    wide = torch.zeros((3, 40 + b.pages.shape[1]), dtype=torch.int32, device=dev)
     wide[:, 5:5 + b.pages.shape[1]] = b.pages
     assert torch.equal(shared_prefix_attention(b.q.to(dev), b.cache, wide[:, 5:5 + b.pages.shape[1]], b.lens_dev, b.groups, b.shared, b.ends), want)
 
 
 @BOTH
-def test_values_that_are_not_finite(dev, qt):
+@KERNELS
+def test_values_that_are_not_finite(dev, kernel, qt):
     """An infinity or a NaN in what is common reaches all of the group and no other; one in a sequence's own part that sequence alone."""
     for where in ("common", "own"):
         for bad in (float("inf"), float("nan"), -float("inf")):
-            b = Batch(dev, [3, 2], [400, 300], [1, 2, 1, 1, 1], [5, 6, 30, 4, 5], 4, 2, 64, 16, qt)
+            b = Batch(dev, [3, 2], [400, 300], [1, 2, 1, 1, 1], [5, 6, 30, 4, 5], 4, 2, 64, 16, qt, kernel=kernel)
             at = 130 if where == "common" else 400
             slot = b.whole[1].long()[at // 16] * 16 + at % 16
             k, v = b.kv[1][0][at:at + 1].clone(), b.kv[1][1][at:at + 1].clone()
@@ -252,17 +275,19 @@ def test_values_that_are_not_finite(dev, qt):
             b.check(got, only={3, 4} if where == "common" else {0, 2, 3, 4})
 
 
-def test_sums_beyond_fp32_stay_finite_where_their_average_is(dev):
-    b = Batch(dev, [2], [1024], [1, 1], [3, 5], 2, 1, 64, 16, ops.BF16)
+@KERNELS
+def test_sums_beyond_fp32_stay_finite_where_their_average_is(dev, kernel):
+    b = Batch(dev, [2], [1024], [1, 1], [3, 5], 2, 1, 64, 16, ops.BF16, kernel=kernel)
     b.cache.v.fill_(3e38)
     got = b().float()
     assert bool(torch.isfinite(got).all()) and float((got / 3e38 - 1).abs().max()) < 0.02
 
 
-def test_a_query_that_is_not_a_number(dev):
+@KERNELS
+def test_a_query_that_is_not_a_number(dev, kernel):
     """It gives NaN, and the other queries what they have without it, within the bound of each: a wavefront that meets the NaN sets the maxima of
     all its rows right, so the others' weights exp2(s - m) are rounded to bf16 with another m (u in the bound, either way)."""
-    b = Batch(dev, [3], [512], [1, 1, 1], [3, 5, 200], 4, 2, 128, 16, ops.BF16)
+    b = Batch(dev, [3], [512], [1, 1, 1], [3, 5, 200], 4, 2, 128, 16, ops.BF16, kernel=kernel)
     clean = b.q.clone()
     b.q[1, 2, 7] = torch.nan
     got = b()
@@ -274,8 +299,10 @@ def test_a_query_that_is_not_a_number(dev):
         _close(got[i:i + 1, keep], want[:, keep], most[:, keep], f"sequence {i}")
 
 
-def test_lengths_and_groups_that_are_none_stay_within_the_tensors(dev):
-    b = Batch(dev, [4, 3], [260, 900], [1, 5, 1, 2, 1, 40, 1], [1, 9, 3, 4, 5, 46, 700], 8, 2, 128, 16, ops.BF16)
+@KERNELS
+def test_lengths_and_groups_that_are_none_stay_within_the_tensors(dev, kernel):
+    b = Batch(dev, [4, 3], [260, 900], [1, 5, 1, 2, 1, 40, 1], [1, 9, 3, 4, 5, 46, 700], 8, 2, 128, 16, ops.BF16, kernel=kernel)
+    assert b.counts
     q = b.q.to(dev)
     for groups, shared, ends, lens in (([0, 9000, -5], [10 ** 9, -7], None, None), ([5, 2, 7], [900, 900], None, None), ([0, 7, 3], [128, 256], None, None), ([0, 4, 7], [2 ** 31 - 1, 2 ** 31 - 1], None, None),
                                        ([0, 4, 7], [260, 900], [0, 60, -1, 10, 51, 20, 3, 51], None), ([0, 4, 7], [260, 900], [50, 0, 50, 0, 50, 0, 50, 0], None),
@@ -289,9 +316,10 @@ def test_lengths_and_groups_that_are_none_stay_within_the_tensors(dev):
 
 
 @BOTH
-def test_captured_steps_see_new_lengths_groups_and_queries(dev, qt):
+@KERNELS
+def test_captured_steps_see_new_lengths_groups_and_queries(dev, kernel, qt):
     counts, shared = [5, 3], [700, 300]
-    b = Batch(dev, counts, shared, [1] * 8, [1, 2, 3, 40, 500, 6, 7, 130], 8, 2, 128, 16, qt)
+    b = Batch(dev, counts, shared, [1] * 8, [1, 2, 3, 40, 500, 6, 7, 130], 8, 2, 128, 16, qt, kernel=kernel)
     q = b.q.to(dev)
     args = (b.cache, b.whole, b.lens_dev, b.groups, b.shared)
     shared_prefix_attention(q, *args)
