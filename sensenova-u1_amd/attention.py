@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from typing import Optional, Sequence, Union
 
 import torch
@@ -31,14 +32,9 @@ class _TableStruct(ctypes.Structure):
     _fields_ = [("turns", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double), ("interleaved", ctypes.c_int32)]
 
 
-class _AxesStruct(ctypes.Structure):
-    _fields_ = [("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double),
-                ("interleaved", ctypes.c_int32), ("parts", ctypes.c_int32), ("part", ctypes.c_int32 * 4)]
-
-
-class _NormStruct(ctypes.Structure):
-    _fields_ = [("weight", ctypes.c_void_p * 4), ("elements", ctypes.c_int32 * 4), ("parts", ctypes.c_int32), ("weight_type", ctypes.c_int32),
-                ("eps", ctypes.c_float)]
+# sngguf_rotary_axes and sngguf_head_norm as bytes, which ctypes hands on by their address (half the time of a Structure that is made and filled)
+_AXES = struct.Struct("PPqd6i")     # turns, axis, pairs, magnitude, interleaved, parts, part[4]
+_NORM = struct.Struct("4P6if4x")    # weight[4], elements[4], parts, weight_type, eps
 
 
 class _CacheStruct(ctypes.Structure):
@@ -192,7 +188,7 @@ class RotaryTable:
     ``turns``: float64 on the device, one for each pair; pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with
     ``interleaved``; elements behind the 2 * pairs first are left as they are.  ``for_model`` makes it of a checkpoint's settings."""
 
-    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes", "_axes_address")
+    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes")
 
     def __init__(self, turns: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -204,8 +200,7 @@ class RotaryTable:
         self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self.magnitude, self.interleaved)
         self._address = ctypes.addressof(self._struct)
         # (the same as a table of one axis and one part, where heads are normed as well)
-        self._axes = _AxesStruct(turns.data_ptr(), None, turns.shape[0], self.magnitude, self.interleaved, 1, (2 * turns.shape[0], 0, 0, 0))
-        self._axes_address = ctypes.addressof(self._axes)
+        self._axes = _AXES.pack(turns.data_ptr(), 0, turns.shape[0], self.magnitude, self.interleaved, 1, 2 * turns.shape[0], 0, 0, 0)
 
     @classmethod
     def for_model(cls, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_context: int = 0,
@@ -246,7 +241,7 @@ class RotaryAxes:
     counted from part to part (default: one part).  With ``interleaved`` pairs are (2 i, 2 i + 1) throughout.  Elements behind are
     left as they are.  An axis that positions do not have counts as the nearest that they have."""
 
-    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes", "_axes_address")
+    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes")
 
     def __init__(self, turns: torch.Tensor, axis: torch.Tensor, parts: Optional[Sequence[int]] = None, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -254,15 +249,14 @@ class RotaryAxes:
         pairs = turns.shape[0]
         axis = _numbers(axis, torch.int32, pairs, "RotaryAxes", "axis")
         _same_device("RotaryAxes", turns.get_device(), axis)
-        self.parts = parts = (2 * pairs,) if parts is None else tuple(int(n) for n in parts)
-        if not 1 <= len(parts) <= 4 or any(n < 2 or n % 2 for n in parts) or sum(parts) != 2 * pairs:
+        parts = (2 * pairs,) if parts is None else tuple(parts)
+        if not 1 <= len(parts) <= 4 or min(parts) < 2 or any(n % 2 for n in parts) or sum(parts) != 2 * pairs:
             raise SnGgufError(f"RotaryAxes: parts of {parts} elements (one to four, even) do not hold {pairs} pairs")
         if not math.isfinite(magnitude):
             raise SnGgufError("RotaryAxes: the magnitude is not finite")
         self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
-        self.axis, self.interleaved, self.magnitude = axis, bool(interleaved), float(magnitude)
-        self._axes = _AxesStruct(turns.data_ptr(), axis.data_ptr(), pairs, self.magnitude, self.interleaved, len(parts), parts + (0,) * (4 - len(parts)))
-        self._axes_address = ctypes.addressof(self._axes)
+        self.axis, self.parts, self.interleaved, self.magnitude = axis, parts, bool(interleaved), float(magnitude)
+        self._axes = _AXES.pack(turns.data_ptr(), axis.data_ptr(), pairs, magnitude, self.interleaved, len(parts), *parts, *(0, 0, 0)[len(parts) - 1:])
 
     @classmethod
     def for_model(cls, parts: Sequence[tuple], interleaved: bool = False, device="cuda") -> "RotaryAxes":
@@ -283,29 +277,33 @@ class HeadNorm:
     itself (one: the whole head); their elements, multiples of 8, are a head's together.  Their memory is read at every call: a change in place counts, a tensor
     put in a module's place does not."""
 
-    __slots__ = ("weights", "eps", "dim", "_struct", "_address", "_index")
+    __slots__ = ("weights", "eps", "dim", "_norm", "_index")
 
     def __init__(self, *weights: torch.Tensor, eps: float = 1e-6) -> None:
         if not 1 <= len(weights) <= 4:
             raise SnGgufError(f"HeadNorm: {len(weights)} parts (one to four are possible)")
+        kind, index, at, sizes, kept = weights[0].dtype, weights[0].get_device(), [], [], []
         for w in weights:
-            if w.dtype not in (_BF16, torch.float32) or w.dtype != weights[0].dtype or w.dim() != 1 or w.shape[0] < 8 or w.shape[0] % 8 or not w.is_cuda:
+            size = w.shape[0] if w.dim() == 1 else 0
+            if w.dtype is not kind or size < 8 or size % 8 or w.get_device() != index or index < 0 or (kind is not _BF16 and kind is not torch.float32):
                 raise SnGgufError("HeadNorm: weights must be bf16 or fp32 [a multiple of 8] on a HIP device, of one type, "
-                                  f"got {[(str(w.dtype), tuple(w.shape), str(w.device)) for w in weights]}")
-            if w.requires_grad and torch.is_grad_enabled():
-                raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
+                                  f"got {[(str(x.dtype), tuple(x.shape), str(x.device)) for x in weights]}")
+            if w.requires_grad:
+                if torch.is_grad_enabled():
+                    raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
+                w = w.detach()          # (what a parameter's .data is set to later does not take this memory away)
+            address = w.data_ptr()
+            if address % 16 or w.stride(0) != 1:
+                w = w.clone(memory_format=torch.contiguous_format)
+                address = w.data_ptr()
+            kept.append(w)
+            at.append(address)
+            sizes.append(size)
         if not (math.isfinite(eps) and eps >= 0):
             raise SnGgufError(f"HeadNorm: eps is {eps}")
-        self._index = weights[0].get_device()
-        _same_device("HeadNorm", self._index, *weights)
-        # (detached: what a parameter's .data is set to later does not take this memory away)
-        weights = [w.detach() for w in weights]
-        self.weights = weights = tuple(w if (w.stride(0) == 1 and w.data_ptr() % 16 == 0) else w.clone(memory_format=torch.contiguous_format) for w in weights)
-        self.eps, self.dim = float(eps), sum(w.shape[0] for w in weights)
-        rest = (0,) * (4 - len(weights))
-        self._struct = _NormStruct(tuple(w.data_ptr() for w in weights) + rest, tuple(w.shape[0] for w in weights) + rest, len(weights),
-                                   ops._OUT_CODE[weights[0].dtype], self.eps)
-        self._address = ctypes.addressof(self._struct)
+        self.weights, self.eps, self.dim, self._index = tuple(kept), float(eps), sum(sizes), index
+        rest = (0, 0, 0)[len(at) - 1:]
+        self._norm = _NORM.pack(*at, *rest, *sizes, *rest, len(at), 2 if kind is _BF16 else 0, eps)
 
 
 def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tensor, table, q_norm: Optional[HeadNorm], k_norm: Optional[HeadNorm]):
@@ -326,7 +324,7 @@ def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tens
             raise SnGgufError(f"{what}: a norm of {norm.dim} elements on device {norm._index} does not go with heads of {dim} on device {index}")
     if dim > 512:
         raise SnGgufError(f"{what}: heads of {dim} elements (up to 512 are normed or turned by several positions)")
-    return positions, (positions.data_ptr(), axes, stride), q_norm and q_norm._address, k_norm and k_norm._address
+    return positions, (positions.data_ptr(), axes, stride), q_norm and q_norm._norm, k_norm and k_norm._norm
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: Union[RotaryTable, RotaryAxes], inplace: bool = False,
@@ -367,7 +365,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             q_at, k_at = k_at, None
     if tokens and heads:
         if wide:
-            _launch(index, "sngguf_head_rotary", table._axes_address, *at, tokens, dim, q_at, *first, k_at, *rest)
+            _launch(index, "sngguf_head_rotary", table._axes, *at, tokens, dim, q_at, *first, k_at, *rest)
         else:
             _launch(index, "sngguf_rotary", table._address, positions.data_ptr(), tokens, dim, *first, *rest)
     return q_out, k_out
@@ -461,7 +459,7 @@ class PagedKVCache:
         _same_device(what, self._index, q, positions, table.turns)
         out, ot, oh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
         if tokens and wide:
-            _launch(self._index, "sngguf_cache_write_head_rotary", self._address, table._axes_address, *at, q_at, q.data_ptr(), heads, qt, qh, out.data_ptr(),
+            _launch(self._index, "sngguf_cache_write_head_rotary", self._address, table._axes, *at, q_at, q.data_ptr(), heads, qt, qh, out.data_ptr(),
                     ot, oh, k_at, *rows)
         elif tokens:
             _launch(self._index, "sngguf_cache_write_rotary", self._address, table._address, positions.data_ptr(), q.data_ptr(), heads, qt, qh, out.data_ptr(),

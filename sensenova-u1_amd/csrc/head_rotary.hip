@@ -14,6 +14,8 @@
 //  * head_pairs_kernel, pairs half a part apart in parts of multiples of 16 elements: a lane has eight pairs, both of their elements.
 //  * head_rotary_kernel, neighbouring pairs, any parts or rows: a lane has eight elements; those that they are turned with, where they are not among
 //    the eight, are read beside them.  Shapes for which the other is no form, so it is kept simple.
+#include <type_traits>
+
 #include "head_rotary.hpp"
 #include "rotary_cache_device.hpp"
 
@@ -293,8 +295,8 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
             void* pages = value ? a.v_pages : a.k_pages;
             uint16_t* scales = value ? a.v_scales : a.k_scales;
             const u32x4_t held = value ? k_raw : y;
-            if (scales) cache_piece<true>(pages, scales, a, slot, h, e, held);
-            else cache_piece<false>(pages, scales, a, slot, h, e, held);
+            if (scales) cache_piece<true>(cache_place<true>(pages, scales, a, slot, h), a, e, held);
+            else cache_piece<false>(cache_place<false>(pages, scales, a, slot, h), a, e, held);
         }
     }
 }
@@ -496,14 +498,18 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
             if (slot >= 0 && slot < a.slot_count) {
                 void* pages = value ? a.v_pages : a.k_pages;
                 uint16_t* scales = value ? a.v_scales : a.k_scales;
+                auto both = [&](auto q8_) {
+                    constexpr bool Q8 = decltype(q8_)::value;
+                    const CachePlace to = cache_place<Q8>(pages, scales, a, slot, h);
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int e = 8 * (unit + half * lanes);
-                    if (e >= a.dim) continue;
-                    const u32x4_t held = value ? (half ? k_raw.b : k_raw.a) : *reinterpret_cast<const u32x4_t*>(room + e);
-                    if (scales) cache_piece<true>(pages, scales, a, slot, h, e, held);
-                    else cache_piece<false>(pages, scales, a, slot, h, e, held);
-                }
+                    for (int half = 0; half < 2; half++) {
+                        const int e = 8 * (unit + half * lanes);
+                        if (e >= a.dim) continue;
+                        cache_piece<Q8>(to, a, e, value ? (half ? k_raw.b : k_raw.a) : *reinterpret_cast<const u32x4_t*>(room + e));
+                    }
+                };
+                if (scales) both(std::integral_constant<bool, true>());
+                else both(std::integral_constant<bool, false>());
             }
             __builtin_amdgcn_wave_barrier();             // (the room is written again)
         }

@@ -19,25 +19,32 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kFill = 256, kFillTokens = 1024;       // threads and tokens of a workgroup of the second launch
 constexpr int kStaged = 4096;                        // sequences whose ends it keeps in LDS
 
-// Sum of x over the workgroup's threads up to this one, and over all of them.  `part`: one for each wavefront.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
+// Sums that stop at `most` (below 2^31), which is all that is asked of them: so 32 bits do, and such sums may be taken in any order.
+__device__ __forceinline__ uint32_t add_up_to(uint32_t x, uint32_t y, uint32_t most) { return x + y < most ? x + y : most; }
+
+// x of the workgroup's threads in front of this one, and of all of them, added up to `most`; x is no more than that.  `part`: one for each
+// wavefront, that no call before used.  (In a wavefront: row shifts, then a row's last value handed on.)
+__device__ __forceinline__ uint32_t block_sum_before(uint32_t x, uint32_t most, uint32_t* part, uint32_t& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up((long long)x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();                                 // (the sums of the call before are read)
+#define SNGGUF_STEP(CONTROL, ROWS) x = add_up_to(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CONTROL, ROWS, 0xF, false), most);
+    SNGGUF_STEP(0x111, 0xF)
+    SNGGUF_STEP(0x112, 0xF)
+    SNGGUF_STEP(0x114, 0xF)
+    SNGGUF_STEP(0x118, 0xF)
+    SNGGUF_STEP(0x142, 0xA)
+    SNGGUF_STEP(0x143, 0xC)
+#undef SNGGUF_STEP
     if (lane == 63) part[wave] = x;
+    const uint32_t in_wave = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x138, 0xF, 0xF, false);      // the lane before's
     __syncthreads();
     total = 0;
-    int64_t before = 0;
+    uint32_t before = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
-        if (w < wave) before += part[w];
-        total += part[w];
+        if (w == wave) before = total;
+        total = add_up_to(total, part[w], most);
     }
-    return x + before;
+    return add_up_to(before, in_wave, most);
 }
 
 __device__ __forceinline__ int32_t clamped(int64_t x, int64_t lo, int64_t hi) { return (int32_t)(x < lo ? lo : x > hi ? hi : x); }
@@ -46,6 +53,7 @@ __device__ __forceinline__ int32_t pages_of(int64_t tokens, int shift) { return 
 // What the ring holds: pages that are there, and the place of the first
 __device__ __forceinline__ int32_t ring_count(const PageArgs& a) { return clamped(a.cursor[1] - a.cursor[0], 0, a.ring); }
 __device__ __forceinline__ int32_t ring_place(int64_t at, int32_t ring) {
+    if ((at >> 32) == 0) return (int32_t)((uint32_t)at % (uint32_t)ring);
     const int64_t r = at % ring;
     return (int32_t)(r < 0 ? r + ring : r);
 }
@@ -89,41 +97,45 @@ __device__ __forceinline__ void fill_token(const PageArgs& a, int64_t t, int32_t
 
 template <bool ONE>
 __global__ __launch_bounds__(kThreads) void page_append_kernel(PageArgs a) {
-    __shared__ int64_t part[kWaves];
+    __shared__ uint32_t part[2][2][kWaves];
+    __shared__ unsigned long long missing;
     __shared__ int32_t ends[ONE ? kOneLaunchSequences + 1 : 1];
     __shared__ PageSequence of[ONE ? kOneLaunchSequences : 1];
+    touch_arguments(a);
     const int tid = threadIdx.x;
     const int64_t most = (int64_t)a.width << a.page_shift;
     const int64_t taken = a.cursor[0], given = a.cursor[1];
     const int32_t there = ring_count(a), first = ring_place(taken, a.ring);
-    int64_t rows = 0, wanted = 0, missing = 0;
+    const uint32_t room_rows = (uint32_t)a.tokens, room_pages = 0x7FFFFFFFu;
+    uint32_t rows = 0, wanted = 0;
     if (tid == 0) {
         a.ends[0] = 0;
+        missing = 0;
         if constexpr (ONE) ends[0] = 0;
     }
     for (int64_t base = 0; base < a.sequences; base += kThreads) {
         const int64_t i = base + tid;
         const bool mine = i < a.sequences;
-        int64_t n = mine ? a.added[i] : 0;
-        n = n < 0 ? 0 : n;
+        const int turn = (base / kThreads) & 1;
+        const int32_t asked = mine ? a.added[i] : 0;
         const int32_t length = mine ? clamped(a.lens[i], 0, most) : 0;
-        int64_t sum;
-        const int64_t up = rows + block_scan(n, part, sum);
         // (more new tokens than there are rows: those behind the last row are none)
-        const int64_t e0 = up - n < a.tokens ? up - n : a.tokens, e1 = up < a.tokens ? up : a.tokens;
-        rows += sum;
-        const int64_t whole = length + (e1 - e0);
+        const uint32_t n = asked < 0 ? 0 : (uint32_t)asked < room_rows ? (uint32_t)asked : room_rows;
+        uint32_t sum;
+        const uint32_t e0 = add_up_to(rows, block_sum_before(n, room_rows, part[turn][0], sum), room_rows), e1 = add_up_to(e0, n, room_rows);
+        rows = add_up_to(rows, sum, room_rows);
+        const int64_t whole = length + (int64_t)(e1 - e0);
         const int32_t has = pages_of(length, a.page_shift), wants = pages_of(whole < most ? whole : most, a.page_shift) - has;
-        const int64_t before = wanted + block_scan(wants, part, sum) - wants;
-        wanted += sum;
-        const int32_t gets = clamped(there - before, 0, wants);
+        const uint32_t before = add_up_to(wanted, block_sum_before((uint32_t)wants, room_pages, part[turn][1], sum), room_pages);
+        wanted = add_up_to(wanted, sum, room_pages);
+        const int32_t gets = clamped((int64_t)there - before, 0, wants);
         const int64_t room = (int64_t)(has + gets) << a.page_shift;
         PageSequence q;
         q.length = length;
         q.after = (int32_t)(whole < room ? whole : room);
         q.pages = has;
         q.ring_at = gets ? ring_step(first, before, a.ring) : 0;
-        missing += whole - q.after;
+        if (whole > q.after) atomicAdd(&missing, (unsigned long long)(whole - q.after));
         if (mine) {
             a.ends[i + 1] = (int32_t)e1;
             a.lens_out[i] = q.after;
@@ -131,16 +143,14 @@ __global__ __launch_bounds__(kThreads) void page_append_kernel(PageArgs a) {
             else a.of[i] = q;
         }
     }
-    int64_t all;
-    block_scan(missing, part, all);
+    __syncthreads();
     if (tid == 0) {
-        *a.missing = clamped(all, 0, 0x7FFFFFFF);
-        a.cursor_out[0] = taken + (wanted < there ? wanted : there);
+        *a.missing = missing < 0x7FFFFFFFull ? (int32_t)missing : 0x7FFFFFFF;
+        a.cursor_out[0] = taken + (wanted < (uint32_t)there ? wanted : there);
         a.cursor_out[1] = given;
     }
     if constexpr (ONE) {
-        __syncthreads();
-        const int32_t total = (int32_t)(rows < a.tokens ? rows : a.tokens);
+        const int32_t total = (int32_t)rows;
         for (int64_t t = tid; t < a.tokens; t += kThreads) {
             if (t < total) {
                 const int32_t i = sequence_of(ends, (int32_t)a.sequences, (int32_t)t);
@@ -176,29 +186,28 @@ __global__ __launch_bounds__(kFill) void page_fill_kernel(PageArgs a) {
 
 // Pages of the sequences that are done back into the ring, in the order of the sequences; a wavefront copies one's.
 __global__ __launch_bounds__(kThreads) void page_release_kernel(PageArgs a) {
-    __shared__ int64_t part[kWaves];
-    __shared__ int64_t offset[kThreads];
-    __shared__ int32_t from[kThreads], count[kThreads];
+    __shared__ uint32_t part[kWaves];
+    __shared__ int32_t offset[kThreads], from[kThreads], count[kThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t most = (int64_t)a.width << a.page_shift;
     const int64_t given = a.cursor[1];
     const int32_t room = a.ring - ring_count(a), first = ring_place(given, a.ring);
-    int64_t back = 0;
+    const uint32_t all = 0x7FFFFFFFu;
+    uint32_t back = 0;
     for (int64_t base = 0; base < a.sequences; base += kThreads) {
         const int64_t i = base + tid;
         const bool done = i < a.sequences && a.done[i];
         const int32_t has = done ? pages_of(clamped(a.lens[i], 0, most), a.page_shift) : 0;
         const int32_t held = done && a.held ? clamped(a.held[i], 0, has) : 0;
-        int64_t sum;
-        const int64_t up = block_scan(has - held, part, sum);
-        offset[tid] = back + up - (has - held);
+        uint32_t sum;
+        offset[tid] = (int32_t)add_up_to(back, block_sum_before((uint32_t)(has - held), all, part, sum), all);
         from[tid] = held;
         count[tid] = has - held;
-        back += sum;
+        back = add_up_to(back, sum, all);
         __syncthreads();
         for (int k = wave; k < kThreads && base + k < a.sequences; k += kWaves) {
             const int32_t* row = a.pages + (base + k) * a.width + from[k];
-            for (int32_t j = lane; j < count[k] && offset[k] + j < room; j += 64) a.free[ring_step(first, offset[k] + j, a.ring)] = row[j];
+            for (int32_t j = lane; j < count[k] && j < (int64_t)room - offset[k]; j += 64) a.free[ring_step(first, (int64_t)offset[k] + j, a.ring)] = row[j];
         }
         if (done) {
             a.lens[i] = 0;
@@ -206,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void page_release_kernel(PageArgs a) {
         }
         __syncthreads();
     }
-    if (tid == 0) a.cursor[1] = given + (back < room ? back : room);
+    if (tid == 0) a.cursor[1] = given + (back < (uint32_t)room ? back : room);
 }
 
 // A workgroup a sequence: one that is empty starts with whole pages of its parent, which stay the parent's.

@@ -165,10 +165,10 @@ __global__ __launch_bounds__(kThreads) void rotary_cache_kernel(RotaryCacheArgs 
             if (slot < 0 || slot >= a.slot_count) return;
             if (h < a.kv_heads) {
                 const bf16_t* p = a.k + (t0 + t) * a.k_token + h * a.k_head;
-                cache_piece<CACHE == 2>(a.k_pages, a.k_scales, a, slot, h, 8 * u, ROTARY ? turned8(p, 8 * u, a, cs_all + t * a.pairs) : load8(p + 8 * u, a.wide));
+                cache_piece<CACHE == 2>(cache_place<CACHE == 2>(a.k_pages, a.k_scales, a, slot, h), a, 8 * u, ROTARY ? turned8(p, 8 * u, a, cs_all + t * a.pairs) : load8(p + 8 * u, a.wide));
             } else {
                 h -= a.kv_heads;
-                cache_piece<CACHE == 2>(a.v_pages, a.v_scales, a, slot, h, 8 * u, load8(a.v + (t0 + t) * a.v_token + h * a.v_head + 8 * u, a.wide));
+                cache_piece<CACHE == 2>(cache_place<CACHE == 2>(a.v_pages, a.v_scales, a, slot, h), a, 8 * u, load8(a.v + (t0 + t) * a.v_token + h * a.v_head + 8 * u, a.wide));
             }
         });
     }

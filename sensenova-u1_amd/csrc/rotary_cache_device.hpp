@@ -46,10 +46,10 @@ __device__ __forceinline__ void store8(bf16_t* p, u32x4_t v, bool wide) {
 
 // Eight elements into a run: four neighbouring lanes hold it.  Returns the whole numbers, and the scale for the run.
 //
-// q = rint(x / d) without a division for each: with r = 1 / d to a step, t = x r is off by less than 2^-15, and q = rint(t) can
-// be wrong only if x / d is that near to a half.  It then is one: x has 8 significant bits and d at most 11, so |x / d - (n + 1/2)|, a multiple
-// of 2^-12 at least for numbers in reach, is 0 or more than that.  x - q d is exact, so 2 |x - q d| = d tells, and the even one is taken.
-// (Largest magnitudes are compared as whole numbers, which bf16 without its sign is ordered as, NaN above all.)
+// q = rint(x / d) without a division for each: with r = 1 / d to a step, t = x r is off by at most 2^-22 of itself, and t + (x - t d) r by 2^-44,
+// before it is rounded.  That gives the same whole number: x has 8 significant bits and d at most 11, so x / d is a half exactly, which the
+// second t then is too, or further from one than 2^-13.  (Checked over all x and d.)
+// Largest magnitudes are compared as whole numbers, which bf16 without its sign is ordered as, NaN above all.
 __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
     u16x2_t m = {0, 0};
@@ -73,17 +73,18 @@ __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
     u32x2_t out = {0u, 0u};
     if (d > 0.f) {
         constexpr float kWhole = 12582912.f;           // 1.5 x 2^23: added to a small number, it rounds it to a whole one in its low bits
-        const float r = __builtin_amdgcn_rcpf(d), most = 127.f * d;
+        const float r = __builtin_amdgcn_rcpf(d);
         float x[8];
         unpack8(p, x);
+        if (d >= 512.f) {                              // (only then are there larger ones than 127 d, but for d's own rounding)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_fmed3f(x[i], -127.f * 512.f, 127.f * 512.f);
+        }
         uint32_t q[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float within = __builtin_amdgcn_fmed3f(x[i], -most, most);
-            const float u = within * r + kWhole;
-            const float off = __builtin_fmaf(-(u - kWhole), d, within);
-            q[i] = __builtin_bit_cast(uint32_t, u);
-            if (2.f * __builtin_fabsf(off) == d && (q[i] & 1u)) q[i] += off > 0.f ? 1u : 0xFFFFFFFFu;
+            const float t = x[i] * r;
+            q[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(__builtin_fmaf(-t, d, x[i]), r, t) + kWhole);
         }
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -93,18 +94,28 @@ __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
     return out;
 }
 
+// Where a token's head lies in one half of the cache: its elements, and its first scale
+struct CachePlace {
+    uint8_t* row;
+    uint16_t* scale;
+};
+template <bool Q8>
+__device__ __forceinline__ CachePlace cache_place(void* pages, uint16_t* scales, const RotaryCacheArgs& a, int64_t slot, int head) {
+    const uint32_t page = (uint32_t)(slot >> a.page_shift), row = (uint32_t)slot & ((1u << a.page_shift) - 1);
+    const uint64_t at = (uint64_t)page * (uint32_t)a.kv_heads + (uint32_t)head;
+    return {static_cast<uint8_t*>(pages) + ((at << a.page_shift) + row) * (uint32_t)(a.dim * (Q8 ? 1 : 2)), scales + ((at * (uint32_t)(a.dim >> 5) << a.page_shift) + row)};
+}
+
 // One piece (eight elements from e on) of a token's head into the cache.
 template <bool Q8>
-__device__ __forceinline__ void cache_piece(void* pages, uint16_t* scales, const RotaryCacheArgs& a, int64_t slot, int head, int e, u32x4_t v) {
-    const int64_t page = slot >> a.page_shift, row = slot & ((1 << a.page_shift) - 1);
-    const int64_t at = page * a.kv_heads + head;
+__device__ __forceinline__ void cache_piece(const CachePlace& to, const RotaryCacheArgs& a, int e, u32x4_t v) {
     if constexpr (Q8) {
         uint16_t scale;
         const u32x2_t q = quantise8(v, scale);
-        *reinterpret_cast<u32x2_t*>(static_cast<int8_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e) = q;
-        if ((e & 31) == 0) scales[((at * (a.dim >> 5) + (e >> 5)) << a.page_shift) + row] = scale;
+        *reinterpret_cast<u32x2_t*>(to.row + e) = q;
+        if ((e & 31) == 0) to.scale[(uint32_t)(e >> 5) << a.page_shift] = scale;
     } else {
-        *reinterpret_cast<u32x4_t*>(static_cast<bf16_t*>(pages) + ((at << a.page_shift) + row) * a.dim + e) = v;
+        *reinterpret_cast<u32x4_t*>(to.row + 2 * e) = v;
     }
 }
 

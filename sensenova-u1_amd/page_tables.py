@@ -12,8 +12,8 @@ Nothing here synchronises or reads a length on the host, so a captured step repl
 """
 from __future__ import annotations
 
-import ctypes
 import functools
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -23,9 +23,8 @@ from .attention import _launch, _launch_with_workspace, _numbers, _same_device
 from .ops import SnGgufError
 
 
-class _TablesStruct(ctypes.Structure):
-    _fields_ = [("pages", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("held", ctypes.c_void_p), ("free", ctypes.c_void_p), ("cursor", ctypes.c_void_p),
-                ("sequences", ctypes.c_int64), ("width", ctypes.c_int64), ("ring", ctypes.c_int64), ("page_size", ctypes.c_int64)]
+# sngguf_page_tables as bytes: pages, lens, held, free, cursor, sequences, width, ring, page_size
+_TABLES = struct.Struct("5P4q")
 
 
 class PageStep(NamedTuple):
@@ -55,7 +54,7 @@ class PageTables:
     belong to another sequence (``fork``), None where none do.  ``PageTables.empty`` makes them; the constructor takes tensors that are there.  Calls
     change them in place, on the current stream."""
 
-    __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_struct", "_address", "_index")
+    __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_tables", "_index")
 
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor, page_size: int, held: Optional[torch.Tensor] = None) -> None:
         if not pages.is_cuda:
@@ -68,15 +67,16 @@ class PageTables:
         if width * page_size > (1 << 31) - 65536 or sequences >= 1 << 24:
             raise SnGgufError(f"PageTables: {sequences} sequences of {width} pages of {page_size} tokens are too many")
         for name, x, dtype, count in (("lens", lens, torch.int32, sequences), ("free", free, torch.int32, None), ("cursor", cursor, torch.int64, 2), ("held", held, torch.int32, sequences)):
-            if x is not None and (_numbers(x, dtype, count, "PageTables", name) is not x or not x.is_contiguous()):
+            if x is not None and _numbers(x, dtype, count, "PageTables", name) is not x:
                 raise SnGgufError(f"PageTables: {name} must be contiguous")
-        if free.shape[0] < 1 or free.shape[0] >= 1 << 31:
-            raise SnGgufError(f"PageTables: a ring of {free.shape[0]} pages")
+        ring = free.shape[0]
+        if not 1 <= ring < 1 << 31:
+            raise SnGgufError(f"PageTables: a ring of {ring} pages")
         self._index = pages.get_device()
         _same_device("PageTables", self._index, lens, free, cursor, held)
         self.pages, self.lens, self.free, self.cursor, self.held, self.page_size = pages, lens, free, cursor, held, int(page_size)
-        self._struct = _TablesStruct(pages.data_ptr(), lens.data_ptr(), ops._ptr(held), free.data_ptr(), cursor.data_ptr(), sequences, width, free.shape[0], self.page_size)
-        self._address = ctypes.addressof(self._struct)
+        self._tables = _TABLES.pack(pages.data_ptr(), lens.data_ptr(), 0 if held is None else held.data_ptr(), free.data_ptr(), cursor.data_ptr(), sequences, width, ring,
+                                    self.page_size)
 
     @classmethod
     def empty(cls, sequences: int, width: int, pages: int, page_size: int, device="cuda") -> "PageTables":
@@ -100,11 +100,13 @@ class PageTables:
         _same_device(what, self._index, new)
         if not 0 <= tokens < 1 << 31:
             raise SnGgufError(f"{what}: {tokens} rows")
-        positions, slots = new.new_empty((2, tokens), dtype=torch.int64).unbind()
-        ends, missing = new.new_empty(sequences + 1), new.new_empty(1)
-        lens, cursor = (self.lens, self.cursor) if inplace else (torch.empty_like(self.lens), torch.empty_like(self.cursor))
+        # (two allocations, each cut in one call)
+        positions, slots, cursor = self.cursor.new_empty(2 * tokens + 2).split((tokens, tokens, 2))
+        ends, lens, missing = new.new_empty(2 * sequences + 2).split((sequences + 1, sequences, 1))
+        if inplace:
+            lens, cursor = self.lens, self.cursor
         if sequences:
-            _launch_with_workspace(self._index, _workspace(sequences, tokens), "sngguf_page_append", self._address, new.data_ptr(), tokens, ends.data_ptr(), lens.data_ptr(),
+            _launch_with_workspace(self._index, _workspace(sequences, tokens), "sngguf_page_append", self._tables, new.data_ptr(), tokens, ends.data_ptr(), lens.data_ptr(),
                                    cursor.data_ptr(), positions.data_ptr(), slots.data_ptr(), missing.data_ptr())
         else:
             for x in (ends, missing, positions):
@@ -123,7 +125,7 @@ class PageTables:
         done = _numbers(done, done.dtype, self.pages.shape[0], what, "done")
         _same_device(what, self._index, done)
         if self.pages.shape[0]:
-            _launch(self._index, "sngguf_page_release", self._address, done.data_ptr())
+            _launch(self._index, "sngguf_page_release", self._tables, done.data_ptr())
 
     def fork(self, parent: torch.Tensor, common: torch.Tensor) -> None:
         """Sequence i with ``parent[i]`` >= 0 (int32 [sequences], -1: none) starts with that one's first ``common[i]`` tokens, rounded down to whole pages:
@@ -136,4 +138,4 @@ class PageTables:
         if self.held is None:
             raise SnGgufError(f"{what}: these tables have no record of pages held (`held`)")
         if sequences:
-            _launch(self._index, "sngguf_page_fork", self._address, parent.data_ptr(), common.data_ptr())
+            _launch(self._index, "sngguf_page_fork", self._tables, parent.data_ptr(), common.data_ptr())

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from sensenova_u1_amd import HeadNorm, RotaryAxes, ops
-from sensenova_u1_amd.attention import _AxesStruct, _CacheStruct, _NormStruct
+from sensenova_u1_amd.attention import _AXES, _NORM, _CacheStruct
 
 E_TYPE, E_SHAPE, E_NULL, E_ALIGN = -1, -2, -3, -4
 _BUF = ctypes.create_string_buffer(4096 + 64)
@@ -14,15 +14,15 @@ NAN, INF = float("nan"), float("inf")
 
 
 def _axes(turns=P, axis=P, pairs=16, magnitude=1.0, interleaved=0, parts=2, part=(16, 16, 0, 0)):
-    return _AxesStruct(turns, axis, pairs, magnitude, interleaved, parts, part)
+    return _AXES.pack(turns or 0, axis or 0, pairs, magnitude, interleaved, parts, *part)
 
 
 def _norm(weight=(P, P, None, None), elements=(32, 32, 0, 0), parts=2, kind=2, eps=1e-6):
-    return _NormStruct(weight, elements, parts, kind, eps)
+    return _NORM.pack(*(w or 0 for w in weight), *elements, parts, kind, eps)
 
 
 def _at(s):
-    return None if s is None else ctypes.addressof(s)
+    return s if s is None or isinstance(s, bytes) else ctypes.addressof(s)
 
 
 def _rotary(table=_axes(), positions=P, axes=3, tokens=3, dim=64, q_norm=_norm(), k_norm=_norm(), q=P, heads=2, out=P, k=P, k_heads=1, k_out=P):
@@ -80,3 +80,15 @@ def test_host_tensors():
 def test_settings(parts):
     with pytest.raises(ops.SnGgufError, match="are not known"):
         RotaryAxes.for_model(parts, device="cpu")
+
+
+def test_the_packed_structures_are_those_of_the_header():
+    class Axes(ctypes.Structure):
+        _fields_ = [("turns", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("pairs", ctypes.c_int64), ("magnitude", ctypes.c_double), ("interleaved", ctypes.c_int32),
+                    ("parts", ctypes.c_int32), ("part", ctypes.c_int32 * 4)]
+
+    class Norm(ctypes.Structure):
+        _fields_ = [("weight", ctypes.c_void_p * 4), ("elements", ctypes.c_int32 * 4), ("parts", ctypes.c_int32), ("weight_type", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+    assert bytes(Axes(5, 7, 3, 1.25, 1, 2, (4, 2, 0, 0))) == _AXES.pack(5, 7, 3, 1.25, 1, 2, 4, 2, 0, 0) and ctypes.sizeof(Axes) == _AXES.size
+    assert bytes(Norm((1, 2, 3, 4), (8, 16, 24, 32), 4, 2, 0.5)) == _NORM.pack(1, 2, 3, 4, 8, 16, 24, 32, 4, 2, 0.5) and ctypes.sizeof(Norm) == _NORM.size

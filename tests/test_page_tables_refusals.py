@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from sensenova_u1_amd import PageTables, ops
-from sensenova_u1_amd.page_tables import _TablesStruct
+from sensenova_u1_amd.page_tables import _TABLES
 
 E_SHAPE, E_NULL, E_ALIGN = -2, -3, -4
 _BUF = ctypes.create_string_buffer(4096 + 64)
@@ -13,15 +13,11 @@ P = (ctypes.addressof(_BUF) + 63) // 64 * 64
 
 
 def _tables(pages=P, lens=P, held=P, free=P, cursor=P, sequences=4, width=4, ring=8, page=16):
-    return _TablesStruct(pages, lens, held, free, cursor, sequences, width, ring, page)
-
-
-def _at(s):
-    return None if s is None else ctypes.addressof(s)
+    return _TABLES.pack(pages or 0, lens or 0, held or 0, free or 0, cursor or 0, sequences, width, ring, page)
 
 
 def _append(tables=_tables(), added=P, tokens=4, ends=P, lens=P, cursor=P, positions=P, slots=P, missing=P, ws=None, nbytes=0):
-    return ops.load_library().sngguf_page_append(_at(tables), added, tokens, ends, lens, cursor, positions, slots, missing, ws, nbytes, None)
+    return ops.load_library().sngguf_page_append(tables, added, tokens, ends, lens, cursor, positions, slots, missing, ws, nbytes, None)
 
 
 @pytest.mark.parametrize("bad,code", [(dict(sequences=-1), E_SHAPE), (dict(sequences=1 << 24), E_SHAPE), (dict(width=0), E_SHAPE), (dict(width=1 << 27), E_SHAPE), (dict(ring=0), E_SHAPE),
@@ -31,7 +27,7 @@ def _append(tables=_tables(), added=P, tokens=4, ends=P, lens=P, cursor=P, posit
 def test_tables(bad, code):
     lib = ops.load_library()
     t = _tables(**bad)
-    assert _append(tables=t) == code and lib.sngguf_page_release(_at(t), P, None) == code and lib.sngguf_page_fork(_at(t), P, P, None) == code
+    assert _append(tables=t) == code and lib.sngguf_page_release(t, P, None) == code and lib.sngguf_page_fork(t, P, P, None) == code
 
 
 def test_calls():
@@ -44,10 +40,10 @@ def test_calls():
         assert _append(**bad) == E_SHAPE, bad
     for bad in (dict(added=P + 2), dict(positions=P + 4), dict(cursor=P + 4), dict(tokens=8193, ws=P + 8, nbytes=64)):
         assert _append(**bad) == E_ALIGN, bad
-    assert lib.sngguf_page_release(_at(t), None, None) == E_NULL
-    assert lib.sngguf_page_fork(_at(t), None, P, None) == E_NULL and lib.sngguf_page_fork(_at(_tables(held=None)), P, P, None) == E_NULL
+    assert lib.sngguf_page_release(t, None, None) == E_NULL
+    assert lib.sngguf_page_fork(t, None, P, None) == E_NULL and lib.sngguf_page_fork(_tables(held=None), P, P, None) == E_NULL
     none = _tables(sequences=0, pages=None, lens=None, held=None, free=None, cursor=None)
-    assert _append(tables=none, added=None) == 0 and lib.sngguf_page_release(_at(none), None, None) == 0 and lib.sngguf_page_fork(_at(none), None, None, None) == 0
+    assert _append(tables=none, added=None) == 0 and lib.sngguf_page_release(none, None, None) == 0 and lib.sngguf_page_fork(none, None, None, None) == 0
     for sequences, tokens, nbytes in ((1024, 8192, 0), (1025, 1, 1025 * 16), (4, 8193, 64), (0, 9000, 0), (-1, 9000, 0), (4, -1, 0)):
         assert lib.sngguf_page_append_workspace_bytes(sequences, tokens) == nbytes
 
@@ -57,3 +53,10 @@ def test_host_tensors():
                  lambda: PageTables.empty(4, 4, 0, 16, device="cpu")):
         with pytest.raises(ops.SnGgufError):
             call()
+
+
+def test_the_packed_structure_is_that_of_the_header():
+    class Tables(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "lens", "held", "free", "cursor")] + [(n, ctypes.c_int64) for n in ("sequences", "width", "ring", "page_size")]
+
+    assert bytes(Tables(1, 2, 3, 4, 5, 6, 7, 8, 9)) == _TABLES.pack(1, 2, 3, 4, 5, 6, 7, 8, 9) and ctypes.sizeof(Tables) == _TABLES.size
