@@ -49,12 +49,13 @@ __device__ __forceinline__ float wave_total(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
-// Choices for the key tiles of a split: what fills all workgroups that run at once, to the sixteenth, as splits are whole; where
-// none of them does, what does in any case
-constexpr int kTries = 3;
-__device__ __forceinline__ float choice(float fill, int i) { return __builtin_ceilf(fill * (1.f + i / 16.f)); }
+// What a launch has to do, in a wavefront's entries
+struct LaunchSums {
+    float work;              // row tiles x key tiles
+    uint32_t row_tiles, entries;
+};
 
-// An entry's launch (-1: none), its row tiles and key tiles, and how many workgroups of a head it would take by each choice
+// An entry's launch (-1: none), its row tiles and key tiles
 struct Entry {
     int launch;
     uint32_t row_tiles, key_tiles;
@@ -76,16 +77,16 @@ __device__ __forceinline__ Entry entry_of(const SharedLaunch* launch, const Atte
 }  // namespace
 
 // W wavefronts.  ONE: there are no more entries than threads, and what a phase hands to the next stays in LDS and registers.
-// The kernel runs through once, on one compute unit, and its code comes from memory as it goes: what is done for each launch is a
-// loop that is not unrolled, and what is done once for each of them is done by as many lanes.
+// It runs through once, on one compute unit, so its time is that of one instruction after the other: sums that do not depend on each other are
+// side by side, and what is done once for each launch is done by as many lanes.
 template <int W, bool ONE>
 __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArgs s) {
     constexpr int T = 64 * W;
     touch_arguments(s);
     __shared__ AttentionEntry held[ONE ? T : 1];
     __shared__ SharedLaunch launch[kSharedLaunches];
-    __shared__ float work_of[W][kSharedLaunches];
-    __shared__ uint32_t tiles_of[W][kSharedLaunches], tried[W][kSharedLaunches][kTries], ups[W][kSharedLaunches];
+    __shared__ LaunchSums sums[W][kSharedLaunches];
+    __shared__ uint32_t ups[W][kSharedLaunches];
     const AttentionArgs& a = s.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t groups = s.group_count, sequences = a.sequences;
@@ -125,26 +126,22 @@ __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArg
         if (g + W < groups) group_0 = s.groups[g + W], group_1 = s.groups[g + W + 1], group_shared = s.shared[g + W];
         e0 = e0 < 0 ? 0 : e0 > sequences ? sequences : e0;
         e1 = e1 < e0 ? e0 : e1 > sequences ? sequences : e1;
-        // sequences without new tokens have no say
-        int32_t least = 0x7FFFFFFF, row = 0x7FFFFFFF, q0 = 0x7FFFFFFF, q1 = 0, row_again = 0x7FFFFFFF;
+        // sequences without new tokens have no say; the first and the last of the others tell which queries are the group's
+        int32_t least = 0x7FFFFFFF, row = -1, q0 = 0, q1 = 0, count = 0;
 #pragma unroll 1
-        for (int64_t i = (int64_t)e0 + lane; i < e1; i += 64) {
-            const AttentionEntry e = entries[groups + i];
-            if (e.lq == 0) continue;
-            least = min(least, e.lk - e.lq);
-            row_again = min(row_again, max(row, (int32_t)i));
-            row = min(row, (int32_t)i);
-            q0 = min(q0, e.q0);
-            q1 = max(q1, e.q0 + e.lq);
+        for (int64_t base = e0; base < e1; base += 64) {
+            AttentionEntry e = {};
+            if (base + lane < e1) e = entries[groups + base + lane];
+            const uint64_t live = __ballot(e.lq != 0);
+            if (!live) continue;
+            const int first = __builtin_ctzll(live), last = 63 - __builtin_clzll(live);
+            least = min(least, wave_min(e.lq != 0 ? e.lk - e.lq : 0x7FFFFFFF));
+            if (row < 0) row = (int32_t)base + first, q0 = __builtin_amdgcn_readlane(e.q0, first);
+            q1 = __builtin_amdgcn_readlane(e.q0 + e.lq, last);
+            count += __builtin_popcountll(live);
         }
-        // (two with queries: one lane has two, or two lanes have one)
-        const bool two = __any(row_again != 0x7FFFFFFF) || __builtin_popcountll(__ballot(row != 0x7FFFFFFF)) > 1;
-        least = wave_min(least);
-        row = wave_min(row);
-        q0 = wave_min(q0);
-        q1 = -wave_min(-q1);
         int32_t common = said < least ? said : least;
-        common = common < 0 || !two ? 0 : common / kSharedUnit * kSharedUnit;
+        common = common < 0 || count < 2 || q1 <= q0 ? 0 : common / kSharedUnit * kSharedUnit;
         if (lane == 0) entries[g] = {q0, common ? q1 - q0 : 0, 0, common, row, 1, -1, 0};
         if (common)
 #pragma unroll 1
@@ -155,7 +152,6 @@ __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArg
     }
     __syncthreads();
 
-    // f(entry, its launch and tiles) for this thread's entries, then the wavefront's sums of what f returns, by launch
     AttentionEntry e = {};
     Entry x = {-1, 0, 0};
     if (ONE && tid < all) {
@@ -165,71 +161,37 @@ __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArg
     // ---- all work of each launch, and how many key tiles of it a workgroup takes ---------------------------------------------
     {
         float work[kSharedLaunches] = {};
-        uint32_t tiles[kSharedLaunches] = {};
+        uint32_t tiles[kSharedLaunches] = {}, entries_of[kSharedLaunches] = {};
         auto add = [&](const Entry& y) {
 #pragma unroll
             for (int l = 0; l < kSharedLaunches; l++)
-                if (l == y.launch) work[l] += (float)y.row_tiles * (float)y.key_tiles, tiles[l] += y.row_tiles;
+                if (l == y.launch) work[l] += (float)y.row_tiles * (float)y.key_tiles, tiles[l] += y.row_tiles, entries_of[l]++;
         };
         if constexpr (ONE) add(x);
         else
             for (int64_t v = tid; v < all; v += T) add(entry_of(launch, entries[v], a.group, v < groups));
-#pragma unroll 1
+#pragma unroll
         for (int l = 0; l < kSharedLaunches; l++) {
-            const uint32_t n = l == 0 ? tiles[0] : l == 1 ? tiles[1] : tiles[2];
-            const float w = l == 0 ? work[0] : l == 1 ? work[1] : work[2];
-            const uint32_t count = wave_total(n);
-            const float sum = wave_total(w);
-            if (lane == 0) work_of[wave][l] = sum, tiles_of[wave][l] = count;
+            const uint32_t count = wave_total(tiles[l]), some = wave_total(entries_of[l]);
+            const float sum = wave_total(work[l]);
+            if (lane == 0) sums[wave][l] = {sum, count, some};
         }
     }
     __syncthreads();
-    // (lane l has launch l's) key tiles that fill all workgroups, and those with which n splits of whole numbers of tiles, which are at most one
-    // more than their fraction for each row tile, do in any case
-    float fill = kNever, safe = kNever;
-    if (lane < kSharedLaunches) {
+    // (lane l has launch l's.)  Workgroups of many rows are one or two a compute unit: as many as run at once.  Splits of c key tiles are at most one
+    // more than their fraction for each row tile, so c = work / (workgroups - row tiles) does in any case; a single entry's are as many as fit.
+    // Those of few rows are short, and some may follow others: the last split of a row tile is half as long as the others on average.
+    float chunk_of = kNever;
+    if (lane < kSharedLaunches && launch[lane].want) {
         float sum = 0.f, count = 0.f;
+        uint32_t some = 0;
 #pragma unroll
-        for (int w = 0; w < W; w++) sum += work_of[w][lane], count += (float)tiles_of[w][lane];
-        const float want = (float)launch[lane].want, least = (float)launch[lane].least;
-        const float all_work = sum * (float)a.kv_heads, left = want - count * (float)a.kv_heads;
-        if (want > 0.f) fill = fmaxf(all_work * __builtin_amdgcn_rcpf(want), least);
-        if (left > 0.f) safe = fmaxf(all_work * __builtin_amdgcn_rcpf(left) * 1.0001f, least);
-    }
-    uint32_t counts[kSharedLaunches][kTries] = {};
-    auto add_tries = [&](const Entry& y) {
-        const float base = __shfl(fill, y.launch < 0 ? 0 : y.launch);
-#pragma unroll
-        for (int i = 0; i < kTries; i++) {
-            const uint32_t n = y.row_tiles * (uint32_t)__builtin_ceilf((float)y.key_tiles * __builtin_amdgcn_rcpf(choice(base, i)) * 0.99999f);
-#pragma unroll
-            for (int l = 0; l < kSharedLaunches; l++)
-                if (l == y.launch) counts[l][i] += n;
-        }
-    };
-    if constexpr (ONE) add_tries(x);
-    else
-        for (int64_t base = 0; base < all; base += T) {
-            const int64_t v = base + tid;
-            add_tries(v < all ? entry_of(launch, entries[v], a.group, v < groups) : Entry{-1, 0, 0});
-        }
-#pragma unroll 1
-    for (int l = 0; l < kSharedLaunches; l++)
-#pragma unroll
-        for (int i = 0; i < kTries; i++) {
-            const uint32_t n = wave_total(l == 0 ? counts[0][i] : l == 1 ? counts[1][i] : counts[2][i]);
-            if (lane == 0) tried[wave][l][i] = n;
-        }
-    __syncthreads();
-    // (a lane for each launch and choice)
-    uint64_t hits;
-    {
-        const int l = lane / kTries, i = lane % kTries;
-        const bool listed = l < kSharedLaunches;
-        uint64_t n = 0;
-#pragma unroll
-        for (int w = 0; w < W; w++) n += listed ? tried[w][l][i] : 0;
-        hits = __ballot(listed && n * (uint32_t)a.kv_heads <= (uint64_t)(listed ? launch[l].want : 0));
+        for (int w = 0; w < W; w++) sum += sums[w][lane].work, count += (float)sums[w][lane].row_tiles, some += sums[w][lane].entries;
+        const float want = (float)launch[lane].want;
+        sum *= (float)a.kv_heads;
+        count *= (float)a.kv_heads;
+        float at_once = lane == 1 ? fmaxf(want - 0.5f * count, 0.5f * want) : some == 1 ? count * __builtin_floorf(want * __builtin_amdgcn_rcpf(count) * 1.00001f) : want - count;
+        if (at_once > 0.f) chunk_of = __builtin_ceilf(fmaxf(sum * __builtin_amdgcn_rcpf(at_once) * 0.99999f, (float)launch[lane].least));
     }
 
     // ---- which workgroups take an entry ------------------------------------------------------------------------------------
@@ -246,14 +208,12 @@ __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArg
             }
         }
         const int mine = x.launch < 0 ? 0 : x.launch;
-        const uint32_t hit = (uint32_t)(hits >> (kTries * mine)) & ((1u << kTries) - 1);
-        const float by_choice = choice(__shfl(fill, mine), __builtin_ctz(hit | 1u << kTries)), in_any_case = __builtin_ceilf(__shfl(safe, mine));
-        const float c = hit ? by_choice : in_any_case;
+        const float c = __shfl(chunk_of, mine);
         const uint32_t chunk = c < kNever ? (uint32_t)c : 0x7FFFFFFFu;
         const uint32_t splits = x.key_tiles > chunk ? (x.key_tiles + chunk - 1) / chunk : 1;
         const uint32_t slots = x.row_tiles * splits;             // (no launch: none)
         uint32_t up = 0;
-#pragma unroll 1
+#pragma unroll
         for (int l = 0; l < kSharedLaunches; l++) {
             const uint32_t sum = wave_scan(l == x.launch ? slots : 0);
             if (l == x.launch) up = sum;
@@ -340,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedA
         int64_t step;
     };
     auto part_of = [&](const AttentionEntry& x) -> Part {
-        if (x.first < 0) return {nullptr, nullptr, 0, 0};
+        if (x.first < 0 || token - (uint32_t)x.q0 >= (uint32_t)x.lq) return {nullptr, nullptr, 0, 0};
         const int l = x.flags >> 8;
         const SharedLaunch& y = l == 0 ? s.launch[0] : l == 1 ? s.launch[1] : s.launch[2];
         const uint32_t row = (token - (uint32_t)x.q0) * (uint32_t)a.group + place, tile = row >> y.row_shift;
