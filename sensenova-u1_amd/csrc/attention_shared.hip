@@ -407,7 +407,7 @@ int launch_shared_plan(const SharedArgs& s, hipStream_t stream) {
 // dim: of the kernels, 64, 128 or 256
 int launch_shared_join(const SharedArgs& s, int dim, hipStream_t stream) {
     const int64_t queries = s.a.tokens_q * s.a.heads;
-    const bool wide = queries <= 1024;
+    const bool wide = queries <= 4096;
     const dim3 grid((unsigned)(wide ? queries : (queries + 3) / 4));
 #define SNGGUF_GO(D)                                                                                                    \
     if (dim == D) {                                                                                                     \

@@ -25,7 +25,7 @@ struct PageArgs {
     const int32_t *parent, *common;
 };
 
-constexpr int64_t kOneLaunchSequences = 1024, kOneLaunchTokens = 8192;
+constexpr int64_t kOneLaunchSequences = 1024, kOneLaunchTokens = 4096;
 
 int launch_page_append(const PageArgs& a, bool one, hipStream_t stream);
 int launch_page_release(const PageArgs& a, hipStream_t stream);

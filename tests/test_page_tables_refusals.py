@@ -34,17 +34,17 @@ def test_calls():
     lib = ops.load_library()
     t = _tables()
     assert _append(tables=None) == E_NULL and lib.sngguf_page_release(None, P, None) == E_NULL and lib.sngguf_page_fork(None, P, P, None) == E_NULL
-    for bad in (dict(added=None), dict(ends=None), dict(lens=None), dict(cursor=None), dict(positions=None), dict(slots=None), dict(missing=None), dict(tokens=8193)):
+    for bad in (dict(added=None), dict(ends=None), dict(lens=None), dict(cursor=None), dict(positions=None), dict(slots=None), dict(missing=None), dict(tokens=4097)):
         assert _append(**bad) == E_NULL, bad
-    for bad in (dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=8193, ws=P, nbytes=63)):
+    for bad in (dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=4097, ws=P, nbytes=63)):
         assert _append(**bad) == E_SHAPE, bad
-    for bad in (dict(added=P + 2), dict(positions=P + 4), dict(cursor=P + 4), dict(tokens=8193, ws=P + 8, nbytes=64)):
+    for bad in (dict(added=P + 2), dict(positions=P + 4), dict(cursor=P + 4), dict(tokens=4097, ws=P + 8, nbytes=64)):
         assert _append(**bad) == E_ALIGN, bad
     assert lib.sngguf_page_release(t, None, None) == E_NULL
     assert lib.sngguf_page_fork(t, None, P, None) == E_NULL and lib.sngguf_page_fork(_tables(held=None), P, P, None) == E_NULL
     none = _tables(sequences=0, pages=None, lens=None, held=None, free=None, cursor=None)
     assert _append(tables=none, added=None) == 0 and lib.sngguf_page_release(none, None, None) == 0 and lib.sngguf_page_fork(none, None, None, None) == 0
-    for sequences, tokens, nbytes in ((1024, 8192, 0), (1025, 1, 1025 * 16), (4, 8193, 64), (0, 9000, 0), (-1, 9000, 0), (4, -1, 0)):
+    for sequences, tokens, nbytes in ((1024, 4096, 0), (1025, 1, 1025 * 16), (4, 4097, 64), (0, 9000, 0), (-1, 9000, 0), (4, -1, 0)):
         assert lib.sngguf_page_append_workspace_bytes(sequences, tokens) == nbytes
 
 
