@@ -10,9 +10,13 @@
 //
 //  * The plan: lengths lie on the device, so a kernel of one workgroup finds how many tokens each group has in common (no more than
 //    its sequences have in front of their new ones, in whole key tiles: what is left over is read as each one's own), deals the work
-//    of each launch over its workgroups, and writes down which workgroup does what.
+//    of each launch over its workgroups, and writes down for each of these what it does.  4.8 us, the time of its 900 instructions one after the
+//    other.
 //  * The join: half a wavefront lies along a query's elements and takes some partial results at a time.  Weights are scaled by 2^-16, so that
 //    no sum leaves fp32 whose average does not (there are fewer than 2^16 splits).
+// Measured, 32 query and 8 key / value heads of 128, passes back to back: 64 single tokens over 16384 common keys and 1 to 400 of their own in bf16
+// 62 us (sngguf_paged_attention 447): plan, common keys 28 (17 GFLOP in 256-row workgroups of nine key tiles, half of whose time is their start and
+// 33 MB of partial results), own keys 14, join 11; 32 over 8192 and up to 900 in 8 bits 43.5 (73): plan, one launch of 30, join 6.
 #include "attention_shared.hpp"
 
 namespace sngguf {

@@ -8,10 +8,14 @@
 // bits and reduced to the nearest whole turn there; everything else is fp32, rounded to bf16 once (norm, weight and rotation
 // by themselves would round three times, and be off by 1.7 times as much).
 //
-// Bound by memory: an element is two bytes in and two out, for some ten operations.  Neighbouring lanes have a head between them, its
-// sums of squares are added up across them in the vector unit, and all of it is read before any of it is written, so a call may work
-// in place.  A lane keeps to the same elements of all heads, so weights, cosines and sines are fetched once for a token.
-//  * head_pairs_kernel, pairs half a part apart in parts of multiples of 16 elements: a lane has eight pairs, both of their elements.
+// Bound by memory: an element is two bytes in and two out, for some ten operations; and next by its instructions, which is why heads are divided
+// as they are.  Neighbouring lanes have a head between them, its sums of squares are added up across them in the vector unit, and all of it is
+// read before any of it is written, so a call may work in place.  A lane keeps to the same elements of all heads, so weights,
+// cosines and sines are fetched once for a token.
+//  * head_pairs_kernel, pairs half a part apart in parts of multiples of 16 elements: a lane has eight pairs, both of their elements, and a
+//    workgroup up to four tokens.  4096 tokens of 40 heads of 128: 15.5 us (84 MB, 5.4 TB/s), with two norms a head 17.5; as eight elements a lane,
+//    with the others from the lane that has them, and one token a workgroup 20.9 and 33.4.  5003 tokens of 32 query and 8 + 8 heads, two
+//    norms, keys and values written in 8 bits: 29.8 us (113 MB, 3.8 TB/s).  One token: 3 us, all latency.
 //  * head_rotary_kernel, neighbouring pairs, any parts or rows: a lane has eight elements; those that they are turned with, where they are not among
 //    the eight, are read beside them.  Shapes for which the other is no form, so it is kept simple.
 #include <type_traits>
@@ -305,12 +309,15 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(HeadRotaryArgs a)
 // Rows start at 16-byte boundaries.
 __device__ __forceinline__ u32x4_t piece_at(const bf16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 
-template <bool CACHE, int NORM>
+// SHIFT: 2^SHIFT lanes have a head.  Known for normed heads of 80 to 128 elements, whose sums then need no choices (4096 tokens 17.5 against
+// 18.2 us, one token 5.2 against 5.8 with its graph node; written in 8 bits level); -1: a.lane_shift says.
+template <bool CACHE, int NORM, int SHIFT>
 __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) {
     extern __shared__ __attribute__((aligned(16))) float2 cs_all[];    // [token][pair], then (CACHE) [team][dim] bf16
     touch_arguments(a);
-    const int tid = threadIdx.x, lanes = 1 << a.lane_shift, teams = kThreads >> a.lane_shift;
-    const int team = tid >> a.lane_shift, unit = tid & (lanes - 1);
+    const int lane_shift = SHIFT >= 0 ? SHIFT : a.lane_shift;
+    const int tid = threadIdx.x, lanes = 1 << lane_shift, teams = kThreads >> lane_shift;
+    const int team = tid >> lane_shift, unit = tid & (lanes - 1);
     const bool there = 16 * unit < a.dim;
     const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_block;
     const int count = (int)(a.tokens - t0 < a.tokens_per_block ? a.tokens - t0 : a.tokens_per_block);
@@ -426,13 +433,17 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
             float sa = 0.f, sb = 0.f, ra = 0.f, rb = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) sa = __builtin_fmaf(u[j], u[j], sa), sb = __builtin_fmaf(v[j], v[j], sb);
-#pragma unroll 1
-            for (int p = 0; p < n.parts; p++) {
+            auto part = [&](int p) {
                 const float mine = (w.part_a == p ? sa : 0.f) + (w.part_b == p ? sb : 0.f);
-                const float r = rstd_of(lanes_sum(mine, a.lane_shift), norm_one_over(n, p), n.eps);
+                const float r = rstd_of(lanes_sum(mine, lane_shift), norm_one_over(n, p), n.eps);
                 if (w.part_a == p) ra = r;
                 if (w.part_b == p) rb = r;
-            }
+            };
+            // (one or two parts are the usual ones: side by side)
+            part(0);
+            part(1);
+#pragma unroll 1
+            for (int p = 2; p < n.parts; p++) part(p);
 #pragma unroll
             for (int j = 0; j < 8; j++) u[j] = u[j] * ra * weight_of(w, 0, j), v[j] = v[j] * rb * weight_of(w, 1, j);
             if (!rotates) return {pack8(u), pack8(v)};
@@ -545,9 +556,10 @@ int launch_head_rotary(const HeadRotaryArgs& a0, int cache, hipStream_t stream) 
     const int kind = !norm ? kNormNone : one.bf16 ? kNormHalf : kNormWide;
 #define SNGGUF_GO(C)                                                                                                    \
     if ((cache != 0) == C) {                                                                                            \
-        if (pairs && kind == kNormNone) head_pairs_kernel<C, kNormNone><<<grid, kThreads, lds, stream>>>(a);            \
-        else if (pairs && kind == kNormHalf) head_pairs_kernel<C, kNormHalf><<<grid, kThreads, lds, stream>>>(a);       \
-        else if (pairs) head_pairs_kernel<C, kNormWide><<<grid, kThreads, lds, stream>>>(a);                            \
+        if (pairs && kind == kNormNone) head_pairs_kernel<C, kNormNone, -1><<<grid, kThreads, lds, stream>>>(a);        \
+        else if (pairs && kind == kNormHalf && a.lane_shift == 3) head_pairs_kernel<C, kNormHalf, 3><<<grid, kThreads, lds, stream>>>(a); \
+        else if (pairs && kind == kNormHalf) head_pairs_kernel<C, kNormHalf, -1><<<grid, kThreads, lds, stream>>>(a);   \
+        else if (pairs) head_pairs_kernel<C, kNormWide, -1><<<grid, kThreads, lds, stream>>>(a);                        \
         else if (a.interleaved && norm) head_rotary_kernel<kNeighbours, C, true><<<grid, kThreads, lds, stream>>>(a);   \
         else if (a.interleaved) head_rotary_kernel<kNeighbours, C, false><<<grid, kThreads, lds, stream>>>(a);          \
         else if (norm) head_rotary_kernel<kAnyHalves, C, true><<<grid, kThreads, lds, stream>>>(a);                     \

@@ -12,7 +12,7 @@
 //
 // All of it is bound by memory.  A workgroup takes a few tokens: its threads first make one (cosine, sine) pair each, in LDS,
 // then work through the tokens' heads in pieces of 16 bytes.  8192 tokens of 40 heads of 128: 35.7 us, 4.7 TB/s; 5003 tokens of 32 query
-// and 8 + 8 heads, keys and values written in 8 bits: 27 us, 4.2 TB/s; 40000 tokens read back: 53 us, 4.7 TB/s (nontemporal stores: 58).
+// and 8 + 8 heads, keys and values written in 8 bits: 23.4 us, 4.8 TB/s; 40000 tokens read back: 53 us, 4.7 TB/s (nontemporal stores: 58).
 #include "rotary_cache_device.hpp"
 
 namespace sngguf {
