@@ -540,11 +540,11 @@ int launch_head_rotary(const HeadRotaryArgs& a0, int cache, hipStream_t stream) 
     if (pairs && cache && a.lane_shift < 2) a.lane_shift = 2;        // (four lanes for a run of the 8-bit cache)
     const int teams = kThreads >> a.lane_shift;
     const int64_t heads = (int64_t)a.q_heads + (cache ? 2 * a.kv_heads : a.k_heads);
-    // as many tokens as give each team a head; where there are tokens enough for four workgroups a compute unit, up to four times as many, as
-    // finding its elements and weights costs a workgroup as much as two heads do (4096 tokens of 40 normed heads, 1 / 2 / 4 / 8 tokens a workgroup:
-    // 31.5 / 25.0 / 20.3 / 22.4 us)
+    // as many tokens as give each team a head; where there are tokens enough for two workgroups a compute unit, up to four times as many, as
+    // finding its elements and weights costs a workgroup as much as two heads do (40 normed heads, 1 / 2 / 4 tokens a workgroup: 4096 tokens
+    // 27.8 / 21.5 / 17.3 us, 3000 - / 18.0 / 14.8, 2048 16.8 / 13.1 / 12.6; eight: 4096 22.4, 33000 137.8 against 133.7)
     const int64_t fill = heads * 8 <= teams ? 8 : heads < teams ? teams / heads : 1;
-    const int64_t spare = a.tokens / (1024 * fill);
+    const int64_t spare = a.tokens / (512 * fill);
     const int64_t tokens = fill * (spare < 1 ? 1 : spare > 4 ? 4 : spare), room = 2048 / a.pairs;       // (16 KB of cosines and sines)
     a.tokens_per_block = (int32_t)(tokens < room ? tokens : room);
     const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
