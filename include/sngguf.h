@@ -431,7 +431,7 @@ typedef struct sngguf_rotary_axes {
 } sngguf_rotary_axes;
 
 /* Norm of single heads: `parts` parts (1 .. 4) of elements[] elements each (multiples of 8, together a whole head), y = weight x /
- * sqrt(mean of the part's x^2 + eps) in fp32.  weight[]: device, [elements] of one type, 16-byte aligned: bf16 (weight_type 2) or
+ * sqrt(mean of the part's x^2 + eps) in fp32 (a part whose sum of squares is beyond it becomes zeros).  weight[]: device, [elements] of one type, 16-byte aligned: bf16 (weight_type 2) or
  * fp32 (weight_type 0). */
 typedef struct sngguf_head_norm {
     const void* weight[4];
@@ -494,7 +494,8 @@ int sngguf_cache_read(const sngguf_kv_cache* cache, const int64_t* slots, int64_
  * The tables of many sequences over a paged cache, all in device memory: pages [sequences][width], the pages of each sequence in order;
  * lens [sequences], its tokens; held [sequences] (NULL: none), leading pages of a row that belong to another sequence; free
  * [ring], page numbers in a ring of which those from cursor[0] (taken so far) up to cursor[1] (given so far) are there, the c-th
- * at place c mod ring.  page_size as in a cache; width * page_size below 2^31 - 65536, sequences below 2^24.
+ * at place c mod ring.  page_size as in a cache; width * page_size below 2^31 - 65536, sequences below 2^24.  No two of these share memory, and what
+ * a call only reads shares none with what it writes.
  */
 typedef struct sngguf_page_tables {
     int32_t *pages, *lens, *held, *free;

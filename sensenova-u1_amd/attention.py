@@ -258,6 +258,9 @@ class RotaryAxes:
         self.axis, self.parts, self.interleaved, self.magnitude = axis, parts, bool(interleaved), float(magnitude)
         self._axes = _AXES.pack(turns.data_ptr(), axis.data_ptr(), pairs, magnitude, self.interleaved, len(parts), *parts, *(0, 0, 0)[len(parts) - 1:])
 
+    def __reduce__(self):               # (a copy has the addresses of its own tensors)
+        return RotaryAxes, (self.turns, self.axis, self.parts, self.interleaved, self.magnitude)
+
     @classmethod
     def for_model(cls, parts: Sequence[tuple], interleaved: bool = False, device="cuda") -> "RotaryAxes":
         """The table of a head whose parts turn by an axis each: ``parts`` holds (elements, axis, base) of each part, with wavelengths
@@ -275,7 +278,8 @@ class HeadNorm:
 
     ``weights``: one to four tensors [elements] on the device, bf16 or fp32, for the consecutive parts of a head that are normed each by
     itself (one: the whole head); their elements, multiples of 8, are a head's together.  Their memory is read at every call: a change in place counts, a tensor
-    put in a module's place does not."""
+    put in a module's place does not.  (Weights that do not start at a 16-byte boundary, or are not neighbours, are copied, and stay as they are now.)  A part
+    whose squares add up to more than 32 bits hold, from magnitudes of 1.8e19 on, becomes zeros."""
 
     __slots__ = ("weights", "eps", "dim", "_norm", "_index")
 
@@ -304,6 +308,9 @@ class HeadNorm:
         self.weights, self.eps, self.dim, self._index = tuple(kept), float(eps), sum(sizes), index
         rest = (0, 0, 0)[len(at) - 1:]
         self._norm = _NORM.pack(*at, *rest, *sizes, *rest, len(at), 2 if kind is _BF16 else 0, eps)
+
+    def __reduce__(self):               # (a copy has the addresses of its own tensors)
+        return functools.partial(HeadNorm, eps=self.eps), self.weights
 
 
 def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tensor, table, q_norm: Optional[HeadNorm], k_norm: Optional[HeadNorm]):

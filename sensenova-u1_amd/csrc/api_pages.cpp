@@ -15,6 +15,28 @@ constexpr int64_t kMostSequences = (int64_t)1 << 24;  // a workgroup of 256 thre
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+struct Bytes {
+    const void* at;
+    int64_t count;
+};
+// Whether `x` shares no byte with any of them
+template <int N>
+bool apart(const Bytes& x, const Bytes (&others)[N]) {
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at);
+    for (const Bytes& y : others) {
+        const uintptr_t y0 = reinterpret_cast<uintptr_t>(y.at);
+        if (x.at && y.at && x0 < y0 + (uintptr_t)y.count && y0 < x0 + (uintptr_t)x.count) return false;
+    }
+    return true;
+}
+
+// Whether the tables' arrays share no byte (a call writes some while others of its threads still read)
+bool tables_apart(const PageArgs& a) {
+    const Bytes pages = {a.pages, a.sequences * a.width * 4}, lens = {a.lens, a.sequences * 4}, held = {a.held, a.sequences * 4}, free = {a.free, (int64_t)a.ring * 4}, cursor = {a.cursor, 16};
+    const Bytes behind_pages[] = {lens, held, free, cursor}, behind_lens[] = {held, free, cursor}, behind_held[] = {free, cursor}, behind_free[] = {cursor};
+    return apart(pages, behind_pages) && apart(lens, behind_lens) && apart(held, behind_held) && apart(free, behind_free);
+}
+
 int check_tables(const sngguf_page_tables* t, PageArgs& a) {
     if (!t) return SNGGUF_E_NULLPTR;
     if (t->sequences < 0 || t->sequences >= kMostSequences || t->width < 1 || t->ring < 1 || t->ring >= kMost || t->page_size < 16 || t->page_size > 4096 ||
@@ -59,6 +81,9 @@ int sngguf_page_append(const sngguf_page_tables* tables, const int32_t* added, i
     if (!aligned(added, 4) || !aligned(ends, 4) || !aligned(lens_out, 4) || !aligned(cursor_out, 8) || !aligned(positions, 8) || !aligned(slots, 8) ||
         !aligned(missing, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
+    const Bytes written[] = {{a.pages, a.sequences * a.width * 4}, {lens_out, a.sequences * 4},  {cursor_out, 16},   {ends, (a.sequences + 1) * 4},
+                             {missing, 4},                          {positions, tokens * 8},      {slots, tokens * 8}};
+    if (!tables_apart(a) || !apart({added, a.sequences * 4}, written)) return SNGGUF_E_BADSHAPE;
     a.added = added;
     a.tokens = tokens;
     a.ends = ends;
@@ -76,6 +101,8 @@ int sngguf_page_release(const sngguf_page_tables* tables, const uint8_t* done, v
     const int rc = check_tables(tables, a);
     if (rc != SNGGUF_OK || a.sequences == 0) return rc;
     if (!done) return SNGGUF_E_NULLPTR;
+    const Bytes written[] = {{a.lens, a.sequences * 4}, {a.held, a.sequences * 4}, {a.free, (int64_t)a.ring * 4}, {a.cursor, 16}};
+    if (!tables_apart(a) || !apart({done, a.sequences}, written)) return SNGGUF_E_BADSHAPE;
     a.done = done;
     return sngguf::launch_page_release(a, static_cast<hipStream_t>(stream));
 }
@@ -86,6 +113,8 @@ int sngguf_page_fork(const sngguf_page_tables* tables, const int32_t* parent, co
     if (rc != SNGGUF_OK || a.sequences == 0) return rc;
     if (!parent || !common || !a.held) return SNGGUF_E_NULLPTR;
     if (!aligned(parent, 4) || !aligned(common, 4)) return SNGGUF_E_ALIGN;
+    const Bytes written[] = {{a.pages, a.sequences * a.width * 4}, {a.lens, a.sequences * 4}, {a.held, a.sequences * 4}};
+    if (!tables_apart(a) || !apart({parent, a.sequences * 4}, written) || !apart({common, a.sequences * 4}, written)) return SNGGUF_E_BADSHAPE;
     a.parent = parent;
     a.common = common;
     return sngguf::launch_page_fork(a, static_cast<hipStream_t>(stream));

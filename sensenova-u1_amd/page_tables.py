@@ -51,7 +51,7 @@ class PageTables:
     ``pages``: int32 [sequences][width], the pages of each sequence in order.  ``lens``: int32 [sequences].  ``free``: int32 [ring], page
     numbers in a ring of at least as many places as there are pages; ``cursor``: int64 [2], how many have been taken from it and given to
     it so far (the c-th lies at place c mod ring, so those from ``cursor[0]`` up to ``cursor[1]`` are there).  ``held``: int32 [sequences], leading pages of a row that
-    belong to another sequence (``fork``), None where none do.  ``PageTables.empty`` makes them; the constructor takes tensors that are there.  Calls
+    belong to another sequence (``fork``), None where none do.  No two of them share memory, nor with what a call is given.  ``PageTables.empty`` makes them; the constructor takes tensors that are there.  Calls
     change them in place, on the current stream."""
 
     __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_tables", "_index")
@@ -77,6 +77,9 @@ class PageTables:
         self.pages, self.lens, self.free, self.cursor, self.held, self.page_size = pages, lens, free, cursor, held, int(page_size)
         self._tables = _TABLES.pack(pages.data_ptr(), lens.data_ptr(), 0 if held is None else held.data_ptr(), free.data_ptr(), cursor.data_ptr(), sequences, width, ring,
                                     self.page_size)
+
+    def __reduce__(self):               # (a copy has the addresses of its own tensors)
+        return PageTables, (self.pages, self.lens, self.free, self.cursor, self.page_size, self.held)
 
     @classmethod
     def empty(cls, sequences: int, width: int, pages: int, page_size: int, device="cuda") -> "PageTables":

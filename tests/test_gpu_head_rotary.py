@@ -1,5 +1,7 @@
 """Norms of single heads and rotation by several positions, to tensors and into the cache, against 64 bits."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -224,6 +226,40 @@ def test_into_the_cache(dev, quant, tokens, q_heads, kv_heads, dim, parts, norm,
     copy = qkv.clone()
     cache.write_rotary(copy[:, :q_heads], copy[:, q_heads:q_heads + kv_heads], copy[:, q_heads + kv_heads:], positions, table, slots, inplace=True, **norms)
     assert torch.equal(copy[:, :q_heads], got) and torch.equal(copy[:, q_heads:], qkv[:, q_heads:])
+
+
+@pytest.mark.parametrize("tokens", [1023, 1024, 2049, 5003])
+@pytest.mark.parametrize("q_heads,k_heads,dim,parts,norm", [(6, 2, 64, (32, 16, 16), (32, 32)), (40, 0, 32, (32,), ()), (2, 1, 80, (36,), (80,))])
+def test_many_tokens(dev, tokens, q_heads, k_heads, dim, parts, norm):
+    """Several tokens a workgroup, the last one's fewer."""
+    gen = torch.Generator().manual_seed(tokens)
+    q, k = _values(gen, tokens, q_heads, dim), _values(gen, tokens, k_heads, dim)
+    turns, axis = _table(gen, parts, 2)
+    positions, weights = torch.randint(0, 5000, (2, tokens), generator=gen), _weights(gen, norm)
+    table = RotaryAxes(turns.to(dev), axis.to(dev), parts)
+    norms = dict.fromkeys(("q_norm", "k_norm"), HeadNorm(*(w.to(dev) for w in weights))) if norm else {}
+    q2, k2 = rotary(q.to(dev), k.to(dev), positions.to(dev), table, **norms)
+    for got, x in ((q2, q), (k2, k)):
+        if x.numel():
+            _close(got, *ho.head(x, positions, turns, axis, parts, weights=weights, eps=1e-6))
+    if k_heads and dim % 32 == 0:
+        cache, slots = PagedKVCache.empty(-(-tokens // 64), k_heads, 64, dim, ops.BF16, dev), torch.randperm(tokens, generator=gen).to(dev)
+        assert torch.equal(cache.write_rotary(q.to(dev), k.to(dev), k.to(dev), positions.to(dev), table, slots, **norms), q2)
+        assert torch.equal(cache.read(slots)[0], k2) and torch.equal(cache.read(slots)[1].cpu(), k)
+
+
+def test_copies_have_tensors_of_their_own(dev):
+    gen = torch.Generator().manual_seed(9)
+    q, at = _values(gen, 3, 2, 64).to(dev), torch.randint(0, 99, (2, 3), generator=gen).to(dev)
+    axes, norm = RotaryAxes.for_model([(32, 0, 1e4), (32, 1, 1e4)], device=dev), HeadNorm(*(w.to(dev) for w in _weights(gen, (32, 32))), eps=1e-4)
+    want = rotary(q, None, at, axes, q_norm=norm)[0]
+    copies = [(copy.copy(axes), copy.copy(norm)), copy.deepcopy((axes, norm)), pickle.loads(pickle.dumps((axes, norm)))]
+    assert copies[0][1].weights[0] is norm.weights[0]
+    for t in (axes.turns, axes.axis, *norm.weights):
+        t.zero_()
+    assert not torch.equal(rotary(q, None, at, copies[0][0], q_norm=copies[0][1])[0], want)
+    for a, n in copies[1:]:
+        assert torch.equal(rotary(q, None, at, a, q_norm=n)[0], want)
 
 
 def test_captured_and_on_another_stream(dev):

@@ -1,4 +1,6 @@
 """The tables of many sequences against a program on the host: every number is equal."""
+import copy
+import pickle
 import random
 
 import pytest
@@ -187,3 +189,32 @@ def test_what_is_refused(dev):
                  lambda: tables.release(torch.zeros(3, dtype=torch.bool, device=dev)), lambda: tables.fork(new, new[:2]), lambda: PageTables(**good).fork(new, new)):
         with pytest.raises(ops.SnGgufError):
             call()
+
+
+def test_copies_have_tensors_of_their_own(dev):
+    tables, oracle = PageTables.empty(3, 4, 12, 16, dev), Tables(3, 4, 12, 16)
+    _step(tables, oracle, [20, 0, 3], 23, dev)
+    for other in (copy.deepcopy(tables), pickle.loads(pickle.dumps(tables))):
+        before = [t.clone() for t in (tables.pages, tables.lens, tables.cursor, tables.free)]
+        their = copy.deepcopy(oracle)
+        _step(other, their, [1, 40, 13], 54, dev)
+        other.release(torch.tensor([True, False, False], device=dev))
+        their.release([True, False, False])
+        _same(other, their)
+        assert all(torch.equal(a, b) for a, b in zip(before, (tables.pages, tables.lens, tables.cursor, tables.free)))
+    same = copy.copy(tables)
+    assert same.lens is tables.lens
+    _step(same, oracle, [5, 5, 5], 15, dev)
+    _same(tables, oracle)
+
+
+def test_numbers_in_the_tables_own_memory_are_refused(dev):
+    tables = PageTables.empty(4, 4, 8, 16, dev)
+    room = torch.zeros(5, dtype=torch.int32, device=dev)
+    shifted = PageTables(tables.pages, room[1:], tables.free, tables.cursor, 16, held=tables.held)
+    done = tables.lens.view(torch.uint8)[:4]
+    for call in (lambda: tables.append(tables.lens, 4), lambda: shifted.append(room[:4], 4), lambda: tables.append(tables.pages[0], 4), lambda: tables.release(done),
+                 lambda: tables.fork(tables.held, room[:4]), lambda: PageTables(tables.pages, tables.pages[0], tables.free, tables.cursor, 16).append(room[:4], 4)):
+        with pytest.raises(ops.SnGgufError):
+            call()
+    assert tables.append(tables.lens, 4, inplace=False).missing.item() == 0          # (nothing of it is written)

@@ -48,6 +48,34 @@ def test_calls():
         assert lib.sngguf_page_append_workspace_bytes(sequences, tokens) == nbytes
 
 
+def test_memory_that_is_shared():
+    lib = ops.load_library()
+    # arrays 256 bytes apart; each moved into another in turn (a ring of 8, 4 sequences of 4 pages, 4 rows)
+    at = {name: P + 256 * i for i, name in enumerate(("pages", "lens", "held", "free", "cursor", "added", "ends", "positions", "slots", "missing"))}
+    size = dict(pages=64, lens=16, held=16, free=32, cursor=16, added=16, ends=20, positions=32, slots=32, missing=4)
+
+    def tables(at):
+        return _tables(**{n: at[n] for n in ("pages", "lens", "held", "free", "cursor")})
+
+    def append(at):
+        return _append(tables(at), **{n: at[n] for n in ("added", "ends", "lens", "cursor", "positions", "slots", "missing")})
+
+    arrays = ("pages", "lens", "held", "free", "cursor")
+    for x in arrays:
+        for y in arrays:
+            if x != y:
+                bad = {**at, x: at[y] + size[y] // 8 * 8 - 8}
+                assert append(bad) == E_SHAPE and lib.sngguf_page_release(tables(bad), at["added"], None) == E_SHAPE, (x, y)
+                assert lib.sngguf_page_fork(tables(bad), at["added"], at["ends"], None) == E_SHAPE, (x, y)
+    for y in ("pages", "lens", "cursor", "ends", "positions", "slots", "missing"):
+        assert append({**at, "added": at[y] + size[y] - 4}) == E_SHAPE, y
+    for y in ("lens", "held", "free", "cursor"):
+        assert lib.sngguf_page_release(tables(at), at[y] + size[y] - 1, None) == E_SHAPE, y
+    for y in ("pages", "lens", "held"):
+        for of in ((at[y] + size[y] - 4, at["ends"]), (at["ends"], at[y] - 12)):
+            assert lib.sngguf_page_fork(tables(at), *of, None) == E_SHAPE, y
+
+
 def test_host_tensors():
     for call in (lambda: PageTables.empty(4, 4, 8, 16, device="cpu"), lambda: PageTables.empty(-1, 4, 8, 16, device="cpu"), lambda: PageTables.empty(4, 0, 8, 16, device="cpu"),
                  lambda: PageTables.empty(4, 4, 0, 16, device="cpu")):
