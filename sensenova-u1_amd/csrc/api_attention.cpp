@@ -145,7 +145,9 @@ constexpr int64_t kMostKeys = kMost - 65536;          // of a sequence: a few ti
 
 constexpr int kRowsLeast = 2, kRowsKeys = 128;        // key tiles that a split has at least; keys of a tile
 constexpr int kTilesLeast = 16, kTilesKeys = 64;     // (a workgroup costs as much as five tiles before its first and behind its last)
-constexpr int kCommonLeast = 4;                       // the same for keys that sequences have in common, whose rows have no other work
+// The same for keys that sequences have in common, whose rows have no other work (64 over 4096 / 16 over 16384 / 200 over 2048 tokens, bf16, with
+// 2: 52.4 / 42.4 / 59.5 us, 4: 49.6 / 42.7 / 59.1, 8: 53.5 / 41.6 / 60.7, 16: 61.8 / 50.2 / 70.3)
+constexpr int kCommonLeast = 4;
 
 int kernel_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // The kernel for many rows, bound by its arithmetic, has two more
@@ -271,6 +273,7 @@ SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_
     // wavefronts than with larger tiles.  bf16, 16 sequences of 4 heads a group over 8192 / 16384 / 32768 common keys 31.7 / 44.6 / 75.9 us
     // against 36.4 / 43.3 / 56.2, 64 over 512 / 2048 25.0 / 40.8 against 37.9 / 41.4; 8 bits, 16 over 16384 / 32768 39.2 / 54.6 against 45.1 /
     // 54.6, 32 over 8192 / 16384 40.1 / 55.3 against 43.9 / 51.4.
+    // (As tiles of 32 rows, the common keys read half as often: 8 bits 3 us less to 1 more, bf16 level to 6 more; of 64 rows 7 to 30 more.)
     const PagedPlan own = paged_plan(tokens, sequences, max_new, keys, heads, kv_heads, dim);
     const int64_t mean = tokens * group / groups;
     const bool few_common = own.few && (double)mean * (double)keys <= (q8 ? 1.5 : 0.875) * (double)(1 << 20);
@@ -280,6 +283,8 @@ SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_
         p.launch[1] = planned((own.many ? sequences : row_tiles(tokens, sequences, group, rows)) + (few_common ? row_tiles(tokens, groups, group, rows) : 0), rows, own.a.want,
                               keys / kRowsKeys + 1, kRowsLeast);
     if (own.many) p.launch[2] = planned(row_tiles(tokens, sequences, group, own.b.rows), own.b.rows, own.b.want, keys / kTilesKeys + 1, kTilesLeast);
+    // Else 128 or 256 rows a workgroup: 64 / 128 sequences over 16384 / 8192 in bf16 60.6 / 72.6 us with 256, 63.9 / 74.5 with 128; 64 over 4096 49.5
+    // against 46.7; 8 bits level.
     if (!few_common) {
         const int many = many_dim(dim) <= 192 && mean > 128 ? 256 : 128;
         p.launch[0] = planned(row_tiles(tokens, groups, group, many), many, many_at_a_time(many, d), keys / kTilesKeys, kCommonLeast);

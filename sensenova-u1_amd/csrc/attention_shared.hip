@@ -15,8 +15,8 @@
 //  * The join: half a wavefront lies along a query's elements and takes some partial results at a time.  Weights are scaled by 2^-16, so that
 //    no sum leaves fp32 whose average does not (there are fewer than 2^16 splits).
 // Measured, 32 query and 8 key / value heads of 128, passes back to back: 64 single tokens over 16384 common keys and 1 to 400 of their own in bf16
-// 62 us (sngguf_paged_attention 447): plan, common keys 28 (17 GFLOP in 256-row workgroups of nine key tiles, half of whose time is their start and
-// 33 MB of partial results), own keys 14, join 11; 32 over 8192 and up to 900 in 8 bits 43.5 (73): plan, one launch of 30, join 6.
+// 59 us (sngguf_paged_attention 447): plan, common keys 28 (17 GFLOP in 256-row workgroups of eight key tiles, half of whose time is their start and
+// 33 MB of partial results), own keys 14, join 9; 32 over 8192 and up to 900 in 8 bits 43 (73): plan, one launch of 30, join 6.
 #include "attention_shared.hpp"
 
 namespace sngguf {
@@ -275,11 +275,11 @@ __global__ __launch_bounds__(64 * W) void attention_shared_plan_kernel(SharedArg
     }
 }
 
-// A query's partial results summed.  TEAMS half wavefronts have a query: two, or all eight of the workgroup where queries are few.
+// A query's partial results summed.  TEAMS half wavefronts have a query, eight or four of them a workgroup, or two (a wavefront, four a workgroup).
 template <int DT, int TEAMS>
-__global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(SharedArgs s) {
+__global__ __launch_bounds__(TEAMS == 2 ? kThreads : 32 * TEAMS) void attention_shared_join_kernel(SharedArgs s) {
     constexpr int PER = DT / 32;             // elements of a lane
-    constexpr int CHUNK = 4;                 // partial results that a team asks for at once
+    constexpr int CHUNK = 2;                 // partial results that a team asks for at once (4: up to 1 us more in a pass, 8: 2 to 5)
     __shared__ float room[TEAMS > 2 ? TEAMS : 1][DT + 2];
     touch_arguments(s);
     const AttentionArgs& a = s.a;
@@ -411,11 +411,14 @@ int launch_shared_plan(const SharedArgs& s, hipStream_t stream) {
 // dim: of the kernels, 64, 128 or 256
 int launch_shared_join(const SharedArgs& s, int dim, hipStream_t stream) {
     const int64_t queries = s.a.tokens_q * s.a.heads;
-    const bool wide = queries <= 4096;
-    const dim3 grid((unsigned)(wide ? queries : (queries + 3) / 4));
+    // Passes with eight / four / two teams: 64 queries of many splits 37.2 / 40.5 / 48.2 us, 512 42.0 / 44.2 / 51.3; 2048 of 35 parts 59.4 / 59.0 /
+    // 61.7, of 17 48.9 / 48.5 / 47.9; 4096 72.7 / 68.7 / 69.4; 6400 of 10 - / 64.7 / 59.2
+    const int teams = queries <= 1024 ? 8 : queries <= 4096 ? 4 : 2;
+    const dim3 grid((unsigned)(teams > 2 ? queries : (queries + 3) / 4));
 #define SNGGUF_GO(D)                                                                                                    \
     if (dim == D) {                                                                                                     \
-        if (wide) attention_shared_join_kernel<D, 8><<<grid, kThreads, 0, stream>>>(s);                                 \
+        if (teams == 8) attention_shared_join_kernel<D, 8><<<grid, 32 * 8, 0, stream>>>(s);                             \
+        else if (teams == 4) attention_shared_join_kernel<D, 4><<<grid, 32 * 4, 0, stream>>>(s);                        \
         else attention_shared_join_kernel<D, 2><<<grid, kThreads, 0, stream>>>(s);                                      \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }

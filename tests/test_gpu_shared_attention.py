@@ -176,6 +176,17 @@ def test_long_common_parts_are_split(dev, dim, kernel, qt):
         b.check(b(), only={0, 1, count - 1})
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("count", [60, 150])
+@KERNELS
+def test_joins_of_many_queries(dev, dim, count, kernel):
+    """From 1024 and from 4096 queries on (32 a token) fewer lanes have one, and partial results come in turns."""
+    own = [1 + i % 20 for i in range(count)]
+    own[3] = 3000
+    b = Batch(dev, [count], [1300], [1] * count, own, 32, 4, dim, 64, ops.BF16, count + dim, kernel=kernel)
+    b.check(b(), only={0, 3, count // 2, count - 1})
+
+
 @BOTH
 def test_long_own_parts_are_split(dev, qt):
     b = Batch(dev, [3], [256], [1, 1, 2], [6000, 5, 3000], 4, 1, 128, 64, qt)
