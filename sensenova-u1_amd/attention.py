@@ -605,7 +605,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.T
     lie in the pages of the first of them that has queries; the other ones' pages hold the same there (``PageTables.fork`` makes them the same pages).
     No more counts as common than every sequence of the group with queries has in front of its new tokens; sequences of no group, or of a group of
     one, have nothing in common.  The result is that of ``paged_attention`` but for the order of its sums; everything else is as there, and where
-    nothing would be gained (few keys, or many new tokens of each sequence) it is what runs."""
+    nothing would be gained (few keys, by the width of the tables, or many new tokens of each sequence) it is what runs."""
     what = "shared_prefix_attention"
     q, qt, qh, pages, lens, ends_q, scale = _paged(what, q, cache, pages, lens, ends_q, max_new, scale, 0)
     (tokens, heads, dim), (sequences, width) = q.shape, pages.shape
