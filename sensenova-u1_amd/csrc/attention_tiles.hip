@@ -617,13 +617,13 @@ __global__ __launch_bounds__(64 * W, DT <= 128 || W == 8 ? 2 : 1) void attention
 // dim: of the kernel, 64, 96, 128, 192 or 256; rows: of a workgroup, 128 or (up to 192 elements) 256
 int launch_attention_tiles(const AttentionArgs& a, int rows, int dim, int source, hipStream_t stream) {
     const bool planned = a.map != nullptr;
-#define SNGGUF_GO(D, S, W, N, P)                                                                                         \
-    if (dim == D && source == S && rows == 32 * W && planned == P) {                                                                    \
+#define SNGGUF_GO(D, S, W, N, P)                                                                                        \
+    if (dim == D && source == S && rows == 32 * W && planned == P) {                                                    \
         constexpr int kLds = N * 2 * Tile<D>::kBytes;                                                                   \
         static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_tiles_kernel<D, S, W, N, P>), \
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds);           \
         if (attr != hipSuccess) return SNGGUF_E_LAUNCH;                                                                 \
-        attention_tiles_kernel<D, S, W, N, P><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                        \
+        attention_tiles_kernel<D, S, W, N, P><<<dim3((unsigned)a.grid), 64 * W, kLds, stream>>>(a);                     \
         return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;                                           \
     }
     // (three stages where a compute unit has room for them; 8-bit tiles pass through registers and need two)

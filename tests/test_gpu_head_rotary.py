@@ -160,6 +160,38 @@ def test_far_negative_and_missing_positions(dev):
     _close(got, *ho.head(q, positions, turns, axis, (64, 64)))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("axes", [4, 5, 9])
+def test_more_axes(dev, axes, interleaved):
+    gen = torch.Generator().manual_seed(axes)
+    q, positions = _values(gen, 21, 3, 128), torch.randint(-50, 5000, (axes, 21), generator=gen)
+    turns, axis = _table(gen, (64, 32, 32), axes)
+    axis[:3] = torch.tensor([-1, axes, axes - 1], dtype=torch.int32)
+    table, weights = RotaryAxes(turns.to(dev), axis.to(dev), (64, 32, 32), interleaved), _weights(gen, (128,))
+    got, _ = rotary(q.to(dev), None, positions.to(dev), table, q_norm=HeadNorm(weights[0].to(dev)))
+    _close(got, *ho.head(q, positions, turns, axis, (64, 32, 32), interleaved, weights=weights))
+    # positions of some of many axes, every other token, one axis for all
+    many = torch.randint(-50, 5000, (axes, 2 * 21), generator=gen)
+    got, _ = rotary(q.to(dev), None, many.to(dev)[:, ::2], table)
+    _close(got, *ho.head(q, many[:, ::2], turns, axis, (64, 32, 32), interleaved))
+    got, _ = rotary(q.to(dev), None, many[:1, :21].to(dev).expand(axes, 21), table)
+    _close(got, *ho.head(q, many[:1, :21].expand(axes, 21), turns, axis, (64, 32, 32), interleaved))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_magnitudes(dev, interleaved):
+    """Parts of very small and very large elements; squares beyond 32 bits make a part zeros."""
+    gen = torch.Generator().manual_seed(3)
+    turns, axis = _table(gen, (64,), 1)
+    table, weights, at = RotaryAxes(turns.to(dev), axis.to(dev), (64,), interleaved), _weights(gen, (64,)), torch.arange(5)[None]
+    norm = HeadNorm(weights[0].to(dev), eps=0.0)
+    for size in (1e-19, 1e-12, 1e17):
+        q = (_values(gen, 5, 2, 64).float() * size).to(torch.bfloat16)
+        _close(rotary(q.to(dev), None, at.to(dev), table, q_norm=norm)[0], *ho.head(q, at, turns, axis, (64,), interleaved, weights=weights, eps=0.0))
+    q = torch.full((5, 2, 64), 1e30, dtype=torch.bfloat16)
+    assert not rotary(q.to(dev), None, at.to(dev), table, q_norm=norm)[0].any()
+
+
 @pytest.mark.parametrize("parts", [(64,), (32, 16, 16), (50, 6)])
 def test_rows_that_are_not_finite_and_rows_of_zeros(dev, parts):
     gen = torch.Generator().manual_seed(5)
