@@ -361,14 +361,15 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
         u32x4_t a, b;
     };
     const int q_items = count * a.q_heads, k_items = count * others;
-    auto load_q = [&](const Item& x) -> Words {
-        Words w = {u32x4_t{0u, 0u, 0u, 0u}, u32x4_t{0u, 0u, 0u, 0u}};
-        if (x.t < count && there) {
-            const bf16_t* p = a.q + (t0 + x.t) * a.q_token + x.h * a.q_head;
-            w = {piece_at(p + ea), piece_at(p + eb)};
-        }
-        return w;
+    // (behind the last item the first one's words again, which go nowhere)
+    const bf16_t* const q_first = a.q + t0 * a.q_token;
+    auto load_q = [&](const Item& x, int64_t at) -> Words {
+        const bf16_t* p = q_first + (x.t < count ? at : 0);
+        return {piece_at(p + ea), piece_at(p + eb)};
     };
+    // how far an item's row is from the one before it, of the same token's run of heads or with another step of tokens
+    const int64_t q_step = q_hop * a.q_token + q_rest * a.q_head, q_wrap = a.q_token - a.q_heads * a.q_head;
+    const int64_t out_step = q_hop * a.q_out_token + q_rest * a.q_out_head, out_wrap = a.q_out_token - a.q_heads * a.q_out_head;
     // values go to the cache as they are: pieces `unit` and `unit` + lanes
     auto load_k = [&](const Item& x, int64_t& slot) -> Words {
         Words w = {u32x4_t{0u, 0u, 0u, 0u}, u32x4_t{0u, 0u, 0u, 0u}};
@@ -387,7 +388,8 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
     };
     Item x = first_item(a.q_heads), y = others ? first_item(others) : Item{count, 0};
     int64_t slot;
-    Words q_raw = load_q(x), k_raw = load_k(y, slot);
+    int64_t q_at = x.t * a.q_token + x.h * a.q_head, out_at = (t0 + x.t) * a.q_out_token + x.h * a.q_out_head;
+    Words q_raw = load_q(x, q_at), k_raw = load_k(y, slot);
 
     // ---- weights: asked for here, used behind the angles -----------------------------------------------------------------------
     struct Weights {
@@ -397,17 +399,24 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
     auto ask_weights = [&](const HeadNormArgs& n) -> Weights {
         Weights w;
         int start_a, start_b;
-        w.part_a = norm_part(n, there ? ea : 0, start_a);
-        w.part_b = norm_part(n, there ? eb : 0, start_b);
-        if (NORM == kNormNone || n.parts == 0) return w;
-        const int at_a = (there ? ea : 0) - start_a, at_b = (there ? eb : 0) - start_b;
+        const int part_a = norm_part(n, ea, start_a), part_b = norm_part(n, eb, start_b), at_a = ea - start_a, at_b = eb - start_b;
+        // (behind the head's elements: weights of its first ones, and a part that is none)
+        w.part_a = there && n.parts ? part_a : -1;
+        w.part_b = there && n.parts ? part_b : -1;
+        if (NORM == kNormNone) return w;
+        if (n.parts == 0) {                              // heads without a norm beside others with one: times 1
+            const uint32_t one = NORM == kNormWide ? 0x3F800000u : 0x3F803F80u;
+#pragma unroll
+            for (u32x4_t& x : w.word) x = u32x4_t{one, one, one, one};
+            return w;
+        }
         if constexpr (NORM == kNormWide) {
-            const u32x4_t* pa = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, w.part_a)) + at_a);
-            const u32x4_t* pb = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, w.part_b)) + at_b);
+            const u32x4_t* pa = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, part_a)) + at_a);
+            const u32x4_t* pb = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(norm_weight(n, part_b)) + at_b);
             w.word[0] = pa[0], w.word[1] = pa[1], w.word[2] = pb[0], w.word[3] = pb[1];
         } else {
-            w.word[0] = piece_at(static_cast<const bf16_t*>(norm_weight(n, w.part_a)) + at_a);
-            w.word[1] = piece_at(static_cast<const bf16_t*>(norm_weight(n, w.part_b)) + at_b);
+            w.word[0] = piece_at(static_cast<const bf16_t*>(norm_weight(n, part_a)) + at_a);
+            w.word[1] = piece_at(static_cast<const bf16_t*>(norm_weight(n, part_b)) + at_b);
         }
         return w;
     };
@@ -429,8 +438,8 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
         float u[8], v[8];
         unpack8(raw.a, u);
         unpack8(raw.b, v);
-        if (NORM && n.parts) {
-            float sa = 0.f, sb = 0.f, ra = 0.f, rb = 0.f;
+        if constexpr (NORM != kNormNone) {
+            float sa = 0.f, sb = 0.f, ra = n.parts ? 0.f : 1.f, rb = ra;
 #pragma unroll
             for (int j = 0; j < 8; j++) sa = __builtin_fmaf(u[j], u[j], sa), sb = __builtin_fmaf(v[j], v[j], sb);
             auto part = [&](int p) {
@@ -446,39 +455,42 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
             for (int p = 2; p < n.parts; p++) part(p);
 #pragma unroll
             for (int j = 0; j < 8; j++) u[j] = u[j] * ra * weight_of(w, 0, j), v[j] = v[j] * rb * weight_of(w, 1, j);
-            if (!rotates) return {pack8(u), pack8(v)};
         } else if (!rotates) {
             return raw;
         }
-        const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(cs_all + t * a.pairs + pair);
-        float p[8], q[8];
+        if (rotates) {
+            const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(cs_all + t * a.pairs + pair);
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const f32x4_t w2 = cs[j / 2];
+            for (int j = 0; j < 8; j += 2) {
+                const f32x4_t w2 = cs[j / 2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float c = w2[2 * i], s = w2[2 * i + 1];
-                if constexpr (NORM) {
-                    p[j + i] = __builtin_fmaf(u[j + i], c, -(v[j + i] * s));
-                    q[j + i] = __builtin_fmaf(v[j + i], c, u[j + i] * s);
-                } else {                                 // (as the rotation by one position has it, to the bit)
-                    p[j + i] = u[j + i] * c - v[j + i] * s;
-                    q[j + i] = v[j + i] * c + u[j + i] * s;
+                for (int i = j; i < j + 2; i++) {
+                    const float c = w2[2 * (i - j)], s = w2[2 * (i - j) + 1], x = u[i], z = v[i];
+                    if constexpr (NORM) {
+                        u[i] = __builtin_fmaf(x, c, -(z * s));
+                        v[i] = __builtin_fmaf(z, c, x * s);
+                    } else {                             // (as the rotation by one position has it, to the bit)
+                        u[i] = x * c - z * s;
+                        v[i] = z * c + x * s;
+                    }
                 }
             }
         }
-        return {pack8(p), pack8(q)};
+        return {pack8(u), pack8(v)};
     };
 
     for (int i0 = 0; i0 < q_items; i0 += teams) {
         const Item next = next_item(x, q_hop, q_rest, a.q_heads);
-        const Words ahead = load_q(next);
+        const bool wraps = next.t != x.t + q_hop;
+        q_at += wraps ? q_step + q_wrap : q_step;
+        const Words ahead = load_q(next, q_at);
         const Words out = turn(q_raw, x.t, a.q_norm, qw);
         if (x.t < count && there) {
-            bf16_t* p = a.q_out + (t0 + x.t) * a.q_out_token + x.h * a.q_out_head;
+            bf16_t* p = a.q_out + out_at;
             *reinterpret_cast<u32x4_t*>(p + ea) = out.a;
             *reinterpret_cast<u32x4_t*>(p + eb) = out.b;
         }
+        out_at += wraps ? out_step + out_wrap : out_step;
         x = next;
         q_raw = ahead;
     }
