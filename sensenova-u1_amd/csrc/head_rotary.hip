@@ -324,19 +324,19 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
     const int turned = 2 * a.pairs;
 
     // ---- this lane's pieces --------------------------------------------------------------------------------------------------
-    int ea, eb, pair = 0;
-    const bool rotates = there && 8 * unit < a.pairs;
-    ea = there ? turned + 16 * (unit - (a.pairs >> 3)) : 0;
-    eb = ea + 8;
+    // (lanes behind the head's elements do what its first one does, so that nothing depends on them but the sums that they have no part in)
+    const int of = there ? unit : 0;
+    const bool rotates = 8 * of < a.pairs;
+    int ea = turned + 16 * (of - (a.pairs >> 3)), eb = ea + 8, pair = 0;
     {
         int start = 0, first = 0;
 #pragma unroll
         for (int p = 0; p < kMostParts; p++) {
-            const int n = p < a.parts ? a.part[p] : 0, at = 8 * unit - first;
+            const int n = p < a.parts ? a.part[p] : 0, at = 8 * of - first;
             if (rotates && at >= 0 && at < n / 2) {
                 ea = start + at;
                 eb = ea + n / 2;
-                pair = 8 * unit;
+                pair = 8 * of;
             }
             start += n;
             first += n / 2;
@@ -360,36 +360,27 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
     struct Words {
         u32x4_t a, b;
     };
-    const int q_items = count * a.q_heads, k_items = count * others;
-    // (behind the last item the first one's words again, which go nowhere)
-    const bf16_t* const q_first = a.q + t0 * a.q_token;
-    auto load_q = [&](const Item& x, int64_t at) -> Words {
-        const bf16_t* p = q_first + (x.t < count ? at : 0);
-        return {piece_at(p + ea), piece_at(p + eb)};
+    auto words_at = [&](const bf16_t* p) -> Words { return {piece_at(p + ea), piece_at(p + eb)}; };
+    // Loads have no branches of their own, since a lane whose words are on their way in another branch would wait for them: behind the last item
+    // the first one's words again, which go nowhere; values, which go to the cache as they are, as pieces `unit` and `unit` + lanes.
+    const int vb = 8 * (unit + lanes) < a.dim ? 8 * (unit + lanes) : 0;
+    auto load_cached = [&](const Item& x, int64_t& slot) -> Words {
+        const bool in = x.t < count;
+        const int64_t token = t0 + (in ? x.t : 0);
+        int h = in ? x.h : 0;
+        const bool value = h >= a.kv_heads;
+        h -= value ? a.kv_heads : 0;
+        const bf16_t* p = (value ? a.v : a.k) + token * (value ? a.v_token : a.k_token) + h * (value ? a.v_head : a.k_head);
+        slot = a.slots[token];
+        return {piece_at(p + (value ? 8 * unit : ea)), piece_at(p + (value ? vb : eb))};
     };
-    // how far an item's row is from the one before it, of the same token's run of heads or with another step of tokens
-    const int64_t q_step = q_hop * a.q_token + q_rest * a.q_head, q_wrap = a.q_token - a.q_heads * a.q_head;
-    const int64_t out_step = q_hop * a.q_out_token + q_rest * a.q_out_head, out_wrap = a.q_out_token - a.q_heads * a.q_out_head;
-    // values go to the cache as they are: pieces `unit` and `unit` + lanes
-    auto load_k = [&](const Item& x, int64_t& slot) -> Words {
-        Words w = {u32x4_t{0u, 0u, 0u, 0u}, u32x4_t{0u, 0u, 0u, 0u}};
-        slot = -1;
-        if (x.t >= count) return w;
-        if (CACHE) slot = a.slots[t0 + x.t];
-        if (CACHE && x.h >= a.kv_heads) {
-            const bf16_t* p = a.v + (t0 + x.t) * a.v_token + (x.h - a.kv_heads) * a.v_head;
-            if (8 * unit < a.dim) w.a = piece_at(p + 8 * unit);
-            if (8 * (unit + lanes) < a.dim) w.b = piece_at(p + 8 * (unit + lanes));
-        } else if (there) {
-            const bf16_t* p = a.k + (t0 + x.t) * a.k_token + x.h * a.k_head;
-            w = {piece_at(p + ea), piece_at(p + eb)};
-        }
-        return w;
-    };
-    Item x = first_item(a.q_heads), y = others ? first_item(others) : Item{count, 0};
-    int64_t slot;
-    int64_t q_at = x.t * a.q_token + x.h * a.q_head, out_at = (t0 + x.t) * a.q_out_token + x.h * a.q_out_head;
-    Words q_raw = load_q(x, q_at), k_raw = load_k(y, slot);
+    const Item x0 = first_item(a.q_heads);
+    Item y = others ? first_item(others) : Item{count, 0};
+    int64_t slot = -1;
+    const Words q_raw = words_at(a.q + t0 * a.q_token + (x0.t < count ? x0.t * a.q_token + x0.h * a.q_head : 0));
+    Words k_raw = {};
+    if constexpr (CACHE) k_raw = load_cached(y, slot);
+    else if (others) k_raw = words_at(a.k + t0 * a.k_token + (y.t < count ? y.t * a.k_token + y.h * a.k_head : 0));
 
     // ---- weights: asked for here, used behind the angles -----------------------------------------------------------------------
     struct Weights {
@@ -400,9 +391,8 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
         Weights w;
         int start_a, start_b;
         const int part_a = norm_part(n, ea, start_a), part_b = norm_part(n, eb, start_b), at_a = ea - start_a, at_b = eb - start_b;
-        // (behind the head's elements: weights of its first ones, and a part that is none)
-        w.part_a = there && n.parts ? part_a : -1;
-        w.part_b = there && n.parts ? part_b : -1;
+        w.part_a = n.parts ? part_a : -1;
+        w.part_b = n.parts ? part_b : -1;
         if (NORM == kNormNone) return w;
         if (n.parts == 0) {                              // heads without a norm beside others with one: times 1
             const uint32_t one = NORM == kNormWide ? 0x3F800000u : 0x3F803F80u;
@@ -442,6 +432,7 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
             float sa = 0.f, sb = 0.f, ra = n.parts ? 0.f : 1.f, rb = ra;
 #pragma unroll
             for (int j = 0; j < 8; j++) sa = __builtin_fmaf(u[j], u[j], sa), sb = __builtin_fmaf(v[j], v[j], sb);
+            if (!there) sa = sb = 0.f;
             auto part = [&](int p) {
                 const float mine = (w.part_a == p ? sa : 0.f) + (w.part_b == p ? sb : 0.f);
                 const float r = rstd_of(lanes_sum(mine, lane_shift), norm_one_over(n, p), n.eps);
@@ -479,36 +470,53 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
         return {pack8(u), pack8(v)};
     };
 
-    for (int i0 = 0; i0 < q_items; i0 += teams) {
-        const Item next = next_item(x, q_hop, q_rest, a.q_heads);
-        const bool wraps = next.t != x.t + q_hop;
-        q_at += wraps ? q_step + q_wrap : q_step;
-        const Words ahead = load_q(next, q_at);
-        const Words out = turn(q_raw, x.t, a.q_norm, qw);
-        if (x.t < count && there) {
-            bf16_t* p = a.q_out + out_at;
-            *reinterpret_cast<u32x4_t*>(p + ea) = out.a;
-            *reinterpret_cast<u32x4_t*>(p + eb) = out.b;
-        }
-        out_at += wraps ? out_step + out_wrap : out_step;
-        x = next;
-        q_raw = ahead;
+    // All items of the queries, or of the keys.  Where each team has one, its words are stored without a branch, as stores that may have been
+    // skipped would have to be waited for with the loads in front of them.
+    auto rows = [&](Item x, Words raw, int heads, int hop, int rest, const bf16_t* from, int64_t token, int64_t head, bf16_t* to, int64_t to_token, int64_t to_head,
+                    const HeadNormArgs& n, const Weights& w) {
+        const int items = count * heads;
+        // how far an item's row is from the one before it, in the same run of heads or with one more token
+        const int64_t step = hop * token + rest * head, wrap = token - heads * head, to_step = hop * to_token + rest * to_head, to_wrap = to_token - heads * to_head;
+        const bf16_t* p = from + t0 * token + x.t * token + x.h * head;
+        bf16_t* out = to + (t0 + x.t) * to_token + x.h * to_head;
+        int i0 = 0;
+        auto item = [&](auto all) {
+            const Item next = next_item(x, hop, rest, heads);
+            const bool wraps = next.t != x.t + hop;
+            Words ahead;
+            if (i0 + teams < items) {
+                p += wraps ? step + wrap : step;
+                ahead = words_at(next.t < count ? p : from + t0 * token);
+            }
+            const bool in = decltype(all)::value || x.t < count;
+            const Words y = turn(raw, in ? x.t : 0, n, w);
+            if (in) {
+                *reinterpret_cast<u32x4_t*>(out + ea) = y.a;
+                *reinterpret_cast<u32x4_t*>(out + eb) = y.b;
+            }
+            out += wraps ? to_step + to_wrap : to_step;
+            x = next;
+            raw = ahead;
+            i0 += teams;
+        };
+        while (i0 + teams <= items) item(std::true_type());
+        if (i0 < items) item(std::false_type());
+    };
+    rows(x0, q_raw, a.q_heads, q_hop, q_rest, a.q, a.q_token, a.q_head, a.q_out, a.q_out_token, a.q_out_head, a.q_norm, qw);
+    if constexpr (!CACHE) {
+        if (others) rows(y, k_raw, others, k_hop, k_rest, a.k, a.k_token, a.k_head, a.k_out, a.k_out_token, a.k_out_head, a.k_norm, kw);
+        return;
     }
+    const int k_items = count * others;
     bf16_t* room = reinterpret_cast<bf16_t*>(cs_all + a.tokens_per_block * a.pairs) + team * a.dim;
     for (int i0 = 0; i0 < k_items; i0 += teams) {
         const Item next = next_item(y, k_hop, k_rest, others);
         int64_t slot_ahead;
-        const Words ahead = load_k(next, slot_ahead);
-        const bool value = CACHE && y.h >= a.kv_heads;
+        const Words ahead = load_cached(next, slot_ahead);
+        const bool value = y.h >= a.kv_heads;
         Words out = k_raw;
-        if (!CACHE || __any(!value)) out = turn(k_raw, y.t, a.k_norm, kw);
-        if constexpr (!CACHE) {
-            if (y.t < count && there) {
-                bf16_t* p = a.k_out + (t0 + y.t) * a.k_out_token + y.h * a.k_out_head;
-                *reinterpret_cast<u32x4_t*>(p + ea) = out.a;
-                *reinterpret_cast<u32x4_t*>(p + eb) = out.b;
-            }
-        } else {
+        if (__any(!value)) out = turn(k_raw, y.t < count ? y.t : 0, a.k_norm, kw);
+        {
             // through LDS, so that four neighbouring lanes have a run of 32 elements (a head's lanes are one wavefront's)
             if (there && !value) {
                 *reinterpret_cast<u32x4_t*>(room + ea) = out.a;
@@ -518,7 +526,7 @@ __global__ __launch_bounds__(kThreads) void head_pairs_kernel(HeadRotaryArgs a) 
             __builtin_amdgcn_wave_barrier();
             const int h = value ? y.h - a.kv_heads : y.h;
             // slots outside the cache (padding is marked by negative ones) are passed over; the lanes of a run agree
-            if (slot >= 0 && slot < a.slot_count) {
+            if (y.t < count && slot >= 0 && slot < a.slot_count) {
                 void* pages = value ? a.v_pages : a.k_pages;
                 uint16_t* scales = value ? a.v_scales : a.k_scales;
                 auto both = [&](auto q8_) {
