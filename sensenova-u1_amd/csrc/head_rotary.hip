@@ -13,9 +13,9 @@
 // read before any of it is written, so a call may work in place.  A lane keeps to the same elements of all heads, so weights,
 // cosines and sines are fetched once for a token.
 //  * head_pairs_kernel, pairs half a part apart in parts of multiples of 16 elements: a lane has eight pairs, both of their elements, and a
-//    workgroup up to four tokens.  4096 tokens of 40 heads of 128: 15.5 us (84 MB, 5.4 TB/s), with two norms a head 17.5; as eight elements a lane,
+//    workgroup up to four tokens.  4096 tokens of 40 heads of 128: 15.3 us (84 MB, 5.5 TB/s), with two norms a head 17.4; as eight elements a lane,
 //    with the others from the lane that has them, and one token a workgroup 20.9 and 33.4.  5003 tokens of 32 query and 8 + 8 heads, two
-//    norms, keys and values written in 8 bits: 29.8 us (113 MB, 3.8 TB/s).  One token: 3 us, all latency.
+//    norms, keys and values written in 8 bits: 28 us (113 MB, 4.0 TB/s).  One token: 3 us, all latency.
 //  * head_rotary_kernel, neighbouring pairs, any parts or rows: a lane has eight elements; those that they are turned with, where they are not among
 //    the eight, are read beside them.  Shapes for which the other is no form, so it is kept simple.
 #include <type_traits>
@@ -562,7 +562,7 @@ int launch_head_rotary(const HeadRotaryArgs& a0, int cache, hipStream_t stream) 
     const int64_t heads = (int64_t)a.q_heads + (cache ? 2 * a.kv_heads : a.k_heads);
     // as many tokens as give each team a head; where there are tokens enough for two workgroups a compute unit, up to four times as many, as
     // finding its elements and weights costs a workgroup as much as two heads do (40 normed heads, 1 / 2 / 4 tokens a workgroup: 4096 tokens
-    // 27.8 / 21.5 / 17.3 us, 3000 - / 18.0 / 14.8, 2048 16.8 / 13.1 / 12.6; eight: 4096 22.4, 33000 137.8 against 133.7)
+    // 27.9 / 21.0 / 17.4 us, 3000 22.2 / 17.6 / 14.3, 2048 16.6 / 12.6 / 12.3; eight: 33000 139.7 against 134.4)
     const int64_t fill = heads * 8 <= teams ? 8 : heads < teams ? teams / heads : 1;
     const int64_t spare = a.tokens / (512 * fill);
     const int64_t tokens = fill * (spare < 1 ? 1 : spare > 4 ? 4 : spare), room = 2048 / a.pairs;       // (16 KB of cosines and sines)
