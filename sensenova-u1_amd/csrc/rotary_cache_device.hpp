@@ -48,7 +48,9 @@ __device__ __forceinline__ void store8(bf16_t* p, u32x4_t v, bool wide) {
 //
 // q = rint(x / d) without a division for each: with r = 1 / d to a step, t = x r is off by at most 2^-22 of itself, and t + (x - t d) r by 2^-44,
 // before it is rounded.  That gives the same whole number: x has 8 significant bits and d at most 11, so x / d is a half exactly, which the
-// second t then is too, or further from one than 2^-13.  (Checked over all x and d.)
+// second t then is too, or further from one than 2^-13.  (Checked over all largest magnitudes of a run, all x up to them and r off by a step either way.)
+// No whole number is beyond 127 then, but where d is held to 512 or rounded down by more than 2^-8 of itself, as a scale below the smallest
+// normal one, 2^-14, may be: at 2^-24 by a third, where x / d is up to 190.  Only there are x held to 127 d.
 // Largest magnitudes are compared as whole numbers, which bf16 without its sign is ordered as, NaN above all.
 __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
@@ -76,9 +78,10 @@ __device__ __forceinline__ u32x2_t quantise8(u32x4_t p, uint16_t& scale) {
         const float r = __builtin_amdgcn_rcpf(d);
         float x[8];
         unpack8(p, x);
-        if (d >= 512.f) {                              // (only then are there larger ones than 127 d, but for d's own rounding)
+        if (d >= 512.f || d < 0x1p-14f) {
+            const float most = 127.f * d;
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_fmed3f(x[i], -127.f * 512.f, 127.f * 512.f);
+            for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
         }
         uint32_t q[8];
 #pragma unroll
