@@ -240,7 +240,8 @@ int launch_page_append(const PageArgs& a, bool one, hipStream_t stream) {
         page_append_kernel<true><<<1, kThreads, 0, stream>>>(a);
     } else {
         page_append_kernel<false><<<1, kThreads, 0, stream>>>(a);
-        if (a.tokens && hipGetLastError() == hipSuccess) page_fill_kernel<<<dim3((unsigned)((a.tokens + kFill - 1) / kFill)), kFill, 0, stream>>>(a);
+        if (hipGetLastError() != hipSuccess) return SNGGUF_E_LAUNCH;      // (asking clears it)
+        if (a.tokens) page_fill_kernel<<<dim3((unsigned)((a.tokens + kFill - 1) / kFill)), kFill, 0, stream>>>(a);
     }
     return hipGetLastError() == hipSuccess ? SNGGUF_OK : SNGGUF_E_LAUNCH;
 }
