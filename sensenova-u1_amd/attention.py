@@ -47,6 +47,11 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
+def _memory(*tensors: Optional[torch.Tensor]):
+    """What holds the memory of tensors whose addresses are kept: a tensor may be given other memory (``.data``)."""
+    return [t.untyped_storage() for t in tensors if t is not None]
+
+
 def _stream(index: int) -> int:
     return ops._raw_stream(index) if ops._raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
@@ -188,7 +193,7 @@ class RotaryTable:
     ``turns``: float64 on the device, one for each pair; pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with
     ``interleaved``; elements behind the 2 * pairs first are left as they are.  ``for_model`` makes it of a checkpoint's settings."""
 
-    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes")
+    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes", "_memory")
 
     def __init__(self, turns: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -200,6 +205,7 @@ class RotaryTable:
         self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self.magnitude, self.interleaved)
         self._address = ctypes.addressof(self._struct)
         # (the same as a table of one axis and one part, where heads are normed as well)
+        self._memory = _memory(turns)
         self._axes = _AXES.pack(turns.data_ptr(), 0, turns.shape[0], self.magnitude, self.interleaved, 1, 2 * turns.shape[0], 0, 0, 0)
 
     @classmethod
@@ -241,7 +247,7 @@ class RotaryAxes:
     counted from part to part (default: one part).  With ``interleaved`` pairs are (2 i, 2 i + 1) throughout.  Elements behind are
     left as they are.  An axis that positions do not have counts as the nearest that they have."""
 
-    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes")
+    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes", "_memory")
 
     def __init__(self, turns: torch.Tensor, axis: torch.Tensor, parts: Optional[Sequence[int]] = None, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -256,6 +262,7 @@ class RotaryAxes:
             raise SnGgufError("RotaryAxes: the magnitude is not finite")
         self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
         self.axis, self.parts, self.interleaved, self.magnitude = axis, parts, bool(interleaved), float(magnitude)
+        self._memory = _memory(turns, axis)
         self._axes = _AXES.pack(turns.data_ptr(), axis.data_ptr(), pairs, magnitude, self.interleaved, len(parts), *parts, *(0, 0, 0)[len(parts) - 1:])
 
     def __reduce__(self):               # (a copy has the addresses of its own tensors)
@@ -281,7 +288,7 @@ class HeadNorm:
     put in a module's place does not.  (Weights that do not start at a 16-byte boundary, or are not neighbours, are copied, and stay as they are now.)  A part
     whose squares add up to more than 32 bits hold, from magnitudes of 1.8e19 on, becomes zeros."""
 
-    __slots__ = ("weights", "eps", "dim", "_norm", "_index")
+    __slots__ = ("weights", "eps", "dim", "_norm", "_index", "_memory")
 
     def __init__(self, *weights: torch.Tensor, eps: float = 1e-6) -> None:
         if not 1 <= len(weights) <= 4:
@@ -292,10 +299,10 @@ class HeadNorm:
             if w.dtype is not kind or size < 8 or size % 8 or w.get_device() != index or index < 0 or (kind is not _BF16 and kind is not torch.float32):
                 raise SnGgufError("HeadNorm: weights must be bf16 or fp32 [a multiple of 8] on a HIP device, of one type, "
                                   f"got {[(str(x.dtype), tuple(x.shape), str(x.device)) for x in weights]}")
-            if w.requires_grad:
-                if torch.is_grad_enabled():
-                    raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
-                w = w.detach()          # (what a parameter's .data is set to later does not take this memory away)
+            if w.requires_grad and torch.is_grad_enabled():
+                raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
+            if w.requires_grad or type(w) is not torch.Tensor:
+                w = w.detach()          # (a parameter's .data may be set to another tensor, which is not what is read)
             address = w.data_ptr()
             if address % 16 or w.stride(0) != 1:
                 w = w.clone(memory_format=torch.contiguous_format)
@@ -306,6 +313,7 @@ class HeadNorm:
         if not (math.isfinite(eps) and eps >= 0):
             raise SnGgufError(f"HeadNorm: eps is {eps}")
         self.weights, self.eps, self.dim, self._index = tuple(kept), float(eps), sum(sizes), index
+        self._memory = _memory(*kept)
         rest = (0, 0, 0)[len(at) - 1:]
         self._norm = _NORM.pack(*at, *rest, *sizes, *rest, len(at), 2 if kind is _BF16 else 0, eps)
 
@@ -389,7 +397,7 @@ class PagedKVCache:
 
     Token t of a sequence lies at slot ``page_of_the_sequence[t // page_size] * page_size + t % page_size``."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index", "_shared")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index", "_shared", "_memory")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
         if not k.is_cuda:
@@ -407,6 +415,7 @@ class PagedKVCache:
         index = k.get_device()
         _same_device("PagedKVCache", index, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._memory = _memory(k, v, k_scale, v_scale)
         self.quant_type = ops.Q8_0 if q8 else ops.BF16
         self.pages, self.kv_heads, self.page_size, self.dim, self._index = pages, kv_heads, page, dim, index
         at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None)

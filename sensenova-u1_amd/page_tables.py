@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import ops
-from .attention import _launch, _launch_with_workspace, _numbers, _same_device
+from .attention import _launch, _launch_with_workspace, _memory, _numbers, _same_device
 from .ops import SnGgufError
 
 
@@ -54,7 +54,7 @@ class PageTables:
     belong to another sequence (``fork``), None where none do.  No two of them share memory, nor with what a call is given.  ``PageTables.empty`` makes them; the constructor takes tensors that are there.  Calls
     change them in place, on the current stream."""
 
-    __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_tables", "_index")
+    __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_tables", "_index", "_lens_at", "_cursor_at", "_memory")
 
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor, page_size: int, held: Optional[torch.Tensor] = None) -> None:
         if not pages.is_cuda:
@@ -75,7 +75,9 @@ class PageTables:
         self._index = pages.get_device()
         _same_device("PageTables", self._index, lens, free, cursor, held)
         self.pages, self.lens, self.free, self.cursor, self.held, self.page_size = pages, lens, free, cursor, held, int(page_size)
-        self._tables = _TABLES.pack(pages.data_ptr(), lens.data_ptr(), 0 if held is None else held.data_ptr(), free.data_ptr(), cursor.data_ptr(), sequences, width, ring,
+        self._memory = _memory(pages, lens, free, cursor, held)
+        self._lens_at, self._cursor_at = lens.data_ptr(), cursor.data_ptr()
+        self._tables = _TABLES.pack(pages.data_ptr(), self._lens_at, 0 if held is None else held.data_ptr(), free.data_ptr(), self._cursor_at, sequences, width, ring,
                                     self.page_size)
 
     def __reduce__(self):               # (a copy has the addresses of its own tensors)
@@ -107,10 +109,12 @@ class PageTables:
         positions, slots, cursor = self.cursor.new_empty(2 * tokens + 2).split((tokens, tokens, 2))
         ends, lens, missing = new.new_empty(2 * sequences + 2).split((sequences + 1, sequences, 1))
         if inplace:
-            lens, cursor = self.lens, self.cursor
+            lens, cursor, lens_at, cursor_at = self.lens, self.cursor, self._lens_at, self._cursor_at
+        else:
+            lens_at, cursor_at = lens.data_ptr(), cursor.data_ptr()
         if sequences:
-            _launch_with_workspace(self._index, _workspace(sequences, tokens), "sngguf_page_append", self._tables, new.data_ptr(), tokens, ends.data_ptr(), lens.data_ptr(),
-                                   cursor.data_ptr(), positions.data_ptr(), slots.data_ptr(), missing.data_ptr())
+            _launch_with_workspace(self._index, _workspace(sequences, tokens), "sngguf_page_append", self._tables, new.data_ptr(), tokens, ends.data_ptr(), lens_at, cursor_at,
+                                   positions.data_ptr(), slots.data_ptr(), missing.data_ptr())
         else:
             for x in (ends, missing, positions):
                 x.zero_()
