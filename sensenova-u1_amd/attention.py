@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 import struct
 from typing import Optional, Sequence, Union
 
@@ -47,9 +48,15 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
-def _memory(*tensors: Optional[torch.Tensor]):
-    """What holds the memory of tensors whose addresses are kept: a tensor may be given other memory (``.data``)."""
-    return [t.untyped_storage() for t in tensors if t is not None]
+def _field(name: str) -> property:
+    """A field that calls have by its address: it can be written into, not replaced."""
+    held = operator.attrgetter("_" + name)
+
+    def refuse(self, value):
+        if value is not held(self):     # (x.field += 1 ends here with the field itself)
+            raise SnGgufError(f"{type(self).__name__}: {name} cannot be replaced (calls use what it was made with)")
+
+    return property(held, refuse)
 
 
 def _stream(index: int) -> int:
@@ -193,20 +200,21 @@ class RotaryTable:
     ``turns``: float64 on the device, one for each pair; pairs are elements (i, i + pairs), or (2 i, 2 i + 1) with
     ``interleaved``; elements behind the 2 * pairs first are left as they are.  ``for_model`` makes it of a checkpoint's settings."""
 
-    __slots__ = ("turns", "interleaved", "magnitude", "_struct", "_address", "_axes", "_memory")
+    __slots__ = ("_turns", "_interleaved", "_magnitude", "_struct", "_address", "_axes", "_memory")
+    turns, interleaved, magnitude = map(_field, ("turns", "interleaved", "magnitude"))
 
     def __init__(self, turns: torch.Tensor, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
             raise SnGgufError(f"RotaryTable: turns must be float64 [pairs] on a HIP device, got {turns.dtype} {tuple(turns.shape)} on '{turns.device}'")
         if not math.isfinite(magnitude):
             raise SnGgufError("RotaryTable: the magnitude is not finite")
-        self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
-        self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
-        self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self.magnitude, self.interleaved)
+        self._turns = turns = turns if turns.is_contiguous() else turns.contiguous()
+        self._interleaved, self._magnitude = bool(interleaved), float(magnitude)
+        self._struct = _TableStruct(turns.data_ptr(), turns.shape[0], self._magnitude, self._interleaved)
         self._address = ctypes.addressof(self._struct)
         # (the same as a table of one axis and one part, where heads are normed as well)
-        self._memory = _memory(turns)
-        self._axes = _AXES.pack(turns.data_ptr(), 0, turns.shape[0], self.magnitude, self.interleaved, 1, 2 * turns.shape[0], 0, 0, 0)
+        self._memory = turns.untyped_storage()      # (a tensor may be given other memory: its .data)
+        self._axes = _AXES.pack(turns.data_ptr(), 0, turns.shape[0], self._magnitude, self._interleaved, 1, 2 * turns.shape[0], 0, 0, 0)
 
     @classmethod
     def for_model(cls, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_context: int = 0,
@@ -247,7 +255,8 @@ class RotaryAxes:
     counted from part to part (default: one part).  With ``interleaved`` pairs are (2 i, 2 i + 1) throughout.  Elements behind are
     left as they are.  An axis that positions do not have counts as the nearest that they have."""
 
-    __slots__ = ("turns", "axis", "parts", "interleaved", "magnitude", "_axes", "_memory")
+    __slots__ = ("_turns", "_axis", "_parts", "_interleaved", "_magnitude", "_axes", "_memory")
+    turns, axis, parts, interleaved, magnitude = map(_field, ("turns", "axis", "parts", "interleaved", "magnitude"))
 
     def __init__(self, turns: torch.Tensor, axis: torch.Tensor, parts: Optional[Sequence[int]] = None, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
@@ -260,13 +269,13 @@ class RotaryAxes:
             raise SnGgufError(f"RotaryAxes: parts of {parts} elements (one to four, even) do not hold {pairs} pairs")
         if not math.isfinite(magnitude):
             raise SnGgufError("RotaryAxes: the magnitude is not finite")
-        self.turns = turns = turns if turns.is_contiguous() else turns.contiguous()
-        self.axis, self.parts, self.interleaved, self.magnitude = axis, parts, bool(interleaved), float(magnitude)
-        self._memory = _memory(turns, axis)
-        self._axes = _AXES.pack(turns.data_ptr(), axis.data_ptr(), pairs, magnitude, self.interleaved, len(parts), *parts, *(0, 0, 0)[len(parts) - 1:])
+        self._turns = turns = turns if turns.is_contiguous() else turns.contiguous()
+        self._axis, self._parts, self._interleaved, self._magnitude = axis, parts, bool(interleaved), float(magnitude)
+        self._memory = turns.untyped_storage(), axis.untyped_storage()
+        self._axes = _AXES.pack(turns.data_ptr(), axis.data_ptr(), pairs, magnitude, self._interleaved, len(parts), *parts, *(0, 0, 0)[len(parts) - 1:])
 
     def __reduce__(self):               # (a copy has the addresses of its own tensors)
-        return RotaryAxes, (self.turns, self.axis, self.parts, self.interleaved, self.magnitude)
+        return RotaryAxes, (self._turns, self._axis, self._parts, self._interleaved, self._magnitude)
 
     @classmethod
     def for_model(cls, parts: Sequence[tuple], interleaved: bool = False, device="cuda") -> "RotaryAxes":
@@ -288,12 +297,13 @@ class HeadNorm:
     put in a module's place does not.  (Weights that do not start at a 16-byte boundary, or are not neighbours, are copied, and stay as they are now.)  A part
     whose squares add up to more than 32 bits hold, from magnitudes of 1.8e19 on, becomes zeros."""
 
-    __slots__ = ("weights", "eps", "dim", "_norm", "_index", "_memory")
+    __slots__ = ("_weights", "_eps", "_dim", "_norm", "_index", "_memory")
+    weights, eps, dim = map(_field, ("weights", "eps", "dim"))
 
     def __init__(self, *weights: torch.Tensor, eps: float = 1e-6) -> None:
         if not 1 <= len(weights) <= 4:
             raise SnGgufError(f"HeadNorm: {len(weights)} parts (one to four are possible)")
-        kind, index, at, sizes, kept = weights[0].dtype, weights[0].get_device(), [], [], []
+        kind, index, at, sizes, kept, memory = weights[0].dtype, weights[0].get_device(), [], [], [], []
         for w in weights:
             size = w.shape[0] if w.dim() == 1 else 0
             if w.dtype is not kind or size < 8 or size % 8 or w.get_device() != index or index < 0 or (kind is not _BF16 and kind is not torch.float32):
@@ -308,17 +318,18 @@ class HeadNorm:
                 w = w.clone(memory_format=torch.contiguous_format)
                 address = w.data_ptr()
             kept.append(w)
+            memory.append(w.untyped_storage())
             at.append(address)
             sizes.append(size)
         if not (math.isfinite(eps) and eps >= 0):
             raise SnGgufError(f"HeadNorm: eps is {eps}")
-        self.weights, self.eps, self.dim, self._index = tuple(kept), float(eps), sum(sizes), index
-        self._memory = _memory(*kept)
+        self._weights, self._eps, self._dim, self._index = tuple(kept), float(eps), sum(sizes), index
+        self._memory = memory
         rest = (0, 0, 0)[len(at) - 1:]
         self._norm = _NORM.pack(*at, *rest, *sizes, *rest, len(at), 2 if kind is _BF16 else 0, eps)
 
     def __reduce__(self):               # (a copy has the addresses of its own tensors)
-        return functools.partial(HeadNorm, eps=self.eps), self.weights
+        return functools.partial(HeadNorm, eps=self._eps), self._weights
 
 
 def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tensor, table, q_norm: Optional[HeadNorm], k_norm: Optional[HeadNorm]):
@@ -329,14 +340,14 @@ def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tens
         if positions.stride(1) != 1 and tokens > 1:
             positions = positions.contiguous()
         axes, stride = positions.shape[0], positions.stride(0)
-        if 2 * table.turns.shape[0] > dim:
-            raise SnGgufError(f"{what}: {table.turns.shape[0]} pairs do not fit heads of {dim} elements")
-        _same_device(what, index, table.axis)
+        if 2 * table._turns.shape[0] > dim:
+            raise SnGgufError(f"{what}: {table._turns.shape[0]} pairs do not fit heads of {dim} elements")
+        _same_device(what, index, table._axis)
     else:
         positions, axes, stride = _numbers(positions, torch.int64, tokens, what, "positions"), 1, 0
     for norm in (q_norm, k_norm):
-        if norm is not None and (norm.dim != dim or norm._index != index):
-            raise SnGgufError(f"{what}: a norm of {norm.dim} elements on device {norm._index} does not go with heads of {dim} on device {index}")
+        if norm is not None and (norm._dim != dim or norm._index != index):
+            raise SnGgufError(f"{what}: a norm of {norm._dim} elements on device {norm._index} does not go with heads of {dim} on device {index}")
     if dim > 512:
         raise SnGgufError(f"{what}: heads of {dim} elements (up to 512 are normed or turned by several positions)")
     return positions, (positions.data_ptr(), axes, stride), q_norm and q_norm._norm, k_norm and k_norm._norm
@@ -358,7 +369,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         positions, at, q_at, k_at = _axes_of("rotary", index, tokens, dim, positions, table, q_norm, k_norm)
     else:
         positions = _numbers(positions, torch.int64, tokens, "rotary", "positions")
-    _same_device("rotary", index, k, positions, table.turns)
+    _same_device("rotary", index, k, positions, table._turns)
     if k is not None:
         k, kt, kh = _heads(k, "rotary", "k")
         if k.shape[0] != tokens or k.shape[2] != dim:
@@ -397,7 +408,8 @@ class PagedKVCache:
 
     Token t of a sequence lies at slot ``page_of_the_sequence[t // page_size] * page_size + t % page_size``."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim", "_struct", "_address", "_index", "_shared", "_memory")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_quant_type", "_pages", "_kv_heads", "_page_size", "_dim", "_struct", "_address", "_index", "_shared", "_memory")
+    k, v, k_scale, v_scale, quant_type, pages, kv_heads, page_size, dim = map(_field, ("k", "v", "k_scale", "v_scale", "quant_type", "pages", "kv_heads", "page_size", "dim"))
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
         if not k.is_cuda:
@@ -414,12 +426,12 @@ class PagedKVCache:
                 raise SnGgufError("PagedKVCache: an int8 cache has contiguous fp16 scales [pages][kv_heads][dim / 32][page_size], a bf16 cache none")
         index = k.get_device()
         _same_device("PagedKVCache", index, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self._memory = _memory(k, v, k_scale, v_scale)
-        self.quant_type = ops.Q8_0 if q8 else ops.BF16
-        self.pages, self.kv_heads, self.page_size, self.dim, self._index = pages, kv_heads, page, dim, index
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._memory = [x.untyped_storage() for x in (k, v, k_scale, v_scale) if x is not None]
+        self._quant_type = ops.Q8_0 if q8 else ops.BF16
+        self._pages, self._kv_heads, self._page_size, self._dim, self._index = pages, kv_heads, page, dim, index
         at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None)
-        self._struct = _CacheStruct(*at, pages, page, kv_heads, dim, self.quant_type)
+        self._struct = _CacheStruct(*at, pages, page, kv_heads, dim, self._quant_type)
         count = pages * kv_heads * page * dim
         self._shared = abs(at[0] - at[1]) < (count if q8 else 2 * count) or (q8 and abs(at[2] - at[3]) < count // 16)
         self._address = ctypes.addressof(self._struct)
@@ -435,14 +447,14 @@ class PagedKVCache:
         return cls(k, v, *scales)
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (self._k, self._v, self._k_scale, self._v_scale) if t is not None)
 
     def _rows(self, k, v, slots, what):
         if self._shared:
             raise SnGgufError(f"{what}: the cache's keys and values share memory")
         (k, kt, kh), (v, vt, vh) = _heads(k, what, "k"), _heads(v, what, "v")
-        if k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[2] != self.dim:
-            raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with a cache of {self.kv_heads} heads of {self.dim}")
+        if k.shape != v.shape or k.shape[1] != self._kv_heads or k.shape[2] != self._dim:
+            raise SnGgufError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with a cache of {self._kv_heads} heads of {self._dim}")
         slots = _numbers(slots, torch.int64, k.shape[0], what, "slots")
         _same_device(what, self._index, k, v, slots)
         return k, v, slots, (k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), k.shape[0])
@@ -463,7 +475,7 @@ class PagedKVCache:
         q, qt, qh = _heads(q, what, "q")
         k, v, slots, rows = self._rows(k, v, slots, what)
         tokens, heads, dim = q.shape
-        if k.shape[0] != tokens or dim != self.dim:
+        if k.shape[0] != tokens or dim != self._dim:
             raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
         if inplace and (q is not q0 or not _apart(q) or (q.numel() and (_rows_share(q, k) or _rows_share(q, v)))):
             raise SnGgufError(f"{what}: in place needs rows that share no element, the elements of a head next to each other")
@@ -472,7 +484,7 @@ class PagedKVCache:
             positions, at, q_at, k_at = _axes_of(what, self._index, tokens, dim, positions, table, q_norm, k_norm)
         else:
             positions = _numbers(positions, torch.int64, tokens, what, "positions")
-        _same_device(what, self._index, q, positions, table.turns)
+        _same_device(what, self._index, q, positions, table._turns)
         out, ot, oh = (q, qt, qh) if inplace else (_new(q), heads * dim, dim)
         if tokens and wide:
             _launch(self._index, "sngguf_cache_write_head_rotary", self._address, table._axes, *at, q_at, q.data_ptr(), heads, qt, qh, out.data_ptr(),
@@ -487,7 +499,7 @@ class PagedKVCache:
         slots = _numbers(slots, torch.int64, None, "PagedKVCache.read", "slots")
         _same_device("PagedKVCache.read", self._index, slots)
         tokens = slots.shape[0]
-        k = self.k.new_empty((tokens, self.kv_heads, self.dim), dtype=_BF16)
+        k = self._k.new_empty((tokens, self._kv_heads, self._dim), dtype=_BF16)
         v = torch.empty_like(k)
         if tokens:
             _launch(self._index, "sngguf_cache_read", self._address, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
@@ -562,9 +574,9 @@ def _paged(what: str, q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor,
     """The checked arguments of a call over a cache: (q, its token and head strides, pages, lens, ends_q, scale)"""
     q, qt, qh = _heads(q, what, "q", True)
     tokens, heads, dim = q.shape
-    if dim != cache.dim:
-        raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with a cache of heads of {cache.dim}")
-    scale = _check_options(what, heads, cache.kv_heads, dim, scale, window)
+    if dim != cache._dim:
+        raise SnGgufError(f"{what}: q {tuple(q.shape)} does not go with a cache of heads of {cache._dim}")
+    scale = _check_options(what, heads, cache._kv_heads, dim, scale, window)
     if not 0 <= max_new < 1 << 63:
         raise SnGgufError(f"{what}: max_new is {max_new}")
     lens = _numbers(lens, torch.int32, None, what, "lens")
@@ -572,8 +584,8 @@ def _paged(what: str, q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor,
     if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != sequences:
         raise SnGgufError(f"{what}: pages must be int32 [{sequences}][width], got {pages.dtype} {tuple(pages.shape)}")
     width = pages.shape[1]
-    if width * cache.page_size > (1 << 31) - 65536:
-        raise SnGgufError(f"{what}: {width} pages of {cache.page_size} tokens a sequence are too many")
+    if width * cache._page_size > (1 << 31) - 65536:
+        raise SnGgufError(f"{what}: {width} pages of {cache._page_size} tokens a sequence are too many")
     if (width > 1 and pages.stride(1) != 1) or (sequences > 1 and pages.stride(0) < width):
         pages = pages.contiguous()
     if ends_q is not None:
@@ -596,11 +608,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.Tensor, l
     what = "paged_attention"
     q, qt, qh, pages, lens, ends_q, scale = _paged(what, q, cache, pages, lens, ends_q, max_new, scale, window)
     (tokens, heads, dim), (sequences, width) = q.shape, pages.shape
-    out, ot, oh = _output(out, q, what, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    out, ot, oh = _output(out, q, what, cache._k, cache._v, cache._k_scale, cache._v_scale)
     if tokens and sequences:
         if ends_q is None:
             max_new = 1
-        nbytes = _paged_workspace(tokens, sequences, max_new, width * cache.page_size, heads, cache.kv_heads, dim)
+        nbytes = _paged_workspace(tokens, sequences, max_new, width * cache._page_size, heads, cache._kv_heads, dim)
         _launch_with_workspace(cache._index, nbytes, "sngguf_paged_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
                                pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, max_new, scale, window, out.data_ptr(), ot, oh)
     return out
@@ -626,11 +638,11 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, pages: torch.T
     _same_device(what, cache._index, groups, shared)
     if not count:
         return paged_attention(q, cache, pages, lens, ends_q, max_new, scale, out=out)
-    out, ot, oh = _output(out, q, what, cache.k, cache.v, cache.k_scale, cache.v_scale)
+    out, ot, oh = _output(out, q, what, cache._k, cache._v, cache._k_scale, cache._v_scale)
     if tokens and sequences:
         if ends_q is None:
             max_new = 1
-        nbytes = _shared_workspace(tokens, sequences, count, max_new, width * cache.page_size, heads, cache.kv_heads, dim, cache.quant_type)
+        nbytes = _shared_workspace(tokens, sequences, count, max_new, width * cache._page_size, heads, cache._kv_heads, dim, cache._quant_type)
         _launch_with_workspace(cache._index, nbytes, "sngguf_shared_attention", q.data_ptr(), tokens, heads, qt, qh, cache._address, pages.data_ptr(),
                                pages.stride(0), width, lens.data_ptr(), ops._ptr(ends_q), sequences, groups.data_ptr(), shared.data_ptr(), count, max_new, scale,
                                out.data_ptr(), ot, oh)

@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import ops
-from .attention import _launch, _launch_with_workspace, _memory, _numbers, _same_device
+from .attention import _field, _launch, _launch_with_workspace, _numbers, _same_device
 from .ops import SnGgufError
 
 
@@ -52,9 +52,10 @@ class PageTables:
     numbers in a ring of at least as many places as there are pages; ``cursor``: int64 [2], how many have been taken from it and given to
     it so far (the c-th lies at place c mod ring, so those from ``cursor[0]`` up to ``cursor[1]`` are there).  ``held``: int32 [sequences], leading pages of a row that
     belong to another sequence (``fork``), None where none do.  No two of them share memory, nor with what a call is given.  ``PageTables.empty`` makes them; the constructor takes tensors that are there.  Calls
-    change them in place, on the current stream."""
+    change them in place, on the current stream.  They can be written into, not replaced."""
 
-    __slots__ = ("pages", "lens", "free", "cursor", "held", "page_size", "_tables", "_index", "_lens_at", "_cursor_at", "_memory")
+    __slots__ = ("_pages", "_lens", "_free", "_cursor", "_held", "_page_size", "_tables", "_index", "_sequences", "_lens_at", "_cursor_at", "_memory")
+    pages, lens, free, cursor, held, page_size = map(_field, ("pages", "lens", "free", "cursor", "held", "page_size"))
 
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor, page_size: int, held: Optional[torch.Tensor] = None) -> None:
         if not pages.is_cuda:
@@ -72,16 +73,16 @@ class PageTables:
         ring = free.shape[0]
         if not 1 <= ring < 1 << 31:
             raise SnGgufError(f"PageTables: a ring of {ring} pages")
-        self._index = pages.get_device()
+        self._index, self._sequences = pages.get_device(), sequences
         _same_device("PageTables", self._index, lens, free, cursor, held)
-        self.pages, self.lens, self.free, self.cursor, self.held, self.page_size = pages, lens, free, cursor, held, int(page_size)
-        self._memory = _memory(pages, lens, free, cursor, held)
+        self._pages, self._lens, self._free, self._cursor, self._held, self._page_size = pages, lens, free, cursor, held, int(page_size)
+        self._memory = pages.untyped_storage(), lens.untyped_storage(), free.untyped_storage(), cursor.untyped_storage(), None if held is None else held.untyped_storage()
         self._lens_at, self._cursor_at = lens.data_ptr(), cursor.data_ptr()
         self._tables = _TABLES.pack(pages.data_ptr(), self._lens_at, 0 if held is None else held.data_ptr(), free.data_ptr(), self._cursor_at, sequences, width, ring,
-                                    self.page_size)
+                                    self._page_size)
 
     def __reduce__(self):               # (a copy has the addresses of its own tensors)
-        return PageTables, (self.pages, self.lens, self.free, self.cursor, self.page_size, self.held)
+        return PageTables, (self._pages, self._lens, self._free, self._cursor, self._page_size, self._held)
 
     @classmethod
     def empty(cls, sequences: int, width: int, pages: int, page_size: int, device="cuda") -> "PageTables":
@@ -98,18 +99,19 @@ class PageTables:
 
         Sequences that outgrow their pages get free ones, in order.  A token for which there is none, or whose sequence's row of pages is
         full, has slot -1 and does not count in ``lens``; ``missing`` says how many there are.  Not ``inplace``, lengths and cursor stay as they
-        were, and only ``pages`` is filled in, behind what the lengths reach: the same step again gives the same."""
+        were, and only ``pages`` is filled in, behind what the lengths reach: the same step again gives the same.  ``tables.lens.copy_(step.lens)`` and
+        ``tables.cursor.copy_(step.cursor)`` take such a step over."""
         what = "PageTables.append"
-        sequences = self.pages.shape[0]
+        sequences = self._sequences
         new = _numbers(new, torch.int32, sequences, what, "new")
         _same_device(what, self._index, new)
         if not 0 <= tokens < 1 << 31:
             raise SnGgufError(f"{what}: {tokens} rows")
         # (two allocations, each cut in one call)
-        positions, slots, cursor = self.cursor.new_empty(2 * tokens + 2).split((tokens, tokens, 2))
+        positions, slots, cursor = self._cursor.new_empty(2 * tokens + 2).split((tokens, tokens, 2))
         ends, lens, missing = new.new_empty(2 * sequences + 2).split((sequences + 1, sequences, 1))
         if inplace:
-            lens, cursor, lens_at, cursor_at = self.lens, self.cursor, self._lens_at, self._cursor_at
+            lens, cursor, lens_at, cursor_at = self._lens, self._cursor, self._lens_at, self._cursor_at
         else:
             lens_at, cursor_at = lens.data_ptr(), cursor.data_ptr()
         if sequences:
@@ -120,7 +122,7 @@ class PageTables:
                 x.zero_()
             slots.fill_(-1)
             if not inplace:
-                cursor.copy_(self.cursor)
+                cursor.copy_(self._cursor)
         return PageStep(ends, lens, positions, slots, cursor, missing)
 
     def release(self, done: torch.Tensor) -> None:
@@ -129,9 +131,9 @@ class PageTables:
         what = "PageTables.release"
         if done.dtype not in (torch.bool, torch.uint8):
             raise SnGgufError(f"{what}: done must be bool or uint8, got {done.dtype}")
-        done = _numbers(done, done.dtype, self.pages.shape[0], what, "done")
+        done = _numbers(done, done.dtype, self._sequences, what, "done")
         _same_device(what, self._index, done)
-        if self.pages.shape[0]:
+        if self._sequences:
             _launch(self._index, "sngguf_page_release", self._tables, done.data_ptr())
 
     def fork(self, parent: torch.Tensor, common: torch.Tensor) -> None:
@@ -139,10 +141,10 @@ class PageTables:
         it holds their pages, and the parent owns them.  Nothing happens to a sequence that has tokens, or whose parent is no sequence or one that
         has a parent in the same call.  What ``shared_prefix_attention`` reads once for all of them."""
         what = "PageTables.fork"
-        sequences = self.pages.shape[0]
+        sequences = self._sequences
         parent, common = _numbers(parent, torch.int32, sequences, what, "parent"), _numbers(common, torch.int32, sequences, what, "common")
         _same_device(what, self._index, parent, common)
-        if self.held is None:
+        if self._held is None:
             raise SnGgufError(f"{what}: these tables have no record of pages held (`held`)")
         if sequences:
             _launch(self._index, "sngguf_page_fork", self._tables, parent.data_ptr(), common.data_ptr())

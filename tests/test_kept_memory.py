@@ -84,6 +84,36 @@ def test_a_norm_of_parameters_shows_the_weights_that_it_reads():
     assert [w.data_ptr() for w in x.weights] == at == list(_NORM.unpack(x._norm)[:2]) and [w.data_ptr() for w in copy.copy(x).weights] == at
 
 
+FIELDS = {"HeadNorm": "weights eps dim", "RotaryTable": "turns interleaved magnitude", "RotaryAxes": "turns axis parts interleaved magnitude",
+          "PageTables": "pages lens free cursor held page_size", "PagedKVCache": "k v k_scale v_scale quant_type pages kv_heads page_size dim"}
+
+
+@pytest.mark.parametrize("name,field", [(name, f) for name, fields in FIELDS.items() for f in fields.split()])
+def test_fields_cannot_be_replaced(name, field):
+    x = _made(name, Standing)[0]
+    held = getattr(x, field)
+    setattr(x, field, held)             # (as x.field += 1 does)
+    for value in (held.clone() if isinstance(held, torch.Tensor) else "other", None):
+        with pytest.raises(ops.SnGgufError, match=f"{name}: {field} cannot be replaced"):
+            setattr(x, field, value)
+    with pytest.raises(AttributeError):
+        delattr(x, field)
+    assert getattr(x, field) is held and getattr(copy.copy(x), field) is not None
+
+
+@pytest.mark.gpu
+def test_a_step_that_was_not_in_place_is_taken_over(dev):
+    tables, same = (PageTables.empty(3, 4, 12, 16, dev) for _ in range(2))
+    for new in ([5, 0, 20], [13, 1, 30], [0, 40, 1]):
+        new = torch.tensor(new, dtype=torch.int32, device=dev)
+        step, want = tables.append(new, 50, inplace=False), same.append(new, 50)
+        with pytest.raises(ops.SnGgufError, match="lens cannot be replaced"):
+            tables.lens = step.lens
+        tables.lens.copy_(step.lens)
+        tables.cursor.copy_(step.cursor)
+        assert all(torch.equal(a, b) for a, b in zip(step, want)) and torch.equal(tables.pages, same.pages) and torch.equal(tables.lens, same.lens)
+
+
 @pytest.mark.gpu
 def test_calls_read_what_they_were_made_with(dev):
     gen = torch.Generator().manual_seed(1)
