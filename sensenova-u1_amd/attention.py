@@ -321,7 +321,7 @@ class HeadNorm:
             memory.append(w.untyped_storage())
             at.append(address)
             sizes.append(size)
-        if not (math.isfinite(eps) and eps >= 0):
+        if not 0 <= eps <= 3.4028234663852886e38:       # (the largest number of 32 bits)
             raise SnGgufError(f"HeadNorm: eps is {eps}")
         self._weights, self._eps, self._dim, self._index = tuple(kept), float(eps), sum(sizes), index
         self._memory = memory

@@ -7,6 +7,8 @@ import torch
 from sensenova_u1_amd import HeadNorm, RotaryAxes, ops
 from sensenova_u1_amd.attention import _AXES, _NORM, _CacheStruct
 
+from .test_kept_memory import Standing
+
 E_TYPE, E_SHAPE, E_NULL, E_ALIGN = -1, -2, -3, -4
 _BUF = ctypes.create_string_buffer(4096 + 64)
 P = (ctypes.addressof(_BUF) + 63) // 64 * 64
@@ -92,3 +94,11 @@ def test_the_packed_structures_are_those_of_the_header():
 
     assert bytes(Axes(5, 7, 3, 1.25, 1, 2, (4, 2, 0, 0))) == _AXES.pack(5, 7, 3, 1.25, 1, 2, 4, 2, 0, 0) and ctypes.sizeof(Axes) == _AXES.size
     assert bytes(Norm((1, 2, 3, 4), (8, 16, 24, 32), 4, 2, 0.5)) == _NORM.pack(1, 2, 3, 4, 8, 16, 24, 32, 4, 2, 0.5) and ctypes.sizeof(Norm) == _NORM.size
+
+
+@pytest.mark.parametrize("eps", [1e300, 3.5e38, -3.5e38, INF, NAN, -1e-9])
+def test_an_eps_that_32_bits_do_not_hold(eps):
+    weight = torch.Tensor._make_subclass(Standing, torch.ones(64))
+    with pytest.raises(ops.SnGgufError, match="HeadNorm: eps is"):
+        HeadNorm(weight, eps=eps)
+    assert HeadNorm(weight, eps=3.4028234663852886e38).eps == 3.4028234663852886e38
