@@ -507,7 +507,8 @@ typedef struct sngguf_page_tables {
  * ends [sequences + 1] where each one's rows start and end (cut at `tokens`), positions and slots [tokens] of each row (0 and -1 behind the last), lens_out
  * [sequences] and cursor_out [2] what lens and cursor are behind the step (they may be the tables' own), and pages filled in for
  * sequences that outgrow theirs, taken from the ring in the order of the sequences.  Tokens for which there is no page, or
- * whose row of pages is full, have slot -1 and no part in lens_out; missing[0] counts them.  workspace (16-byte aligned) of
+ * whose row of pages is full, have slot -1 and no part in lens_out; missing[0] counts them.  What is written shares no memory with anything else, but
+ * that lens_out may be lens and cursor_out cursor.  workspace (16-byte aligned) of
  * sngguf_page_append_workspace_bytes(sequences, tokens) bytes, NULL where that is 0. */
 int64_t sngguf_page_append_workspace_bytes(int64_t sequences, int64_t tokens);
 int sngguf_page_append(const sngguf_page_tables* tables, const int32_t* added, int64_t tokens, int32_t* ends, int32_t* lens_out, int64_t* cursor_out,

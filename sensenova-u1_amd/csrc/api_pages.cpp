@@ -19,14 +19,15 @@ struct Bytes {
     const void* at;
     int64_t count;
 };
+bool overlap(const Bytes& x, const Bytes& y) {
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at), y0 = reinterpret_cast<uintptr_t>(y.at);
+    return x.at && y.at && x.count && y.count && x0 < y0 + (uintptr_t)y.count && y0 < x0 + (uintptr_t)x.count;
+}
 // Whether `x` shares no byte with any of them
 template <int N>
 bool apart(const Bytes& x, const Bytes (&others)[N]) {
-    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at);
-    for (const Bytes& y : others) {
-        const uintptr_t y0 = reinterpret_cast<uintptr_t>(y.at);
-        if (x.at && y.at && x0 < y0 + (uintptr_t)y.count && y0 < x0 + (uintptr_t)x.count) return false;
-    }
+    for (const Bytes& y : others)
+        if (overlap(x, y)) return false;
     return true;
 }
 
@@ -81,9 +82,16 @@ int sngguf_page_append(const sngguf_page_tables* tables, const int32_t* added, i
     if (!aligned(added, 4) || !aligned(ends, 4) || !aligned(lens_out, 4) || !aligned(cursor_out, 8) || !aligned(positions, 8) || !aligned(slots, 8) ||
         !aligned(missing, 4) || !aligned(workspace, 16))
         return SNGGUF_E_ALIGN;
-    const Bytes written[] = {{a.pages, a.sequences * a.width * 4}, {lens_out, a.sequences * 4},  {cursor_out, 16},   {ends, (a.sequences + 1) * 4},
-                             {missing, 4},                          {positions, tokens * 8},      {slots, tokens * 8}};
-    if (!tables_apart(a) || !apart({added, a.sequences * 4}, written)) return SNGGUF_E_BADSHAPE;
+    // What is written, the tables' lengths and cursor among it where they are given for it, and nothing else in part
+    const Bytes written[] = {{lens_out, a.sequences * 4}, {cursor_out, 16}, {ends, (a.sequences + 1) * 4}, {missing, 4}, {positions, tokens * 8}, {slots, tokens * 8}, {workspace, need}};
+    const Bytes tables_of[] = {{a.pages, a.sequences * a.width * 4}, {a.held, a.sequences * 4}, {a.free, (int64_t)a.ring * 4}, {a.lens, a.sequences * 4}, {a.cursor, 16}};
+    if (!tables_apart(a) || !apart({added, a.sequences * 4}, written) || overlap({added, a.sequences * 4}, tables_of[0])) return SNGGUF_E_BADSHAPE;
+    for (const Bytes& x : written) {
+        for (const Bytes& y : written)
+            if (&x != &y && overlap(x, y)) return SNGGUF_E_BADSHAPE;
+        for (const Bytes& y : tables_of)
+            if (overlap(x, y) && !(x.at == y.at && ((x.at == lens_out && y.at == a.lens) || (x.at == cursor_out && y.at == a.cursor)))) return SNGGUF_E_BADSHAPE;
+    }
     a.added = added;
     a.tokens = tokens;
     a.ends = ends;

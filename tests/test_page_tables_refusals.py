@@ -76,6 +76,32 @@ def test_memory_that_is_shared():
             assert lib.sngguf_page_fork(tables(at), *of, None) == E_SHAPE, y
 
 
+@pytest.mark.parametrize("tokens,two", [(4, False), (4, True)])
+def test_outputs_that_are_shared(tokens, two):
+    # arrays 64 KB apart, outputs not in place; with 1025 sequences a workspace as well
+    n = 1025 if two else 4
+    names = ("pages", "lens", "held", "free", "cursor", "added", "lens_out", "cursor_out", "ends", "missing", "positions", "slots", "workspace")
+    room = ctypes.create_string_buffer(14 << 16)
+    at = {name: (ctypes.addressof(room) + 63) // 64 * 64 + (i << 16) for i, name in enumerate(names)}
+    size = dict(pages=16 * n, lens=4 * n, held=4 * n, free=32, cursor=16, added=4 * n, lens_out=4 * n, cursor_out=16, ends=4 * n + 4, missing=4, positions=8 * tokens, slots=8 * tokens, workspace=16 * n)
+    written = names[6:] if two else names[6:-1]
+
+    def append(at):
+        return _append(_tables(sequences=n, **{x: at[x] for x in names[:5]}), at["added"], tokens, at["ends"], at["lens_out"], at["cursor_out"], at["positions"], at["slots"], at["missing"],
+                       at["workspace"], 16 * n if two else 0)
+
+    for x in written:
+        for y in names[:5] + written:
+            if x == y:
+                continue
+            for offset in {0, max(0, size[y] // 16 * 16 - 16), (size[y] - 1) // 8 * 8}:
+                if (offset == 0 and (x, y) in (("lens_out", "lens"), ("cursor_out", "cursor"))) or (x == "workspace" and offset % 16):
+                    continue
+                assert append({**at, x: at[y] + offset}) == E_SHAPE, (x, y, offset)
+    for x in ("lens", "cursor"):
+        assert append({**at, x + "_out": at[x], "ends": at[x]}) == E_SHAPE
+
+
 def test_host_tensors():
     for call in (lambda: PageTables.empty(4, 4, 8, 16, device="cpu"), lambda: PageTables.empty(-1, 4, 8, 16, device="cpu"), lambda: PageTables.empty(4, 0, 8, 16, device="cpu"),
                  lambda: PageTables.empty(4, 4, 0, 16, device="cpu")):
