@@ -253,19 +253,19 @@ class RotaryAxes:
     ``turns``: float64, ``axis``: int32, both on the device, one entry for each pair.  ``parts``: elements of the stretches, one to four, into
     which the first 2 * pairs elements of a head are cut; the pairs of one of n elements are (i, i + n / 2) of it, and pairs are
     counted from part to part (default: one part).  With ``interleaved`` pairs are (2 i, 2 i + 1) throughout.  Elements behind are
-    left as they are.  An axis that positions do not have counts as the nearest that they have."""
+    left as they are.  An axis that positions do not have counts as the nearest that they have.  Fields cannot be replaced."""
 
-    __slots__ = ("_turns", "_axis", "_parts", "_interleaved", "_magnitude", "_axes", "_memory")
+    __slots__ = ("_turns", "_axis", "_parts", "_interleaved", "_magnitude", "_axes", "_pairs", "_memory")
     turns, axis, parts, interleaved, magnitude = map(_field, ("turns", "axis", "parts", "interleaved", "magnitude"))
 
     def __init__(self, turns: torch.Tensor, axis: torch.Tensor, parts: Optional[Sequence[int]] = None, interleaved: bool = False, magnitude: float = 1.0) -> None:
         if turns.dtype != torch.float64 or turns.dim() != 1 or turns.shape[0] < 1 or not turns.is_cuda:
             raise SnGgufError(f"RotaryAxes: turns must be float64 [pairs] on a HIP device, got {turns.dtype} {tuple(turns.shape)} on '{turns.device}'")
-        pairs = turns.shape[0]
+        self._pairs = pairs = turns.shape[0]
         axis = _numbers(axis, torch.int32, pairs, "RotaryAxes", "axis")
         _same_device("RotaryAxes", turns.get_device(), axis)
         parts = (2 * pairs,) if parts is None else tuple(parts)
-        if not 1 <= len(parts) <= 4 or min(parts) < 2 or any(n % 2 for n in parts) or sum(parts) != 2 * pairs:
+        if not 1 <= len(parts) <= 4 or min(parts) < 2 or [n for n in parts if n % 2] or sum(parts) != 2 * pairs:
             raise SnGgufError(f"RotaryAxes: parts of {parts} elements (one to four, even) do not hold {pairs} pairs")
         if not math.isfinite(magnitude):
             raise SnGgufError("RotaryAxes: the magnitude is not finite")
@@ -295,7 +295,8 @@ class HeadNorm:
     ``weights``: one to four tensors [elements] on the device, bf16 or fp32, for the consecutive parts of a head that are normed each by
     itself (one: the whole head); their elements, multiples of 8, are a head's together.  Their memory is read at every call: a change in place counts, a tensor
     put in a module's place does not.  (Weights that do not start at a 16-byte boundary, or are not neighbours, are copied, and stay as they are now.)  A part
-    whose squares add up to more than 32 bits hold, from magnitudes of 1.8e19 on, becomes zeros."""
+    whose squares add up to more than 32 bits hold, from magnitudes of 1.8e19 on, becomes zeros; with an ``eps`` of zero, or near it, one of magnitudes below
+    1e-19 loses digits, and below 2.6e-23, where squares vanish, it is not finite.  Fields cannot be replaced."""
 
     __slots__ = ("_weights", "_eps", "_dim", "_norm", "_index", "_memory")
     weights, eps, dim = map(_field, ("weights", "eps", "dim"))
@@ -305,13 +306,13 @@ class HeadNorm:
             raise SnGgufError(f"HeadNorm: {len(weights)} parts (one to four are possible)")
         kind, index, at, sizes, kept, memory = weights[0].dtype, weights[0].get_device(), [], [], [], []
         for w in weights:
-            size = w.shape[0] if w.dim() == 1 else 0
+            size = w.numel() if w.dim() == 1 else 0
             if w.dtype is not kind or size < 8 or size % 8 or w.get_device() != index or index < 0 or (kind is not _BF16 and kind is not torch.float32):
                 raise SnGgufError("HeadNorm: weights must be bf16 or fp32 [a multiple of 8] on a HIP device, of one type, "
                                   f"got {[(str(x.dtype), tuple(x.shape), str(x.device)) for x in weights]}")
-            if w.requires_grad and torch.is_grad_enabled():
-                raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
-            if w.requires_grad or type(w) is not torch.Tensor:
+            if type(w) is not torch.Tensor or w.requires_grad:
+                if w.requires_grad and torch.is_grad_enabled():
+                    raise SnGgufError("HeadNorm: forward only, but a weight requires a gradient")
                 w = w.detach()          # (a parameter's .data may be set to another tensor, which is not what is read)
             address = w.data_ptr()
             if address % 16 or w.stride(0) != 1:
@@ -335,13 +336,14 @@ class HeadNorm:
 def _axes_of(what: str, index: int, tokens: int, dim: int, positions: torch.Tensor, table, q_norm: Optional[HeadNorm], k_norm: Optional[HeadNorm]):
     """(positions, their axes, elements from one axis to the next) where heads are normed or turned by several positions, and the norms' addresses"""
     if isinstance(table, RotaryAxes):
-        if positions.dtype != torch.int64 or positions.dim() != 2 or positions.shape[1] != tokens or positions.shape[0] < 1:
-            raise SnGgufError(f"{what}: positions must be torch.int64 [axes][{tokens}], got {positions.dtype} {tuple(positions.shape)}")
+        shape = positions.shape
+        if positions.dtype != torch.int64 or len(shape) != 2 or shape[1] != tokens or shape[0] < 1:
+            raise SnGgufError(f"{what}: positions must be torch.int64 [axes][{tokens}], got {positions.dtype} {tuple(shape)}")
         if positions.stride(1) != 1 and tokens > 1:
             positions = positions.contiguous()
-        axes, stride = positions.shape[0], positions.stride(0)
-        if 2 * table._turns.shape[0] > dim:
-            raise SnGgufError(f"{what}: {table._turns.shape[0]} pairs do not fit heads of {dim} elements")
+        axes, stride = shape[0], positions.stride(0)
+        if 2 * table._pairs > dim:
+            raise SnGgufError(f"{what}: {table._pairs} pairs do not fit heads of {dim} elements")
         _same_device(what, index, table._axis)
     else:
         positions, axes, stride = _numbers(positions, torch.int64, tokens, what, "positions"), 1, 0
@@ -427,7 +429,7 @@ class PagedKVCache:
         index = k.get_device()
         _same_device("PagedKVCache", index, v, k_scale, v_scale)
         self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
-        self._memory = [x.untyped_storage() for x in (k, v, k_scale, v_scale) if x is not None]
+        self._memory = k.untyped_storage(), v.untyped_storage(), *((k_scale.untyped_storage(), v_scale.untyped_storage()) if q8 else ())
         self._quant_type = ops.Q8_0 if q8 else ops.BF16
         self._pages, self._kv_heads, self._page_size, self._dim, self._index = pages, kv_heads, page, dim, index
         at = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q8 else None, v_scale.data_ptr() if q8 else None)

@@ -60,17 +60,18 @@ class PageTables:
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor, page_size: int, held: Optional[torch.Tensor] = None) -> None:
         if not pages.is_cuda:
             raise SnGgufError(f"sn_gguf ops run on a HIP device only, got page tables on '{pages.device}'; there is no CPU implementation")
-        if pages.dtype != torch.int32 or pages.dim() != 2 or not pages.is_contiguous() or pages.shape[1] < 1:
-            raise SnGgufError(f"PageTables: pages must be contiguous int32 [sequences][width], got {pages.dtype} {tuple(pages.shape)}")
+        shape = pages.shape
+        if pages.dtype != torch.int32 or len(shape) != 2 or not pages.is_contiguous() or shape[1] < 1:
+            raise SnGgufError(f"PageTables: pages must be contiguous int32 [sequences][width], got {pages.dtype} {tuple(shape)}")
         if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
             raise SnGgufError(f"PageTables: pages of 16 .. 4096 tokens (a power of two) are needed, got {page_size}")
-        sequences, width = pages.shape
+        sequences, width = shape
         if width * page_size > (1 << 31) - 65536 or sequences >= 1 << 24:
             raise SnGgufError(f"PageTables: {sequences} sequences of {width} pages of {page_size} tokens are too many")
         for name, x, dtype, count in (("lens", lens, torch.int32, sequences), ("free", free, torch.int32, None), ("cursor", cursor, torch.int64, 2), ("held", held, torch.int32, sequences)):
             if x is not None and _numbers(x, dtype, count, "PageTables", name) is not x:
                 raise SnGgufError(f"PageTables: {name} must be contiguous")
-        ring = free.shape[0]
+        ring = free.numel()
         if not 1 <= ring < 1 << 31:
             raise SnGgufError(f"PageTables: a ring of {ring} pages")
         self._index, self._sequences = pages.get_device(), sequences
