@@ -431,7 +431,8 @@ typedef struct sngguf_rotary_axes {
 } sngguf_rotary_axes;
 
 /* Norm of single heads: `parts` parts (1 .. 4) of elements[] elements each (multiples of 8, together a whole head), y = weight x /
- * sqrt(mean of the part's x^2 + eps) in fp32 (a part whose sum of squares is beyond it becomes zeros).  weight[]: device, [elements] of one type, 16-byte aligned: bf16 (weight_type 2) or
+ * sqrt(mean of the part's x^2 + eps) in fp32 (a part whose sum of squares is beyond it becomes zeros; without eps, one
+ * whose squares vanish in it is not finite).  weight[]: device, [elements] of one type, 16-byte aligned: bf16 (weight_type 2) or
  * fp32 (weight_type 0). */
 typedef struct sngguf_head_norm {
     const void* weight[4];

@@ -250,6 +250,7 @@ struct SharedPlan {
 //    128, bf16, 8 sequences of 4300 keys at most 23.5 us against 22.2, 32 of 1250 22.8 against 25.9, 64 of 700 25.0 against 26.7; 8 bits, 8 of 4300
 //    23.4 against 21.5, 4 of 16600 30.1 against 30.8);
 //  * where they have 256 rows each on average, whose tiles are full already (two of 256 tokens and four of one, 6016 keys in common: 107 us against 96).
+//    An average: a prompt of some thousand tokens among single tokens sends these there as well, which then read what is common each by itself.
 bool shared_alone(int64_t tokens, int64_t sequences, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
     return (double)sequences * (double)keys * (double)(kv_heads * dim) < (double)(40 << 20) || tokens * (heads / kv_heads) >= 256 * sequences;
 }
@@ -258,7 +259,9 @@ SharedPlan shared_plan(int64_t tokens, int64_t sequences, int64_t groups, int64_
     SharedPlan p = {};
     const int64_t group = heads / kv_heads;
     const int d = kernel_dim(dim);
-    // (one more for what a quotient leaves)
+    // Room for every row tile and, where keys are split, for `want` workgroups more.  With c key tiles a split, an entry of r row tiles and k key tiles takes
+    // r ceil(k / c) <= r k / c + r (1 - 1 / c) workgroups, and c is chosen for a sum of r k / c of no more than `want`, within
+    // 1e-5 of it: over all entries, being whole, no more than want + row tiles.  An entry that found no room would be passed over by the join.
     auto planned = [&](int64_t tiles, int rows, int want, int64_t key_tiles, int64_t least) {
         Launch x;
         x.rows = rows;

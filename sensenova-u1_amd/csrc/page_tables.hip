@@ -9,7 +9,9 @@
 // Two prefix sums over the sequences, then each token by itself.  Little memory is moved (a few bytes a sequence, 16 a token), so
 // the time is launches and latencies: one workgroup does a step of up to 1024 sequences and 4096 tokens, sums, tables and tokens; larger
 // ones are two launches, whose second has a thread for each token.  Passes back to back: 256 sequences of one new token 4.6 us (as two launches
-// 6.0), 16 of 128 5.3 (6.2), 16 of 256 6.9 (6.3), 16 of 500 9.5 (6.5); 37 prompts in 111000 rows 6.6.
+// 6.0), 16 of 128 5.3 (6.2), 16 of 256 6.9 (6.3), 16 of 500 9.5 (6.5); 37 prompts in 111000 rows 6.6.  On the device the two are level at 3000 to 3500
+// rows (1000 sequences of 2 6.1 and 7.5, of 4 8.4 and 7.5), but a second launch costs a call that is not replayed 4.7 us of the host's time (11.9 and 16.6
+// at every one of these sizes): so 4096.
 #include "page_tables.hpp"
 
 namespace sngguf {
